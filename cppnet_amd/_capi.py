@@ -151,6 +151,12 @@ SIGNATURES: dict[str, tuple] = {
     "cnhip_global_avgpool_backward": (i32, [vp, vp, i64, i64, i64, i64, vp]),
     "cnhip_global_maxpool_forward": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, vp]),
     "cnhip_global_maxpool_backward": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, vp]),
+    "cnhip_token_embedding_forward": (i32, [vp, vp, vp, i64, i64, i64, i64, f32, vp, i32, vp]),
+    "cnhip_token_embedding_backward": (i32, [vp, vp, vp, i64, i64, i64, i64, f32, i32, i32, vp]),
+    "cnhip_attention_forward": (i32, [vp] * 5 + [i64] * 6 + [f32, i32, vp, vp, i32, vp]),
+    "cnhip_attention_backward": (i32, [vp] * 9 + [i64] * 6 + [f32, i32, vp, vp, i32, vp]),
+    "cnhip_linear_ce_forward": (i32, [vp] * 6 + [i64] * 3 + [i32, vp, vp]),
+    "cnhip_linear_ce_head": (i32, [vp] * 9 + [i64] * 3 + [i32, i32, vp, vp]),
     "cnhip_rnn_forward": (i32, [vp] * 5 + [i64] * 4 + [vp]),
     "cnhip_rnn_backward": (i32, [vp] * 9 + [i64] * 4 + [vp]),
 }

@@ -480,3 +480,99 @@ def rnn_backward(X, W_ih, W_hh, Y, dY, gW_ih, gW_hh, gb, dX, B, S, I, H) -> None
     _capi.call("cnhip_rnn_backward", *(_p(t) for t in (X, W_ih, W_hh, Y, dY, gW_ih, gW_hh, gb, dX)), B, S, I,
                H, _stream())
 
+
+# ---- language-model operators ----
+def _held(device_of, *operands) -> list:
+    """Pointers of (tensor, name, values, dtype) operands, None for no tensor.
+    Each has to be a contiguous tensor of that many values on device_of's device."""
+    ptrs = []
+    for t, name, n, dtype in operands:
+        ptrs.append(_p(t, name))
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+        if t.numel() != n:
+            raise ValueError(f"{name}: expected {n} values, got {t.numel()}")
+        if t.device != device_of.device:
+            raise ValueError(f"{name} is on {t.device}, not on {device_of.device}")
+    return ptrs
+
+
+def _call_on(t, name: str, *args) -> None:
+    """Calls an entry point on t's device, on that device's current stream."""
+    with torch.cuda.device(t.device):
+        _capi.call(name, *args, _stream())
+
+
+def _positive(**sizes) -> None:
+    for name, n in sizes.items():
+        if n <= 0:
+            raise ValueError(f"{name} must be positive, got {n}")
+
+
+def token_embedding_forward(ids, Wt, out, B, S, V, D, scale: float = 1.0, oob=None, rows=ROWS_REF) -> None:
+    """out [B, S, D] = scale * Wt[ids], Wt token-major (the ColMajor [D, V] of a tied Linear)."""
+    _positive(B=B, S=S, V=V, D=D)
+    f, i = torch.float32, torch.int32
+    p = _held(out, (ids, "ids", B * S, i), (Wt, "Wt", V * D, f), (out, "out", B * S * D, f), (oob, "oob", 1, i))
+    _call_on(out, "cnhip_token_embedding_forward", *p[:3], B, S, V, D, scale, p[3], rows)
+
+
+def token_embedding_backward(ids, dY, gWt, B, S, V, D, scale: float = 1.0, accumulate: bool = False,
+                             rows=ROWS_REF) -> None:
+    """gWt (+)= scale * the sums of dY's rows by token."""
+    _positive(B=B, S=S, V=V, D=D)
+    f, i = torch.float32, torch.int32
+    p = _held(gWt, (ids, "ids", B * S, i), (dY, "dY", B * S * D, f), (gWt, "gWt", V * D, f))
+    _call_on(gWt, "cnhip_token_embedding_backward", *p, B, S, V, D, scale, int(accumulate), rows)
+
+
+def _attention_scale(scale, head_dim: int) -> float:
+    return head_dim ** -0.5 if scale is None else scale
+
+
+def attention_forward(q, k, v, out, lse, B, Sq, Sk, heads, kv_heads, head_dim, causal: bool = False, k_len=None,
+                      q_start=None, scale=None, rows=ROWS_REF) -> None:
+    """out = softmax(scale q k^T) v per head, lse its log-sum-exp (None: not wanted); scale None: 1/sqrt(head_dim).
+    k_len: keys of each sample; q_start: position of its first query (causal); int32 [B]."""
+    _positive(B=B, Sq=Sq, Sk=Sk, heads=heads, kv_heads=kv_heads, head_dim=head_dim)
+    f, i, nq, nk = torch.float32, torch.int32, B * Sq * heads * head_dim, B * Sk * kv_heads * head_dim
+    p = _held(out, (q, "q", nq, f), (k, "k", nk, f), (v, "v", nk, f), (out, "out", nq, f),
+              (lse, "lse", B * Sq * heads, f), (k_len, "k_len", B, i), (q_start, "q_start", B, i))
+    _call_on(out, "cnhip_attention_forward", *p[:5], B, Sq, Sk, heads, kv_heads, head_dim,
+             _attention_scale(scale, head_dim), int(causal), *p[5:], rows)
+
+
+def attention_backward(q, k, v, out, lse, dout, dq, dk, dv, B, Sq, Sk, heads, kv_heads, head_dim, causal: bool = False,
+                       k_len=None, q_start=None, scale=None, rows=ROWS_REF) -> None:
+    """dq, dk, dv from dout and the forward's out and lse, with the forward's arguments."""
+    _positive(B=B, Sq=Sq, Sk=Sk, heads=heads, kv_heads=kv_heads, head_dim=head_dim)
+    f, i, nq, nk = torch.float32, torch.int32, B * Sq * heads * head_dim, B * Sk * kv_heads * head_dim
+    p = _held(dq, (q, "q", nq, f), (k, "k", nk, f), (v, "v", nk, f), (out, "out", nq, f),
+              (lse, "lse", B * Sq * heads, f), (dout, "dout", nq, f), (dq, "dq", nq, f), (dk, "dk", nk, f),
+              (dv, "dv", nk, f), (k_len, "k_len", B, i), (q_start, "q_start", B, i))
+    _call_on(dq, "cnhip_attention_backward", *p[:9], B, Sq, Sk, heads, kv_heads, head_dim,
+             _attention_scale(scale, head_dim), int(causal), *p[9:], rows)
+
+
+def linear_ce_forward(X, W, b, targets, loss, lse, batch: int, in_features: int, classes: int,
+                      reduction: str = "mean", oob=None) -> None:
+    """Cross-entropy of X W + b against class ids (outside [0, classes): no target), and lse [batch]."""
+    _positive(batch=batch, in_features=in_features, classes=classes)
+    f, i = torch.float32, torch.int32
+    p = _held(loss, (X, "X", batch * in_features, f), (W, "W", in_features * classes, f), (b, "b", classes, f),
+              (targets, "targets", batch, i), (loss, "loss", 1, f), (lse, "lse", batch, f), (oob, "oob", 1, i))
+    _call_on(loss, "cnhip_linear_ce_forward", *p[:6], batch, in_features, classes, _red(reduction), p[6])
+
+
+def linear_ce_head(X, W, b, targets, loss, lse, dX, dW, db, batch: int, in_features: int, classes: int,
+                   reduction: str = "mean", accumulate: bool = False, oob=None) -> None:
+    """linear_ce_forward with the gradients: dX overwritten, dW and db overwritten or added to."""
+    _positive(batch=batch, in_features=in_features, classes=classes)
+    f, i = torch.float32, torch.int32
+    p = _held(loss, (X, "X", batch * in_features, f), (W, "W", in_features * classes, f), (b, "b", classes, f),
+              (targets, "targets", batch, i), (loss, "loss", 1, f), (lse, "lse", batch, f),
+              (dX, "dX", batch * in_features, f), (dW, "dW", in_features * classes, f), (db, "db", classes, f),
+              (oob, "oob", 1, i))
+    _call_on(loss, "cnhip_linear_ce_head", *p[:9], batch, in_features, classes, _red(reduction), int(accumulate), p[9])

@@ -741,6 +741,84 @@ int cnhip_rnn_backward(const float* X, const float* W_ih, const float* W_hh, con
                        const float* dY, float* gW_ih, float* gW_hh, float* gb, float* dX,
                        int64_t B, int64_t S, int64_t I, int64_t H, cnhip_stream_t stream);
 
+/* ---- language-model operators --------------------------------------------
+ * Embedding with a scale, attention that keeps no probabilities and a Linear
+ * with cross-entropy that keeps no logits.  The reference has none of the
+ * three in this form; they stand beside its Embedding (embedding.cpp:46-175),
+ * MultiHeadAttention (attention.cpp:60-569) and SoftmaxCrossEntropy
+ * (softmax_cross_entropy.cpp:118-195).
+ *
+ * Workspace is the stream's reusable scratch, as for every other entry point:
+ * to capture a call with cnhip_graph_begin_capture, run it once uncaptured at
+ * the same sizes first.  Calls on different streams may overlap; calls on one
+ * stream from several host threads at once are not supported.  Every sum runs
+ * in an order fixed by the arguments, so equal calls give equal bits.
+ *
+ * Token embedding: out[p, d] = scale * Wt[d + D id_p], ids ColMajor [B, S],
+ * out a [B, S, D] sequence in either row order.  Ids outside [0, V) give zero
+ * rows, take no part in the gradient, and are counted into *oob_count (may be
+ * NULL; added to, not cleared), so padding may carry any negative id.
+ * backward: gWt[d + D v] (+)= scale * sum of dY[p, d] over the rows with id v,
+ * in ascending order of the ids' storage in runs of 16, the runs in order.  accumulate 0
+ * overwrites the whole table's gradient (zeros for unused ids), 1 adds to the
+ * rows of the ids that occur and touches no other.  With tied weights gWt is
+ * the dW that cnhip_linear_ce_head wrote.  B*S < 2^30. */
+int cnhip_token_embedding_forward(const int32_t* ids, const float* Wt, float* out, int64_t B,
+                                  int64_t S, int64_t V, int64_t D, float scale,
+                                  int32_t* oob_count, int rows, cnhip_stream_t stream);
+int cnhip_token_embedding_backward(const int32_t* ids, const float* dY, float* gWt, int64_t B,
+                                   int64_t S, int64_t V, int64_t D, float scale, int accumulate,
+                                   int rows, cnhip_stream_t stream);
+/* Attention core of `heads` heads over `kv_heads` key heads (heads %
+ * kv_heads == 0; query head h reads key head h / (heads / kv_heads)), no
+ * projections: q, out [B, Sq, heads*head_dim], k, v [B, Sk, kv_heads*head_dim]
+ * in either row order, head h in columns [h head_dim, (h+1) head_dim).
+ *   S_ij = scale q_i k_j over the keys j that query i of sample b reads,
+ *   out_i = sum_j exp(S_ij - lse_i) v_j,  lse_i = log sum_j exp(S_ij).
+ * A query reads the keys j < k_len[b] (device int32 [B]; NULL: all Sk; values
+ * are cut to [0, Sk]), and with causal != 0 only those with j <= q_start[b] + i
+ * (device int32 [B], the position of the sample's first query among the keys;
+ * NULL: Sk - Sq).  So a padded batch passes its lengths, and a decoding step
+ * over a cache of capacity Sk passes k_len = the tokens held and q_start =
+ * k_len - Sq.  Keys and values at and past k_len are never used, whatever they
+ * hold; a query that reads no key gives a zero row and lse = -inf.  A NaN or
+ * infinity in a key or value that only some queries of the batch may read can
+ * reach the causal rows just before it.
+ * lse [B*Sq, heads] has q's rows; it may be NULL in the forward.
+ * backward: gradients of q, k and v (overwritten; zeros for keys at and past
+ * k_len) from out, lse and dout; the probabilities are formed again, dk and dv
+ * are summed over the heads that share a key head.  head_dim <= 128,
+ * B * heads <= 65535. */
+int cnhip_attention_forward(const float* q, const float* k, const float* v, float* out,
+                            float* lse, int64_t B, int64_t Sq, int64_t Sk, int64_t heads,
+                            int64_t kv_heads, int64_t head_dim, float scale, int causal,
+                            const int32_t* k_len, const int32_t* q_start, int rows,
+                            cnhip_stream_t stream);
+int cnhip_attention_backward(const float* q, const float* k, const float* v, const float* out,
+                             const float* lse, const float* dout, float* dq, float* dk,
+                             float* dv, int64_t B, int64_t Sq, int64_t Sk, int64_t heads,
+                             int64_t kv_heads, int64_t head_dim, float scale, int causal,
+                             const int32_t* k_len, const int32_t* q_start, int rows,
+                             cnhip_stream_t stream);
+/* Linear to `classes` logits with softmax cross-entropy against class ids:
+ * z = X W + b (X [batch, in_features], W [in_features, classes], b may be
+ * NULL), lse [batch] = log sum exp of each row of z, *loss = the sum over the
+ * rows with a target of lse - z_target, divided by their number for
+ * CNHIP_REDUCE_MEAN (0 where no row has one).  targets: device int32 [batch];
+ * a row whose target is outside [0, classes) has none: no loss, no gradient.
+ * Targets >= classes are counted into *oob_count (may be NULL; added to).
+ * head: also dX [batch, in_features] (overwritten), dW and db (added to with
+ * accumulate, else overwritten; db NULL exactly where b is).  No logits
+ * outlive the call; the rows go through in pieces that bound the workspace. */
+int cnhip_linear_ce_forward(const float* X, const float* W, const float* b,
+                            const int32_t* targets, float* loss, float* lse, int64_t batch,
+                            int64_t in_features, int64_t classes, int reduction,
+                            int32_t* oob_count, cnhip_stream_t stream);
+int cnhip_linear_ce_head(const float* X, const float* W, const float* b, const int32_t* targets,
+                         float* loss, float* lse, float* dX, float* dW, float* db, int64_t batch,
+                         int64_t in_features, int64_t classes, int reduction, int accumulate,
+                         int32_t* oob_count, cnhip_stream_t stream);
+
 /* ---- DataLoader batch assembly (ref: dataloader.cpp:68-88) ----
  * src: the dataset sample-major (sample n's F values at src + n*F), N
  * samples; idx: B int32 sample indices (one outside [0, N) yields zeros);
