@@ -7,13 +7,22 @@
 //   dX = G W^T,  dW (+)= X^T G,  db (+)= column sums of G.
 //
 // The rows go through in pieces whose logits fill a bounded workspace: a
-// piece's logits are formed, turned into its part of G where they lie, and
-// multiplied into dX and dW while they are at hand.
+// piece's logits are formed, turned into its part of G, and multiplied into dX
+// and dW while they are at hand.  Keeping the piece's logits for that moment
+// makes three products of 2 N D V flops; forming them again vocabulary piece
+// by vocabulary piece would make four.
+//
+// The products run on the fp16 matrix cores over operands packed as pairs
+// (mfma_pair.hpp).  X, W and a piece's G are packed once each and serve two
+// products apiece, one along their rows and one across.  The first product
+// leaves each row's maximum and sum of exponentials over the 128 columns that
+// a wave holds, so the logits are read once more only, to become G.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
 
 #include "common.hpp"
+#include "mfma_pair.hpp"
 
 namespace cnhip {
 
@@ -23,106 +32,412 @@ int gemm_f32(int trans_a, int trans_b, int64_t M, int64_t N, int64_t K, float al
 
 namespace {
 
-constexpr int kStatCols = 64;  // columns that a wave reduces for its rows
+using pr::f32x16;
+using pr::f32x4;
+using pr::f32x4u;
+using pr::u32x4;
+
+// What the kernels of a call share, at the head of its workspace.
+struct CeState {
+  int held;        // rows of the batch with a target
+  uint32_t x_max;  // the largest finite |X| of those rows and |W|, as bits
+  uint32_t w_max;
+};
 
 struct CeArgs {
   const int32_t* t;
-  int64_t N, V;
+  const float *X, *W, *b;
+  int64_t N, D, V;
   int64_t row0, R;     // the piece's first row, and its rows
   float* Z;            // the piece's logits [R, V]
-  float2* stat;        // [col blocks][R]: maximum and sum of exp(z - maximum)
+  float2* stat;        // [stat_blocks][R]: maximum and sum of exp(z - maximum)
   int64_t stat_blocks;
   float *lse, *row_loss;
-  int* held;           // rows of the batch with a target
+  CeState* state;
+  uint32_t* row_max;   // [N]: the largest finite |X| of a row without a target
+  char *xp, *wp, *gp;  // packed X [N x D], W^T [V x D], the piece's G [R x V]
+  int steps_d, steps_v;
+  float* db_part;      // [ceil(R / 256)][V], or null
   int32_t* oob;
   int mean;
 };
 
-// Rows of the batch with a target (one block), and the count of targets past
-// the last class.
-__global__ void __launch_bounds__(1024) ce_count_kernel(const int32_t* __restrict__ t, int64_t N, int64_t V, int* held,
-                                                        int32_t* oob) {
+__device__ __forceinline__ bool has_target(const CeArgs& a, int64_t n) {
+  const int32_t t = a.t[n];
+  return t >= 0 && t < a.V;
+}
+// The exponent that row n of X is packed with: one for all rows with a target,
+// whose products with G are summed, and one of its own for a row without.
+__device__ __forceinline__ int x_exp(const CeArgs& a, int64_t n) {
+  return pr::scale_exp(has_target(a, n) ? a.state->x_max : a.row_max[n]);
+}
+// G is 2^kGExp times its value before the division by the number of rows
+constexpr int kGExp = 15;
+__device__ __forceinline__ float grad_factor(const CeArgs& a) {
+  const int held = a.state->held;
+  return a.mean ? 1.f / (float)(held > 0 ? held : 1) : 1.f;
+}
+
+// Rows of the batch with a target (one block), the count of targets past the
+// last class, and the state's other words cleared.
+__global__ void __launch_bounds__(1024) ce_count_kernel(CeArgs a) {
   __shared__ int total[2];
   if (threadIdx.x < 2) total[threadIdx.x] = 0;
   __syncthreads();
   int n = 0, past = 0;
-  for (int64_t i = threadIdx.x; i < N; i += 1024) {
-    n += t[i] >= 0 && t[i] < V;
-    past += t[i] >= V;
+  for (int64_t i = threadIdx.x; i < a.N; i += 1024) {
+    n += has_target(a, i);
+    past += a.t[i] >= a.V;
+    a.row_max[i] = 0u;
   }
   atomicAdd(&total[0], n);
   atomicAdd(&total[1], past);
   __syncthreads();
   if (threadIdx.x == 0) {
-    *held = total[0];
-    if (oob && total[1]) atomicAdd(oob, total[1]);
+    *a.state = CeState{total[0], 0u, 0u};
+    if (a.oob && total[1]) atomicAdd(a.oob, total[1]);
   }
 }
 
-// a lane per row, kStatCols columns
-__global__ void __launch_bounds__(64) ce_stat_kernel(CeArgs a) {
-  const int64_t r = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (r >= a.R) return;
-  const int64_t c0 = (int64_t)blockIdx.y * kStatCols, c1 = c0 + kStatCols < a.V ? c0 + kStatCols : a.V;
-  float m = -INFINITY, s = 0.f;
-  for (int64_t c = c0; c < c1; ++c) {
-    const float z = a.Z[r + a.R * c], mn = fmaxf(m, z), base = mn == -INFINITY ? 0.f : mn;
-    s = s * expf(m - base) + expf(z - base);
-    m = mn;
+// The largest finite |W| and |X|, the latter over the rows with a target, and
+// of each row without: what those hold must not set the others' scale.
+__global__ void __launch_bounds__(256) ce_max_kernel(CeArgs a, int w_blocks) {
+  uint32_t m = 0;
+  const bool w = (int)blockIdx.x < w_blocks;
+  if (w) {
+    const int64_t n = a.V * a.D, n4 = n / 4, step = (int64_t)w_blocks * 256;
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (; i + 3 * step < n4; i += 4 * step) {
+      f32x4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const f32x4u*>(a.W + 4 * (i + u * step));
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max(m, pr::finite_bits(x[u][e]));
+    }
+    for (; i < n4; i += step) {
+      const f32x4 x = *reinterpret_cast<const f32x4u*>(a.W + 4 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = max(m, pr::finite_bits(x[e]));
+    }
+    if (blockIdx.x == 0 && (int64_t)threadIdx.x < n % 4) m = max(m, pr::finite_bits(a.W[4 * n4 + threadIdx.x]));
+  } else {
+    const int64_t bx = (int64_t)blockIdx.x - w_blocks, strips = (a.N + 255) / 256;
+    const int64_t n = bx % strips * 256 + threadIdx.x, d0 = bx / strips * 16;
+    if (n < a.N) {
+      for (int64_t d = d0; d < (d0 + 16 < a.D ? d0 + 16 : a.D); ++d) m = max(m, pr::finite_bits(a.X[n + a.N * d]));
+      if (!has_target(a, n)) {
+        if (m) atomicMax(a.row_max + n, m);
+        m = 0;
+      }
+    }
   }
-  a.stat[(int64_t)blockIdx.y * a.R + r] = float2{m, s};
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+  if ((threadIdx.x & 63) == 0 && m) atomicMax(w ? &a.state->w_max : &a.state->x_max, m);
 }
 
-__global__ void __launch_bounds__(64) ce_row_kernel(CeArgs a) {
-  const int64_t r = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (r >= a.R) return;
+__device__ __forceinline__ void put_frag(char* p, int64_t block, int steps, int step, const float (&x)[8]) {
+  u32x4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t h, l;
+    pr::split2(x[2 * e], x[2 * e + 1], h, l);
+    hi[e] = h;
+    lo[e] = l;
+  }
+  char* q = p + (block * steps + step) * (2 * pr::kFrag) + (threadIdx.x & 63) * 16;
+  *reinterpret_cast<u32x4*>(q) = hi;
+  *reinterpret_cast<u32x4*>(q + pr::kFrag) = lo;
+}
+
+// X and W^T packed, a wave per fragment of 32 rows x 16 k.  Of rows without a
+// target only finite values enter: whatever they hold, a zero of G times it is
+// zero.
+__global__ void __launch_bounds__(256) ce_pack_kernel(CeArgs a, int64_t w_frags, int64_t x_frags) {
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  float x[8];
+  if (f < w_frags) {
+    const float s = pr::exp2i(pr::scale_exp(a.state->w_max));
+    const int64_t v = f / a.steps_d * 32 + r;
+    const int step = (int)(f % a.steps_d);
+    const int64_t d0 = step * 16 + 8 * h;
+    const float* p = a.W + v * a.D + d0;
+    if (v < a.V && d0 + 8 <= a.D) {
+      const f32x4 u = *reinterpret_cast<const f32x4u*>(p), w = *reinterpret_cast<const f32x4u*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = u[e] * s;
+        x[4 + e] = w[e] * s;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = v < a.V && d0 + e < a.D ? p[e] * s : 0.f;
+    }
+    put_frag(a.wp, f / a.steps_d, a.steps_d, step, x);
+    return;
+  }
+  f -= w_frags;
+  if (f >= x_frags) return;
+  // neighbouring waves take neighbouring row blocks: their reads run along a column
+  const int64_t blocks = (a.N + 31) / 32, n = f % blocks * 32 + r;
+  const int step = (int)(f / blocks);
+  const bool in = n < a.N, held = in && has_target(a, n);
+  const float s = in ? pr::exp2i(x_exp(a, n)) : 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int64_t d = step * 16 + 8 * h + e;
+    x[e] = in && d < a.D ? a.X[n + a.N * d] : 0.f;
+    if (!held) x[e] = x[e] - x[e] == 0.f ? x[e] : 0.f;
+    x[e] *= s;
+  }
+  put_frag(a.xp, f % blocks, a.steps_d, step, x);
+}
+
+// ------------------------------------------------------------- the products
+// Element (m, n) of a product goes to out[n + ld m].
+struct Out {
+  float* p;
+  int64_t ld;
+  float* part;      // split sums [splits][M][N], or null
+  int accumulate;
+  int exp_a, exp_b; // which scales to take out: 0 X, 1 W, 2 G
+};
+
+__device__ __forceinline__ int scale_of(const CeState& s, int which) {
+  return which == 0 ? pr::scale_exp(s.x_max) : which == 1 ? pr::scale_exp(s.w_max) : kGExp;
+}
+// store(where, element) for the elements of a tile that this lane holds and
+// that exist, where = p + n + ld m
+template <class F>
+__device__ __forceinline__ void each(const pr::Acc& acc, int tm, int tn, int M, int N, float* p, int64_t ld,
+                                     F&& store) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m0 = tm * pr::TM + (wave >> 2) * 128, m1 = m0 + 4 * (lane >> 5);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
+    if (n >= N) continue;
+    float* q = p + n + ld * m1;
+    if (m0 + 128 <= M) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) store(q + ld * (32 * i + 8 * (e / 4) + e % 4), acc.x[i][j][e]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int m = 32 * i + 8 * (e / 4) + e % 4;
+          if (m1 + m < M) store(q + ld * m, acc.x[i][j][e]);
+        }
+    }
+  }
+}
+
+// Logits of a piece (M: classes, N: rows): stored, with each row's maximum and
+// sum of exponentials over the wave's 128 classes.
+__global__ void __launch_bounds__(pr::GNT, 2) ce_logits_kernel(pr::GemmArgs g, CeArgs a) {
+  __shared__ __align__(16) char lds[pr::kGemmLds];
+  int tm, tn;
+  pr::tile_of((int)blockIdx.x, (g.M + pr::TM - 1) / pr::TM, (g.N + pr::TN - 1) / pr::TN, tm, tn);
+  pr::Acc acc;
+  pr::gemm_tile<false, false>(g, tm, tn, 0, g.steps, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int ez[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
+    ez[j] = -pr::scale_exp(a.state->w_max) - x_exp(a, a.row0 + min(n, g.N - 1));
+  }
+  const int m0 = tm * pr::TM + (wave >> 2) * 128;
+  if (m0 >= g.M) return;
+  const bool whole = m0 + 128 <= g.M;
+  auto row = [&](int i, int e) { return m0 + 32 * i + 8 * (e / 4) + 4 * (lane >> 5) + e % 4; };
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float b = a.b ? a.b[min(row(i, e), g.M - 1)] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc.x[i][j][e] = pr::times_exp2(acc.x[i][j][e], ez[j]) + b;
+    }
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc.x[i][j][e] = row(i, e) < g.M ? acc.x[i][j][e] : -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, acc.x[i][j][e]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        sum += __builtin_amdgcn_exp2f((acc.x[i][j][e] - base) * 1.4426950408889634f);
+    sum += __shfl_xor(sum, 32, 64);
+    if (n >= g.N) continue;
+    if (lane < 32) a.stat[(int64_t)(tm * 2 + (wave >> 2)) * a.R + n] = float2{top, sum};
+  }
+  each(acc, tm, tn, g.M, g.N, a.Z, a.R, [](float* p, float x) { *p = x; });
+}
+
+// dX (A: W across its rows, B: G) and dW (A: G, B: X, both across their rows)
+template <bool TA, bool TB>
+__global__ void __launch_bounds__(pr::GNT, 2) ce_grads_kernel(pr::GemmArgs g, CeArgs a, Out o) {
+  __shared__ __align__(16) char lds[pr::kGemmLds];
+  int tm, tn;
+  pr::tile_of((int)blockIdx.x, (g.M + pr::TM - 1) / pr::TM, (g.N + pr::TN - 1) / pr::TN, tm, tn);
+  const int t0 = (int)blockIdx.y * g.steps_per_split, t1 = min(g.steps, t0 + g.steps_per_split);
+  pr::Acc acc;
+  pr::gemm_tile<TA, TB>(g, tm, tn, t0, t1, lds, acc);
+  if (o.part) {
+    each(acc, tm, tn, g.M, g.N, o.part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float* p, float x) { *p = x; });
+    return;
+  }
+  const int eo = -scale_of(*a.state, o.exp_a) - scale_of(*a.state, o.exp_b);
+  const float factor = grad_factor(a);
+  if (o.accumulate)
+    each(acc, tm, tn, g.M, g.N, o.p, o.ld, [&](float* p, float x) { *p += pr::times_exp2(x, eo) * factor; });
+  else
+    each(acc, tm, tn, g.M, g.N, o.p, o.ld, [&](float* p, float x) { *p = pr::times_exp2(x, eo) * factor; });
+}
+
+__global__ void __launch_bounds__(256) ce_reduce_kernel(CeArgs a, Out o, int M, int N, int splits) {
+  const int64_t total = (int64_t)M * N;
+  const int eo = -scale_of(*a.state, o.exp_a) - scale_of(*a.state, o.exp_b);
+  const float factor = grad_factor(a);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float x = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) x += o.part[s * total + i];
+    float* p = o.p + i % N + o.ld * (i / N);
+    x = pr::times_exp2(x, eo) * factor;
+    *p = o.accumulate ? *p + x : x;
+  }
+}
+
+// ------------------------------------------------------------- row by row
+// lse and loss of 64 rows a block; the 16 waves share the row's parts.
+__global__ void __launch_bounds__(1024) ce_row_kernel(CeArgs a) {
+  __shared__ float2 part[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = (int64_t)blockIdx.x * 64 + lane;
   float m = -INFINITY, s = 0.f;
-  for (int64_t q = 0; q < a.stat_blocks; ++q) {
-    const float2 x = a.stat[q * a.R + r];
+  auto add = [&](float2 x) {
     const float mn = fmaxf(m, x.x), base = mn == -INFINITY ? 0.f : mn;
     s = s * expf(m - base) + x.y * expf(x.x - base);
     m = mn;
-  }
+  };
+  if (r < a.R)
+    for (int64_t q = wave; q < a.stat_blocks; q += 16) add(a.stat[q * a.R + r]);
+  part[wave][lane] = float2{m, s};
+  __syncthreads();
+  if (wave || r >= a.R) return;
+  for (int w = 1; w < 16; ++w) add(part[w][lane]);
   const float lse = m + logf(s);
-  const int32_t t = a.t[a.row0 + r];
-  a.lse[a.row0 + r] = lse;
-  a.row_loss[a.row0 + r] = t >= 0 && t < a.V ? lse - a.Z[r + a.R * (int64_t)t] : 0.f;
+  const int64_t n = a.row0 + r;
+  a.lse[n] = lse;
+  a.row_loss[n] = has_target(a, n) ? lse - a.Z[r + a.R * (int64_t)a.t[n]] : 0.f;
 }
 
-// Z -> G where it lies
+// The piece's G packed, a wave for a step of 16 classes and eight blocks of 32
+// rows; with its column sums where they are wanted.
 __global__ void __launch_bounds__(256) ce_grad_kernel(CeArgs a) {
-  const int64_t total = a.R * a.V;
-  const int held = *a.held;
-  const float f = a.mean ? 1.f / (float)(held > 0 ? held : 1) : 1.f;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i % a.R, c = i / a.R;
-    const int32_t t = a.t[a.row0 + r];
-    float g = 0.f;
-    if (t >= 0 && t < a.V) g = (expf(a.Z[i] - a.lse[a.row0 + r]) - (c == t ? 1.f : 0.f)) * f;
-    a.Z[i] = g;
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t groups = (a.R + 255) / 256, blocks = (a.R + 31) / 32;
+  const int64_t grp = w % groups;
+  const int step = (int)(w / groups);
+  if (step >= a.steps_v) return;
+  const int64_t v0 = (int64_t)step * 16 + 8 * h;
+  const float one = pr::exp2i(kGExp);
+  float sum[8] = {};
+#pragma unroll 2
+  for (int64_t b = grp * 8; b < (grp * 8 + 8 < blocks ? grp * 8 + 8 : blocks); ++b) {
+    const int64_t n = b * 32 + r;
+    const bool in = n < a.R;
+    const int32_t t = in ? a.t[a.row0 + n] : -1;
+    const bool held = t >= 0 && t < a.V;
+    const float lse = in ? a.lse[a.row0 + n] : 0.f;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = in && v0 + e < a.V ? a.Z[n + a.R * (v0 + e)] : -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = __builtin_amdgcn_exp2f((x[e] - lse) * 1.4426950408889634f) - (v0 + e == t ? 1.f : 0.f);
+      x[e] = held && v0 + e < a.V ? x[e] * one : 0.f;
+      sum[e] += x[e];
+    }
+    put_frag(a.gp, b, a.steps_v, step, x);
   }
+  if (!a.db_part) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum[e] += __shfl_xor(sum[e], o, 64);
+    if (r == 0 && v0 + e < a.V) a.db_part[grp * a.V + v0 + e] = sum[e];
+  }
+}
+
+// db (+)= the sums of the groups of rows, in order
+__global__ void __launch_bounds__(256) ce_db_kernel(CeArgs a, float* db, int accumulate) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (v >= a.V) return;
+  float s = 0.f;
+  for (int64_t q = 0; q < (a.R + 255) / 256; ++q) s += a.db_part[q * a.V + v];
+  s = pr::times_exp2(s, -kGExp) * grad_factor(a);
+  db[v] = accumulate ? db[v] + s : s;
 }
 
 // the losses of the rows in a fixed order (one block)
-__global__ void __launch_bounds__(1024) ce_loss_kernel(const float* __restrict__ row_loss, int64_t N,
-                                                       const int* __restrict__ held, int mean,
-                                                       float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) ce_loss_kernel(CeArgs a, float* __restrict__ loss) {
   __shared__ float part[1024];
   float s = 0.f;
-  for (int64_t i = threadIdx.x; i < N; i += 1024) s += row_loss[i];
+  for (int64_t i = threadIdx.x; i < a.N; i += 1024) s += a.row_loss[i];
   part[threadIdx.x] = s;
   __syncthreads();
   for (int w = 512; w > 0; w >>= 1) {
     if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
     __syncthreads();
   }
-  if (threadIdx.x == 0) *loss = mean ? part[0] / (float)(*held > 0 ? *held : 1) : part[0];
+  const int held = a.state->held;
+  if (threadIdx.x == 0) *loss = a.mean ? part[0] / (float)(held > 0 ? held : 1) : part[0];
 }
 
 struct CeGrads {
   float *dX, *dW, *db;
   int accumulate;
 };
+
+struct Split {
+  int splits, steps;
+};
+// Splits of a contraction so that the tiles fill the 256 CUs, each at least 16
+// steps (256 k) long.
+Split split_of(int64_t M, int64_t N, int steps) {
+  const int64_t tiles = (M + pr::TM - 1) / pr::TM * ((N + pr::TN - 1) / pr::TN);
+  int64_t s = tiles >= 224 ? 1 : 256 / tiles;
+  if (s > steps / 16) s = steps / 16;
+  if (s < 1) s = 1;
+  int per = (int)((steps + s - 1) / s);
+  per = (per + 1) / 2 * 2;
+  return Split{(steps + per - 1) / per, per};
+}
 
 int run(const float* X, const float* W, const float* b, const int32_t* targets, float* loss, float* lse,
         const CeGrads* g, int64_t N, int64_t D, int64_t V, int reduction, int32_t* oob, hipStream_t st,
@@ -131,7 +446,7 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
                 (long long)D, (long long)V);
   CNHIP_REQUIRE(X && W && targets && loss && lse, "%s: NULL pointer", who);
   CNHIP_REQUIRE(reduction == CNHIP_REDUCE_MEAN || reduction == CNHIP_REDUCE_SUM, "%s: bad reduction %d", who, reduction);
-  CNHIP_REQUIRE(V < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && D < ((int64_t)1 << 31), "%s: too large", who);
+  CNHIP_REQUIRE(V < ((int64_t)1 << 30) && N < ((int64_t)1 << 30) && D < ((int64_t)1 << 22), "%s: too large", who);
   if (g) {
     CNHIP_REQUIRE(g->dX && g->dW, "%s: NULL pointer", who);
     CNHIP_REQUIRE(!b == !g->db, "%s: db goes with b", who);
@@ -139,43 +454,103 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   }
   CeArgs a{};
   a.t = targets;
+  a.X = X;
+  a.W = W;
+  a.b = b;
   a.N = N;
+  a.D = D;
   a.V = V;
   a.lse = lse;
   a.oob = oob;
   a.mean = reduction == CNHIP_REDUCE_MEAN;
-  a.stat_blocks = (V + kStatCols - 1) / kStatCols;
-  CNHIP_REQUIRE(a.stat_blocks <= 65535, "%s: too many classes", who);
-  const int64_t most = (int64_t)1 << 28;  // logits of a piece
-  int64_t R = most / V;
-  R = R < 1 ? 1 : R >= N ? N : R >= 256 ? R / 256 * 256 : R;
-  const size_t z = (size_t)R * (size_t)V * sizeof(float), s = (size_t)a.stat_blocks * (size_t)R * sizeof(float2);
+  a.steps_d = (int)((D + 31) / 32 * 2);
+  a.steps_v = (int)((V + 31) / 32 * 2);
+  a.stat_blocks = (V + 127) / 128;
+  // rows of a piece: 2^26 logits, but 1024 rows at least, so that the
+  // gradients of W are read and written once in 1024 rows at most
+  const int64_t most = ((int64_t)1 << 26) / V;
+  int64_t R = most < 1024 ? 1024 : most / 256 * 256;
+  if (R > N) R = N;
+  const int64_t Rp = (R + 31) / 32 * 32, Np = (N + 31) / 32 * 32, Vp = (V + 31) / 32 * 32, Dp = (D + 31) / 32 * 32;
+  const Split sx = split_of(D, R, a.steps_v), sw = split_of(V, D, (int)(Rp / 16));
+  size_t at = 0;
+  auto place = [&](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  const size_t o_state = place(sizeof(CeState)), o_loss = place((size_t)N * 4), o_rows = place((size_t)N * 4), o_x = place((size_t)(Np * Dp) * 4),
+               o_w = place((size_t)(Vp * Dp) * 4), o_z = place((size_t)R * (size_t)V * 4),
+               o_stat = place((size_t)a.stat_blocks * (size_t)R * 8);
+  const size_t o_g = place(g ? (size_t)(Rp * Vp) * 4 : 0), o_db = place(g && g->db ? (size_t)((R + 255) / 256 * V) * 4 : 0);
+  const size_t px = sx.splits > 1 ? (size_t)sx.splits * (size_t)(D * R) * 4 : 0,
+               pw = sw.splits > 1 ? (size_t)sw.splits * (size_t)(V * D) * 4 : 0;
+  const size_t o_part = place(g ? (px > pw ? px : pw) : 0);
   void* ws = nullptr;
-  CNHIP_TRY(scratch(st, kScratchLayer, z + 16 + s + (size_t)N * sizeof(float) + 16, &ws, who));
-  char* p = static_cast<char*>(ws);
-  a.Z = reinterpret_cast<float*>(p);
-  a.stat = reinterpret_cast<float2*>(p + (z + 15) / 16 * 16);
-  a.row_loss = reinterpret_cast<float*>(a.stat + a.stat_blocks * R);
-  a.held = reinterpret_cast<int*>(a.row_loss + N);
-  hipLaunchKernelGGL(ce_count_kernel, dim3(1), dim3(1024), 0, st, targets, N, V, a.held, oob);
+  CNHIP_TRY(scratch(st, kScratchLayer, at, &ws, who));
+  char* base = static_cast<char*>(ws);
+  a.state = reinterpret_cast<CeState*>(base + o_state);
+  a.row_loss = reinterpret_cast<float*>(base + o_loss);
+  a.row_max = reinterpret_cast<uint32_t*>(base + o_rows);
+  a.xp = base + o_x;
+  a.wp = base + o_w;
+  a.Z = reinterpret_cast<float*>(base + o_z);
+  a.stat = reinterpret_cast<float2*>(base + o_stat);
+  a.gp = base + o_g;
+  a.db_part = g && g->db ? reinterpret_cast<float*>(base + o_db) : nullptr;
+  float* part = reinterpret_cast<float*>(base + o_part);
+
+  hipLaunchKernelGGL(ce_count_kernel, dim3(1), dim3(1024), 0, st, a);
   CNHIP_TRY(check_launch(who));
+  const int64_t wb = (V * D / 16 + 255) / 256, w_blocks = wb < 1 ? 1 : wb > 2048 ? 2048 : wb;
+  const int64_t x_blocks = (N + 255) / 256 * ((D + 15) / 16);
+  CNHIP_REQUIRE(w_blocks + x_blocks < ((int64_t)1 << 31), "%s: too large", who);
+  hipLaunchKernelGGL(ce_max_kernel, dim3((unsigned)(w_blocks + x_blocks)), dim3(256), 0, st, a, (int)w_blocks);
+  CNHIP_TRY(check_launch(who));
+  const int64_t w_frags = Vp / 32 * a.steps_d, x_frags = Np / 32 * a.steps_d;
+  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)((w_frags + x_frags + 3) / 4)), dim3(256), 0, st, a, w_frags, x_frags);
+  CNHIP_TRY(check_launch(who));
+
+  const pr::Packed pw_{a.wp, (int)(Vp / 32), a.steps_d};
+  auto tiles = [](int64_t M, int64_t Nn) { return (M + pr::TM - 1) / pr::TM * ((Nn + pr::TN - 1) / pr::TN); };
   for (int64_t r0 = 0; r0 < N; r0 += R) {
     a.row0 = r0;
     a.R = N - r0 < R ? N - r0 : R;
-    CNHIP_TRY(gemm_f32(0, 0, a.R, V, D, 1.f, X + r0, N, W, D, 0.f, a.Z, a.R, b, 0, st, who));
-    hipLaunchKernelGGL(ce_stat_kernel, dim3((unsigned)((a.R + 63) / 64), (unsigned)a.stat_blocks), dim3(64), 0, st, a);
-    CNHIP_TRY(check_launch(who));
-    hipLaunchKernelGGL(ce_row_kernel, dim3((unsigned)((a.R + 63) / 64)), dim3(64), 0, st, a);
+    const int rb = (int)((a.R + 31) / 32);
+    const pr::Packed px_{a.xp + (r0 / 32) * a.steps_d * (2 * pr::kFrag), rb, a.steps_d};
+    const pr::Packed pg_{a.gp, rb, a.steps_v};
+    {
+      const pr::GemmArgs ga{pw_, px_, (int)V, (int)a.R, a.steps_d, a.steps_d, a.steps_d / 2};
+      hipLaunchKernelGGL(ce_logits_kernel, dim3((unsigned)tiles(V, a.R)), dim3(pr::GNT), 0, st, ga, a);
+      CNHIP_TRY(check_launch(who));
+    }
+    hipLaunchKernelGGL(ce_row_kernel, dim3((unsigned)((a.R + 63) / 64)), dim3(1024), 0, st, a);
     CNHIP_TRY(check_launch(who));
     if (!g) continue;
-    hipLaunchKernelGGL(ce_grad_kernel, dim3(elementwise_grid(a.R * V, 256)), dim3(256), 0, st, a);
-    CNHIP_TRY(check_launch(who));
     const int add = g->accumulate || r0 > 0;
-    CNHIP_TRY(gemm_f32(0, 1, a.R, D, V, 1.f, a.Z, a.R, W, D, 0.f, g->dX + r0, N, nullptr, 0, st, who));
-    CNHIP_TRY(gemm_f32(1, 0, D, V, a.R, 1.f, X + r0, N, a.Z, a.R, add ? 1.f : 0.f, g->dW, D, nullptr, 0, st, who));
-    if (g->db) CNHIP_TRY(cnhip_column_sum(a.Z, g->db, a.R, V, add, st));
+    hipLaunchKernelGGL(ce_grad_kernel, dim3((unsigned)(((a.R + 255) / 256 * a.steps_v + 3) / 4)), dim3(256), 0, st, a);
+    CNHIP_TRY(check_launch(who));
+    if (g->db) {
+      hipLaunchKernelGGL(ce_db_kernel, dim3((unsigned)((V + 255) / 256)), dim3(256), 0, st, a, g->db, add);
+      CNHIP_TRY(check_launch(who));
+    }
+    auto grads = [&](auto kernel, const pr::Packed& A, const pr::Packed& B, int64_t M, int64_t Nn, int steps, Split sp,
+                     Out o) -> int {
+      const pr::GemmArgs ga{A, B, (int)M, (int)Nn, steps, sp.steps, steps / 2};
+      const int splits = (steps + sp.steps - 1) / sp.steps;
+      o.part = splits > 1 ? part : nullptr;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)tiles(M, Nn), (unsigned)splits), dim3(pr::GNT), 0, st, ga, a, o);
+      CNHIP_TRY(check_launch(who));
+      if (splits == 1) return CNHIP_OK;
+      hipLaunchKernelGGL(ce_reduce_kernel, dim3(elementwise_grid(M * Nn, 256)), dim3(256), 0, st, a, o, (int)M, (int)Nn,
+                         splits);
+      return check_launch(who);
+    };
+    CNHIP_TRY(grads(ce_grads_kernel<true, false>, pw_, pg_, D, a.R, a.steps_v, sx,
+                    Out{g->dX + r0, N, nullptr, 0, 1, 2}));
+    CNHIP_TRY(grads(ce_grads_kernel<true, true>, pg_, px_, V, D, 2 * rb, sw, Out{g->dW, D, nullptr, add, 0, 2}));
   }
-  hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(1024), 0, st, a.row_loss, N, a.held, a.mean, loss);
+  hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(1024), 0, st, a, loss);
   return check_launch(who);
 }
 

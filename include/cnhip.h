@@ -807,6 +807,8 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
  * CNHIP_REDUCE_MEAN (0 where no row has one).  targets: device int32 [batch];
  * a row whose target is outside [0, classes) has none: no loss, no gradient.
  * Targets >= classes are counted into *oob_count (may be NULL; added to).
+ * Such a row's X reaches nothing but its lse, in which values that are not
+ * finite count as zeros.
  * head: also dX [batch, in_features] (overwritten), dW and db (added to with
  * accumulate, else overwritten; db NULL exactly where b is).  No logits
  * outlive the call; the rows go through in pieces that bound the workspace. */
