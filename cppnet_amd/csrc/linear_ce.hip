@@ -54,7 +54,8 @@ struct CeArgs {
   int64_t stat_blocks;
   float *lse, *row_loss;
   CeState* state;
-  uint32_t* row_max;   // [N]: the largest finite |X| of a row without a target
+  uint32_t *row_max, *w_part;  // largest finite |X| of each row, |W| of each block's part
+  int w_blocks;
   char *xp, *wp, *gp;  // packed X [N x D], W^T [V x D], the piece's G [R x V]
   int steps_d, steps_v;
   float* db_part;      // [ceil(R / 256)][V], or null
@@ -78,35 +79,21 @@ __device__ __forceinline__ float grad_factor(const CeArgs& a) {
   return a.mean ? 1.f / (float)(held > 0 ? held : 1) : 1.f;
 }
 
-// Rows of the batch with a target (one block), the count of targets past the
-// last class, and the state's other words cleared.
-__global__ void __launch_bounds__(1024) ce_count_kernel(CeArgs a) {
-  __shared__ int total[2];
-  if (threadIdx.x < 2) total[threadIdx.x] = 0;
-  __syncthreads();
-  int n = 0, past = 0;
-  for (int64_t i = threadIdx.x; i < a.N; i += 1024) {
-    n += has_target(a, i);
-    past += a.t[i] >= a.V;
-    a.row_max[i] = 0u;
-  }
-  atomicAdd(&total[0], n);
-  atomicAdd(&total[1], past);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    *a.state = CeState{total[0], 0u, 0u};
-    if (a.oob && total[1]) atomicAdd(a.oob, total[1]);
-  }
+__device__ __forceinline__ uint32_t wave_max(uint32_t m) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+  return m;
 }
 
-// The largest finite |W| and |X|, the latter over the rows with a target, and
-// of each row without: what those hold must not set the others' scale.
-__global__ void __launch_bounds__(256) ce_max_kernel(CeArgs a, int w_blocks) {
+// The largest finite |W| of each of the first w_blocks blocks' parts, then of
+// each row of X (64 rows a block, the 16 waves share the columns).
+__global__ void __launch_bounds__(1024) ce_max_kernel(CeArgs a) {
+  __shared__ uint32_t part[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t m = 0;
-  const bool w = (int)blockIdx.x < w_blocks;
-  if (w) {
-    const int64_t n = a.V * a.D, n4 = n / 4, step = (int64_t)w_blocks * 256;
-    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if ((int)blockIdx.x < a.w_blocks) {
+    const int64_t n = a.V * a.D, n4 = n / 4, step = (int64_t)a.w_blocks * 1024;
+    int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x;
     for (; i + 3 * step < n4; i += 4 * step) {
       f32x4 x[4];
 #pragma unroll
@@ -122,20 +109,75 @@ __global__ void __launch_bounds__(256) ce_max_kernel(CeArgs a, int w_blocks) {
       for (int e = 0; e < 4; ++e) m = max(m, pr::finite_bits(x[e]));
     }
     if (blockIdx.x == 0 && (int64_t)threadIdx.x < n % 4) m = max(m, pr::finite_bits(a.W[4 * n4 + threadIdx.x]));
-  } else {
-    const int64_t bx = (int64_t)blockIdx.x - w_blocks, strips = (a.N + 255) / 256;
-    const int64_t n = bx % strips * 256 + threadIdx.x, d0 = bx / strips * 16;
-    if (n < a.N) {
-      for (int64_t d = d0; d < (d0 + 16 < a.D ? d0 + 16 : a.D); ++d) m = max(m, pr::finite_bits(a.X[n + a.N * d]));
-      if (!has_target(a, n)) {
-        if (m) atomicMax(a.row_max + n, m);
-        m = 0;
-      }
+    m = wave_max(m);
+    if (lane == 0) part[0][wave] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 16; ++w) m = max(m, part[0][w]);
+      a.w_part[blockIdx.x] = m;
+    }
+    return;
+  }
+  const int64_t n = ((int64_t)blockIdx.x - a.w_blocks) * 64 + lane;
+  if (n < a.N) {
+    int64_t d = wave;
+    for (; d + 7 * 16 < a.D; d += 8 * 16) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = a.X[n + a.N * (d + 16 * u)];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) m = max(m, pr::finite_bits(x[u]));
+    }
+    for (; d < a.D; d += 16) m = max(m, pr::finite_bits(a.X[n + a.N * d]));
+  }
+  part[wave][lane] = m;
+  __syncthreads();
+  if (wave || n >= a.N) return;
+  for (int w = 1; w < 16; ++w) m = max(m, part[w][lane]);
+  a.row_max[n] = m;
+}
+
+// The call's state (one block): the rows of the batch with a target, the
+// largest finite |X| of those, the largest |W|; and the targets past the last
+// class added to the caller's count.
+__global__ void __launch_bounds__(1024) ce_state_kernel(CeArgs a) {
+  __shared__ uint32_t total[4];
+  if (threadIdx.x < 4) total[threadIdx.x] = 0;
+  __syncthreads();
+  int n = 0, past = 0;
+  uint32_t x = 0, w = 0;
+  constexpr int U = 8;  // loads under way at a time
+  for (int64_t i0 = threadIdx.x; i0 < a.N; i0 += U * 1024) {
+    int32_t t[U];
+    uint32_t m[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * 1024;
+      t[u] = i < a.N ? a.t[i] : -1;
+      m[u] = i < a.N ? a.row_max[i] : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool held = t[u] >= 0 && t[u] < a.V;
+      n += held;
+      past += t[u] >= a.V;
+      if (held) x = max(x, m[u]);
     }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-  if ((threadIdx.x & 63) == 0 && m) atomicMax(w ? &a.state->w_max : &a.state->x_max, m);
+  for (int i = threadIdx.x; i < a.w_blocks; i += 1024) w = max(w, a.w_part[i]);
+  x = wave_max(x);
+  w = wave_max(w);
+  atomicAdd(&total[0], (uint32_t)n);
+  atomicAdd(&total[1], (uint32_t)past);
+  if ((threadIdx.x & 63) == 0) {
+    atomicMax(&total[2], x);
+    atomicMax(&total[3], w);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *a.state = CeState{(int)total[0], total[2], total[3]};
+    if (a.oob && total[1]) atomicAdd(a.oob, (int)total[1]);
+  }
 }
 
 __device__ __forceinline__ void put_frag(char* p, int64_t block, int steps, int step, const float (&x)[8]) {
@@ -209,11 +251,12 @@ struct Out {
 __device__ __forceinline__ int scale_of(const CeState& s, int which) {
   return which == 0 ? pr::scale_exp(s.x_max) : which == 1 ? pr::scale_exp(s.w_max) : kGExp;
 }
-// store(where, element) for the elements of a tile that this lane holds and
-// that exist, where = p + n + ld m
-template <class F>
-__device__ __forceinline__ void each(const pr::Acc& acc, int tm, int tn, int M, int N, float* p, int64_t ld,
-                                     F&& store) {
+// p[n + ld m] = value(element), or += for ADD, for the elements of a tile that
+// this lane holds and that exist.  ADD reads all of a column before it writes
+// one, so the reads are under way together.
+template <bool ADD, class F>
+__device__ __forceinline__ void put_tile(const pr::Acc& acc, int tm, int tn, int M, int N, float* __restrict__ p,
+                                         int64_t ld, F&& value) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = tm * pr::TM + (wave >> 2) * 128, m1 = m0 + 4 * (lane >> 5);
 #pragma unroll
@@ -221,19 +264,28 @@ __device__ __forceinline__ void each(const pr::Acc& acc, int tm, int tn, int M, 
     const int n = tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
     if (n >= N) continue;
     float* q = p + n + ld * m1;
+    auto row = [](int i, int e) { return 32 * i + 8 * (e / 4) + e % 4; };
     if (m0 + 128 <= M) {
+      float old[4][16];
+      if (ADD) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) old[i][e] = q[ld * row(i, e)];
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) store(q + ld * (32 * i + 8 * (e / 4) + e % 4), acc.x[i][j][e]);
+        for (int e = 0; e < 16; ++e) q[ld * row(i, e)] = ADD ? old[i][e] + value(acc.x[i][j][e]) : value(acc.x[i][j][e]);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int m = 32 * i + 8 * (e / 4) + e % 4;
-          if (m1 + m < M) store(q + ld * m, acc.x[i][j][e]);
-        }
+        for (int e = 0; e < 16; ++e)
+          if (m1 + row(i, e) < M) {
+            float* at = q + ld * row(i, e);
+            *at = ADD ? *at + value(acc.x[i][j][e]) : value(acc.x[i][j][e]);
+          }
     }
   }
 }
@@ -293,7 +345,7 @@ __global__ void __launch_bounds__(pr::GNT, 2) ce_logits_kernel(pr::GemmArgs g, C
     if (n >= g.N) continue;
     if (lane < 32) a.stat[(int64_t)(tm * 2 + (wave >> 2)) * a.R + n] = float2{top, sum};
   }
-  each(acc, tm, tn, g.M, g.N, a.Z, a.R, [](float* p, float x) { *p = x; });
+  put_tile<false>(acc, tm, tn, g.M, g.N, a.Z, a.R, [](float x) { return x; });
 }
 
 // dX (A: W across its rows, B: G) and dW (A: G, B: X, both across their rows)
@@ -306,15 +358,14 @@ __global__ void __launch_bounds__(pr::GNT, 2) ce_grads_kernel(pr::GemmArgs g, Ce
   pr::Acc acc;
   pr::gemm_tile<TA, TB>(g, tm, tn, t0, t1, lds, acc);
   if (o.part) {
-    each(acc, tm, tn, g.M, g.N, o.part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float* p, float x) { *p = x; });
+    put_tile<false>(acc, tm, tn, g.M, g.N, o.part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float x) { return x; });
     return;
   }
   const int eo = -scale_of(*a.state, o.exp_a) - scale_of(*a.state, o.exp_b);
   const float factor = grad_factor(a);
-  if (o.accumulate)
-    each(acc, tm, tn, g.M, g.N, o.p, o.ld, [&](float* p, float x) { *p += pr::times_exp2(x, eo) * factor; });
-  else
-    each(acc, tm, tn, g.M, g.N, o.p, o.ld, [&](float* p, float x) { *p = pr::times_exp2(x, eo) * factor; });
+  auto value = [&](float x) { return pr::times_exp2(x, eo) * factor; };
+  if (o.accumulate) put_tile<true>(acc, tm, tn, g.M, g.N, o.p, o.ld, value);
+  else put_tile<false>(acc, tm, tn, g.M, g.N, o.p, o.ld, value);
 }
 
 __global__ void __launch_bounds__(256) ce_reduce_kernel(CeArgs a, Out o, int M, int N, int splits) {
@@ -473,13 +524,16 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   if (R > N) R = N;
   const int64_t Rp = (R + 31) / 32 * 32, Np = (N + 31) / 32 * 32, Vp = (V + 31) / 32 * 32, Dp = (D + 31) / 32 * 32;
   const Split sx = split_of(D, R, a.steps_v), sw = split_of(V, D, (int)(Rp / 16));
+  const int64_t wb = V * D / (16 * 1024);  // 16 values a thread and more
+  a.w_blocks = (int)(wb < 1 ? 1 : wb > 1024 ? 1024 : wb);
   size_t at = 0;
   auto place = [&](size_t bytes) {
     const size_t p = at;
     at += (bytes + 255) / 256 * 256;
     return p;
   };
-  const size_t o_state = place(sizeof(CeState)), o_loss = place((size_t)N * 4), o_rows = place((size_t)N * 4), o_x = place((size_t)(Np * Dp) * 4),
+  const size_t o_state = place(sizeof(CeState)), o_loss = place((size_t)N * 4), o_rows = place((size_t)N * 4),
+               o_wpart = place((size_t)a.w_blocks * 4), o_x = place((size_t)(Np * Dp) * 4),
                o_w = place((size_t)(Vp * Dp) * 4), o_z = place((size_t)R * (size_t)V * 4),
                o_stat = place((size_t)a.stat_blocks * (size_t)R * 8);
   const size_t o_g = place(g ? (size_t)(Rp * Vp) * 4 : 0), o_db = place(g && g->db ? (size_t)((R + 255) / 256 * V) * 4 : 0);
@@ -492,6 +546,7 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   a.state = reinterpret_cast<CeState*>(base + o_state);
   a.row_loss = reinterpret_cast<float*>(base + o_loss);
   a.row_max = reinterpret_cast<uint32_t*>(base + o_rows);
+  a.w_part = reinterpret_cast<uint32_t*>(base + o_wpart);
   a.xp = base + o_x;
   a.wp = base + o_w;
   a.Z = reinterpret_cast<float*>(base + o_z);
@@ -500,12 +555,9 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   a.db_part = g && g->db ? reinterpret_cast<float*>(base + o_db) : nullptr;
   float* part = reinterpret_cast<float*>(base + o_part);
 
-  hipLaunchKernelGGL(ce_count_kernel, dim3(1), dim3(1024), 0, st, a);
+  hipLaunchKernelGGL(ce_max_kernel, dim3((unsigned)(a.w_blocks + (N + 63) / 64)), dim3(1024), 0, st, a);
   CNHIP_TRY(check_launch(who));
-  const int64_t wb = (V * D / 16 + 255) / 256, w_blocks = wb < 1 ? 1 : wb > 2048 ? 2048 : wb;
-  const int64_t x_blocks = (N + 255) / 256 * ((D + 15) / 16);
-  CNHIP_REQUIRE(w_blocks + x_blocks < ((int64_t)1 << 31), "%s: too large", who);
-  hipLaunchKernelGGL(ce_max_kernel, dim3((unsigned)(w_blocks + x_blocks)), dim3(256), 0, st, a, (int)w_blocks);
+  hipLaunchKernelGGL(ce_state_kernel, dim3(1), dim3(1024), 0, st, a);
   CNHIP_TRY(check_launch(who));
   const int64_t w_frags = Vp / 32 * a.steps_d, x_frags = Np / 32 * a.steps_d;
   hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)((w_frags + x_frags + 3) / 4)), dim3(256), 0, st, a, w_frags, x_frags);

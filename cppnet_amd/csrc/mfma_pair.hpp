@@ -150,10 +150,9 @@ struct Stage {
       }
     }
   }
-  __device__ __forceinline__ void copy(int t, char* buf) const {
+  __device__ __forceinline__ void copy(int t, int u, char* buf) const {
     const int64_t at = TR ? (int64_t)(t >> 1) * step + (t & 1) * 256 : (int64_t)t * step;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) copy16(src[u] + at, buf + lds[u]);
+    copy16(src[u] + at, buf + lds[u]);
   }
 };
 
@@ -214,38 +213,21 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc.x[i][j] = f32x16{};
-  auto copy = [&](int t) {
+  // piece u (0 .. 3) of step t's copies; past the last step the last is copied
+  // again, so that the wait counts stay the same
+  auto copy = [&](int t, int u) {
     char* buf = lds + (t & (kStages - 1)) * kStage;
-    // past the last step the last is copied again: the wait counts stay the same
     const int s = t < t1 ? t : t1 - 1;
-    sa.copy(s, buf);
-    sb.copy(s, buf + kStage / 2);
+    if (u < 2) sa.copy(s, u, buf);
+    else sb.copy(s, u - 2, buf + kStage / 2);
   };
-  auto read = [&](int t, Frags& f) {
+  // fragment u (0 .. 11) of step t, in the order of their first use
+  auto read = [&](int t, int u, Frags& f) {
     const char* buf = lds + (t & (kStages - 1)) * kStage;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) f.b[j][q] = frag<TB>(buf + kStage / 2, 2 * wn + j, q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f.a[i][q] = frag<TA>(buf, 4 * wm + i, q);
-    }
-  };
-  auto mfma = [&](Frags& f, uint32_t sign) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f.a[i][q] = flip(f.a[i][q], sign);
-    auto term = [&](int x, int y) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          acc.x[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[i][x], f.b[j][y], acc.x[i][j], 0, 0, 0);
-    };
-    term(1, 0);
-    term(0, 1);
-    term(0, 0);
+    if (u < 2) f.b[u][0] = frag<TB>(buf + kStage / 2, 2 * wn + u, 0);
+    else if (u < 6) f.a[u - 2][1] = frag<TA>(buf, 4 * wm + u - 2, 1);
+    else if (u < 8) f.b[u - 6][1] = frag<TB>(buf + kStage / 2, 2 * wn + u - 6, 1);
+    else f.a[u - 8][0] = frag<TA>(buf, 4 * wm + u - 8, 0);
   };
   Frags f0, f1;
   auto step = [&](int t, Frags& now, Frags& next) {
@@ -258,14 +240,28 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc.x[i][j] = -acc.x[i][j];
     }
-    copy(t + 4);
-    read(t + 1, next);
-    mfma(now, t >= g.half ? 0x80008000u : 0u);
-    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t sign = t >= g.half ? 0x80008000u : 0u;
+    // a MFMA keeps the matrix pipe for 32 cycles and the wave for 4: the reads,
+    // copies and sign changes go between them
+#pragma unroll
+    for (int u = 0; u < 12; ++u) {
+      const int i = u % 4, x = u < 4 ? 1 : 0, y = u >= 4 && u < 8 ? 1 : 0;
+      if (u < 8) now.a[i][x] = flip(now.a[i][x], sign);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        acc.x[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.a[i][x], now.b[j][y], acc.x[i][j], 0, 0, 0);
+      read(t + 1, u, next);
+      if (u % 3 == 0) copy(t + 4, u / 3);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
-  for (int u = 0; u < 4; ++u) copy(t0 + u);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) copy(t0 + t, u);
   wait_and_meet<12>();
-  read(t0, f0);
+#pragma unroll
+  for (int u = 0; u < 12; ++u) read(t0, u, f0);
   for (int t = t0; t < t1; t += 2) {
     step(t, f0, f1);
     if (t + 1 < t1) step(t + 1, f1, f0);
