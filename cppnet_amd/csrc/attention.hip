@@ -25,6 +25,7 @@
 #include <cmath>
 
 #include "common.hpp"
+#include "mfma_pair.hpp"
 
 namespace cnhip {
 namespace {
@@ -379,6 +380,558 @@ __global__ void __launch_bounds__(NT) att_dkv_kernel(AttArgs a) {
   store_row<DHP>(a.dv.at(b, at, (int64_t)kh * a.dh), a.dv.col, stored, a.dh, 1.f, dv);
 }
 
+// ------------------------------------------------------- packed operands
+// Long sequences run on the fp16 matrix cores: q, k, v and dout are packed as
+// pairs (mfma_pair.hpp), 32 steps x 16 features a fragment, once for each pass,
+// and tiles of 32 keys (or queries) go from memory to LDS as they lie.  A tile
+// serves as the operand whose lanes are its rows (ds_read_b128) and, turned by
+// ds_read_b64_tr_b16, as the one whose lanes are features.  The order in which
+// a turned read takes the rows is that of the accumulator registers, so
+// probabilities and their gradients are split into their two terms in the
+// registers and multiplied without leaving them.
+//
+// Scales.  Each operand has one power of two per sample and key head (over the
+// heads that share it).  Probabilities are at most 1 and enter times 2^14.
+// dS = P (dP - delta) is bounded by 2 max ||dout_i|| max ||v_j||, whose power
+// of two scales it.
+struct Scale {
+  uint32_t largest;  // |x|, bits
+  float norm;        // largest row's Euclidean norm
+};
+
+struct PackArgs {
+  Seq<const float> x[4];  // q, k, v, dout
+  char* p[4];
+  Scale* part[4];         // [B][kv_heads][slots]
+  int slots[4], chunks[4], chunk_rows[4], blocks[4];
+  int steps;              // of 16 features
+};
+
+struct PairArgs {
+  AttArgs a;
+  PackArgs p;
+};
+
+// The operand's scale over its slots, the same in every lane.
+__device__ __forceinline__ Scale scale_of(const PackArgs& p, int which, int64_t bkh) {
+  uint32_t m = 0;
+  float n = 0.f;
+  for (int i = threadIdx.x & 63; i < p.slots[which]; i += 64) {
+    const Scale s = p.part[which][bkh * p.slots[which] + i];
+    m = max(m, s.largest);
+    n = fmaxf(n, s.norm);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    n = fmaxf(n, __shfl_xor(n, o, 64));
+  }
+  return Scale{(uint32_t)__builtin_amdgcn_readfirstlane((int)m),
+               __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(n)))};
+}
+
+// Rows of operand `which` that a sample has (past them k and v count as zeros).
+__device__ __forceinline__ int rows_of(const AttArgs& a, int which, int b) {
+  return which == 1 || which == 2 ? keys_of(a, b) : a.Sq;
+}
+
+// The scale of a chunk of rows of one head: a wave per 32 rows, four a block.
+template <int OPS>
+__global__ void __launch_bounds__(NT) att_scale_kernel(PairArgs g) {
+  __shared__ Scale part[4];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int which = (int)blockIdx.z;
+  if (which >= OPS) return;
+  const AttArgs& a = g.a;
+  const bool kv = which == 1 || which == 2;
+  const int heads = kv ? a.kv_heads : a.heads;
+  const int b = (int)blockIdx.y / a.heads, head = (int)blockIdx.y % a.heads;
+  if (head >= heads || (int)blockIdx.x >= g.p.chunks[which]) return;
+  const int rows = rows_of(a, which, b);
+  const Seq<const float>& x = g.p.x[which];
+  uint32_t m = 0;
+  float norm = 0.f;
+  const int c0 = (int)blockIdx.x * g.p.chunk_rows[which];
+  for (int r0 = c0 + 32 * wave; r0 < c0 + g.p.chunk_rows[which] && r0 < rows; r0 += 128) {
+    const int r = r0 + (lane & 31);
+    float s = 0.f;
+    if (r < rows) {
+      const float* p = x.at(b, r, (int64_t)head * a.dh);
+      for (int d = lane >> 5; d < a.dh; d += 16) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = d + 2 * u < a.dh ? p[(d + 2 * u) * x.col] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const uint32_t bits = pr::finite_bits(v[u]);
+          m = max(m, bits);
+          s = fmaf(__uint_as_float(bits), __uint_as_float(bits), s);
+        }
+      }
+    }
+    s += other_half(s);
+    norm = fmaxf(norm, s);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    norm = fmaxf(norm, __shfl_xor(norm, o, 64));
+  }
+  // squares that leave the range: the bound by the largest value
+  if (lane == 0)
+    part[wave] = Scale{m, norm > 1e-30f && norm < 1e37f ? sqrtf(norm) : __uint_as_float(m) * sqrtf((float)a.dh)};
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  Scale s = part[0];
+  for (int w = 1; w < 4; ++w) {
+    s.largest = max(s.largest, part[w].largest);
+    s.norm = fmaxf(s.norm, part[w].norm);
+  }
+  const int kh = kv ? head : head / a.group, slot = (kv ? 0 : head % a.group) * g.p.chunks[which] + (int)blockIdx.x;
+  g.p.part[which][((int64_t)b * a.kv_heads + kh) * g.p.slots[which] + slot] = s;
+}
+
+// A wave packs 32 rows of one head; of dout it also leaves delta.
+template <int OPS>
+__global__ void __launch_bounds__(NT) att_pack_kernel(PairArgs g) {
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, h = lane >> 5;
+  const int which = (int)blockIdx.z;
+  if (which >= OPS) return;
+  const AttArgs& a = g.a;
+  const bool kv = which == 1 || which == 2;
+  const int heads = kv ? a.kv_heads : a.heads;
+  const int b = (int)blockIdx.y / a.heads, head = (int)blockIdx.y % a.heads;
+  const int blk = (int)blockIdx.x * 4 + wave;
+  if (head >= heads || blk >= g.p.blocks[which]) return;
+  const int kh = kv ? head : head / a.group;
+  const float f = pr::exp2i(pr::scale_exp(scale_of(g.p, which, (int64_t)b * a.kv_heads + kh).largest));
+  const int rows = rows_of(a, which, b), r = blk * 32 + (lane & 31);
+  const bool held = r < rows;
+  const Seq<const float>& x = g.p.x[which];
+  const float* p = x.at(b, held ? r : 0, (int64_t)head * a.dh);
+  const float* o = which == 3 ? a.o.at(b, held ? r : 0, (int64_t)head * a.dh) : nullptr;
+  char* q = g.p.p[which] + (((int64_t)b * heads + head) * g.p.blocks[which] + blk) * g.p.steps * (2 * pr::kFrag) + lane * 16;
+  float delta = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < g.p.steps; ++s) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = 16 * s + 8 * h + e;
+      v[e] = held && d < a.dh ? p[d * x.col] : 0.f;
+      if (which == 3 && held && d < a.dh) delta = fmaf(v[e], o[d * a.o.col], delta);
+    }
+    pr::u32x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t w0, w1;
+      pr::split2(v[2 * e] * f, v[2 * e + 1] * f, w0, w1);
+      hi[e] = w0;
+      lo[e] = w1;
+    }
+    *reinterpret_cast<pr::u32x4*>(q + s * (2 * pr::kFrag)) = hi;
+    *reinterpret_cast<pr::u32x4*>(q + s * (2 * pr::kFrag) + pr::kFrag) = lo;
+  }
+  if (which != 3) return;
+  delta += other_half(delta);
+  if (held && h == 0) a.delta[((int64_t)b * a.heads + head) * a.Sq + r] = delta;
+}
+
+// This block's (head of a sample, 128 rows of it): XCDs take contiguous runs
+// of heads, whose keys then stay in one L2; a head's last rows, which read the
+// most keys under a causal mask, go first.
+__device__ __forceinline__ void place(int tiles, int heads, int& tile, int& bh) {
+  const int total = tiles * heads, bid = (int)blockIdx.x, xcd = bid & 7, base = total >> 3, rem = total & 7;
+  const int id = xcd * base + min(xcd, rem) + (bid >> 3);
+  bh = id / tiles;
+  tile = tiles - 1 - id % tiles;
+}
+
+// Fragments of this lane's own row: packed feature step s, plane q.
+template <int KS>
+struct RowFrags {
+  pr::f16x8 x[KS][2];
+  // base: the head's packed rows
+  __device__ __forceinline__ void load(const char* base, int row, bool held) {
+    const char* p = base + (int64_t)(row >> 5) * KS * (2 * pr::kFrag) + (((int)threadIdx.x >> 5 & 1) * 32 + (row & 31)) * 16;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        x[s][q] = held ? *reinterpret_cast<const pr::f16x8*>(p + (2 * s + q) * pr::kFrag) : pr::f16x8{};
+  }
+};
+
+// acc (rows of the tile x rows of the lanes) = tile x^T over the features
+template <int KS>
+__device__ __forceinline__ f32x16 dot_pairs(const char* tile, const RowFrags<KS>& x) {
+  const char* p = tile + ((int)threadIdx.x & 63) * 16;
+  f32x16 acc = {};
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const pr::f16x8 a0 = *reinterpret_cast<const pr::f16x8*>(p + 2 * s * pr::kFrag);
+    const pr::f16x8 a1 = *reinterpret_cast<const pr::f16x8*>(p + (2 * s + 1) * pr::kFrag);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, x.x[s][0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, x.x[s][1], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, x.x[s][0], acc, 0, 0, 0);
+  }
+  return acc;
+}
+
+// A score tile's registers as the B operand of two steps of 16 rows, in terms.
+struct TileFrags {
+  pr::f16x8 x[2][2];
+  __device__ __forceinline__ void split(const f32x16& p) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      pr::u32x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t w0, w1;
+        pr::split2(p[8 * t + 2 * e], p[8 * t + 2 * e + 1], w0, w1);
+        hi[e] = w0;
+        lo[e] = w1;
+      }
+      x[t][0] = __builtin_bit_cast(pr::f16x8, hi);
+      x[t][1] = __builtin_bit_cast(pr::f16x8, lo);
+    }
+  }
+};
+
+// acc (features x rows of the lanes) += tile^T p over the rows of the tile.
+// Element i of half-wave h in p's step t is row 16 t + 8 (i / 4) + 4 h + i % 4.
+template <int KS>
+__device__ __forceinline__ void add_pairs(const char* tile, const TileFrags& p, f32x16 (&acc)[KS / 2]) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const int lane = (int)threadIdx.x & 63, j = lane & 15;
+  const char* base = tile + (lane >> 4 & 1) * (2 * pr::kFrag) + ((j & 3) >> 1) * 512 + (4 * (lane >> 5) + (j >> 2)) * 16 +
+                     (j & 1) * 8;
+  auto frag = [&](int i, int t, int q) {
+    const char* at = base + 2 * i * (2 * pr::kFrag) + q * pr::kFrag + t * 256;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 128));
+    return __builtin_bit_cast(pr::f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < KS / 2; ++i) {
+      const pr::f16x8 a0 = frag(i, t, 0), a1 = frag(i, t, 1);
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, p.x[t][0], acc[i], 0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, p.x[t][1], acc[i], 0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, p.x[t][0], acc[i], 0, 0, 0);
+    }
+}
+
+// Copies of a tile of two operands into LDS (the first, then the second), the
+// fragments shared out among the block's four waves.
+template <int KS>
+__device__ __forceinline__ void copy_tile(const char* first, const char* second, char* lds) {
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  constexpr int PIECES = 2 * KS;  // of 1024 bytes, of one operand
+#pragma unroll
+  for (int u = 0; u < PIECES / 4; ++u) {
+    const int at = (4 * u + wave) * pr::kFrag;
+    pr::copy16(first + at + lane * 16, lds + at);
+    pr::copy16(second + at + lane * 16, lds + PIECES * pr::kFrag + at);
+  }
+}
+
+constexpr float kPExp = 14.f;  // probabilities enter times 2^14
+
+template <int DHP>
+constexpr int pair_waves() { return DHP <= 64 ? 2 : 1; }
+
+// Forward: a wave holds 32 queries of one head.
+template <int DHP>
+__global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int tiles) {
+  constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
+  __shared__ __align__(16) char lds[2][2 * TILE];
+  const AttArgs& a = g.a;
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  int tile, bh;
+  place(tiles, a.B * a.heads, tile, bh);
+  const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
+  const int64_t bkh = (int64_t)b * a.kv_heads + kh;
+  const int i = tile * 128 + 32 * wave + (lane & 31);
+  const bool held = i < a.Sq;
+  const int n = keys_of(a, b);
+  const int64_t start = start_of(a, b);
+  const int lim = held ? limit(a, n, start, i) : 0;
+  const int end = limit(a, n, start, min(tile * 128 + 127, a.Sq - 1));  // limits grow with the row
+  const int ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest), ev = pr::scale_exp(scale_of(g.p, 2, bkh).largest);
+  const int eq = pr::scale_exp(scale_of(g.p, 0, bkh).largest);
+  // not zero, so that a masked score stays -inf
+  const float c = fmaxf(pr::times_exp2(fabsf(a.scale) * kLog2e, -eq - ek), 0x1p-126f);
+  RowFrags<KS> q;
+  q.load(g.p.p[0] + (int64_t)bh * g.p.blocks[0] * TILE, held ? i : 0, held);
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) q.x[s][u] = pr::flip(q.x[s][u], 0x80008000u);
+  }
+  const char* kp = g.p.p[1] + bkh * g.p.blocks[1] * TILE;
+  const char* vp = g.p.p[2] + bkh * g.p.blocks[2] * TILE;
+  f32x16 o[DHP / 32] = {};
+  float m = -INFINITY, l = 0.f;  // maximum of t = scale log2(e) s, sum of 2^(14 + t - m)
+  if (end > 0) copy_tile<KS>(kp, vp, lds[0]);
+  for (int j0 = 0, t = 0; j0 < end; j0 += 32, ++t) {
+    pr::wait_and_meet<0>();
+    if (j0 + 32 < end) copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, vp + (int64_t)(t + 1) * TILE, lds[(t + 1) & 1]);
+    if (!__any(lim > j0)) continue;
+    const char* buf = lds[t & 1];
+    f32x16 s = dot_pairs<KS>(buf, q);
+    if (!__all(lim >= j0 + 32)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = j0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+        s[e] = j < lim ? s[e] : -INFINITY;
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+    top = fmaxf(top, other_half(top)) * c;
+    const float mn = fmaxf(m, top);
+    if (__any(mn > m)) {
+      const float f = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DHP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= f;
+      m = mn;
+    }
+    const float base = (m == -INFINITY ? 0.f : m) - kPExp;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -base));
+      sum += s[e];
+    }
+    l += sum;
+    TileFrags p;
+    p.split(s);
+    add_pairs<KS>(buf + TILE, p, o);
+  }
+  l += other_half(l);
+  const float f = lim > 0 ? 1.f / l : 0.f;
+#pragma unroll
+  for (int d = 0; d < DHP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = pr::times_exp2(o[d][e] * f, -ev);
+  store_row<DHP>(a.out.at(b, held ? i : 0, (int64_t)head * a.dh), a.out.col, held, a.dh, 1.f, o);
+  if (a.lse && held && lane < 32)
+    a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] =
+        lim > 0 ? (m + log2f(pr::times_exp2(l, -(int)kPExp))) * kLn2 : -INFINITY;
+}
+
+// The exponent of dS: 2 max ||dout|| max ||v|| bounds it.
+__device__ __forceinline__ int grad_exp(const Scale& g, const Scale& v) {
+  const float bound = 2.f * g.norm * v.norm;
+  return pr::scale_exp(__float_as_uint(fminf(bound, 3e38f)));
+}
+
+// dq: a wave holds 32 queries of one head and streams keys and values.
+template <int DHP>
+__global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(PairArgs g, int tiles) {
+  constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
+  __shared__ __align__(16) char lds[2][2 * TILE];
+  const AttArgs& a = g.a;
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  int tile, bh;
+  place(tiles, a.B * a.heads, tile, bh);
+  const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
+  const int64_t bkh = (int64_t)b * a.kv_heads + kh;
+  const int i = tile * 128 + 32 * wave + (lane & 31);
+  const bool held = i < a.Sq;
+  const int n = keys_of(a, b);
+  const int64_t start = start_of(a, b);
+  const int lim = held ? limit(a, n, start, i) : 0;
+  const int end = limit(a, n, start, min(tile * 128 + 127, a.Sq - 1));
+  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bkh);
+  const int eq = pr::scale_exp(scale_of(g.p, 0, bkh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
+  const int eg = pr::scale_exp(sg.largest), ev = pr::scale_exp(sv.largest), ed = grad_exp(sg, sv);
+  const float c = pr::times_exp2(a.scale * kLog2e, -eq - ek), cd = pr::times_exp2(1.f, ed - eg - ev);
+  RowFrags<KS> q, go;
+  q.load(g.p.p[0] + (int64_t)bh * g.p.blocks[0] * TILE, held ? i : 0, held);
+  go.load(g.p.p[3] + (int64_t)bh * g.p.blocks[3] * TILE, held ? i : 0, held);
+  const float lse = held ? lse2_of(a, b, head, i) : INFINITY;
+  const float delta = held ? pr::times_exp2(a.delta[(int64_t)bh * a.Sq + i], ed) : 0.f;
+  const char* kp = g.p.p[1] + bkh * g.p.blocks[1] * TILE;
+  const char* vp = g.p.p[2] + bkh * g.p.blocks[2] * TILE;
+  f32x16 acc[DHP / 32] = {};
+  if (end > 0) copy_tile<KS>(kp, vp, lds[0]);
+  for (int j0 = 0, t = 0; j0 < end; j0 += 32, ++t) {
+    pr::wait_and_meet<0>();
+    if (j0 + 32 < end) copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, vp + (int64_t)(t + 1) * TILE, lds[(t + 1) & 1]);
+    if (!__any(lim > j0)) continue;
+    const char* buf = lds[t & 1];
+    f32x16 s = dot_pairs<KS>(buf, q);
+    const f32x16 dp = dot_pairs<KS>(buf + TILE, go);
+    const bool whole = __all(lim >= j0 + 32);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int j = j0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * fmaf(dp[e], cd, -delta);
+      s[e] = whole || j < lim ? p : 0.f;
+    }
+    TileFrags p;
+    p.split(s);
+    add_pairs<KS>(buf, p, acc);
+  }
+#pragma unroll
+  for (int d = 0; d < DHP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[d][e] = pr::times_exp2(acc[d][e], -ek - ed);
+  store_row<DHP>(a.dq.at(b, held ? i : 0, (int64_t)head * a.dh), a.dq.col, held, a.dh, a.scale, acc);
+}
+
+// dk, dv: a wave holds 32 keys and streams the queries and output gradients
+// of the heads that share them.
+template <int DHP>
+__global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(PairArgs g, int key_tiles) {
+  constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
+  __shared__ __align__(16) char lds[2][2 * TILE];
+  __shared__ __align__(16) float stat[2][2][32];  // lse (base 2) - 14, scaled delta of the tile's queries
+  const AttArgs& a = g.a;
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  int tile, bkh;
+  place(key_tiles, a.B * a.kv_heads, tile, bkh);
+  tile = key_tiles - 1 - tile;  // the first keys are read by the most queries
+  const int b = bkh / a.kv_heads, kh = bkh % a.kv_heads;
+  const int key0 = tile * 128, key = key0 + 32 * wave + (lane & 31);
+  const int n = keys_of(a, b);
+  const int64_t start = start_of(a, b);
+  const bool held = key < n;
+  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bkh);
+  const int eq = pr::scale_exp(scale_of(g.p, 0, bkh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
+  const int eg = pr::scale_exp(sg.largest), ev = pr::scale_exp(sv.largest), ed = grad_exp(sg, sv);
+  const float c = pr::times_exp2(a.scale * kLog2e, -eq - ek), cd = pr::times_exp2(1.f, ed - eg - ev - (int)kPExp);
+  RowFrags<KS> k, v;
+  k.load(g.p.p[1] + (int64_t)bkh * g.p.blocks[1] * TILE, held ? key : 0, held);
+  v.load(g.p.p[2] + (int64_t)bkh * g.p.blocks[2] * TILE, held ? key : 0, held);
+  // the first tile of queries that reads the block's first key
+  int64_t first = a.causal ? key0 - start : 0;
+  first = first < 0 ? 0 : first / 32;
+  const int per_head = key0 < n && first * 32 < a.Sq ? (int)((a.Sq + 31) / 32 - first) : 0;
+  const int total = per_head * a.group;
+  f32x16 dk[DHP / 32] = {}, dv[DHP / 32] = {};
+  float st = 0.f;
+  int head_next = 0, tile_next = 0;  // of the next tile to be copied
+  auto copy = [&](char* buf) {
+    const int64_t bh = (int64_t)b * a.heads + kh * a.group + head_next;
+    const int64_t at = (bh * g.p.blocks[0] + first + tile_next) * TILE;
+    copy_tile<KS>(g.p.p[0] + at, g.p.p[3] + at, buf);
+    const int64_t i = (first + tile_next) * 32 + (lane & 31);
+    if (wave == 0 && i < a.Sq) {
+      if (lane < 32) st = lse2_of(a, b, kh * a.group + head_next, i) - kPExp;
+      else st = pr::times_exp2(a.delta[bh * a.Sq + i], ed - (int)kPExp);
+    } else {
+      st = lane < 32 ? INFINITY : 0.f;
+    }
+    if (++tile_next == per_head) {
+      tile_next = 0;
+      ++head_next;
+    }
+  };
+  if (total > 0) copy(lds[0]);
+  int ti = 0;
+  for (int t = 0; t < total; ++t) {
+    if (wave == 0) stat[t & 1][lane >> 5][lane & 31] = st;
+    pr::wait_and_meet<0>();
+    const int64_t i0 = (first + ti) * 32;
+    if (++ti == per_head) ti = 0;
+    if (t + 1 < total) copy(lds[(t + 1) & 1]);
+    if (a.causal && start + i0 + 31 < key0 + 32 * wave) continue;  // no query of the tile reads this wave's keys
+    const char* buf = lds[t & 1];
+    f32x16 s = dot_pairs<KS>(buf, k);
+    f32x16 dp = dot_pairs<KS>(buf + TILE, v);
+    const bool whole = __all(held) && (!a.causal || key0 + 32 * wave + 31 <= start + i0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int r = 8 * q + 4 * (lane >> 5);
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[t & 1][0][r]);
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[t & 1][1][r]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool reads = whole || (held && (!a.causal || key <= start + i0 + r + e));
+        s[4 * q + e] = reads ? __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], c, -lse[e])) : 0.f;
+        dp[4 * q + e] = reads ? s[4 * q + e] * fmaf(dp[4 * q + e], cd, -delta[e]) : 0.f;
+      }
+    }
+    TileFrags p;
+    p.split(s);
+    add_pairs<KS>(buf + TILE, p, dv);
+    p.split(dp);
+    add_pairs<KS>(buf, p, dk);
+  }
+#pragma unroll
+  for (int d = 0; d < DHP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      dk[d][e] = pr::times_exp2(dk[d][e], -eq - ed);
+      dv[d][e] = pr::times_exp2(dv[d][e], -eg - (int)kPExp);
+    }
+  const bool stored = key < a.Sk;
+  const int at = stored ? key : 0;
+  store_row<DHP>(a.dk.at(b, at, (int64_t)kh * a.dh), a.dk.col, stored, a.dh, a.scale, dk);
+  store_row<DHP>(a.dv.at(b, at, (int64_t)kh * a.dh), a.dv.col, stored, a.dh, 1.f, dv);
+}
+
+// Lays out the workspace of the packed operands and packs them.  ops: 3 (q, k,
+// v) or 4; delta: where dout's pass leaves it.
+int pack(PairArgs& g, int ops, hipStream_t st, const char* who) {
+  AttArgs& a = g.a;
+  PackArgs& p = g.p;
+  p.steps = a.dh <= 32 ? 2 : a.dh <= 64 ? 4 : a.dh <= 96 ? 6 : 8;
+  size_t bytes = 0, part[4], data[4];
+  auto place_bytes = [&](size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  int most_chunks = 0, most_blocks = 0;
+  for (int w = 0; w < ops; ++w) {
+    const bool kv = w == 1 || w == 2;
+    const int64_t S = kv ? a.Sk : a.Sq, heads = kv ? a.kv_heads : a.heads;
+    p.blocks[w] = (int)((S + 31) / 32);
+    p.chunk_rows[w] = (int)((S + 32 * 128 - 1) / (32 * 128) * 128);  // 32 chunks at most
+    p.chunks[w] = (int)((S + p.chunk_rows[w] - 1) / p.chunk_rows[w]);
+    p.slots[w] = p.chunks[w] * (kv ? 1 : a.group);
+    most_chunks = p.chunks[w] > most_chunks ? p.chunks[w] : most_chunks;
+    most_blocks = p.blocks[w] > most_blocks ? p.blocks[w] : most_blocks;
+    part[w] = place_bytes((size_t)a.B * a.kv_heads * p.slots[w] * sizeof(Scale));
+    data[w] = place_bytes((size_t)a.B * heads * p.blocks[w] * p.steps * 2 * pr::kFrag);
+  }
+  const size_t delta = place_bytes(ops == 4 ? (size_t)a.B * a.heads * a.Sq * sizeof(float) : 0);
+  void* ws = nullptr;
+  CNHIP_TRY(scratch(st, kScratchLayer, bytes, &ws, who));
+  char* base = static_cast<char*>(ws);
+  for (int w = 0; w < ops; ++w) {
+    p.part[w] = reinterpret_cast<Scale*>(base + part[w]);
+    p.p[w] = base + data[w];
+  }
+  a.delta = reinterpret_cast<float*>(base + delta);
+  p.x[0] = a.q;
+  p.x[1] = a.k;
+  p.x[2] = a.v;
+  p.x[3] = a.dout;
+  const dim3 gs((unsigned)most_chunks, (unsigned)(a.B * a.heads), (unsigned)ops);
+  const dim3 gp((unsigned)((most_blocks + 3) / 4), (unsigned)(a.B * a.heads), (unsigned)ops);
+  if (ops == 3) hipLaunchKernelGGL(att_scale_kernel<3>, gs, dim3(NT), 0, st, g);
+  else hipLaunchKernelGGL(att_scale_kernel<4>, gs, dim3(NT), 0, st, g);
+  CNHIP_TRY(check_launch(who));
+  if (ops == 3) hipLaunchKernelGGL(att_pack_kernel<3>, gp, dim3(NT), 0, st, g);
+  else hipLaunchKernelGGL(att_pack_kernel<4>, gp, dim3(NT), 0, st, g);
+  return check_launch(who);
+}
+
+// Whether a pass runs on packed operands.
+bool use_pairs(const AttArgs& a) { return a.Sq >= 64 && a.Sk >= 64; }
+
 constexpr int kMaxHeadDim = 128;
 
 template <class T>
@@ -386,18 +939,21 @@ Seq<T> seq(T* p, int64_t B, int64_t S, int rows) {
   return rows == CNHIP_ROWS_REF ? Seq<T>{p, 1, B, B * S} : Seq<T>{p, S, 1, B * S};
 }
 
-// f(the kernel's feature padding as an integral constant, whether a step's
-// neighbours are adjacent)
+// f(the features of a row padded to the kernel's as an integral constant)
+template <class F>
+void by_width(int dh, F&& f) {
+  if (dh <= 32) f(std::integral_constant<int, 32>{});
+  else if (dh <= 64) f(std::integral_constant<int, 64>{});
+  else if (dh <= 96) f(std::integral_constant<int, 96>{});
+  else f(std::integral_constant<int, 128>{});
+}
+// the same, and whether a step's neighbours are adjacent
 template <class F>
 void dispatch(int dh, bool unit, F&& f) {
-  auto by = [&](auto d) {
+  by_width(dh, [&](auto d) {
     if (unit) f(d, std::true_type{});
     else f(d, std::false_type{});
-  };
-  if (dh <= 32) by(std::integral_constant<int, 32>{});
-  else if (dh <= 64) by(std::integral_constant<int, 64>{});
-  else if (dh <= 96) by(std::integral_constant<int, 96>{});
-  else by(std::integral_constant<int, 128>{});
+  });
 }
 
 int check_args(const char* who, int64_t B, int64_t Sq, int64_t Sk, int64_t heads, int64_t kv_heads, int64_t dh,
@@ -416,6 +972,7 @@ int check_args(const char* who, int64_t B, int64_t Sq, int64_t Sk, int64_t heads
   CNHIP_REQUIRE(causal || !q_start, "%s: q_start needs causal", who);
   CNHIP_REQUIRE(std::isfinite(scale), "%s: scale is not finite", who);
   CNHIP_REQUIRE(B <= 65535 && heads <= 65535 && B * heads <= 65535, "%s: B * heads exceeds 65535", who);
+  CNHIP_REQUIRE(B * heads * ((Sq > Sk ? Sq : Sk) / 128 + 1) < (int64_t)1 << 31, "%s: too many rows", who);
   CNHIP_REQUIRE(Sq < (1 << 30) && Sk < (1 << 30) && Sq * (heads / kv_heads) < (int64_t)1 << 31,
                 "%s: sequence too long", who);
   return CNHIP_OK;
@@ -464,6 +1021,16 @@ int cnhip_attention_forward(const float* q, const float* k, const float* v, floa
       cnhip::base_args(q, k, v, B, Sq, Sk, heads, kv_heads, head_dim, scale, causal, k_len, q_start, rows);
   a.out = cnhip::seq(out, B, Sq, rows);
   a.lse = lse;
+  if (cnhip::use_pairs(a)) {
+    cnhip::PairArgs g{a, {}};
+    CNHIP_TRY(cnhip::pack(g, 3, st, who));
+    const int tiles = (int)((Sq + 127) / 128);
+    cnhip::by_width(a.dh, [&](auto d) {
+      hipLaunchKernelGGL((cnhip::att_fwd_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st,
+                         g, tiles);
+    });
+    return cnhip::check_launch(who);
+  }
   const dim3 grid((unsigned)((a.group * Sq + 127) / 128), (unsigned)(B * kv_heads));
   cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
     hipLaunchKernelGGL((cnhip::att_fwd_kernel<d(), unit()>), grid, dim3(cnhip::NT), 0, st, a);
@@ -487,6 +1054,21 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
   a.dk = cnhip::seq(dk, B, Sk, rows);
   a.dv = cnhip::seq(dv, B, Sk, rows);
   a.lse_in = lse;
+  if (cnhip::use_pairs(a)) {
+    cnhip::PairArgs g{a, {}};
+    CNHIP_TRY(cnhip::pack(g, 4, st, who));
+    const int tiles = (int)((Sq + 127) / 128), key_tiles = (int)((Sk + 127) / 128);
+    cnhip::by_width(a.dh, [&](auto d) {
+      hipLaunchKernelGGL((cnhip::att_dkv_pair_kernel<d()>), dim3((unsigned)(key_tiles * B * kv_heads)), dim3(cnhip::NT),
+                         0, st, g, key_tiles);
+    });
+    CNHIP_TRY(cnhip::check_launch(who));
+    cnhip::by_width(a.dh, [&](auto d) {
+      hipLaunchKernelGGL((cnhip::att_dq_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st, g,
+                         tiles);
+    });
+    return cnhip::check_launch(who);
+  }
   void* ws = nullptr;
   CNHIP_TRY(cnhip::scratch(st, cnhip::kScratchLayer, (size_t)(B * heads * Sq) * sizeof(float), &ws, who));
   a.delta = static_cast<float*>(ws);

@@ -7,10 +7,20 @@ one rounding per product and per addition, doubled because the matrix cores cut
 the low bits of a sum where an fp32 adder rounds them, and 8 more for the few
 roundings around the sum (scales, exponentials to 2 ulp, a division).  Errors
 of intermediate values are carried to the outputs to first order, exactly as
-the formulas chain them; second-order terms are covered by a factor 1.05."""
+the formulas chain them; second-order terms are covered by a factor 1.05.
+
+Where an operand is held as a pair of fp16 terms (cppnet_amd/csrc/mfma_pair.hpp)
+a value is kept to 2^-22 of itself, which the 8 more in g cover (2 * 8 u =
+2^-20), but not closer than F = 2^-39 of the operand's largest: the largest is
+scaled to at least 2^14, and the second term is rounded on fp16's subnormal grid
+of 2^-24, so by 2^-25 at most.  Probabilities are scaled by 2^14 exactly, the
+cross-entropy's gradient by 2^15, and dS by the power of two that takes its
+bound 2 max ||dout_i|| max ||v_j|| to 2^14 at least; maxima are those of a
+sample and key head."""
 import numpy as np
 
 U = 2.0 ** -24
+F = 2.0 ** -39
 
 
 def g(n):
@@ -71,30 +81,43 @@ def attention(q, k, v, ok, scale, dout=None):
     # scores: the contraction, and the roundings of scale * log2(e) and of the
     # exponent's difference; from the score's and the maximum's size
     es = np.where(m, g(dh) * abs(scale) * (np.abs(q) @ T(np.abs(K))) + 6 * U * np.abs(np.where(m, s, 0)), 0.0)
+    def most(x):  # the largest of a sample and key head, for every query head
+        x = x.max((2, 3))
+        if x.shape[1] == H:
+            x = x.reshape(B, KH, G).max(2)
+        return np.repeat(x, G, 1)[:, :, None, None]
+
+    aq, aK = np.abs(q), np.abs(K)
+    mq, mk, mv = most(aq), most(np.abs(k0)), most(np.abs(v0))
+    row = lambda x: x.sum(3, keepdims=True)  # noqa: E731
+    es = es + np.where(m, abs(scale) * F * (mq * T(row(aK)) + mk * row(aq)), 0.0)
     es = es.max(3, keepdims=True) + 6 * U * np.abs(top)
     eP = 2 * es + g(Sk)  # relative, of every probability of a row
     aV = P @ np.abs(Vv)
-    eo = eP * aV + g(Sk) * aV
+    eo = eP * aV + g(Sk) * aV + F * (m @ np.abs(Vv)) + F * mv
     el = (es + g(Sk) + 4 * U * np.abs(np.where(np.isfinite(lse), lse, 0))[..., None])[..., 0]
     res = {"out": (out, 1.05 * eo), "lse": (lse, 1.05 * el)}
     if dout is None:
         return res
     do, ado = dout, np.abs(dout)
     dP = do @ T(Vv)
-    edP = g(dh) * (ado @ T(np.abs(Vv)))
+    norm = lambda x: np.sqrt((x * x).sum(3, keepdims=True))  # noqa: E731
+    mdo, bound = most(ado), 2 * most(norm(do)) * most(norm(v0))
+    edP = g(dh) * (ado @ T(np.abs(Vv))) + F * (mdo * T(row(np.abs(Vv))) + mv * row(ado))
     delta = (do * out).sum(3, keepdims=True)
     edelta = g(dh) * (ado * np.abs(out)).sum(3, keepdims=True) + (ado * eo).sum(3, keepdims=True)
     dS = P * (dP - delta) * scale
     eb = 2 * es + el[..., None] + g(0)  # of the probability formed again from lse
     edS = abs(scale) * P * (edP + edelta + (eb + g(0)) * (np.abs(dP) + np.abs(delta)))
+    edS = np.where(m, edS + abs(scale) * F * bound, 0.0)
     aS = np.abs(dS)
-    dq, eq = dS @ K, edS @ np.abs(K) + g(Sk) * (aS @ np.abs(K))
+    dq, eq = dS @ K, edS @ np.abs(K) + g(Sk) * (aS @ np.abs(K)) + F * mk * row(aS)
     share = lambda x: x.reshape(B, KH, G, Sk, dh).sum(2)  # noqa: E731
     n = Sq * G
     dk = share(T(dS) @ q)
-    ek = share(T(edS) @ np.abs(q) + g(n) * (T(aS) @ np.abs(q)))
+    ek = share(T(edS) @ np.abs(q) + g(n) * (T(aS) @ np.abs(q)) + F * mq * row(T(aS)))
     dv = share(T(P) @ do)
-    ev = share(T(P * eb) @ ado + g(n) * (T(P) @ ado))
+    ev = share(T(P * eb + F * m) @ ado + g(n) * (T(P) @ ado) + F * mdo * row(T(P)))
     res.update(dq=(dq, 1.05 * eq), dk=(dk, 1.05 * ek), dv=(dv, 1.05 * ev))
     return res
 
@@ -108,7 +131,9 @@ def linear_ce(X, W, b, t, mean, acc=None):
     count = max(1, held.sum()) if mean else 1
     bb = np.zeros(V) if b is None else b
     z = X @ W + bb
-    ez = g(D) * (np.abs(X) @ np.abs(W) + np.abs(bb))
+    aW, aX = np.abs(W), np.abs(X)
+    mx = np.where(held, aX[held].max() if held.any() else 0.0, aX.max(1))[:, None]
+    ez = g(D) * (aX @ aW + np.abs(bb)) + F * (mx * aW.sum(0) + aW.max() * aX.sum(1, keepdims=True))
     top = z.max(1, keepdims=True)
     p = np.exp(z - top)
     l = p.sum(1, keepdims=True)
@@ -124,9 +149,10 @@ def linear_ce(X, W, b, t, mean, acc=None):
     G[np.arange(N)[held], t[held]] -= 1.0
     G = np.where(held[:, None], G, 0.0) / count
     eG = np.where(held[:, None], P * (es + el + g(0))[:, None], 0.0) / count + 4 * U * np.abs(G)
-    aW, aX = np.abs(W), np.abs(X)
-    dX, eX = G @ W.T, eG @ aW.T + g(V) * (np.abs(G) @ aW.T)
-    dW, eW = X.T @ G, aX.T @ eG + g(N) * (aX.T @ np.abs(G))
+    aG = np.abs(G)
+    eG = eG + np.where(held[:, None], F / count, 0.0)
+    dX, eX = G @ W.T, eG @ aW.T + g(V) * (aG @ aW.T) + F * aW.max() * aG.sum(1, keepdims=True)
+    dW, eW = X.T @ G, aX.T @ eG + g(N) * (aX.T @ aG) + F * mx.max(where=held[:, None], initial=0.0) * aG.sum(0)
     db, eb = G.sum(0), eG.sum(0) + g(N) * np.abs(G).sum(0)
     if acc is not None:
         dW, db = dW + acc[0], db + acc[1]

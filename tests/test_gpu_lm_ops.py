@@ -124,6 +124,12 @@ ATT = [  # B, Sq, Sk, H, KH, dh, causal, k_len, q_start, rows
     (2, 200, 300, 3, 1, 17, False, [300, 299], None, REF),
     (1, 40, 600, 4, 2, 100, False, [-3], None, SAMPLE),
     (2, 513, 513, 2, 1, 64, True, [900, 400], None, SAMPLE),
+    (3, 96, 160, 4, 2, 128, True, [160, 0, 3], None, REF),
+    (1, 300, 300, 2, 1, 96, True, None, None, SAMPLE),
+    (2, 129, 65, 4, 4, 32, False, [65, 64], None, SAMPLE),
+    (3, 200, 700, 8, 2, 64, True, [700, 650, 100], [500, -40, 2000], SAMPLE),
+    (2, 385, 130, 3, 3, 128, True, None, [0, -200], REF),
+    (1, 65, 1100, 5, 5, 81, False, None, None, SAMPLE),
 ]
 
 
