@@ -410,6 +410,7 @@ struct PackArgs {
 struct PairArgs {
   AttArgs a;
   PackArgs p;
+  float *dk_part, *dv_part;  // [B][heads][dh][Sk], where heads share keys
 };
 
 // The operand's scale over its slots, the same in every lane.
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(NT) att_pack_kernel(PairArgs g) {
   const Seq<const float>& x = g.p.x[which];
   const float* p = x.at(b, held ? r : 0, (int64_t)head * a.dh);
   const float* o = which == 3 ? a.o.at(b, held ? r : 0, (int64_t)head * a.dh) : nullptr;
-  char* q = g.p.p[which] + (((int64_t)b * heads + head) * g.p.blocks[which] + blk) * g.p.steps * (2 * pr::kFrag) + lane * 16;
+  char* q = g.p.p[which] + (((int64_t)b * heads + head) * g.p.blocks[which] + blk) * g.p.steps * (2 * pr::kFrag);
   float delta = 0.f;
 #pragma unroll 4
   for (int s = 0; s < g.p.steps; ++s) {
@@ -529,22 +530,30 @@ __global__ void __launch_bounds__(NT) att_pack_kernel(PairArgs g) {
       hi[e] = w0;
       lo[e] = w1;
     }
-    *reinterpret_cast<pr::u32x4*>(q + s * (2 * pr::kFrag)) = hi;
-    *reinterpret_cast<pr::u32x4*>(q + s * (2 * pr::kFrag) + pr::kFrag) = lo;
+    char* at = q + s * (2 * pr::kFrag) + pr::slot(lane, s);
+    *reinterpret_cast<pr::u32x4*>(at) = hi;
+    *reinterpret_cast<pr::u32x4*>(at + pr::kFrag) = lo;
   }
   if (which != 3) return;
   delta += other_half(delta);
   if (held && h == 0) a.delta[((int64_t)b * a.heads + head) * a.Sq + r] = delta;
 }
 
-// This block's (head of a sample, 128 rows of it): XCDs take contiguous runs
-// of heads, whose keys then stay in one L2; a head's last rows, which read the
-// most keys under a causal mask, go first.
-__device__ __forceinline__ void place(int tiles, int heads, int& tile, int& bh) {
-  const int total = tiles * heads, bid = (int)blockIdx.x, xcd = bid & 7, base = total >> 3, rem = total & 7;
-  const int id = xcd * base + min(xcd, rem) + (bid >> 3);
-  bh = id / tiles;
-  tile = tiles - 1 - id % tiles;
+// This block's head of a sample and 128 rows of it.  The longest go first (a
+// head's last rows under a causal mask): `tile` counts from there, over all
+// heads of a tile before the next.  Where the heads divide by the eight XCDs,
+// to which consecutive blocks go in turn, each takes a run of them, whose keys
+// then stay in its L2.
+__device__ __forceinline__ void place(int heads, int& tile, int& bh) {
+  const int bid = (int)blockIdx.x;
+  if (heads % 8 == 0) {
+    const int per = heads / 8, local = bid >> 3;
+    tile = local / per;
+    bh = (bid & 7) * per + local % per;
+  } else {
+    tile = bid / heads;
+    bh = bid % heads;
+  }
 }
 
 // Fragments of this lane's own row: packed feature step s, plane q.
@@ -553,24 +562,26 @@ struct RowFrags {
   pr::f16x8 x[KS][2];
   // base: the head's packed rows
   __device__ __forceinline__ void load(const char* base, int row, bool held) {
-    const char* p = base + (int64_t)(row >> 5) * KS * (2 * pr::kFrag) + (((int)threadIdx.x >> 5 & 1) * 32 + (row & 31)) * 16;
+    const char* p = base + (int64_t)(row >> 5) * KS * (2 * pr::kFrag);
+    const int l = ((int)threadIdx.x & 32) | (row & 31);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int q = 0; q < 2; ++q)
-        x[s][q] = held ? *reinterpret_cast<const pr::f16x8*>(p + (2 * s + q) * pr::kFrag) : pr::f16x8{};
+        x[s][q] = held ? *reinterpret_cast<const pr::f16x8*>(p + (2 * s + q) * pr::kFrag + pr::slot(l, s)) : pr::f16x8{};
   }
 };
 
 // acc (rows of the tile x rows of the lanes) = tile x^T over the features
 template <int KS>
 __device__ __forceinline__ f32x16 dot_pairs(const char* tile, const RowFrags<KS>& x) {
-  const char* p = tile + ((int)threadIdx.x & 63) * 16;
+  const int lane = (int)threadIdx.x & 63;
   f32x16 acc = {};
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    const pr::f16x8 a0 = *reinterpret_cast<const pr::f16x8*>(p + 2 * s * pr::kFrag);
-    const pr::f16x8 a1 = *reinterpret_cast<const pr::f16x8*>(p + (2 * s + 1) * pr::kFrag);
+    const char* p = tile + 2 * s * pr::kFrag + pr::slot(lane, s);
+    const pr::f16x8 a0 = *reinterpret_cast<const pr::f16x8*>(p);
+    const pr::f16x8 a1 = *reinterpret_cast<const pr::f16x8*>(p + pr::kFrag);
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, x.x[s][0], acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, x.x[s][1], acc, 0, 0, 0);
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, x.x[s][0], acc, 0, 0, 0);
@@ -604,24 +615,28 @@ template <int KS>
 __device__ __forceinline__ void add_pairs(const char* tile, const TileFrags& p, f32x16 (&acc)[KS / 2]) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const int lane = (int)threadIdx.x & 63, j = lane & 15;
-  const char* base = tile + (lane >> 4 & 1) * (2 * pr::kFrag) + ((j & 3) >> 1) * 512 + (4 * (lane >> 5) + (j >> 2)) * 16 +
-                     (j & 1) * 8;
+  const int lane = (int)threadIdx.x & 63, j = lane & 15, g = lane >> 4 & 1, half = (j & 3) >> 1;
+  const int row = 4 * (lane >> 5) + (j >> 2), turn = half * 4 + g * 8;
+  const char* base = tile + g * (2 * pr::kFrag) + half * 512 + (j & 1) * 8;
   auto frag = [&](int i, int t, int q) {
     const char* at = base + 2 * i * (2 * pr::kFrag) + q * pr::kFrag + t * 256;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 128));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + (row ^ turn) * 16));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + ((row + 8) ^ turn) * 16));
     return __builtin_bit_cast(pr::f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < 2; ++t) {
+    pr::f16x8 a[KS / 2][2];
 #pragma unroll
-    for (int i = 0; i < KS / 2; ++i) {
-      const pr::f16x8 a0 = frag(i, t, 0), a1 = frag(i, t, 1);
-      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, p.x[t][0], acc[i], 0, 0, 0);
-      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, p.x[t][1], acc[i], 0, 0, 0);
-      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, p.x[t][0], acc[i], 0, 0, 0);
-    }
+    for (int i = 0; i < KS / 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) a[i][q] = frag(i, t, q);
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+#pragma unroll
+      for (int i = 0; i < KS / 2; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][u == 0], p.x[t][u == 1], acc[i], 0, 0, 0);
+  }
 }
 
 // Copies of a tile of two operands into LDS (the first, then the second), the
@@ -651,7 +666,8 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
-  place(tiles, a.B * a.heads, tile, bh);
+  place(a.B * a.heads, tile, bh);
+  tile = tiles - 1 - tile;
   const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
   const int64_t bkh = (int64_t)b * a.kv_heads + kh;
   const int i = tile * 128 + 32 * wave + (lane & 31);
@@ -742,7 +758,8 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
-  place(tiles, a.B * a.heads, tile, bh);
+  place(a.B * a.heads, tile, bh);
+  tile = tiles - 1 - tile;
   const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
   const int64_t bkh = (int64_t)b * a.kv_heads + kh;
   const int i = tile * 128 + 32 * wave + (lane & 31);
@@ -789,19 +806,20 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   store_row<DHP>(a.dq.at(b, held ? i : 0, (int64_t)head * a.dh), a.dq.col, held, a.dh, a.scale, acc);
 }
 
-// dk, dv: a wave holds 32 keys and streams the queries and output gradients
-// of the heads that share them.
+// dk, dv: a wave holds 32 keys and streams the queries and output gradients of
+// one query head; where heads share the keys, into sums of their own
+// ([head of a sample][feature][key], att_share_kernel adds them).
 template <int DHP>
-__global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(PairArgs g, int key_tiles) {
+__global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(PairArgs g) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
   __shared__ __align__(16) char lds[2][2 * TILE];
   __shared__ __align__(16) float stat[2][2][32];  // lse (base 2) - 14, scaled delta of the tile's queries
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  int tile, bkh;
-  place(key_tiles, a.B * a.kv_heads, tile, bkh);
-  tile = key_tiles - 1 - tile;  // the first keys are read by the most queries
-  const int b = bkh / a.kv_heads, kh = bkh % a.kv_heads;
+  int tile, bh;
+  place(a.B * a.heads, tile, bh);  // the first keys are read by the most queries
+  const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
+  const int64_t bkh = (int64_t)b * a.kv_heads + kh;
   const int key0 = tile * 128, key = key0 + 32 * wave + (lane & 31);
   const int n = keys_of(a, b);
   const int64_t start = start_of(a, b);
@@ -811,40 +829,30 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(Pai
   const int eg = pr::scale_exp(sg.largest), ev = pr::scale_exp(sv.largest), ed = grad_exp(sg, sv);
   const float c = pr::times_exp2(a.scale * kLog2e, -eq - ek), cd = pr::times_exp2(1.f, ed - eg - ev - (int)kPExp);
   RowFrags<KS> k, v;
-  k.load(g.p.p[1] + (int64_t)bkh * g.p.blocks[1] * TILE, held ? key : 0, held);
-  v.load(g.p.p[2] + (int64_t)bkh * g.p.blocks[2] * TILE, held ? key : 0, held);
+  k.load(g.p.p[1] + bkh * g.p.blocks[1] * TILE, held ? key : 0, held);
+  v.load(g.p.p[2] + bkh * g.p.blocks[2] * TILE, held ? key : 0, held);
   // the first tile of queries that reads the block's first key
   int64_t first = a.causal ? key0 - start : 0;
   first = first < 0 ? 0 : first / 32;
-  const int per_head = key0 < n && first * 32 < a.Sq ? (int)((a.Sq + 31) / 32 - first) : 0;
-  const int total = per_head * a.group;
+  const int total = key0 < n && first * 32 < a.Sq ? (int)((a.Sq + 31) / 32 - first) : 0;
+  const char* qp = g.p.p[0] + ((int64_t)bh * g.p.blocks[0] + first) * TILE;
+  const char* gp = g.p.p[3] + ((int64_t)bh * g.p.blocks[3] + first) * TILE;
   f32x16 dk[DHP / 32] = {}, dv[DHP / 32] = {};
   float st = 0.f;
-  int head_next = 0, tile_next = 0;  // of the next tile to be copied
-  auto copy = [&](char* buf) {
-    const int64_t bh = (int64_t)b * a.heads + kh * a.group + head_next;
-    const int64_t at = (bh * g.p.blocks[0] + first + tile_next) * TILE;
-    copy_tile<KS>(g.p.p[0] + at, g.p.p[3] + at, buf);
-    const int64_t i = (first + tile_next) * 32 + (lane & 31);
-    if (wave == 0 && i < a.Sq) {
-      if (lane < 32) st = lse2_of(a, b, kh * a.group + head_next, i) - kPExp;
-      else st = pr::times_exp2(a.delta[bh * a.Sq + i], ed - (int)kPExp);
-    } else {
-      st = lane < 32 ? INFINITY : 0.f;
-    }
-    if (++tile_next == per_head) {
-      tile_next = 0;
-      ++head_next;
-    }
+  auto copy = [&](int t) {
+    copy_tile<KS>(qp + (int64_t)t * TILE, gp + (int64_t)t * TILE, lds[t & 1]);
+    const int64_t i = (first + t) * 32 + (lane & 31);
+    if (wave != 0) return;
+    if (i >= a.Sq) st = lane < 32 ? INFINITY : 0.f;
+    else if (lane < 32) st = lse2_of(a, b, head, i) - kPExp;
+    else st = pr::times_exp2(a.delta[(int64_t)bh * a.Sq + i], ed - (int)kPExp);
   };
-  if (total > 0) copy(lds[0]);
-  int ti = 0;
+  if (total > 0) copy(0);
   for (int t = 0; t < total; ++t) {
     if (wave == 0) stat[t & 1][lane >> 5][lane & 31] = st;
     pr::wait_and_meet<0>();
-    const int64_t i0 = (first + ti) * 32;
-    if (++ti == per_head) ti = 0;
-    if (t + 1 < total) copy(lds[(t + 1) & 1]);
+    const int64_t i0 = (first + t) * 32;
+    if (t + 1 < total) copy(t + 1);
     if (a.causal && start + i0 + 31 < key0 + 32 * wave) continue;  // no query of the tile reads this wave's keys
     const char* buf = lds[t & 1];
     f32x16 s = dot_pairs<KS>(buf, k);
@@ -877,8 +885,33 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(Pai
     }
   const bool stored = key < a.Sk;
   const int at = stored ? key : 0;
-  store_row<DHP>(a.dk.at(b, at, (int64_t)kh * a.dh), a.dk.col, stored, a.dh, a.scale, dk);
-  store_row<DHP>(a.dv.at(b, at, (int64_t)kh * a.dh), a.dv.col, stored, a.dh, 1.f, dv);
+  if (a.group == 1) {
+    store_row<DHP>(a.dk.at(b, at, (int64_t)kh * a.dh), a.dk.col, stored, a.dh, a.scale, dk);
+    store_row<DHP>(a.dv.at(b, at, (int64_t)kh * a.dh), a.dv.col, stored, a.dh, 1.f, dv);
+  } else {
+    const int64_t o = (int64_t)bh * a.dh * a.Sk + at;
+    store_row<DHP>(g.dk_part + o, a.Sk, stored, a.dh, a.scale, dk);
+    store_row<DHP>(g.dv_part + o, a.Sk, stored, a.dh, 1.f, dv);
+  }
+}
+
+// dk, dv of a key head: the sums of the heads that share it, in their order.
+__global__ void __launch_bounds__(NT) att_share_kernel(PairArgs g) {
+  const AttArgs& a = g.a;
+  const int key = (int)blockIdx.x * NT + (int)threadIdx.x;
+  if (key >= a.Sk) return;
+  const int b = (int)blockIdx.y / a.kv_heads, kh = (int)blockIdx.y % a.kv_heads;
+  const float* part = blockIdx.z ? g.dv_part : g.dk_part;
+  part += ((int64_t)b * a.heads + (int64_t)kh * a.group) * a.dh * a.Sk + key;
+  const Seq<float>& out = blockIdx.z ? a.dv : a.dk;
+  float* o = out.at(b, key, (int64_t)kh * a.dh);
+  const int64_t head = (int64_t)a.dh * a.Sk;
+#pragma unroll 4
+  for (int d = 0; d < a.dh; ++d) {
+    float s = 0.f;
+    for (int h = 0; h < a.group; ++h) s += part[h * head + (int64_t)d * a.Sk];
+    o[d * out.col] = s;
+  }
 }
 
 // Lays out the workspace of the packed operands and packs them.  ops: 3 (q, k,
@@ -907,9 +940,13 @@ int pack(PairArgs& g, int ops, hipStream_t st, const char* who) {
     data[w] = place_bytes((size_t)a.B * heads * p.blocks[w] * p.steps * 2 * pr::kFrag);
   }
   const size_t delta = place_bytes(ops == 4 ? (size_t)a.B * a.heads * a.Sq * sizeof(float) : 0);
+  const size_t sums = ops == 4 && a.group > 1 ? (size_t)a.B * a.heads * a.dh * a.Sk * sizeof(float) : 0;
+  const size_t dk_part = place_bytes(sums), dv_part = place_bytes(sums);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, bytes, &ws, who));
   char* base = static_cast<char*>(ws);
+  g.dk_part = reinterpret_cast<float*>(base + dk_part);
+  g.dv_part = reinterpret_cast<float*>(base + dv_part);
   for (int w = 0; w < ops; ++w) {
     p.part[w] = reinterpret_cast<Scale*>(base + part[w]);
     p.p[w] = base + data[w];
@@ -1022,7 +1059,7 @@ int cnhip_attention_forward(const float* q, const float* k, const float* v, floa
   a.out = cnhip::seq(out, B, Sq, rows);
   a.lse = lse;
   if (cnhip::use_pairs(a)) {
-    cnhip::PairArgs g{a, {}};
+    cnhip::PairArgs g{a, {}, nullptr, nullptr};
     CNHIP_TRY(cnhip::pack(g, 3, st, who));
     const int tiles = (int)((Sq + 127) / 128);
     cnhip::by_width(a.dh, [&](auto d) {
@@ -1055,14 +1092,20 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
   a.dv = cnhip::seq(dv, B, Sk, rows);
   a.lse_in = lse;
   if (cnhip::use_pairs(a)) {
-    cnhip::PairArgs g{a, {}};
+    cnhip::PairArgs g{a, {}, nullptr, nullptr};
     CNHIP_TRY(cnhip::pack(g, 4, st, who));
     const int tiles = (int)((Sq + 127) / 128), key_tiles = (int)((Sk + 127) / 128);
     cnhip::by_width(a.dh, [&](auto d) {
-      hipLaunchKernelGGL((cnhip::att_dkv_pair_kernel<d()>), dim3((unsigned)(key_tiles * B * kv_heads)), dim3(cnhip::NT),
-                         0, st, g, key_tiles);
+      hipLaunchKernelGGL((cnhip::att_dkv_pair_kernel<d()>), dim3((unsigned)(key_tiles * B * heads)), dim3(cnhip::NT), 0,
+                         st, g);
     });
     CNHIP_TRY(cnhip::check_launch(who));
+    if (a.group > 1) {
+      hipLaunchKernelGGL(cnhip::att_share_kernel,
+                         dim3((unsigned)((Sk + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * kv_heads), 2), dim3(cnhip::NT),
+                         0, st, g);
+      CNHIP_TRY(cnhip::check_launch(who));
+    }
     cnhip::by_width(a.dh, [&](auto d) {
       hipLaunchKernelGGL((cnhip::att_dq_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st, g,
                          tiles);

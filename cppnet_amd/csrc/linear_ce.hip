@@ -189,7 +189,7 @@ __device__ __forceinline__ void put_frag(char* p, int64_t block, int steps, int 
     hi[e] = h;
     lo[e] = l;
   }
-  char* q = p + (block * steps + step) * (2 * pr::kFrag) + (threadIdx.x & 63) * 16;
+  char* q = p + (block * steps + step) * (2 * pr::kFrag) + pr::slot(threadIdx.x & 63, step);
   *reinterpret_cast<u32x4*>(q) = hi;
   *reinterpret_cast<u32x4*>(q + pr::kFrag) = lo;
 }

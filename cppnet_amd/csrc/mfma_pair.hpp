@@ -20,14 +20,17 @@
 // and its accumulators with it, and the drifts of the two halves cancel.
 //
 // Packed layout.  An operand of `rows` rows and a contraction of k is held in
-// fragments of 32 rows x 16 k, two planes (x0, x1) of 1024 bytes each: lane l
-// of the MFMA finds its eight k (8 (l / 32) .. + 7) of row l % 32 at byte 16 l.
-// Fragments of a row block follow each other along k.  Both sizes are padded
-// with zeros to multiples of 32.  Such an operand goes from memory to LDS as
-// it lies (16 bytes a lane, no registers) and from LDS to the MFMA with one
-// ds_read_b128 of 1024 adjacent bytes a plane.  The same packing also serves
-// the product whose contraction runs along its rows: ds_read_b64_tr_b16 turns
-// 4 x 16 halves on the way to the registers.
+// fragments of 32 rows x 16 k, two planes (x0, x1) of 1024 bytes each: row r's
+// eight k of half h (8 h .. 8 h + 7), which lane 32 h + r of the MFMA takes, lie
+// in 16 bytes at slot(32 h + r, step).  Fragments of a row block follow each
+// other along k.  Both sizes are padded with zeros to multiples of 32.  Such an
+// operand goes from memory to LDS as it lies (16 bytes a lane, no registers)
+// and from LDS to the MFMA with one ds_read_b128 over the 1024 bytes of a
+// plane.  The same packing also serves the product whose contraction runs along
+// its rows: ds_read_b64_tr_b16 turns 4 x 16 halves on the way to the registers.
+// Half a wave then takes 4 rows of both halves of two steps; slot's permutation
+// of the rows spreads those over all 64 banks (unpermuted they met in a
+// quarter of them: 6.8 cycles a read for 2).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -64,6 +67,11 @@ __device__ __forceinline__ float times_exp2(float x, int e) { return __builtin_a
 __device__ __forceinline__ uint32_t finite_bits(float x) {
   const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
+}
+
+// Byte of lane l's 16 in a plane of step s.
+__device__ __forceinline__ int slot(int l, int s) {
+  return ((l & 32) | ((l & 31) ^ ((l >> 5) * 4 + (s & 1) * 8))) * 16;
 }
 
 // two values to their terms: w0 = {x0(a), x0(b)}, w1 the remainders
@@ -129,7 +137,7 @@ constexpr int kGemmLds = kStages * kStage;
 //   TR false: piece j = plane j & 1 of the fragment of row block j / 2
 //   TR true (contraction along the packed rows): piece j = for the 16 output
 //     rows of packed step j, both planes of the 16 packed rows of this step:
-//     [plane][k half of 8][row][8 halves]
+//     [plane][k half of 8][slot of the row][8 halves]
 template <bool TR>
 struct Stage {
   const char* src[2];
@@ -158,17 +166,17 @@ struct Stage {
   }
 };
 
-// This lane's fragment of row block `blk` of the tile, plane q.
+// This lane's fragment of row block `blk` of the tile, plane q; t: the step.
 template <bool TR>
-__device__ __forceinline__ f16x8 frag(const char* buf, int blk, int q) {
+__device__ __forceinline__ f16x8 frag(const char* buf, int blk, int q, int t) {
   const int lane = threadIdx.x & 63;
-  if constexpr (!TR) return *reinterpret_cast<const f16x8*>(buf + (2 * blk + q) * kFrag + lane * 16);
+  if constexpr (!TR) return *reinterpret_cast<const f16x8*>(buf + (2 * blk + q) * kFrag + slot(lane, t));
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const int j = lane & 15, k = 8 * (lane >> 5) + (j >> 2);
-  const char* p = buf + (2 * blk + (lane >> 4 & 1)) * kFrag + q * 512 + ((j & 3) >> 1) * 256 + k * 16 + (j & 1) * 8;
-  s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-  s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 64));
+  const int j = lane & 15, g = lane >> 4 & 1, half = (j & 3) >> 1, k = 8 * (lane >> 5) + (j >> 2);
+  const char* p = buf + (2 * blk + g) * kFrag + q * 512 + half * 256 + (j & 1) * 8;
+  s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + (k ^ (half * 4 + g * 8)) * 16));
+  s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + ((k + 4) ^ (half * 4 + g * 8)) * 16));
   return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -224,15 +232,15 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
     else sb.copy(s, u - 2, buf + kStage / 2);
   };
   // fragment u (0 .. 11) of step t, in the order of their first use
-  auto read = [&](int t, int u, Frags& f) {
+  auto read = [&](int t, int odd, int u, Frags& f) {
     const char* buf = lds + (t & (kStages - 1)) * kStage;
-    if (u < 2) f.b[u][0] = frag<TB>(buf + kStage / 2, 2 * wn + u, 0);
-    else if (u < 6) f.a[u - 2][1] = frag<TA>(buf, 4 * wm + u - 2, 1);
-    else if (u < 8) f.b[u - 6][1] = frag<TB>(buf + kStage / 2, 2 * wn + u - 6, 1);
-    else f.a[u - 8][0] = frag<TA>(buf, 4 * wm + u - 8, 0);
+    if (u < 2) f.b[u][0] = frag<TB>(buf + kStage / 2, 2 * wn + u, 0, odd);
+    else if (u < 6) f.a[u - 2][1] = frag<TA>(buf, 4 * wm + u - 2, 1, odd);
+    else if (u < 8) f.b[u - 6][1] = frag<TB>(buf + kStage / 2, 2 * wn + u - 6, 1, odd);
+    else f.a[u - 8][0] = frag<TA>(buf, 4 * wm + u - 8, 0, odd);
   };
   Frags f0, f1;
-  auto step = [&](int t, Frags& now, Frags& next) {
+  auto step = [&](int t, int odd, Frags& now, Frags& next) {
     // step t + 1 has arrived (two younger ones may be on their way), and every
     // wave holds step t in registers: its buffer is free
     wait_and_meet<8>();
@@ -252,7 +260,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         acc.x[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.a[i][x], now.b[j][y], acc.x[i][j], 0, 0, 0);
-      read(t + 1, u, next);
+      read(t + 1, 1 - odd, u, next);
       if (u % 3 == 0) copy(t + 4, u / 3);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -263,10 +271,11 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
     for (int u = 0; u < 4; ++u) copy(t0 + t, u);
   wait_and_meet<12>();
 #pragma unroll
-  for (int u = 0; u < 12; ++u) read(t0, u, f0);
+  for (int u = 0; u < 12; ++u) read(t0, 0, u, f0);
+  // t0 is even, so a step's parity, and with it the slots, is known here
   for (int t = t0; t < t1; t += 2) {
-    step(t, f0, f1);
-    if (t + 1 < t1) step(t + 1, f1, f0);
+    step(t, 0, f0, f1);
+    if (t + 1 < t1) step(t + 1, 1, f1, f0);
   }
   wait_and_meet<0>();  // the copies that went past the end
   if (t1 > g.half) {
