@@ -164,16 +164,65 @@ __device__ __forceinline__ void store_row(float* base, int64_t col, bool held, i
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
-// Forward.  A block owns 128 rows of a key head's queries: row g Sq + i is
-// query i of the g-th of the query heads that share the key head, so a
-// sequence's single queries fill a wave together.
+// Forward of few queries.  A block owns 32 rows of a key head's queries (row
+// g Sq + i is query i of the g-th of the query heads that share the key head,
+// so that single queries of a group fill a wave together) and a run of keys,
+// whose tiles its four waves take in turn, each staging its own through its
+// own part of LDS: no wave waits for another before the end.  There the four
+// join their sums, and where the keys are shared out over several blocks
+// att_join_kernel joins theirs.
+struct SplitArgs {
+  int splits, tiles_per_split;  // of 32 keys
+  float* o;                     // [split][B kv_heads][row tile][feature][32]
+  float2* ml;                   // [split][B kv_heads][row tile][32]: maximum (base 2), sum
+};
+
+// A wave's [DHP][RT] tile on its way to LDS.
 template <int DHP, bool UNIT>
-__global__ void __launch_bounds__(NT) att_fwd_kernel(AttArgs a) {
-  __shared__ __align__(16) float lds[2][DHP * LS];
+struct WaveTile {
+  static constexpr int U = DHP / 8;  // float4s per lane
+  f32x4 v[U];
+  __device__ __forceinline__ void load(const float* base, int64_t row, int64_t col, int valid, int dh) {
+    const int r = 4 * ((int)threadIdx.x & 7), d0 = ((int)threadIdx.x & 63) >> 3;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int d = d0 + 8 * u;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (d < dh) {
+        const float* p = base + r * row + d * col;
+        if (UNIT && r + 3 < valid) {
+          x = *reinterpret_cast<const f32x4u*>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (r + e < valid) x[e] = p[e * row];
+        }
+      }
+      v[u] = x;
+    }
+  }
+  __device__ __forceinline__ void store(float* lds) const {
+    const int r = 4 * ((int)threadIdx.x & 7), d0 = ((int)threadIdx.x & 63) >> 3;
+#pragma unroll
+    for (int u = 0; u < U; ++u) *reinterpret_cast<f32x4*>(lds + (d0 + 8 * u) * LS + r) = v[u];
+  }
+};
+
+// Between a wave's own LDS writes and reads: no other wave touches its part.
+__device__ __forceinline__ void own_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+template <int DHP, bool UNIT>
+__global__ void __launch_bounds__(NT) att_fwd_kernel(AttArgs a, SplitArgs p) {
+  __shared__ __align__(16) float lds[4][2][DHP * LS];
+  __shared__ float2 stat[4][32];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const int b = (int)blockIdx.y / a.kv_heads, kh = (int)blockIdx.y % a.kv_heads;
   const int64_t rows = (int64_t)a.group * a.Sq;
-  const int64_t r = (int64_t)blockIdx.x * 128 + 32 * wave + (lane & 31);
+  const int64_t r = (int64_t)blockIdx.x * 32 + (lane & 31);
   const bool held = r < rows;
   const int head = kh * a.group + (int)(held ? r / a.Sq : 0);
   const int64_t i = held ? r % a.Sq : 0;
@@ -181,38 +230,35 @@ __global__ void __launch_bounds__(NT) att_fwd_kernel(AttArgs a) {
   const int lim = held ? limit(a, n, start_of(a, b), i) : 0;
   float q[DHP / 2];
   load_row<DHP>(a.q.at(b, i, (int64_t)head * a.dh), a.q.col, held, a.dh, q);
-  __shared__ int most;
-  if (threadIdx.x == 0) most = 0;
-  __syncthreads();
-  atomicMax(&most, lim);
-  __syncthreads();
-  const int end = most;
+  int most = lim;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  const int t1 = min((most + RT - 1) / RT, ((int)blockIdx.z + 1) * p.tiles_per_split);
   const float c = a.scale * kLog2e;
   const float* kp = a.k.at(b, 0, (int64_t)kh * a.dh);
   const float* vp = a.v.at(b, 0, (int64_t)kh * a.dh);
 
   f32x16 o[DHP / 32] = {};
   float m = -INFINITY, l = 0.f;  // of t = scale log2(e) s: maximum and sum of 2^(t - m)
-  TileLoad<DHP, UNIT> tk, tv;
-  if (end > 0) {
-    tk.load(kp, a.k.row, a.k.col, n, a.dh);
-    tv.load(vp, a.v.row, a.v.col, n, a.dh);
-  }
-  for (int j0 = 0; j0 < end; j0 += RT) {
-    __syncthreads();
-    tk.store(lds[0]);
-    tv.store(lds[1]);
-    __syncthreads();
-    if (j0 + RT < end) {
-      tk.load(kp + (j0 + RT) * a.k.row, a.k.row, a.k.col, n - j0 - RT, a.dh);
-      tv.load(vp + (j0 + RT) * a.v.row, a.v.row, a.v.col, n - j0 - RT, a.dh);
-    }
-    if (!__any(lim > j0)) continue;
-    f32x16 s = dot_rows<DHP>(lds[0], q);
+  WaveTile<DHP, UNIT> tk, tv;
+  auto load = [&](int t) {
+    const int64_t j = (int64_t)t * RT;
+    tk.load(kp + j * a.k.row, a.k.row, a.k.col, n - t * RT, a.dh);
+    tv.load(vp + j * a.v.row, a.v.row, a.v.col, n - t * RT, a.dh);
+  };
+  int t = (int)blockIdx.z * p.tiles_per_split + wave;
+  if (t < t1) load(t);
+  for (; t < t1; t += 4) {
+    own_lds();
+    tk.store(lds[wave][0]);
+    tv.store(lds[wave][1]);
+    own_lds();
+    if (t + 4 < t1) load(t + 4);
+    f32x16 s = dot_rows<DHP>(lds[wave][0], q);
     float most_s = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int j = j0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+      const int j = t * RT + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
       s[e] = j < lim ? s[e] * c : -INFINITY;
       most_s = fmaxf(most_s, s[e]);
     }
@@ -231,12 +277,72 @@ __global__ void __launch_bounds__(NT) att_fwd_kernel(AttArgs a) {
     for (int d = 0; d < DHP / 32; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] *= f;
-    add_rows<DHP>(lds[1], s, o);
+    add_rows<DHP>(lds[wave][1], s, o);
   }
   l += other_half(l);
-  store_row<DHP>(a.out.at(b, i, (int64_t)head * a.dh), a.out.col, held, a.dh, lim > 0 ? 1.f / l : 0.f, o);
-  if (a.lse && held && lane < 32)
-    a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = lim > 0 ? (m + log2f(l)) * kLn2 : -INFINITY;
+  // the four waves' sums to a common maximum; [feature][row] in the wave's part
+  if (lane < 32) stat[wave][lane] = float2{m, l};
+  __syncthreads();
+  float top = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][lane & 31].x);
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) total += stat[w][lane & 31].y * __builtin_amdgcn_exp2f(stat[w][lane & 31].x - base);
+  const float f = __builtin_amdgcn_exp2f(m - base);
+  float* own = &lds[wave][0][0];
+#pragma unroll
+  for (int d = 0; d < DHP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      own[(32 * d + 8 * (e / 4) + 4 * (lane >> 5) + e % 4) * 32 + (lane & 31)] = o[d][e] * f;
+  __syncthreads();
+  const int64_t at = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  const float inv = p.splits > 1 ? 1.f : lim > 0 ? 1.f / total : 0.f;
+  float* out = a.out.at(b, i, (int64_t)head * a.dh);
+  for (int d = 2 * wave + (lane >> 5); d < a.dh; d += 8) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x += lds[w][0][d * 32 + (lane & 31)];
+    if (p.splits > 1) p.o[(at * a.dh + d) * 32 + (lane & 31)] = x;
+    else if (held) out[d * a.out.col] = x * inv;
+  }
+  if (wave != 0 || lane >= 32) return;
+  if (p.splits > 1) p.ml[at * 32 + lane] = float2{top, total};
+  else if (a.lse && held) a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = lim > 0 ? (top + log2f(total)) * kLn2 : -INFINITY;
+}
+
+// Joins the sums of a row tile's runs of keys, in their order; 32 features a
+// block, a thread per row and four of them.
+__global__ void __launch_bounds__(NT) att_join_kernel(AttArgs a, SplitArgs p) {
+  const int lane = (int)threadIdx.x & 31, part = (int)threadIdx.x >> 5;
+  const int b = (int)blockIdx.y / a.kv_heads, kh = (int)blockIdx.y % a.kv_heads;
+  const int64_t rows = (int64_t)a.group * a.Sq;
+  const int64_t r = (int64_t)blockIdx.x * 32 + lane;
+  if (r >= rows) return;
+  const int head = kh * a.group + (int)(r / a.Sq);
+  const int64_t i = r % a.Sq, step = (int64_t)gridDim.y * gridDim.x, at = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  float top = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.ml[(at + s * step) * 32 + lane].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = 0.f, x[4] = {};
+  const int d0 = (int)blockIdx.z * 32 + 4 * part;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = p.ml[(at + s * step) * 32 + lane];
+    const float f = __builtin_amdgcn_exp2f(ml.x - base);
+    total += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d0 + e < a.dh) x[e] = fmaf(p.o[((at + s * step) * a.dh + d0 + e) * 32 + lane], f, x[e]);
+  }
+  const float inv = total > 0.f ? 1.f / total : top == -INFINITY ? 0.f : NAN;
+  float* out = a.out.at(b, i, (int64_t)head * a.dh);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d0 + e < a.dh) out[(d0 + e) * a.out.col] = x[e] * inv;
+  if (a.lse && part == 0 && blockIdx.z == 0)
+    a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
 // delta[b][head][i] = sum_d dout out
@@ -895,23 +1001,28 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(Pai
   }
 }
 
-// dk, dv of a key head: the sums of the heads that share it, in their order.
+// dk, dv of a key head: the sums of the heads that share it, in their order; a
+// thread per key and four features.
 __global__ void __launch_bounds__(NT) att_share_kernel(PairArgs g) {
   const AttArgs& a = g.a;
-  const int key = (int)blockIdx.x * NT + (int)threadIdx.x;
+  const int key = (int)blockIdx.x * NT + (int)threadIdx.x, widths = (a.dh + 3) / 4;
   if (key >= a.Sk) return;
   const int b = (int)blockIdx.y / a.kv_heads, kh = (int)blockIdx.y % a.kv_heads;
-  const float* part = blockIdx.z ? g.dv_part : g.dk_part;
-  part += ((int64_t)b * a.heads + (int64_t)kh * a.group) * a.dh * a.Sk + key;
-  const Seq<float>& out = blockIdx.z ? a.dv : a.dk;
-  float* o = out.at(b, key, (int64_t)kh * a.dh);
+  const int d0 = (int)blockIdx.z % widths * 4;
+  const bool v = (int)blockIdx.z >= widths;
   const int64_t head = (int64_t)a.dh * a.Sk;
-#pragma unroll 4
-  for (int d = 0; d < a.dh; ++d) {
-    float s = 0.f;
-    for (int h = 0; h < a.group; ++h) s += part[h * head + (int64_t)d * a.Sk];
-    o[d * out.col] = s;
-  }
+  const float* part = (v ? g.dv_part : g.dk_part) + ((int64_t)b * a.heads + (int64_t)kh * a.group) * head + key;
+  const Seq<float>& out = v ? a.dv : a.dk;
+  float* o = out.at(b, key, (int64_t)kh * a.dh);
+  float s[4] = {};
+#pragma unroll 2
+  for (int h = 0; h < a.group; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d0 + e < a.dh) s[e] += part[h * head + (int64_t)(d0 + e) * a.Sk];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d0 + e < a.dh) o[(d0 + e) * out.col] = s[e];
 }
 
 // Lays out the workspace of the packed operands and packs them.  ops: 3 (q, k,
@@ -1068,10 +1179,30 @@ int cnhip_attention_forward(const float* q, const float* k, const float* v, floa
     });
     return cnhip::check_launch(who);
   }
-  const dim3 grid((unsigned)((a.group * Sq + 127) / 128), (unsigned)(B * kv_heads));
+  // Runs of keys: enough blocks for two on every CU, at least two tiles a wave.
+  const int64_t row_tiles = (a.group * Sq + 31) / 32, key_tiles = (Sk + 31) / 32;
+  int64_t splits = 512 / (row_tiles * B * kv_heads);
+  if (splits > key_tiles / 8) splits = key_tiles / 8;
+  if (splits < 1) splits = 1;
+  cnhip::SplitArgs p{};
+  p.tiles_per_split = (int)((key_tiles + splits - 1) / splits);
+  p.splits = (int)((key_tiles + p.tiles_per_split - 1) / p.tiles_per_split);
+  CNHIP_REQUIRE(row_tiles < (int64_t)1 << 31, "%s: too many rows", who);
+  if (p.splits > 1) {
+    const size_t rows32 = (size_t)(p.splits * B * kv_heads * row_tiles) * 32;
+    void* ws = nullptr;
+    CNHIP_TRY(cnhip::scratch(st, cnhip::kScratchLayer, rows32 * (sizeof(float2) + head_dim * sizeof(float)), &ws, who));
+    p.ml = static_cast<float2*>(ws);
+    p.o = reinterpret_cast<float*>(p.ml + rows32);
+  }
+  const dim3 grid((unsigned)row_tiles, (unsigned)(B * kv_heads), (unsigned)p.splits);
   cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
-    hipLaunchKernelGGL((cnhip::att_fwd_kernel<d(), unit()>), grid, dim3(cnhip::NT), 0, st, a);
+    hipLaunchKernelGGL((cnhip::att_fwd_kernel<d(), unit()>), grid, dim3(cnhip::NT), 0, st, a, p);
   });
+  CNHIP_TRY(cnhip::check_launch(who));
+  if (p.splits == 1) return CNHIP_OK;
+  hipLaunchKernelGGL(cnhip::att_join_kernel, dim3((unsigned)row_tiles, (unsigned)(B * kv_heads), (unsigned)((head_dim + 31) / 32)),
+                     dim3(cnhip::NT), 0, st, a, p);
   return cnhip::check_launch(who);
 }
 
@@ -1102,8 +1233,8 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
     CNHIP_TRY(cnhip::check_launch(who));
     if (a.group > 1) {
       hipLaunchKernelGGL(cnhip::att_share_kernel,
-                         dim3((unsigned)((Sk + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * kv_heads), 2), dim3(cnhip::NT),
-                         0, st, g);
+                         dim3((unsigned)((Sk + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * kv_heads), (unsigned)((head_dim + 3) / 4 * 2)),
+                         dim3(cnhip::NT), 0, st, g);
       CNHIP_TRY(cnhip::check_launch(who));
     }
     cnhip::by_width(a.dh, [&](auto d) {
