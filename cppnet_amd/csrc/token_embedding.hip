@@ -18,7 +18,6 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef int32_t i32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // Row of the sequence that the id at j = b + B s belongs to, and the reverse.
 __device__ __forceinline__ int64_t row_of(int64_t j, int64_t B, int64_t S, int rows) {
@@ -28,44 +27,72 @@ __device__ __forceinline__ int64_t id_of(int64_t p, int64_t B, int64_t S, int ro
   return rows == CNHIP_ROWS_REF ? p : p / S + B * (p % S);
 }
 
-// A tile of 64 rows x 64 features: read along the features of the table,
-// turned in LDS, written along the rows of out.
+// A 64 x 64 tile turned through LDS, float4s along either side: element c of
+// row r lies at tile[r][lane_of(r, c)], which spreads both the rows' float4s and
+// the single elements of a column over all banks.
+constexpr int TS = 64;
+__device__ __forceinline__ int lane_of(int r, int c) { return c ^ (r & 60); }
+
+// Four floats from p, of which the first n exist (zeros for the others).
+__device__ __forceinline__ f32x4 get4(const float* p, int64_t n) {
+  if (n >= 4) return *reinterpret_cast<const f32x4u*>(p);
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) x[e] = p[e];
+  return x;
+}
+__device__ __forceinline__ void put4(float* p, int64_t n, f32x4 x) {
+  if (n >= 4) {
+    *reinterpret_cast<f32x4u*>(p) = x;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) p[e] = x[e];
+}
+
+// 64 rows x 64 features: read along the features of the table, turned, written
+// along the rows of out.
 __global__ void __launch_bounds__(256) token_fwd_kernel(const int32_t* __restrict__ ids, const float* __restrict__ Wt,
                                                         float* __restrict__ out, int64_t B, int64_t S, int64_t V,
                                                         int64_t D, float scale, int rows, int32_t* __restrict__ oob) {
-  __shared__ float tile[64][65];
-  __shared__ int64_t tok[64];
+  __shared__ __align__(16) float tile[64][TS];  // [feature][row]
+  __shared__ int32_t tok[64];
   const int64_t N = B * S, p0 = (int64_t)blockIdx.x * 64, d0 = (int64_t)blockIdx.y * 64;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   if (threadIdx.x < 64) {
-    const int64_t p = p0 + tx;
-    int64_t id = p < N ? ids[id_of(p, B, S, rows)] : -1;
+    const int64_t p = p0 + threadIdx.x;
+    const int32_t id = p < N ? ids[id_of(p, B, S, rows)] : -1;
     const bool held = id >= 0 && id < V;
     if (p < N && !held && oob && blockIdx.y == 0) atomicAdd(oob, 1);
-    tok[tx] = held ? id : -1;
+    tok[threadIdx.x] = held ? id : -1;
   }
   __syncthreads();
-  float v[16];
-  const int64_t d = d0 + tx;
+  const int four = 4 * (threadIdx.x & 15), one = threadIdx.x >> 4;
+  f32x4 x[4];
 #pragma unroll
-  for (int u = 0; u < 16; ++u) {
-    const int64_t id = tok[ty + 4 * u];
-    v[u] = d < D && id >= 0 ? scale * Wt[d + D * id] : 0.f;
+  for (int u = 0; u < 4; ++u) {
+    const int32_t id = tok[one + 16 * u];
+    x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (id >= 0) x[u] = get4(Wt + D * (int64_t)id + d0 + four, D - d0 - four);
   }
 #pragma unroll
-  for (int u = 0; u < 16; ++u) tile[ty + 4 * u][tx] = v[u];
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[four + e][lane_of(four + e, one + 16 * u)] = scale * x[u][e];
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < 16; ++u) {
-    const int j = ty + 4 * u;
-    if (p0 + tx < N && d0 + j < D) out[p0 + tx + N * (d0 + j)] = tile[tx][j];
+  for (int u = 0; u < 4; ++u) {
+    const int d = one + 16 * u;
+    if (d0 + d < D) put4(out + p0 + four + N * (d0 + d), N - p0 - four, *reinterpret_cast<const f32x4*>(&tile[d][lane_of(d, four)]));
   }
 }
 
 // ------------------------------------------------------------------ gradient
-// 1. Every id finds its place among the sorted ones (its rank: how many are
-//    smaller, or equal and before it), while dY [N, D] is turned into dYt, a
-//    row's features adjacent (leading dimension Dp, a multiple of 4).
+// 1. The ids are sorted, equal ones in their order (each finds how many are
+//    smaller, or equal and before it; very many by a radix sort), while dY
+//    [N, D] is turned into dYt, a row's features adjacent (leading dimension
+//    Dp, a multiple of 4), and the table's rows that no id names get zeros.
 // 2. The sorted rows are summed in chunks of kChunk, a wave each: a token
 //    whose rows lie inside one chunk is written to the table, the sums of one
 //    that goes on into the next chunk are kept.
@@ -73,6 +100,8 @@ __global__ void __launch_bounds__(256) token_fwd_kernel(const int32_t* __restric
 // Ids outside the table sort last, as V, and are left out.  The order of every
 // sum is fixed by the ids alone.
 constexpr int kChunk = 16;
+
+constexpr int64_t kRankMost = 24576;
 
 struct TokArgs {
   const int32_t* ids;
@@ -92,65 +121,232 @@ __device__ __forceinline__ int32_t key_of(int32_t id, int64_t V) {
   return id >= 0 && id < V ? id : (int32_t)V;
 }
 
-// how many of ids[j0 .. j1) have a key below t
-__device__ __forceinline__ int below(const int32_t* ids, int64_t V, int64_t j0, int64_t j1, int64_t t) {
+// Up to kRankMost ids are sorted by comparing each with every other: 2 N^2
+// instructions over all lanes, beside the turning of dY in the same launch.
+// More take a radix sort in launches of its own.  The whole gradient at width
+// 512 and 32000 ids, comparing against radix sort: 8192 rows 40 and 79 us,
+// 16384 58 and 85, 24576 86 and 90, 32768 125 and 99.
+constexpr int kIdChunk = 8192;  // ids in LDS at a time
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kSortIds = 16;                // ids a block
+constexpr int kSortParts = 256 / kSortIds;  // threads that share an id's comparisons
+
+// how many of this thread's fours of keys in [q0, q1) are below t
+__device__ __forceinline__ int below(const i32x4* keys, int q0, int q1, int part, int32_t t) {
   int n = 0;
-  int64_t j = j0;
-  for (; j + 16 <= j1; j += 16) {
-    i32x4u x[4];
+#pragma unroll 8
+  for (int q = q0 + part; q < q1; q += kSortParts) {
+    const i32x4 x = keys[q];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const i32x4u*>(ids + j + 4 * u);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) n += key_of(x[u][e], V) < t;
+    for (int e = 0; e < 4; ++e) n += x[e] < t;
   }
-  for (; j < j1; ++j) n += key_of(ids[j], V) < t;
   return n;
 }
 
-__global__ void __launch_bounds__(256) token_sort_kernel(TokArgs a, int sort_blocks) {
-  __shared__ float tile[64][65];
-  if ((int)blockIdx.x < sort_blocks) {
-    // 32 ids a block; the eight half-waves share the comparisons of each
-    int* counts = reinterpret_cast<int*>(&tile[0][0]);  // [8][32]
-    const int at = threadIdx.x & 31, part = threadIdx.x >> 5;
-    const int64_t i0 = (int64_t)blockIdx.x * 32, i1 = i0 + 32 < a.N ? i0 + 32 : a.N;
-    const int64_t i = i0 + at;
-    const int32_t key = i < a.N ? key_of(a.ids[i], a.V) : 0;
-    const int64_t per = (a.N + 7) / 8, j0 = part * per, j1 = j0 + per < a.N ? j0 + per : a.N;
-    int n = 0;
-    if (j0 < j1) {
-      // before the block's ids an equal one counts, after them it does not
-      const int64_t a1 = j1 < i0 ? j1 : i0, b0 = j0 > i1 ? j0 : i1;
-      if (j0 < a1) n += below(a.ids, a.V, j0, a1, (int64_t)key + 1);
-      if (b0 < j1) n += below(a.ids, a.V, b0, j1, key);
-      for (int64_t j = j0 > i0 ? j0 : i0; j < (j1 < i1 ? j1 : i1); ++j) n += key_of(a.ids[j], a.V) < (int64_t)key + (j < i);
-    }
-    counts[part * 32 + at] = n;
-    __syncthreads();
-    if (part == 0 && i < a.N) {
-      int rank = 0;
+// Turns tile t of dY into dYt.
+__device__ __forceinline__ void turn_tile(const TokArgs& a, int64_t t, float (*tile)[TS]) {
+  const int64_t tiles = (a.N + 63) / 64, p0 = t % tiles * 64, d0 = t / tiles * 64;
+  const int four = 4 * (threadIdx.x & 15), one = threadIdx.x >> 4;
+  f32x4 x[4];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) rank += counts[q * 32 + at];
-      a.sid[rank] = key;
-      a.order[rank] = (int32_t)row_of(i, a.B, a.S, a.rows);
-    }
-    return;
+  for (int u = 0; u < 4; ++u) {
+    const int64_t d = d0 + one + 16 * u;
+    x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (d < a.D) x[u] = get4(a.dY + p0 + four + a.N * d, a.N - p0 - four);
   }
-  const int64_t t = (int64_t)blockIdx.x - sort_blocks, tiles = (a.N + 63) / 64;
-  const int64_t p0 = t % tiles * 64, d0 = t / tiles * 64;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
 #pragma unroll
-  for (int u = 0; u < 16; ++u) {
-    const int j = ty + 4 * u;
-    tile[j][tx] = p0 + tx < a.N && d0 + j < a.D ? a.dY[p0 + tx + a.N * (d0 + j)] : 0.f;
-  }
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[four + e][lane_of(four + e, one + 16 * u)] = x[u][e];  // [row][feature]
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < 16; ++u) {
-    const int64_t p = p0 + ty + 4 * u;
-    if (p < a.N && d0 + tx < a.Dp) a.dYt[p * a.Dp + d0 + tx] = tile[tx][ty + 4 * u];
+  for (int u = 0; u < 4; ++u) {
+    const int64_t p = p0 + one + 16 * u;
+    if (p < a.N && d0 + four < a.Dp)
+      *reinterpret_cast<f32x4*>(a.dYt + p * a.Dp + d0 + four) = *reinterpret_cast<const f32x4*>(&tile[one + 16 * u][lane_of(one + 16 * u, four)]);
+  }
+}
+
+// Zeros for those of a block's rows of the table that no id names.  The block
+// reads all ids; where they are many it takes more rows.
+__host__ __device__ __forceinline__ int zero_rows(int64_t N) {
+  return N <= 131072 ? 64 : N <= 1048576 ? 512 : 4096;
+}
+
+__device__ __forceinline__ void zero_unused(const TokArgs& a, int64_t blk, unsigned char* used) {
+  const int rows = zero_rows(a.N), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t v0 = blk * rows;
+  for (int r = 4 * threadIdx.x; r < rows; r += 1024) *reinterpret_cast<uint32_t*>(used + r) = 0;
+  __syncthreads();
+  int64_t j = 4 * threadIdx.x;
+#pragma unroll 8
+  for (; j + 4 <= a.N; j += 1024) {
+    const i32x4 x = *reinterpret_cast<const i32x4u*>(a.ids + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (x[e] >= v0 && x[e] < v0 + rows) used[x[e] - v0] = 1;
+  }
+  for (; j < a.N; ++j)
+    if (a.ids[j] >= v0 && a.ids[j] < v0 + rows) used[a.ids[j] - v0] = 1;
+  __syncthreads();
+  for (int r = wave; r < rows && v0 + r < a.V; r += 4) {
+    if (used[r]) continue;
+    float* g = a.gWt + a.D * (v0 + r);
+    for (int64_t d = 4 * lane; d < a.D; d += 256) put4(g + d, a.D - d, f32x4{0.f, 0.f, 0.f, 0.f});
+  }
+}
+
+__global__ void __launch_bounds__(256) token_sort_kernel(TokArgs a, int sort_blocks, int zero_blocks) {
+  __shared__ __align__(16) int32_t lds[kIdChunk];  // ids, or a tile of dY
+  static_assert(sizeof(lds) >= 64 * TS * sizeof(float), "a tile fits");
+  if ((int)blockIdx.x >= sort_blocks) {
+    const int64_t blk = (int64_t)blockIdx.x - sort_blocks;
+    if (blk < zero_blocks) zero_unused(a, blk, reinterpret_cast<unsigned char*>(lds));
+    else turn_tile(a, blk - zero_blocks, reinterpret_cast<float (*)[TS]>(lds));
+    return;
+  }
+  const int at = threadIdx.x % kSortIds, part = threadIdx.x / kSortIds;
+  const int N = (int)a.N, i0 = (int)blockIdx.x * kSortIds, i = i0 + at;
+  const int32_t key = i < N ? key_of(a.ids[i], a.V) : 0;
+  int n = 0;
+  for (int c0 = 0; c0 < N; c0 += kIdChunk) {
+    const int m = N - c0 < kIdChunk ? N - c0 : kIdChunk, m4 = (m + 3) / 4 * 4;
+    __syncthreads();
+#pragma unroll 8
+    for (int j = 4 * threadIdx.x; j < m4; j += 1024) {
+      i32x4 x;
+      if (j + 4 <= m) {
+        x = *reinterpret_cast<const i32x4u*>(a.ids + c0 + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = key_of(x[e], a.V);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = j + e < m ? key_of(a.ids[c0 + j + e], a.V) : INT32_MAX;
+      }
+      *reinterpret_cast<i32x4*>(lds + j) = x;
+    }
+    __syncthreads();
+    // before the block's ids an equal one counts, after them it does not
+    const int lo = min(max(i0 - c0, 0), m4), hi = min(max(i0 + kSortIds - c0, 0), m4);
+    const i32x4* fours = reinterpret_cast<const i32x4*>(lds);
+    n += below(fours, 0, lo / 4, part, key + 1);  // key + 1 <= V + 1 <= INT32_MAX
+    n += below(fours, hi / 4, m4 / 4, part, key);
+    if (lo + part < hi) n += lds[lo + part] < key + (c0 + lo + part < i);
+  }
+  __syncthreads();
+  lds[part * kSortIds + at] = n;
+  __syncthreads();
+  if (part == 0 && i < N) {
+    int rank = 0;
+#pragma unroll
+    for (int q = 0; q < kSortParts; ++q) rank += lds[q * kSortIds + at];
+    a.sid[rank] = key;
+    a.order[rank] = (int32_t)row_of(i, a.B, a.S, a.rows);
+  }
+}
+
+// The radix sort: eight bits a pass, from the lowest; a block counts, then
+// moves, kRadixTile keys, each of its four waves a run of them, 64 at a time,
+// so equal digits keep their order.
+constexpr int kRadixTile = 4096;
+
+struct RadixArgs {
+  const int32_t *key_in, *row_in;  // null in the first pass: the ids and their rows
+  int32_t *key_out, *row_out;
+  int32_t* counts;                 // [256][blocks], then their exclusive sums
+  int shift, blocks;
+};
+
+__device__ __forceinline__ int32_t radix_key(const TokArgs& a, const RadixArgs& r, int64_t i) {
+  return r.key_in ? r.key_in[i] : key_of(a.ids[i], a.V);
+}
+
+__global__ void __launch_bounds__(256) token_radix_count_kernel(TokArgs a, RadixArgs r, int zero_blocks, int turn_blocks) {
+  __shared__ __align__(16) float tile[64][TS];
+  if ((int)blockIdx.x < zero_blocks + turn_blocks) {  // in the first pass
+    if ((int)blockIdx.x < zero_blocks) zero_unused(a, blockIdx.x, reinterpret_cast<unsigned char*>(tile));
+    else turn_tile(a, (int64_t)blockIdx.x - zero_blocks, tile);
+    return;
+  }
+  int32_t* hist = reinterpret_cast<int32_t*>(tile);
+  const int blk = (int)blockIdx.x - zero_blocks - turn_blocks;
+  hist[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blk * kRadixTile;
+  for (int j = threadIdx.x; j < kRadixTile; j += 256)
+    if (i0 + j < a.N) atomicAdd(&hist[radix_key(a, r, i0 + j) >> r.shift & 255], 1);
+  __syncthreads();
+  r.counts[(int64_t)threadIdx.x * r.blocks + blk] = hist[threadIdx.x];
+}
+
+// exclusive sums over counts in place (one block)
+__global__ void __launch_bounds__(1024) token_radix_scan_kernel(RadixArgs r) {
+  __shared__ int32_t wave_sum[16];
+  const int64_t total = (int64_t)256 * r.blocks, per = (total + 1023) / 1024;
+  const int64_t lo = min(total, (int64_t)threadIdx.x * per), hi = min(total, lo + per);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t s = 0;
+#pragma unroll 8
+  for (int64_t i = lo; i < hi; ++i) s += r.counts[i];
+  int32_t x = s;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int32_t y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) wave_sum[wave] = x;
+  __syncthreads();
+  int32_t run = x - s;
+  for (int w = 0; w < wave; ++w) run += wave_sum[w];
+  for (int64_t i = lo; i < hi; ++i) {
+    const int32_t c = r.counts[i];
+    r.counts[i] = run;
+    run += c;
+  }
+}
+
+__global__ void __launch_bounds__(256) token_radix_move_kernel(TokArgs a, RadixArgs r) {
+  __shared__ int32_t at[4][256];  // where a wave's next key of a digit goes
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t i0 = (int64_t)blockIdx.x * kRadixTile + wave * (kRadixTile / 4);
+  for (int w = 0; w < 4; ++w) at[w][threadIdx.x] = 0;
+  __syncthreads();
+  for (int j = lane; j < kRadixTile / 4; j += 64)
+    if (i0 + j < a.N) atomicAdd(&at[wave][radix_key(a, r, i0 + j) >> r.shift & 255], 1);
+  __syncthreads();
+  {
+    int32_t run = r.counts[(int64_t)threadIdx.x * r.blocks + blockIdx.x];
+    for (int w = 0; w < 4; ++w) {
+      const int32_t c = at[w][threadIdx.x];
+      at[w][threadIdx.x] = run;
+      run += c;
+    }
+  }
+  __syncthreads();
+  for (int j = 0; j < kRadixTile / 4; j += 64) {
+    const int64_t i = i0 + j + lane;
+    const bool in = i < a.N;
+    const int32_t key = in ? radix_key(a, r, i) : 0;
+    const int digit = key >> r.shift & 255;
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const uint64_t set = __ballot(digit >> b & 1);
+      same &= digit >> b & 1 ? set : ~set;
+    }
+    const int before = __popcll(same & (((uint64_t)1 << lane) - 1));
+    const int32_t base = at[wave][digit];
+    // every lane has its digit's place before the first of them moves it on
+    __builtin_amdgcn_wave_barrier();
+    if (in && before == 0) at[wave][digit] = base + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    if (in) {
+      r.key_out[base + before] = key;
+      r.row_out[base + before] = r.row_in ? r.row_in[i] : (int32_t)row_of(i, a.B, a.S, a.rows);
+    }
   }
 }
 
@@ -158,44 +354,14 @@ __global__ void __launch_bounds__(256) token_sort_kernel(TokArgs a, int sort_blo
 __device__ __forceinline__ void put(const TokArgs& a, int64_t v, int64_t d, f32x4 x) {
   float* g = a.gWt + a.D * v + d;
   x *= a.scale;
-  if (d + 4 <= a.D) {
-    if (a.accumulate) x += *reinterpret_cast<const f32x4u*>(g);
-    *reinterpret_cast<f32x4u*>(g) = x;
-  } else {
-    for (int e = 0; e < 4; ++e)
-      if (d + e < a.D) g[e] = a.accumulate ? g[e] + x[e] : x[e];
-  }
+  if (a.accumulate) x += get4(g, a.D - d);
+  put4(g, a.D - d, x);
 }
 
-// blocks [0, zero_blocks): zeros for the table's rows that no id names, a wave
-// for 64 rows; then a wave for each chunk and 256 features.
-__global__ void __launch_bounds__(256) token_sum_kernel(TokArgs a, int zero_blocks, int cols) {
+// A wave for each chunk and 256 features.
+__global__ void __launch_bounds__(256) token_sum_kernel(TokArgs a, int cols) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if ((int)blockIdx.x < zero_blocks) {
-    const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 64;
-    if (v0 >= a.V) return;
-    const int64_t v = v0 + lane;
-    int64_t lo = 0, hi = a.N;  // first sorted id that is not below v
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (a.sid[mid] < v) lo = mid + 1;
-      else hi = mid;
-    }
-    uint64_t unused = __ballot(v < a.V && (lo == a.N || a.sid[lo] != v));
-    while (unused) {
-      const int u = __ffsll((unsigned long long)unused) - 1;
-      unused &= unused - 1;
-      float* g = a.gWt + a.D * (v0 + u);
-      for (int64_t d = 4 * lane; d < a.D; d += 256) {
-        if (d + 4 <= a.D) *reinterpret_cast<f32x4u*>(g + d) = f32x4{0.f, 0.f, 0.f, 0.f};
-        else
-          for (int e = 0; e < 4; ++e)
-            if (d + e < a.D) g[d + e] = 0.f;
-      }
-    }
-    return;
-  }
-  const int64_t w = ((int64_t)blockIdx.x - zero_blocks) * 4 + wave;
+  const int64_t w = (int64_t)blockIdx.x * 4 + wave;
   const int c = (int)(w / cols);
   if (c >= a.chunks) return;
   const int64_t d = (w % cols) * 256 + 4 * lane;
@@ -241,13 +407,15 @@ __global__ void __launch_bounds__(64) token_join_kernel(TokArgs a) {
   const int32_t v = a.sid[last];
   if (v >= a.V || a.sid[last + 1] != v) return;
   if (last >= kChunk && a.sid[last - kChunk] == v) return;  // it began before this chunk
-  int64_t lo = last + 1, hi = a.N;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (a.sid[mid] <= v) lo = mid + 1;
-    else hi = mid;
+  // the chunk it ends in: the first whose next entry is another's, 64 at a time
+  int end = c + 1;
+  for (;; end += 64) {
+    const int64_t next = ((int64_t)end + threadIdx.x + 1) * kChunk;
+    const uint64_t ends = __ballot(next >= a.N || a.sid[next] != v);
+    if (!ends) continue;
+    end += __ffsll((unsigned long long)ends) - 1;
+    break;
   }
-  const int end = (int)((lo - 1) / kChunk);
   const int64_t d = (int64_t)blockIdx.y * 256 + 4 * threadIdx.x;
   if (d >= a.Dp) return;
   f32x4 s = *reinterpret_cast<const f32x4*>(a.part + ((int64_t)c * 2 + 1) * a.Dp + d);
@@ -261,7 +429,7 @@ int check_args(const char* who, int64_t B, int64_t S, int64_t V, int64_t D, floa
                 (long long)S, (long long)V, (long long)D);
   CNHIP_REQUIRE(rows == CNHIP_ROWS_REF || rows == CNHIP_ROWS_BY_SAMPLE, "%s: bad row order %d", who, rows);
   CNHIP_REQUIRE(std::isfinite(scale), "%s: scale is not finite", who);
-  CNHIP_REQUIRE(V < ((int64_t)1 << 31) && B < ((int64_t)1 << 30) && S < ((int64_t)1 << 30) &&
+  CNHIP_REQUIRE(V < ((int64_t)1 << 31) - 1 && B < ((int64_t)1 << 30) && S < ((int64_t)1 << 30) &&
                     B * S < ((int64_t)1 << 30),
                 "%s: too many ids or rows", who);
   CNHIP_REQUIRE(D <= 64 * 65535, "%s: embed_dim too large", who);
@@ -308,29 +476,57 @@ int cnhip_token_embedding_backward(const int32_t* ids, const float* dY, float* g
   a.accumulate = accumulate;
   a.scale = scale;
   a.chunks = (int)((a.N + cnhip::kChunk - 1) / cnhip::kChunk);
-  const int64_t tiles = (a.N + 63) / 64 * ((D + 63) / 64), sort_blocks = (a.N + 31) / 32;
+  const int64_t tiles = (a.N + 63) / 64 * ((D + 63) / 64);
+  const bool radix = a.N > cnhip::kRankMost;
+  const int64_t sort_blocks = radix ? (a.N + cnhip::kRadixTile - 1) / cnhip::kRadixTile
+                                    : (a.N + cnhip::kSortIds - 1) / cnhip::kSortIds;
   const int cols = (int)((a.Dp + 255) / 256);
-  const int64_t zero_blocks = accumulate ? 0 : (V + 255) / 256, sum_blocks = ((int64_t)a.chunks * cols + 3) / 4;
-  CNHIP_REQUIRE(tiles + sort_blocks < ((int64_t)1 << 31) && zero_blocks + sum_blocks < ((int64_t)1 << 31),
+  const int zr = cnhip::zero_rows(a.N);
+  const int64_t zero_blocks = accumulate ? 0 : (V + zr - 1) / zr, sum_blocks = ((int64_t)a.chunks * cols + 3) / 4;
+  CNHIP_REQUIRE(tiles + sort_blocks + zero_blocks < ((int64_t)1 << 31) && sum_blocks < ((int64_t)1 << 31),
                 "%s: too large", who);
   const size_t rows_bytes = (size_t)(a.N * a.Dp) * sizeof(float);
   const size_t part_bytes = (size_t)a.chunks * 2 * (size_t)a.Dp * sizeof(float);
-  const size_t ints = (size_t)a.N * sizeof(int32_t);
+  const size_t ints = (size_t)a.N * sizeof(int32_t), counts = (size_t)sort_blocks * 256 * sizeof(int32_t);
   void* ws = nullptr;
-  CNHIP_TRY(cnhip::scratch(st, cnhip::kScratchLayer, rows_bytes + part_bytes + 2 * ints, &ws, who));
+  CNHIP_TRY(cnhip::scratch(st, cnhip::kScratchLayer, rows_bytes + part_bytes + (radix ? 4 * ints + counts : 2 * ints), &ws,
+                           who));
   a.dYt = static_cast<float*>(ws);
   a.part = a.dYt + a.N * a.Dp;
   a.sid = reinterpret_cast<int32_t*>(a.part + (int64_t)a.chunks * 2 * a.Dp);
   a.order = a.sid + a.N;
-  hipLaunchKernelGGL(cnhip::token_sort_kernel, dim3((unsigned)(sort_blocks + tiles)), dim3(256), 0, st, a,
-                     (int)sort_blocks);
-  CNHIP_TRY(cnhip::check_launch(who));
+  if (!radix) {
+    hipLaunchKernelGGL(cnhip::token_sort_kernel, dim3((unsigned)(sort_blocks + zero_blocks + tiles)), dim3(256), 0, st, a,
+                       (int)sort_blocks, (int)zero_blocks);
+    CNHIP_TRY(cnhip::check_launch(who));
+  } else {
+    int bits = 1;
+    while (((int64_t)1 << bits) <= V) ++bits;  // keys are 0 .. V
+    const int passes = (bits + 7) / 8;
+    int32_t* pair[2][2] = {{a.sid, a.order}, {a.order + a.N, a.order + 2 * a.N}};
+    cnhip::RadixArgs r{nullptr, nullptr, nullptr, nullptr, a.order + 3 * a.N, 0, (int)sort_blocks};
+    for (int pass = 0; pass < passes; ++pass) {
+      int32_t** to = pair[(passes - 1 - pass) & 1];  // the last pass ends in sid and order
+      r.key_out = to[0];
+      r.row_out = to[1];
+      r.shift = 8 * pass;
+      const int64_t zero = pass == 0 ? zero_blocks : 0, turn = pass == 0 ? tiles : 0;
+      hipLaunchKernelGGL(cnhip::token_radix_count_kernel, dim3((unsigned)(zero + turn + sort_blocks)), dim3(256), 0, st,
+                         a, r, (int)zero, (int)turn);
+      CNHIP_TRY(cnhip::check_launch(who));
+      hipLaunchKernelGGL(cnhip::token_radix_scan_kernel, dim3(1), dim3(1024), 0, st, r);
+      CNHIP_TRY(cnhip::check_launch(who));
+      hipLaunchKernelGGL(cnhip::token_radix_move_kernel, dim3((unsigned)sort_blocks), dim3(256), 0, st, a, r);
+      CNHIP_TRY(cnhip::check_launch(who));
+      r.key_in = to[0];
+      r.row_in = to[1];
+    }
+  }
   {
     // every row's gradient read once, every row of the table that is written
     cnhip::HbmTimer timer("token_sum_kernel",
                           4.0 * (double)a.N * (double)D + (accumulate ? 8.0 * (double)a.N : 4.0 * (double)V) * (double)D, st);
-    hipLaunchKernelGGL(cnhip::token_sum_kernel, dim3((unsigned)(zero_blocks + sum_blocks)), dim3(256), 0, st, a,
-                       (int)zero_blocks, cols);
+    hipLaunchKernelGGL(cnhip::token_sum_kernel, dim3((unsigned)sum_blocks), dim3(256), 0, st, a, cols);
     CNHIP_TRY(cnhip::check_launch(who));
   }
   hipLaunchKernelGGL(cnhip::token_join_kernel, dim3((unsigned)a.chunks, (unsigned)cols), dim3(64), 0, st, a);

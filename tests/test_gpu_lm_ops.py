@@ -58,6 +58,9 @@ EMB = [  # B, S, V, D, ids, rows
     (3, 5, 7, 33, "padded", SAMPLE), (4, 64, 50, 512, "uniform", SAMPLE), (2, 257, 300, 130, "zipf", REF),
     (5, 401, 3, 66, "uniform", SAMPLE), (7, 300, 5000, 257, "same", SAMPLE), (2, 1024, 999, 40, "padded", SAMPLE),
     (1, 77, 40, 1000, "none", REF), (33, 31, 1025, 3, "zipf", SAMPLE),
+    (3, 4100, 600, 36, "zipf", REF),  # more ids than one piece of the comparing sort
+    (9, 4096, 70000, 36, "zipf", SAMPLE), (5, 8000, 200, 20, "padded", REF), (4, 10007, 65535, 6, "uniform", SAMPLE),
+    (1, 33000, 2, 5, "same", REF),    # the radix sort, one to three passes
 ]
 
 
