@@ -496,8 +496,8 @@ __global__ void __launch_bounds__(NT) att_dkv_kernel(AttArgs a) {
 // probabilities and their gradients are split into their two terms in the
 // registers and multiplied without leaving them.
 //
-// Scales.  Each operand has one power of two per sample and key head (over the
-// heads that share it).  Probabilities are at most 1 and enter times 2^14.
+// Scales.  Each operand has one power of two per head of a sample.
+// Probabilities are at most 1 and enter times 2^14.
 // dS = P (dP - delta) is bounded by 2 max ||dout_i|| max ||v_j||, whose power
 // of two scales it.
 struct Scale {
@@ -508,9 +508,8 @@ struct Scale {
 struct PackArgs {
   Seq<const float> x[4];  // q, k, v, dout
   char* p[4];
-  Scale* part[4];         // [B][kv_heads][slots]
-  int slots[4], chunks[4], chunk_rows[4], blocks[4];
-  int steps;              // of 16 features
+  Scale* part[4];         // [head of a sample][chunks]
+  int chunks[4], chunk_rows[4], blocks[4];
 };
 
 struct PairArgs {
@@ -519,14 +518,15 @@ struct PairArgs {
   float *dk_part, *dv_part;  // [B][heads][dh][Sk], where heads share keys
 };
 
-// The operand's scale over its slots, the same in every lane.
-__device__ __forceinline__ Scale scale_of(const PackArgs& p, int which, int64_t bkh) {
+// The scale of a head (of a sample) over its chunks, the same in every lane.
+__device__ __forceinline__ Scale scale_of(const PackArgs& p, int which, int64_t bh) {
   uint32_t m = 0;
   float n = 0.f;
-  for (int i = threadIdx.x & 63; i < p.slots[which]; i += 64) {
-    const Scale s = p.part[which][bkh * p.slots[which] + i];
-    m = max(m, s.largest);
-    n = fmaxf(n, s.norm);
+  const int i = threadIdx.x & 63;
+  if (i < p.chunks[which]) {
+    const Scale s = p.part[which][bh * p.chunks[which] + i];
+    m = s.largest;
+    n = s.norm;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -542,107 +542,155 @@ __device__ __forceinline__ int rows_of(const AttArgs& a, int which, int b) {
   return which == 1 || which == 2 ? keys_of(a, b) : a.Sq;
 }
 
-// The scale of a chunk of rows of one head: a wave per 32 rows, four a block.
-template <int OPS>
+// The head of operand `which` that block (.., y, z) of a packing launch has;
+// false where the operand has fewer heads.
+struct Operand {
+  int which, b, head;
+  int64_t bh;  // head of a sample, counted through
+  int rows;
+};
+__device__ __forceinline__ bool operand_of(const AttArgs& a, Operand& o) {
+  o.which = (int)blockIdx.z;
+  const int heads = o.which == 1 || o.which == 2 ? a.kv_heads : a.heads;
+  o.b = (int)blockIdx.y / a.heads;
+  o.head = (int)blockIdx.y % a.heads;
+  o.bh = (int64_t)o.b * heads + o.head;
+  o.rows = rows_of(a, o.which, o.b);
+  return o.head < heads;
+}
+
+// 32 rows of a head in a wave's registers: features 16 s + 8 (lane / 32) .. + 7 of
+// row lane % 32 in v[s], zeros where there are none.
+template <int KS>
+struct RowBlock {
+  float v[KS][8];
+  __device__ __forceinline__ void load(const AttArgs& a, const PackArgs& p, const Operand& o, int blk) {
+    const int lane = (int)threadIdx.x & 63, r = blk * 32 + (lane & 31), d0 = 8 * (lane >> 5);
+    const bool held = r < o.rows;
+    const Seq<const float>& x = p.x[o.which];
+    const float* q = x.at(o.b, held ? r : 0, (int64_t)o.head * a.dh);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[s][e] = held && 16 * s + d0 + e < a.dh ? q[(16 * s + d0 + e) * x.col] : 0.f;
+  }
+  // the largest finite value, and the largest row's norm, of the whole wave
+  __device__ __forceinline__ Scale scale(int dh) const {
+    uint32_t m = 0;
+    float n = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t bits = pr::finite_bits(v[s][e]);
+        m = max(m, bits);
+        n = fmaf(__uint_as_float(bits), __uint_as_float(bits), n);
+      }
+    n += other_half(n);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+      n = fmaxf(n, __shfl_xor(n, o, 64));
+    }
+    // squares that leave the range: the bound by the largest value
+    return Scale{m, n > 1e-30f && n < 1e37f ? sqrtf(n) : __uint_as_float(m) * sqrtf((float)dh)};
+  }
+  __device__ __forceinline__ void pack(const PackArgs& p, const Operand& o, int blk, float f) const {
+    const int lane = (int)threadIdx.x & 63;
+    char* q = p.p[o.which] + (o.bh * p.blocks[o.which] + blk) * KS * (2 * pr::kFrag);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      pr::u32x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t w0, w1;
+        pr::split2(v[s][2 * e] * f, v[s][2 * e + 1] * f, w0, w1);
+        hi[e] = w0;
+        lo[e] = w1;
+      }
+      char* at = q + s * (2 * pr::kFrag) + pr::slot(lane, s);
+      *reinterpret_cast<pr::u32x4*>(at) = hi;
+      *reinterpret_cast<pr::u32x4*>(at + pr::kFrag) = lo;
+    }
+  }
+  // delta of the rows, these being dout's
+  __device__ __forceinline__ void delta(const AttArgs& a, const Operand& o, int blk) const {
+    const int lane = (int)threadIdx.x & 63, r = blk * 32 + (lane & 31), d0 = 8 * (lane >> 5);
+    const bool held = r < o.rows;
+    const float* q = a.o.at(o.b, held ? r : 0, (int64_t)o.head * a.dh);
+    float x[KS][8], d = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[s][e] = held && 16 * s + d0 + e < a.dh ? q[(16 * s + d0 + e) * a.o.col] : 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d = fmaf(v[s][e], x[s][e], d);
+    d += other_half(d);
+    if (held && lane < 32) a.delta[o.bh * a.Sq + r] = d;
+  }
+};
+
+// Short sequences, up to 32 rows a wave in one block: scale and packing of a
+// head with one reading.
+template <int KS>
+__global__ void __launch_bounds__(1024) att_pack_head_kernel(PairArgs g) {
+  __shared__ Scale part[16];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
+  Operand o;
+  if (!operand_of(g.a, o)) return;
+  RowBlock<KS> x;
+  x.load(g.a, g.p, o, wave);
+  Scale s = x.scale(g.a.dh);
+  if (lane == 0) part[wave] = s;
+  __syncthreads();
+  for (int w = 0; w < waves; ++w) {
+    s.largest = max(s.largest, part[w].largest);
+    s.norm = fmaxf(s.norm, part[w].norm);
+  }
+  if (threadIdx.x == 0) g.p.part[o.which][o.bh] = s;
+  if (wave >= g.p.blocks[o.which]) return;
+  x.pack(g.p, o, wave, pr::exp2i(pr::scale_exp(s.largest)));
+  if (o.which == 3) x.delta(g.a, o, wave);
+}
+
+// Longer ones: the scale of a chunk of rows of a head, then the packing, a wave
+// per 32 rows in both.
+template <int KS>
 __global__ void __launch_bounds__(NT) att_scale_kernel(PairArgs g) {
   __shared__ Scale part[4];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const int which = (int)blockIdx.z;
-  if (which >= OPS) return;
-  const AttArgs& a = g.a;
-  const bool kv = which == 1 || which == 2;
-  const int heads = kv ? a.kv_heads : a.heads;
-  const int b = (int)blockIdx.y / a.heads, head = (int)blockIdx.y % a.heads;
-  if (head >= heads || (int)blockIdx.x >= g.p.chunks[which]) return;
-  const int rows = rows_of(a, which, b);
-  const Seq<const float>& x = g.p.x[which];
-  uint32_t m = 0;
-  float norm = 0.f;
-  const int c0 = (int)blockIdx.x * g.p.chunk_rows[which];
-  for (int r0 = c0 + 32 * wave; r0 < c0 + g.p.chunk_rows[which] && r0 < rows; r0 += 128) {
-    const int r = r0 + (lane & 31);
-    float s = 0.f;
-    if (r < rows) {
-      const float* p = x.at(b, r, (int64_t)head * a.dh);
-      for (int d = lane >> 5; d < a.dh; d += 16) {
-        float v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = d + 2 * u < a.dh ? p[(d + 2 * u) * x.col] : 0.f;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const uint32_t bits = pr::finite_bits(v[u]);
-          m = max(m, bits);
-          s = fmaf(__uint_as_float(bits), __uint_as_float(bits), s);
-        }
-      }
-    }
-    s += other_half(s);
-    norm = fmaxf(norm, s);
+  Operand o;
+  if (!operand_of(g.a, o) || (int)blockIdx.x >= g.p.chunks[o.which]) return;
+  Scale s{0u, 0.f};
+  const int per = g.p.chunk_rows[o.which] / 32;
+  for (int blk = (int)blockIdx.x * per + wave; blk < ((int)blockIdx.x + 1) * per && blk * 32 < o.rows; blk += 4) {
+    RowBlock<KS> x;
+    x.load(g.a, g.p, o, blk);
+    const Scale t = x.scale(g.a.dh);
+    s.largest = max(s.largest, t.largest);
+    s.norm = fmaxf(s.norm, t.norm);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-    norm = fmaxf(norm, __shfl_xor(norm, o, 64));
-  }
-  // squares that leave the range: the bound by the largest value
-  if (lane == 0)
-    part[wave] = Scale{m, norm > 1e-30f && norm < 1e37f ? sqrtf(norm) : __uint_as_float(m) * sqrtf((float)a.dh)};
+  if (lane == 0) part[wave] = s;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  Scale s = part[0];
   for (int w = 1; w < 4; ++w) {
     s.largest = max(s.largest, part[w].largest);
     s.norm = fmaxf(s.norm, part[w].norm);
   }
-  const int kh = kv ? head : head / a.group, slot = (kv ? 0 : head % a.group) * g.p.chunks[which] + (int)blockIdx.x;
-  g.p.part[which][((int64_t)b * a.kv_heads + kh) * g.p.slots[which] + slot] = s;
+  g.p.part[o.which][o.bh * g.p.chunks[o.which] + blockIdx.x] = s;
 }
 
-// A wave packs 32 rows of one head; of dout it also leaves delta.
-template <int OPS>
+template <int KS>
 __global__ void __launch_bounds__(NT) att_pack_kernel(PairArgs g) {
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, h = lane >> 5;
-  const int which = (int)blockIdx.z;
-  if (which >= OPS) return;
-  const AttArgs& a = g.a;
-  const bool kv = which == 1 || which == 2;
-  const int heads = kv ? a.kv_heads : a.heads;
-  const int b = (int)blockIdx.y / a.heads, head = (int)blockIdx.y % a.heads;
-  const int blk = (int)blockIdx.x * 4 + wave;
-  if (head >= heads || blk >= g.p.blocks[which]) return;
-  const int kh = kv ? head : head / a.group;
-  const float f = pr::exp2i(pr::scale_exp(scale_of(g.p, which, (int64_t)b * a.kv_heads + kh).largest));
-  const int rows = rows_of(a, which, b), r = blk * 32 + (lane & 31);
-  const bool held = r < rows;
-  const Seq<const float>& x = g.p.x[which];
-  const float* p = x.at(b, held ? r : 0, (int64_t)head * a.dh);
-  const float* o = which == 3 ? a.o.at(b, held ? r : 0, (int64_t)head * a.dh) : nullptr;
-  char* q = g.p.p[which] + (((int64_t)b * heads + head) * g.p.blocks[which] + blk) * g.p.steps * (2 * pr::kFrag);
-  float delta = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < g.p.steps; ++s) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = 16 * s + 8 * h + e;
-      v[e] = held && d < a.dh ? p[d * x.col] : 0.f;
-      if (which == 3 && held && d < a.dh) delta = fmaf(v[e], o[d * a.o.col], delta);
-    }
-    pr::u32x4 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t w0, w1;
-      pr::split2(v[2 * e] * f, v[2 * e + 1] * f, w0, w1);
-      hi[e] = w0;
-      lo[e] = w1;
-    }
-    char* at = q + s * (2 * pr::kFrag) + pr::slot(lane, s);
-    *reinterpret_cast<pr::u32x4*>(at) = hi;
-    *reinterpret_cast<pr::u32x4*>(at + pr::kFrag) = lo;
-  }
-  if (which != 3) return;
-  delta += other_half(delta);
-  if (held && h == 0) a.delta[((int64_t)b * a.heads + head) * a.Sq + r] = delta;
+  Operand o;
+  const int blk = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+  if (!operand_of(g.a, o) || blk >= g.p.blocks[o.which]) return;
+  RowBlock<KS> x;
+  x.load(g.a, g.p, o, blk);
+  x.pack(g.p, o, blk, pr::exp2i(pr::scale_exp(scale_of(g.p, o.which, o.bh).largest)));
+  if (o.which == 3) x.delta(g.a, o, blk);
 }
 
 // This block's head of a sample and 128 rows of it.  The longest go first (a
@@ -678,97 +726,141 @@ struct RowFrags {
   }
 };
 
-// acc (rows of the tile x rows of the lanes) = tile x^T over the features
-template <int KS>
-__device__ __forceinline__ f32x16 dot_pairs(const char* tile, const RowFrags<KS>& x) {
+// acc[x] (rows of a tile x rows of the lanes) = tile[x] row[x]^T over the
+// features, for NX pairs of operands at once.  pair(0 .. 7) is called in
+// between, for work on the registers of another tile: a MFMA keeps the matrix
+// pipe for 32 cycles and the wave for 4, so that work runs beside them.
+template <int KS, int NX, class F>
+__device__ __forceinline__ void dot_pairs(const char* const (&tile)[NX], const RowFrags<KS>* const (&row)[NX],
+                                          f32x16 (&acc)[NX], F&& pair) {
   const int lane = (int)threadIdx.x & 63;
-  f32x16 acc = {};
+  pr::f16x8 f[2][NX][2];
+  auto read = [&](int s) {
+#pragma unroll
+    for (int x = 0; x < NX; ++x)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        f[s & 1][x][q] =
+            *reinterpret_cast<const pr::f16x8*>(tile[x] + (2 * s + q) * pr::kFrag + pr::slot(lane, s));
+  };
+  read(0);
+#pragma unroll
+  for (int x = 0; x < NX; ++x) acc[x] = f32x16{};
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    const char* p = tile + 2 * s * pr::kFrag + pr::slot(lane, s);
-    const pr::f16x8 a0 = *reinterpret_cast<const pr::f16x8*>(p);
-    const pr::f16x8 a1 = *reinterpret_cast<const pr::f16x8*>(p + pr::kFrag);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, x.x[s][0], acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, x.x[s][1], acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, x.x[s][0], acc, 0, 0, 0);
+    if (s + 1 < KS) read(s + 1);
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+        acc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[s & 1][x][u == 0], row[x]->x[s][u == 1], acc[x], 0, 0, 0);
+#pragma unroll
+    for (int p = 8 * s / KS; p < 8 * (s + 1) / KS; ++p) pair(p);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  return acc;
 }
 
 // A score tile's registers as the B operand of two steps of 16 rows, in terms.
 struct TileFrags {
-  pr::f16x8 x[2][2];
-  __device__ __forceinline__ void split(const f32x16& p) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      pr::u32x4 hi, lo;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t w0, w1;
-        pr::split2(p[8 * t + 2 * e], p[8 * t + 2 * e + 1], w0, w1);
-        hi[e] = w0;
-        lo[e] = w1;
-      }
-      x[t][0] = __builtin_bit_cast(pr::f16x8, hi);
-      x[t][1] = __builtin_bit_cast(pr::f16x8, lo);
-    }
+  pr::u32x4 w[2][2];
+  // registers 2 p and 2 p + 1
+  __device__ __forceinline__ void split(int p, float a, float b) {
+    uint32_t w0, w1;
+    pr::split2(a, b, w0, w1);
+    w[p / 4][0][p % 4] = w0;
+    w[p / 4][1][p % 4] = w1;
   }
+  __device__ __forceinline__ pr::f16x8 at(int t, int q) const { return __builtin_bit_cast(pr::f16x8, w[t][q]); }
 };
 
-// acc (features x rows of the lanes) += tile^T p over the rows of the tile.
-// Element i of half-wave h in p's step t is row 16 t + 8 (i / 4) + 4 h + i % 4.
-template <int KS>
-__device__ __forceinline__ void add_pairs(const char* tile, const TileFrags& p, f32x16 (&acc)[KS / 2]) {
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const int lane = (int)threadIdx.x & 63, j = lane & 15, g = lane >> 4 & 1, half = (j & 3) >> 1;
-  const int row = 4 * (lane >> 5) + (j >> 2), turn = half * 4 + g * 8;
-  const char* base = tile + g * (2 * pr::kFrag) + half * 512 + (j & 1) * 8;
-  auto frag = [&](int i, int t, int q) {
-    const char* at = base + 2 * i * (2 * pr::kFrag) + q * pr::kFrag + t * 256;
+// Products along a tile's rows: acc[x] (features x rows of the lanes) += tile[x]^T
+// p[x], for NX operands at once.  Element i of half-wave h in half t of p is row
+// 16 t + 8 (i / 4) + 4 h + i % 4.  The work goes in groups of two blocks of 32
+// features (successive MFMAs then do not depend on each other), half 0 of all
+// operands before half 1; a group's fragments are read during the one before.
+// beside(g) is called in group g, for work on other registers.
+template <int KS, int NX>
+struct Adder {
+  static constexpr int W = KS / 2, G = (W + 1) / 2;  // feature blocks, and groups of two
+  static constexpr int GROUPS = 2 * NX * G, HALF = NX * G;
+  pr::f16x8 f[2][2][2];
+
+  __device__ __forceinline__ static pr::f16x8 frag(const char* tile, int i, int t, int q) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int lane = (int)threadIdx.x & 63, j = lane & 15, g = lane >> 4 & 1, half = (j & 3) >> 1;
+    const int row = 4 * (lane >> 5) + (j >> 2), turn = half * 4 + g * 8;
+    const char* at = tile + g * (2 * pr::kFrag) + half * 512 + (j & 1) * 8 + t * 256 + 2 * i * (2 * pr::kFrag) + q * pr::kFrag;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + (row ^ turn) * 16));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + ((row + 8) ^ turn) * 16));
     return __builtin_bit_cast(pr::f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  };
+  }
+  __device__ __forceinline__ void read(const char* const (&tile)[NX], int g) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    pr::f16x8 a[KS / 2][2];
+    for (int x = 0; x < 2; ++x)
+      if (2 * (g % G) + x < W)
 #pragma unroll
-    for (int i = 0; i < KS / 2; ++i)
+        for (int q = 0; q < 2; ++q) f[g & 1][x][q] = frag(tile[g / G % NX], 2 * (g % G) + x, g / HALF, q);
+  }
+  // after read(tile, 0)
+  template <class F>
+  __device__ __forceinline__ void run(const char* const (&tile)[NX], const TileFrags* const (&p)[NX],
+                                      f32x16 (*const (&acc)[NX])[W], F&& beside) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) a[i][q] = frag(i, t, q);
+    for (int g = 0; g < GROUPS; ++g) {
+      if (g + 1 < GROUPS) read(tile, g + 1);
 #pragma unroll
-    for (int u = 0; u < 3; ++u)
+      for (int u = 0; u < 3; ++u)
 #pragma unroll
-      for (int i = 0; i < KS / 2; ++i)
-        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][u == 0], p.x[t][u == 1], acc[i], 0, 0, 0);
+        for (int x = 0; x < 2; ++x) {
+          const int i = 2 * (g % G) + x;
+          if (i >= W) continue;
+          f32x16& o = (*acc[g / G % NX])[i];
+          o = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[g & 1][x][u == 0], p[g / G % NX]->at(g / HALF, u == 1), o, 0, 0, 0);
+        }
+      beside(g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+// calls pair(4 t .. 4 t + 3), the work on a half's registers: part of `parts`
+template <class F>
+__device__ __forceinline__ void pairs_of(int t, int part, int parts, F&& pair) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e * parts / 4 == part) pair(4 * t + e);
+}
+
+// Copies a packed tile into LDS, its fragments shared out among the block's
+// four waves.
+template <int KS>
+__device__ __forceinline__ void copy_tile(const char* tile, char* lds) {
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+#pragma unroll
+  for (int u = 0; u < KS / 2; ++u) {
+    const int at = (4 * u + wave) * pr::kFrag;
+    pr::copy16(tile + at + lane * 16, lds + at);
   }
 }
 
-// Copies of a tile of two operands into LDS (the first, then the second), the
-// fragments shared out among the block's four waves.
-template <int KS>
-__device__ __forceinline__ void copy_tile(const char* first, const char* second, char* lds) {
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  constexpr int PIECES = 2 * KS;  // of 1024 bytes, of one operand
-#pragma unroll
-  for (int u = 0; u < PIECES / 4; ++u) {
-    const int at = (4 * u + wave) * pr::kFrag;
-    pr::copy16(first + at + lane * 16, lds + at);
-    pr::copy16(second + at + lane * 16, lds + PIECES * pr::kFrag + at);
-  }
+// Tiles that a wave's rows [r0, r0 + 32) reach: their keys' limits grow with
+// the row.
+__device__ __forceinline__ int tiles_read(const AttArgs& a, int n, int64_t start, int r0) {
+  return r0 >= a.Sq ? 0 : (limit(a, n, start, min(r0 + 31, a.Sq - 1)) + 31) / 32;
 }
 
 constexpr float kPExp = 14.f;  // probabilities enter times 2^14
 
 template <int DHP>
 constexpr int pair_waves() { return DHP <= 64 ? 2 : 1; }
+template <int DHP>
+constexpr int dkv_waves() { return DHP <= 64 ? 2 : 1; }
 
 // Forward: a wave holds 32 queries of one head.
 template <int DHP>
 __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int tiles) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
-  __shared__ __align__(16) char lds[2][2 * TILE];
+  __shared__ __align__(16) char kbuf[2][TILE], vbuf[2][TILE];
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
@@ -781,9 +873,10 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   const int n = keys_of(a, b);
   const int64_t start = start_of(a, b);
   const int lim = held ? limit(a, n, start, i) : 0;
-  const int end = limit(a, n, start, min(tile * 128 + 127, a.Sq - 1));  // limits grow with the row
+  const int row0 = tile * 128 + 32 * __builtin_amdgcn_readfirstlane(wave);
+  const int mine = tiles_read(a, n, start, row0), all = (limit(a, n, start, min(tile * 128 + 127, a.Sq - 1)) + 31) / 32;
   const int ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest), ev = pr::scale_exp(scale_of(g.p, 2, bkh).largest);
-  const int eq = pr::scale_exp(scale_of(g.p, 0, bkh).largest);
+  const int eq = pr::scale_exp(scale_of(g.p, 0, bh).largest);
   // not zero, so that a masked score stays -inf
   const float c = fmaxf(pr::times_exp2(fabsf(a.scale) * kLog2e, -eq - ek), 0x1p-126f);
   RowFrags<KS> q;
@@ -798,25 +891,24 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   const char* vp = g.p.p[2] + bkh * g.p.blocks[2] * TILE;
   f32x16 o[DHP / 32] = {};
   float m = -INFINITY, l = 0.f;  // maximum of t = scale log2(e) s, sum of 2^(14 + t - m)
-  if (end > 0) copy_tile<KS>(kp, vp, lds[0]);
-  for (int j0 = 0, t = 0; j0 < end; j0 += 32, ++t) {
-    pr::wait_and_meet<0>();
-    if (j0 + 32 < end) copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, vp + (int64_t)(t + 1) * TILE, lds[(t + 1) & 1]);
-    if (!__any(lim > j0)) continue;
-    const char* buf = lds[t & 1];
-    f32x16 s = dot_pairs<KS>(buf, q);
-    if (!__all(lim >= j0 + 32)) {
+  // Step t forms the scores of tile t, and beside them the probabilities of
+  // tile t - 1, which then multiply its values.
+  f32x16 s[1] = {};
+  TileFrags p;
+  float base = 0.f;
+  // tile t's scores masked, the maximum and what it rescales
+  auto top = [&](int t) {
+    if (!__all(lim >= 32 * t + 32)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int j = j0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-        s[e] = j < lim ? s[e] : -INFINITY;
+        const int j = 32 * t + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+        s[0][e] = j < lim ? s[0][e] : -INFINITY;
       }
     }
-    float top = s[0];
+    float most = s[0][0];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-    top = fmaxf(top, other_half(top)) * c;
-    const float mn = fmaxf(m, top);
+    for (int e = 1; e < 16; ++e) most = fmaxf(most, s[0][e]);
+    const float mn = fmaxf(m, fmaxf(most, other_half(most)) * c);
     if (__any(mn > m)) {
       const float f = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
       l *= f;
@@ -826,17 +918,46 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
         for (int e = 0; e < 16; ++e) o[d][e] *= f;
       m = mn;
     }
-    const float base = (m == -INFINITY ? 0.f : m) - kPExp;
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -base));
-      sum += s[e];
+    base = (m == -INFINITY ? 0.f : m) - kPExp;
+  };
+  auto pair = [&](const f32x16& x, int e) {
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(x[2 * e], c, -base)), p1 = __builtin_amdgcn_exp2f(fmaf(x[2 * e + 1], c, -base));
+    l += p0 + p1;
+    p.split(e, p0, p1);
+  };
+  const RowFrags<KS>* const rows[1] = {&q};
+  const TileFrags* const probs[1] = {&p};
+  f32x16 (*const sums[1])[KS / 2] = {&o};
+  if (all > 0) copy_tile<KS>(kp, kbuf[0]);
+  for (int t = 0; t <= all; ++t) {
+    pr::wait_and_meet<0>();
+    if (t + 1 < all) copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, kbuf[(t + 1) & 1]);
+    if (t < all) copy_tile<KS>(vp + (int64_t)t * TILE, vbuf[t & 1]);
+    if (t > mine) continue;
+    const char* const now[1] = {kbuf[t & 1]};
+    if (t == 0) {
+      if (mine > 0) dot_pairs<KS, 1>(now, rows, s, [](int) {});
+      continue;
     }
-    l += sum;
-    TileFrags p;
-    p.split(s);
-    add_pairs<KS>(buf + TILE, p, o);
+    top(t - 1);
+    const char* const before[1] = {vbuf[(t - 1) & 1]};
+    Adder<KS, 1> add;
+    if (t < mine) {
+      f32x16 next[1];
+      dot_pairs<KS, 1>(now, rows, next, [&](int e) {
+        if (e == 7) add.read(before, 0);
+        pair(s[0], e);
+      });
+      s[0] = next[0];
+    } else {
+      add.read(before, 0);
+      // opaque, or the exponentials of both branches move ahead of them
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[0][e] = pr::opaque(s[0][e]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pair(s[0], e);
+    }
+    add.run(before, probs, sums, [](int) {});
   }
   l += other_half(l);
   const float f = lim > 0 ? 1.f / l : 0.f;
@@ -850,6 +971,13 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
         lim > 0 ? (m + log2f(pr::times_exp2(l, -(int)kPExp))) * kLn2 : -INFINITY;
 }
 
+// scale log2(e) over the packed operands' scales; not zero, so that times the
+// score of a key that is not read it stays infinite
+__device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
+  const float c = pr::times_exp2(a.scale * kLog2e, -exps);
+  return copysignf(fmaxf(fabsf(c), 0x1p-126f), c);
+}
+
 // The exponent of dS: 2 max ||dout|| max ||v|| bounds it.
 __device__ __forceinline__ int grad_exp(const Scale& g, const Scale& v) {
   const float bound = 2.f * g.norm * v.norm;
@@ -860,7 +988,7 @@ __device__ __forceinline__ int grad_exp(const Scale& g, const Scale& v) {
 template <int DHP>
 __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(PairArgs g, int tiles) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
-  __shared__ __align__(16) char lds[2][2 * TILE];
+  __shared__ __align__(16) char kbuf[2][TILE], vbuf[2][TILE];
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
@@ -873,11 +1001,13 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   const int n = keys_of(a, b);
   const int64_t start = start_of(a, b);
   const int lim = held ? limit(a, n, start, i) : 0;
-  const int end = limit(a, n, start, min(tile * 128 + 127, a.Sq - 1));
-  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bkh);
-  const int eq = pr::scale_exp(scale_of(g.p, 0, bkh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
+  const int row0 = tile * 128 + 32 * __builtin_amdgcn_readfirstlane(wave);
+  const int mine = tiles_read(a, n, start, row0), all = (limit(a, n, start, min(tile * 128 + 127, a.Sq - 1)) + 31) / 32;
+  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bh);
+  const int eq = pr::scale_exp(scale_of(g.p, 0, bh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
   const int eg = pr::scale_exp(sg.largest), ev = pr::scale_exp(sv.largest), ed = grad_exp(sg, sv);
-  const float c = pr::times_exp2(a.scale * kLog2e, -eq - ek), cd = pr::times_exp2(1.f, ed - eg - ev);
+  const float c = score_factor(a, eq + ek), cd = pr::times_exp2(1.f, ed - eg - ev);
+  const float none = copysignf(INFINITY, -c);  // the score of a key that is not read
   RowFrags<KS> q, go;
   q.load(g.p.p[0] + (int64_t)bh * g.p.blocks[0] * TILE, held ? i : 0, held);
   go.load(g.p.p[3] + (int64_t)bh * g.p.blocks[3] * TILE, held ? i : 0, held);
@@ -886,24 +1016,43 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   const char* kp = g.p.p[1] + bkh * g.p.blocks[1] * TILE;
   const char* vp = g.p.p[2] + bkh * g.p.blocks[2] * TILE;
   f32x16 acc[DHP / 32] = {};
-  if (end > 0) copy_tile<KS>(kp, vp, lds[0]);
-  for (int j0 = 0, t = 0; j0 < end; j0 += 32, ++t) {
-    pr::wait_and_meet<0>();
-    if (j0 + 32 < end) copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, vp + (int64_t)(t + 1) * TILE, lds[(t + 1) & 1]);
-    if (!__any(lim > j0)) continue;
-    const char* buf = lds[t & 1];
-    f32x16 s = dot_pairs<KS>(buf, q);
-    const f32x16 dp = dot_pairs<KS>(buf + TILE, go);
-    const bool whole = __all(lim >= j0 + 32);
+  // dS of a tile's first 16 keys is formed, then that of the others beside the
+  // product of the first
+  f32x16 s[2];
+  TileFrags p;
+  auto pair = [&](int e) {
+    float d[2];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int j = j0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-      const float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * fmaf(dp[e], cd, -delta);
-      s[e] = whole || j < lim ? p : 0.f;
+    for (int u = 0; u < 2; ++u)
+      d[u] = __builtin_amdgcn_exp2f(fmaf(s[0][2 * e + u], c, -lse)) * fmaf(s[1][2 * e + u], cd, -delta);
+    p.split(e, d[0], d[1]);
+  };
+  const RowFrags<KS>* const rows[2] = {&q, &go};
+  const TileFrags* const probs[1] = {&p};
+  f32x16 (*const sums[1])[KS / 2] = {&acc};
+  if (all > 0) {
+    copy_tile<KS>(kp, kbuf[0]);
+    copy_tile<KS>(vp, vbuf[0]);
+  }
+  for (int t = 0; t < all; ++t) {
+    pr::wait_and_meet<0>();
+    if (t + 1 < all) {
+      copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, kbuf[(t + 1) & 1]);
+      copy_tile<KS>(vp + (int64_t)(t + 1) * TILE, vbuf[(t + 1) & 1]);
     }
-    TileFrags p;
-    p.split(s);
-    add_pairs<KS>(buf, p, acc);
+    if (t >= mine) continue;
+    const char* const now[2] = {kbuf[t & 1], vbuf[t & 1]};
+    dot_pairs<KS, 2>(now, rows, s, [](int) {});
+    const char* const keys[1] = {now[0]};
+    Adder<KS, 1> add;
+    add.read(keys, 0);
+    if (!__all(lim >= 32 * t + 32)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        s[0][e] = 32 * t + 8 * (e / 4) + 4 * (lane >> 5) + e % 4 < lim ? s[0][e] : none;
+    }
+    pairs_of(0, 0, 1, pair);
+    add.run(keys, probs, sums, [&](int n) { pairs_of(1, n, add.HALF, pair); });
   }
 #pragma unroll
   for (int d = 0; d < DHP / 32; ++d)
@@ -916,10 +1065,10 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
 // one query head; where heads share the keys, into sums of their own
 // ([head of a sample][feature][key], att_share_kernel adds them).
 template <int DHP>
-__global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(PairArgs g) {
+__global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(PairArgs g) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
-  __shared__ __align__(16) char lds[2][2 * TILE];
-  __shared__ __align__(16) float stat[2][2][32];  // lse (base 2) - 14, scaled delta of the tile's queries
+  __shared__ __align__(16) char qbuf[2][TILE], gbuf[2][TILE];
+  __shared__ __align__(16) float stat[2][2][32];  // lse (base 2) - 14, scaled delta of the tiles' queries
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
@@ -930,10 +1079,11 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(Pai
   const int n = keys_of(a, b);
   const int64_t start = start_of(a, b);
   const bool held = key < n;
-  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bkh);
-  const int eq = pr::scale_exp(scale_of(g.p, 0, bkh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
+  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bh);
+  const int eq = pr::scale_exp(scale_of(g.p, 0, bh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
   const int eg = pr::scale_exp(sg.largest), ev = pr::scale_exp(sv.largest), ed = grad_exp(sg, sv);
-  const float c = pr::times_exp2(a.scale * kLog2e, -eq - ek), cd = pr::times_exp2(1.f, ed - eg - ev - (int)kPExp);
+  const float c = score_factor(a, eq + ek), cd = pr::times_exp2(1.f, ed - eg - ev - (int)kPExp);
+  const float none = copysignf(INFINITY, -c);  // the score of a key that is not read
   RowFrags<KS> k, v;
   k.load(g.p.p[1] + bkh * g.p.blocks[1] * TILE, held ? key : 0, held);
   v.load(g.p.p[2] + bkh * g.p.blocks[2] * TILE, held ? key : 0, held);
@@ -945,42 +1095,57 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dkv_pair_kernel(Pai
   const char* gp = g.p.p[3] + ((int64_t)bh * g.p.blocks[3] + first) * TILE;
   f32x16 dk[DHP / 32] = {}, dv[DHP / 32] = {};
   float st = 0.f;
-  auto copy = [&](int t) {
-    copy_tile<KS>(qp + (int64_t)t * TILE, gp + (int64_t)t * TILE, lds[t & 1]);
+  auto copy = [&](int t, int buf) {
+    copy_tile<KS>(qp + (int64_t)t * TILE, qbuf[buf]);
+    copy_tile<KS>(gp + (int64_t)t * TILE, gbuf[buf]);
     const int64_t i = (first + t) * 32 + (lane & 31);
     if (wave != 0) return;
     if (i >= a.Sq) st = lane < 32 ? INFINITY : 0.f;
     else if (lane < 32) st = lse2_of(a, b, head, i) - kPExp;
     else st = pr::times_exp2(a.delta[(int64_t)bh * a.Sq + i], ed - (int)kPExp);
   };
-  if (total > 0) copy(0);
+  // A wave's first tile is that of the first query that reads its first key.
+  const int64_t skip = a.causal ? key0 + 32 * __builtin_amdgcn_readfirstlane(wave) - start - first * 32 : 0;
+  const int from = (int)(skip < 0 ? 0 : skip / 32 < total ? skip / 32 : total);
+  // the probabilities and dS of a tile's first 16 queries are formed, then those
+  // of the others beside the products of the first
+  f32x16 s[2];
+  TileFrags p, ds;
+  auto pair = [&](const float (*st)[32], int e) {
+    const int r = 8 * (e / 2) + 4 * (lane >> 5) + 2 * (e & 1);
+    const float2 lse = *reinterpret_cast<const float2*>(&st[0][r]);
+    const float2 delta = *reinterpret_cast<const float2*>(&st[1][r]);
+    float w[2] = {__builtin_amdgcn_exp2f(fmaf(s[0][2 * e], c, -lse.x)), __builtin_amdgcn_exp2f(fmaf(s[0][2 * e + 1], c, -lse.y))};
+    float d[2] = {w[0] * fmaf(s[1][2 * e], cd, -delta.x), w[1] * fmaf(s[1][2 * e + 1], cd, -delta.y)};
+    p.split(e, w[0], w[1]);
+    ds.split(e, d[0], d[1]);
+  };
+  const RowFrags<KS>* const rows[2] = {&k, &v};
+  const TileFrags* const probs[2] = {&p, &ds};
+  f32x16 (*const sums[2])[KS / 2] = {&dv, &dk};
+  if (total > 0) copy(0, 0);
   for (int t = 0; t < total; ++t) {
     if (wave == 0) stat[t & 1][lane >> 5][lane & 31] = st;
     pr::wait_and_meet<0>();
-    const int64_t i0 = (first + t) * 32;
-    if (t + 1 < total) copy(t + 1);
-    if (a.causal && start + i0 + 31 < key0 + 32 * wave) continue;  // no query of the tile reads this wave's keys
-    const char* buf = lds[t & 1];
-    f32x16 s = dot_pairs<KS>(buf, k);
-    f32x16 dp = dot_pairs<KS>(buf + TILE, v);
-    const bool whole = __all(held) && (!a.causal || key0 + 32 * wave + 31 <= start + i0);
+    if (t + 1 < total) copy(t + 1, (t + 1) & 1);
+    if (t < from) continue;
+    const char* const now[2] = {qbuf[t & 1], gbuf[t & 1]};
+    dot_pairs<KS, 2>(now, rows, s, [](int) {});
+    const char* const turned[2] = {now[1], now[0]};
+    Adder<KS, 2> add;
+    add.read(turned, 0);
+    const int64_t i0 = start + (first + t) * 32;  // the position of the tile's first query
+    if (!(__all(held) && (!a.causal || key0 + 32 * wave + 31 <= i0))) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int r = 8 * q + 4 * (lane >> 5);
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[t & 1][0][r]);
-      const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[t & 1][1][r]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool reads = whole || (held && (!a.causal || key <= start + i0 + r + e));
-        s[4 * q + e] = reads ? __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], c, -lse[e])) : 0.f;
-        dp[4 * q + e] = reads ? s[4 * q + e] * fmaf(dp[4 * q + e], cd, -delta[e]) : 0.f;
+      for (int e = 0; e < 16; ++e) {
+        const bool reads = held && (!a.causal || key <= i0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4);
+        s[0][e] = reads ? s[0][e] : none;
       }
     }
-    TileFrags p;
-    p.split(s);
-    add_pairs<KS>(buf + TILE, p, dv);
-    p.split(dp);
-    add_pairs<KS>(buf, p, dk);
+    const float (*const st_now)[32] = stat[t & 1];
+    auto work = [&](int e) { pair(st_now, e); };
+    pairs_of(0, 0, 1, work);
+    add.run(turned, probs, sums, [&](int n) { pairs_of(1, n, add.HALF, work); });
   }
 #pragma unroll
   for (int d = 0; d < DHP / 32; ++d)
@@ -1025,30 +1190,37 @@ __global__ void __launch_bounds__(NT) att_share_kernel(PairArgs g) {
     if (d0 + e < a.dh) o[(d0 + e) * out.col] = s[e];
 }
 
+// f(the features of a row padded to the kernel's as an integral constant)
+template <class F>
+void by_width(int dh, F&& f) {
+  if (dh <= 32) f(std::integral_constant<int, 32>{});
+  else if (dh <= 64) f(std::integral_constant<int, 64>{});
+  else if (dh <= 96) f(std::integral_constant<int, 96>{});
+  else f(std::integral_constant<int, 128>{});
+}
+
 // Lays out the workspace of the packed operands and packs them.  ops: 3 (q, k,
-// v) or 4; delta: where dout's pass leaves it.
+// v) or 4; with dout's packing comes delta.
 int pack(PairArgs& g, int ops, hipStream_t st, const char* who) {
   AttArgs& a = g.a;
   PackArgs& p = g.p;
-  p.steps = a.dh <= 32 ? 2 : a.dh <= 64 ? 4 : a.dh <= 96 ? 6 : 8;
+  const int steps = a.dh <= 32 ? 2 : a.dh <= 64 ? 4 : a.dh <= 96 ? 6 : 8;
+  const int most = a.Sq > a.Sk ? a.Sq : a.Sk;
+  const bool one = most <= 512;  // 16 waves of 32 rows
   size_t bytes = 0, part[4], data[4];
   auto place_bytes = [&](size_t n) {
     const size_t at = bytes;
     bytes += (n + 255) / 256 * 256;
     return at;
   };
-  int most_chunks = 0, most_blocks = 0;
   for (int w = 0; w < ops; ++w) {
     const bool kv = w == 1 || w == 2;
     const int64_t S = kv ? a.Sk : a.Sq, heads = kv ? a.kv_heads : a.heads;
     p.blocks[w] = (int)((S + 31) / 32);
-    p.chunk_rows[w] = (int)((S + 32 * 128 - 1) / (32 * 128) * 128);  // 32 chunks at most
-    p.chunks[w] = (int)((S + p.chunk_rows[w] - 1) / p.chunk_rows[w]);
-    p.slots[w] = p.chunks[w] * (kv ? 1 : a.group);
-    most_chunks = p.chunks[w] > most_chunks ? p.chunks[w] : most_chunks;
-    most_blocks = p.blocks[w] > most_blocks ? p.blocks[w] : most_blocks;
-    part[w] = place_bytes((size_t)a.B * a.kv_heads * p.slots[w] * sizeof(Scale));
-    data[w] = place_bytes((size_t)a.B * heads * p.blocks[w] * p.steps * 2 * pr::kFrag);
+    p.chunk_rows[w] = (int)((S + 64 * 128 - 1) / (64 * 128) * 128);  // 64 chunks at most
+    p.chunks[w] = one ? 1 : (int)((S + p.chunk_rows[w] - 1) / p.chunk_rows[w]);
+    part[w] = place_bytes((size_t)a.B * heads * p.chunks[w] * sizeof(Scale));
+    data[w] = place_bytes((size_t)a.B * heads * p.blocks[w] * steps * 2 * pr::kFrag);
   }
   const size_t delta = place_bytes(ops == 4 ? (size_t)a.B * a.heads * a.Sq * sizeof(float) : 0);
   const size_t sums = ops == 4 && a.group > 1 ? (size_t)a.B * a.heads * a.dh * a.Sk * sizeof(float) : 0;
@@ -1067,13 +1239,17 @@ int pack(PairArgs& g, int ops, hipStream_t st, const char* who) {
   p.x[1] = a.k;
   p.x[2] = a.v;
   p.x[3] = a.dout;
-  const dim3 gs((unsigned)most_chunks, (unsigned)(a.B * a.heads), (unsigned)ops);
-  const dim3 gp((unsigned)((most_blocks + 3) / 4), (unsigned)(a.B * a.heads), (unsigned)ops);
-  if (ops == 3) hipLaunchKernelGGL(att_scale_kernel<3>, gs, dim3(NT), 0, st, g);
-  else hipLaunchKernelGGL(att_scale_kernel<4>, gs, dim3(NT), 0, st, g);
-  CNHIP_TRY(check_launch(who));
-  if (ops == 3) hipLaunchKernelGGL(att_pack_kernel<3>, gp, dim3(NT), 0, st, g);
-  else hipLaunchKernelGGL(att_pack_kernel<4>, gp, dim3(NT), 0, st, g);
+  const unsigned bh = (unsigned)(a.B * a.heads), blocks = (unsigned)((most + 31) / 32);
+  by_width(a.dh, [&](auto d) {
+    constexpr int KS = d() / 16;
+    if (one) {
+      hipLaunchKernelGGL(att_pack_head_kernel<KS>, dim3(1, bh, (unsigned)ops), dim3(64 * blocks), 0, st, g);
+    } else {
+      const int chunks = p.chunks[0] > p.chunks[1] ? p.chunks[0] : p.chunks[1];
+      hipLaunchKernelGGL(att_scale_kernel<KS>, dim3((unsigned)chunks, bh, (unsigned)ops), dim3(NT), 0, st, g);
+      hipLaunchKernelGGL(att_pack_kernel<KS>, dim3((blocks + 3) / 4, bh, (unsigned)ops), dim3(NT), 0, st, g);
+    }
+  });
   return check_launch(who);
 }
 
@@ -1087,15 +1263,7 @@ Seq<T> seq(T* p, int64_t B, int64_t S, int rows) {
   return rows == CNHIP_ROWS_REF ? Seq<T>{p, 1, B, B * S} : Seq<T>{p, S, 1, B * S};
 }
 
-// f(the features of a row padded to the kernel's as an integral constant)
-template <class F>
-void by_width(int dh, F&& f) {
-  if (dh <= 32) f(std::integral_constant<int, 32>{});
-  else if (dh <= 64) f(std::integral_constant<int, 64>{});
-  else if (dh <= 96) f(std::integral_constant<int, 96>{});
-  else f(std::integral_constant<int, 128>{});
-}
-// the same, and whether a step's neighbours are adjacent
+// by_width, and whether a step's neighbours are adjacent
 template <class F>
 void dispatch(int dh, bool unit, F&& f) {
   by_width(dh, [&](auto d) {

@@ -44,6 +44,7 @@ namespace pr {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -74,14 +75,22 @@ __device__ __forceinline__ int slot(int l, int s) {
   return ((l & 32) | ((l & 31) ^ ((l >> 5) * 4 + (s & 1) * 8))) * 16;
 }
 
-// two values to their terms: w0 = {x0(a), x0(b)}, w1 the remainders
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+// Keeps the compiler from folding the operation that formed x into what uses it.
+__device__ __forceinline__ float opaque(float x) {
+  asm("" : "+v"(x));
+  return x;
 }
+// Two values to their terms: w0 = {x0(a), x0(b)}, w1 the remainders'.  Values
+// and remainders are opaque: a product that is converted at once, or a
+// remainder, became a v_fma_mixlo_f16 otherwise, and dq came out ten times less
+// exact.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& w0, uint32_t& w1) {
-  const f16x2 h = {(_Float16)a, (_Float16)b};
+  a = opaque(a);
+  b = opaque(b);
+  const f16x2 h = __builtin_convertvector(f32x2{a, b}, f16x2);
+  const f16x2 l = __builtin_convertvector(f32x2{opaque(a - (float)h[0]), opaque(b - (float)h[1])}, f16x2);
   w0 = __builtin_bit_cast(uint32_t, h);
-  w1 = pack2(a - (float)h[0], b - (float)h[1]);
+  w1 = __builtin_bit_cast(uint32_t, l);
 }
 
 // ----------------------------------------------------------- global -> LDS
