@@ -323,11 +323,12 @@ __global__ void __launch_bounds__(NT) att_join_kernel(AttArgs a, SplitArgs p) {
   const int head = kh * a.group + (int)(r / a.Sq);
   const int64_t i = r % a.Sq, step = (int64_t)gridDim.y * gridDim.x, at = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   float top = -INFINITY;
+#pragma unroll 8
   for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.ml[(at + s * step) * 32 + lane].x);
   const float base = top == -INFINITY ? 0.f : top;
   float total = 0.f, x[4] = {};
   const int d0 = (int)blockIdx.z * 32 + 4 * part;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < p.splits; ++s) {
     const float2 ml = p.ml[(at + s * step) * 32 + lane];
     const float f = __builtin_amdgcn_exp2f(ml.x - base);
@@ -345,24 +346,13 @@ __global__ void __launch_bounds__(NT) att_join_kernel(AttArgs a, SplitArgs p) {
     a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
-// delta[b][head][i] = sum_d dout out
-__global__ void __launch_bounds__(NT) att_delta_kernel(AttArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
-  const int b = (int)blockIdx.y / a.heads, head = (int)blockIdx.y % a.heads;
-  if (i >= a.Sq) return;
-  const float* g = a.dout.at(b, i, (int64_t)head * a.dh);
-  const float* o = a.o.at(b, i, (int64_t)head * a.dh);
-  float s = 0.f;
-  for (int d = 0; d < a.dh; ++d) s = fmaf(g[d * a.dout.col], o[d * a.o.col], s);
-  a.delta[(int64_t)blockIdx.y * a.Sq + i] = s;
-}
-
 __device__ __forceinline__ float lse2_of(const AttArgs& a, int b, int head, int64_t i) {
   const float l = a.lse_in[b * a.lse_sample + i * a.lse_row + head * a.lse_col];
   return l == -INFINITY ? INFINITY : l * kLog2e;  // a row that reads no key: every 2^(t - inf) is 0
 }
 
-// dq: a block owns 128 rows as in the forward and streams keys and values.
+// dq: a block owns 128 rows as in the forward and streams keys and values; it
+// leaves delta for the kernel of dk and dv.
 template <int DHP, bool UNIT>
 __global__ void __launch_bounds__(NT) att_dq_kernel(AttArgs a) {
   __shared__ __align__(16) float lds[2][DHP * LS];
@@ -379,7 +369,15 @@ __global__ void __launch_bounds__(NT) att_dq_kernel(AttArgs a) {
   load_row<DHP>(a.q.at(b, i, (int64_t)head * a.dh), a.q.col, held, a.dh, q);
   load_row<DHP>(a.dout.at(b, i, (int64_t)head * a.dh), a.dout.col, held, a.dh, g);
   const float lse = held ? lse2_of(a, b, head, i) : INFINITY;
-  const float delta = held ? a.delta[((int64_t)b * a.heads + head) * a.Sq + i] : 0.f;
+  float delta = 0.f;
+  {
+    float out[DHP / 2];
+    load_row<DHP>(a.o.at(b, i, (int64_t)head * a.dh), a.o.col, held, a.dh, out);
+#pragma unroll
+    for (int s = 0; s < DHP / 2; ++s) delta = fmaf(g[s], out[s], delta);
+    delta += other_half(delta);
+    if (held && lane < 32) a.delta[((int64_t)b * a.heads + head) * a.Sq + i] = delta;
+  }
   __shared__ int most;
   if (threadIdx.x == 0) most = 0;
   __syncthreads();
@@ -559,6 +557,12 @@ __device__ __forceinline__ bool operand_of(const AttArgs& a, Operand& o) {
   return o.head < heads;
 }
 
+// The norm of a row whose squares sum to n; where they leave the range, its
+// bound by the largest value.
+__device__ __forceinline__ float norm_of(float n, uint32_t largest, int dh) {
+  return n > 1e-30f && n < 1e37f ? sqrtf(n) : __uint_as_float(largest) * sqrtf((float)dh);
+}
+
 // 32 rows of a head in a wave's registers: features 16 s + 8 (lane / 32) .. + 7 of
 // row lane % 32 in v[s], zeros where there are none.
 template <int KS>
@@ -592,8 +596,7 @@ struct RowBlock {
       m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
       n = fmaxf(n, __shfl_xor(n, o, 64));
     }
-    // squares that leave the range: the bound by the largest value
-    return Scale{m, n > 1e-30f && n < 1e37f ? sqrtf(n) : __uint_as_float(m) * sqrtf((float)dh)};
+    return Scale{m, norm_of(n, m, dh)};
   }
   __device__ __forceinline__ void pack(const PackArgs& p, const Operand& o, int blk, float f) const {
     const int lane = (int)threadIdx.x & 63;
@@ -655,31 +658,49 @@ __global__ void __launch_bounds__(1024) att_pack_head_kernel(PairArgs g) {
   if (o.which == 3) x.delta(g.a, o, wave);
 }
 
-// Longer ones: the scale of a chunk of rows of a head, then the packing, a wave
-// per 32 rows in both.
+// Longer ones: the scale of a chunk of rows of a head (a lane per row, 256
+// adjacent bytes a load, the four waves a quarter of the features each), then
+// the packing, a wave per 32 rows.
 template <int KS>
 __global__ void __launch_bounds__(NT) att_scale_kernel(PairArgs g) {
-  __shared__ Scale part[4];
+  __shared__ float squares[4][64];
+  __shared__ uint32_t part[4];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const AttArgs& a = g.a;
   Operand o;
-  if (!operand_of(g.a, o) || (int)blockIdx.x >= g.p.chunks[o.which]) return;
-  Scale s{0u, 0.f};
-  const int per = g.p.chunk_rows[o.which] / 32;
-  for (int blk = (int)blockIdx.x * per + wave; blk < ((int)blockIdx.x + 1) * per && blk * 32 < o.rows; blk += 4) {
-    RowBlock<KS> x;
-    x.load(g.a, g.p, o, blk);
-    const Scale t = x.scale(g.a.dh);
-    s.largest = max(s.largest, t.largest);
-    s.norm = fmaxf(s.norm, t.norm);
+  if (!operand_of(a, o) || (int)blockIdx.x >= g.p.chunks[o.which]) return;
+  const Seq<const float>& x = g.p.x[o.which];
+  const int rows = g.p.chunk_rows[o.which];
+  constexpr int U = 4 * KS;
+  uint32_t m = 0;
+  float norm = 0.f;
+  for (int r0 = (int)blockIdx.x * rows; r0 < ((int)blockIdx.x + 1) * rows && r0 < o.rows; r0 += 64) {
+    const int r = r0 + lane;
+    const float* p = x.at(o.b, r < o.rows ? r : 0, (int64_t)o.head * a.dh);
+    float v[U], n = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = r < o.rows && wave * U + u < a.dh ? p[(wave * U + u) * x.col] : 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t bits = pr::finite_bits(v[u]);
+      m = max(m, bits);
+      n = fmaf(__uint_as_float(bits), __uint_as_float(bits), n);
+    }
+    squares[wave][lane] = n;
+    __syncthreads();
+    norm = fmaxf(norm, (squares[0][lane] + squares[1][lane]) + (squares[2][lane] + squares[3][lane]));
+    __syncthreads();
   }
-  if (lane == 0) part[wave] = s;
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) {
+    m = max(m, (uint32_t)__shfl_xor((int)m, i, 64));
+    norm = fmaxf(norm, __shfl_xor(norm, i, 64));
+  }
+  if (lane == 0) part[wave] = m;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int w = 1; w < 4; ++w) {
-    s.largest = max(s.largest, part[w].largest);
-    s.norm = fmaxf(s.norm, part[w].norm);
-  }
-  g.p.part[o.which][o.bh * g.p.chunks[o.which] + blockIdx.x] = s;
+  m = max(max(part[0], part[1]), max(part[2], part[3]));
+  g.p.part[o.which][o.bh * g.p.chunks[o.which] + blockIdx.x] = Scale{m, norm_of(norm, m, a.dh)};
 }
 
 template <int KS>
@@ -1217,7 +1238,7 @@ int pack(PairArgs& g, int ops, hipStream_t st, const char* who) {
     const bool kv = w == 1 || w == 2;
     const int64_t S = kv ? a.Sk : a.Sq, heads = kv ? a.kv_heads : a.heads;
     p.blocks[w] = (int)((S + 31) / 32);
-    p.chunk_rows[w] = (int)((S + 64 * 128 - 1) / (64 * 128) * 128);  // 64 chunks at most
+    p.chunk_rows[w] = (int)((S + 64 * 64 - 1) / (64 * 64) * 64);  // 64 chunks at most
     p.chunks[w] = one ? 1 : (int)((S + p.chunk_rows[w] - 1) / p.chunk_rows[w]);
     part[w] = place_bytes((size_t)a.B * heads * p.chunks[w] * sizeof(Scale));
     data[w] = place_bytes((size_t)a.B * heads * p.blocks[w] * steps * 2 * pr::kFrag);
@@ -1414,18 +1435,15 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
   void* ws = nullptr;
   CNHIP_TRY(cnhip::scratch(st, cnhip::kScratchLayer, (size_t)(B * heads * Sq) * sizeof(float), &ws, who));
   a.delta = static_cast<float*>(ws);
-  hipLaunchKernelGGL(cnhip::att_delta_kernel, dim3((unsigned)((Sq + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * heads)),
-                     dim3(cnhip::NT), 0, st, a);
-  CNHIP_TRY(cnhip::check_launch(who));
-  cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
-    hipLaunchKernelGGL((cnhip::att_dkv_kernel<d(), unit()>),
-                       dim3((unsigned)((Sk + 127) / 128), (unsigned)(B * kv_heads)), dim3(cnhip::NT), 0, st, a);
-  });
-  CNHIP_TRY(cnhip::check_launch(who));
   cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
     hipLaunchKernelGGL((cnhip::att_dq_kernel<d(), unit()>),
                        dim3((unsigned)((a.group * Sq + 127) / 128), (unsigned)(B * kv_heads)), dim3(cnhip::NT), 0, st,
                        a);
+  });
+  CNHIP_TRY(cnhip::check_launch(who));
+  cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
+    hipLaunchKernelGGL((cnhip::att_dkv_kernel<d(), unit()>),
+                       dim3((unsigned)((Sk + 127) / 128), (unsigned)(B * kv_heads)), dim3(cnhip::NT), 0, st, a);
   });
   return cnhip::check_launch(who);
 }

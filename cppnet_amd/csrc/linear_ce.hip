@@ -470,6 +470,252 @@ __global__ void __launch_bounds__(1024) ce_loss_kernel(CeArgs a, float* __restri
   if (threadIdx.x == 0) *loss = a.mean ? part[0] / (float)(held > 0 ? held : 1) : part[0];
 }
 
+// ------------------------------------------------------------ few rows
+// Up to kFewRows rows are one or two columns of 32 lanes: W is then read once or
+// twice and each value used for a handful of products, so the fp32 matrix cores
+// keep up with memory and nothing is packed.  Four launches: logits with row
+// statistics, the rows' losses, G with dW, db and parts of dX, and the sum of
+// those parts.
+constexpr int kFewRows = 64;
+constexpr int kFewClasses = 32;   // classes a block of the first launch
+constexpr int kFewSlice = 64;     // classes a block of the third
+constexpr int kFewWidth = 128;    // features a block of the third: 32 a wave
+
+// 32 classes; the eight waves share out the features, a step of 16 each.
+template <int NB>
+__global__ void __launch_bounds__(512) ce_few_logits_kernel(CeArgs a) {
+  __shared__ float part[8][kFewClasses][64 + 1];
+  __shared__ float2 stat[8][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, r = lane & 31;
+  const int64_t v0 = (int64_t)blockIdx.x * kFewClasses, v = v0 + r;
+  const int N = (int)a.N, steps = (int)((a.D + 15) / 16);
+  bool held[NB], in[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    in[j] = 32 * j + r < N;
+    held[j] = in[j] && has_target(a, 32 * j + r);
+  }
+  float w[2][8], x[2][NB][8];
+  auto load = [&](int s, int b) {
+    const int64_t d0 = 16 * (int64_t)s + 8 * h;
+    const float* p = a.W + v * a.D + d0;
+    if (v < a.V && d0 + 8 <= a.D) {
+      const f32x4 lo = *reinterpret_cast<const f32x4u*>(p), hi = *reinterpret_cast<const f32x4u*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[b][e] = lo[e];
+        w[b][4 + e] = hi[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[b][e] = v < a.V && d0 + e < a.D ? p[e] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[b][j][e] = in[j] && d0 + e < a.D ? a.X[32 * j + r + a.N * (d0 + e)] : 0.f;
+  };
+  f32x16 acc[NB] = {};
+  auto multiply = [&](int b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        float y = x[b][j][e];
+        if (!held[j]) y = y - y == 0.f ? y : 0.f;
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(w[b][e], y, acc[j], 0, 0, 0);
+      }
+  };
+  if (wave < steps) load(wave, 0);
+  for (int s = wave; s < steps; s += 16) {
+    if (s + 8 < steps) load(s + 8, 1);
+    multiply(0);
+    if (s + 16 < steps) load(s + 16, 0);
+    if (s + 8 < steps) multiply(1);
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) part[wave][8 * (e / 4) + 4 * h + e % 4][32 * j + r] = acc[j][e];
+  __syncthreads();
+  // a lane per row, four classes a wave
+  const int n = lane;
+  float z[4], top = -INFINITY;
+  if (n < 32 * NB) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 4 * wave + e;
+      z[e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) z[e] += part[q][c][n];
+      if (a.b && v0 + c < a.V) z[e] += a.b[v0 + c];
+      if (v0 + c >= a.V) z[e] = -INFINITY;
+      else if (n < N) a.Z[n + a.N * (v0 + c)] = z[e];
+      top = fmaxf(top, z[e]);
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += expf(z[e] - base);
+    stat[wave][n] = float2{top, sum};
+  }
+  __syncthreads();
+  if (wave || n >= N) return;
+  float m = -INFINITY, t = 0.f;
+  for (int q = 0; q < 8; ++q) m = fmaxf(m, stat[q][n].x);
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int q = 0; q < 8; ++q) t += stat[q][n].y * expf(stat[q][n].x - base);
+  a.stat[(int64_t)blockIdx.x * a.N + n] = float2{m, t};
+}
+
+// The rows' log-sum-exp and losses, their number and sum (one block).
+__global__ void __launch_bounds__(1024) ce_few_rows_kernel(CeArgs a, float* __restrict__ loss) {
+  __shared__ float2 part[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float m = -INFINITY, s = 0.f;
+  if (lane < a.N) {
+    constexpr int U = 8;
+    for (int64_t q0 = wave; q0 < a.stat_blocks; q0 += 16 * U) {
+      float2 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        x[u] = q0 + 16 * u < a.stat_blocks ? a.stat[(q0 + 16 * u) * a.N + lane] : float2{-INFINITY, 0.f};
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, x[u].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      s *= expf(m - base);
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += x[u].y * expf(x[u].x - base);
+      m = top;
+    }
+  }
+  part[wave][lane] = float2{m, s};
+  __syncthreads();
+  if (wave) return;
+  for (int w = 1; w < 16; ++w) {
+    const float2 x = part[w][lane];
+    const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.f : top;
+    s = s * expf(m - base) + x.y * expf(x.x - base);
+    m = top;
+  }
+  const int32_t t = lane < a.N ? a.t[lane] : -1;
+  const bool held = t >= 0 && t < a.V;
+  const float lse = m + logf(s);
+  if (lane < a.N) a.lse[lane] = lse;
+  float l = held ? lse - a.Z[lane + a.N * (int64_t)t] : 0.f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  const int count = __popcll(__ballot(held)), past = __popcll(__ballot(t >= a.V));
+  if (lane == 0) {
+    a.state->held = count;
+    *loss = a.mean ? l / (float)(count > 0 ? count : 1) : l;
+    if (a.oob && past) atomicAdd(a.oob, past);
+  }
+}
+
+// A slice of classes and 128 features, 32 a wave: G of the slice in LDS, dW and
+// db of it, and its part of dX ([slice][feature][row]).
+template <int NB>
+__global__ void __launch_bounds__(256) ce_few_grads_kernel(CeArgs a, float* dW, float* db, float* part, int accumulate) {
+  constexpr int NR = 32 * NB, LD = NR + 1;
+  __shared__ float G[kFewSlice * LD], xs[kFewWidth * LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, r = lane & 31;
+  const int64_t v0 = (int64_t)blockIdx.x * kFewSlice, d0 = (int64_t)blockIdx.y * kFewWidth, d = d0 + 32 * wave + r;
+  const int N = (int)a.N;
+  const float f = grad_factor(a);
+  // W of the wave's features, and everything else that is read, goes out first
+  float w[kFewSlice / 2];
+#pragma unroll
+  for (int s = 0; s < kFewSlice / 2; ++s) {
+    const int64_t v = v0 + 2 * s + h;
+    w[s] = d < a.D && v < a.V ? a.W[d + a.D * v] : 0.f;
+  }
+  {
+    const int n = threadIdx.x % NR;
+    const int32_t t = n < N ? a.t[n] : -1;
+    const bool held = t >= 0 && t < a.V;
+    const float lse = held ? a.lse[n] : 0.f;
+    constexpr int STEP = 256 / NR, UG = kFewSlice / STEP, UX = kFewWidth / STEP;
+    float z[UG], x[UX];
+#pragma unroll
+    for (int u = 0; u < UG; ++u) {
+      const int64_t v = v0 + threadIdx.x / NR + u * STEP;
+      z[u] = held && v < a.V ? a.Z[n + a.N * v] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < UX; ++u) {
+      const int64_t dx = d0 + threadIdx.x / NR + u * STEP;
+      x[u] = held && dx < a.D ? a.X[n + a.N * dx] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < UG; ++u) {
+      const int c = threadIdx.x / NR + u * STEP;
+      const int64_t v = v0 + c;
+      G[c * LD + n] = held && v < a.V ? (expf(z[u] - lse) - (v == t ? 1.f : 0.f)) * f : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < UX; ++u) xs[(threadIdx.x / NR + u * STEP) * LD + n] = x[u];
+  }
+  __syncthreads();
+  // dX's part: W's features over the classes
+  f32x16 acc[NB] = {};
+#pragma unroll
+  for (int s = 0; s < kFewSlice / 2; ++s)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(w[s], G[(2 * s + h) * LD + 32 * j + r], acc[j], 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int64_t m = d0 + 32 * wave + 8 * (e / 4) + 4 * h + e % 4;
+      if (m < a.D && 32 * j + r < N) part[((int64_t)blockIdx.x * a.D + m) * a.N + 32 * j + r] = acc[j][e];
+    }
+  // dW: G over the rows of the batch
+  constexpr int C = kFewSlice / 32;
+  f32x16 dw[C] = {};
+#pragma unroll 16
+  for (int s = 0; s < NR / 2; ++s) {
+    const float x = xs[(32 * wave + r) * LD + 2 * s + h];
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      dw[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(G[(32 * i + r) * LD + 2 * s + h], x, dw[i], 0, 0, 0);
+  }
+  if (d < a.D) {
+    float* p = dW + d + a.D * (v0 + 4 * h);
+    const int64_t left = a.V - (v0 + 4 * h);
+    auto row = [](int i, int e) { return 32 * i + 8 * (e / 4) + e % 4; };
+    float old[C][16];
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) old[i][e] = accumulate && row(i, e) < left ? p[a.D * row(i, e)] : 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (row(i, e) < left) p[a.D * row(i, e)] = old[i][e] + dw[i][e];
+  }
+  if (db && blockIdx.y == 0 && threadIdx.x < kFewSlice && v0 + threadIdx.x < a.V) {
+    float sum = 0.f;
+    for (int n = 0; n < NR; ++n) sum += G[threadIdx.x * LD + n];
+    float* p = db + v0 + threadIdx.x;
+    *p = accumulate ? *p + sum : sum;
+  }
+}
+
+// dX = the slices' parts, in order
+__global__ void __launch_bounds__(256) ce_few_dx_kernel(const float* __restrict__ part, float* __restrict__ dX, int64_t n,
+                                                        int slices) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+#pragma unroll 16
+  for (int q = 0; q < slices; ++q) s += part[q * n + i];
+  dX[i] = s;
+}
+
 struct CeGrads {
   float *dX, *dW, *db;
   int accumulate;
@@ -488,6 +734,31 @@ Split split_of(int64_t M, int64_t N, int steps) {
   int per = (int)((steps + s - 1) / s);
   per = (per + 1) / 2 * 2;
   return Split{(steps + per - 1) / per, per};
+}
+
+int run_few(CeArgs& a, float* loss, const CeGrads* g, hipStream_t st, const char* who) {
+  const int64_t N = a.N, D = a.D, V = a.V, slices = (V + kFewSlice - 1) / kFewSlice;
+  a.stat_blocks = (V + kFewClasses - 1) / kFewClasses;
+  const size_t z = (size_t)(N * V) * 4, stat = (size_t)(a.stat_blocks * N) * 8, part = g ? (size_t)(slices * D * N) * 4 : 0;
+  void* ws = nullptr;
+  CNHIP_TRY(scratch(st, kScratchLayer, 256 + stat + z + part, &ws, who));
+  a.state = static_cast<CeState*>(ws);
+  a.stat = reinterpret_cast<float2*>(static_cast<char*>(ws) + 256);
+  a.Z = reinterpret_cast<float*>(a.stat + a.stat_blocks * N);
+  float* dx_part = a.Z + N * V;
+  const dim3 logits((unsigned)a.stat_blocks), grads((unsigned)slices, (unsigned)((D + kFewWidth - 1) / kFewWidth));
+  if (N <= 32) hipLaunchKernelGGL(ce_few_logits_kernel<1>, logits, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL(ce_few_logits_kernel<2>, logits, dim3(512), 0, st, a);
+  CNHIP_TRY(check_launch(who));
+  hipLaunchKernelGGL(ce_few_rows_kernel, dim3(1), dim3(1024), 0, st, a, loss);
+  CNHIP_TRY(check_launch(who));
+  if (!g) return CNHIP_OK;
+  if (N <= 32) hipLaunchKernelGGL(ce_few_grads_kernel<1>, grads, dim3(256), 0, st, a, g->dW, g->db, dx_part, g->accumulate);
+  else hipLaunchKernelGGL(ce_few_grads_kernel<2>, grads, dim3(256), 0, st, a, g->dW, g->db, dx_part, g->accumulate);
+  CNHIP_TRY(check_launch(who));
+  hipLaunchKernelGGL(ce_few_dx_kernel, dim3((unsigned)((N * D + 255) / 256)), dim3(256), 0, st, dx_part, g->dX, N * D,
+                     (int)slices);
+  return check_launch(who);
 }
 
 int run(const float* X, const float* W, const float* b, const int32_t* targets, float* loss, float* lse,
@@ -514,6 +785,7 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   a.lse = lse;
   a.oob = oob;
   a.mean = reduction == CNHIP_REDUCE_MEAN;
+  if (N <= kFewRows && D <= 64 * 65535) return run_few(a, loss, g, st, who);
   a.steps_d = (int)((D + 31) / 32 * 2);
   a.steps_v = (int)((V + 31) / 32 * 2);
   a.stat_blocks = (V + 127) / 128;

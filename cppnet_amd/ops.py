@@ -486,21 +486,25 @@ def _held(device_of, *operands) -> list:
     """Pointers of (tensor, name, values, dtype) operands, None for no tensor.
     Each has to be a contiguous tensor of that many values on device_of's device."""
     ptrs = []
+    device = getattr(device_of, "device", None)
     for t, name, n, dtype in operands:
         ptrs.append(_p(t, name))
         if t is None:
             continue
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
         if t.numel() != n:
             raise ValueError(f"{name}: expected {n} values, got {t.numel()}")
-        if t.device != device_of.device:
-            raise ValueError(f"{name} is on {t.device}, not on {device_of.device}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
     return ptrs
 
 
 def _call_on(t, name: str, *args) -> None:
     """Calls an entry point on t's device, on that device's current stream."""
+    if t.device.index == torch.cuda.current_device():
+        _capi.call(name, *args, _stream())
+        return
     with torch.cuda.device(t.device):
         _capi.call(name, *args, _stream())
 

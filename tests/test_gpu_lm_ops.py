@@ -224,7 +224,8 @@ def test_attention_large_scores(gpu):
 # ---------------------------------------------------- Linear + cross-entropy
 CE = [  # N, D, V, bias, targets, reduction, accumulate
     (1, 1, 1, False, "all", "mean", False), (1, 64, 1000, True, "all", "mean", False), (3, 5, 2, True, "some", "sum", True),
-    (64, 32, 100, False, "some", "mean", False), (65, 33, 257, True, "some", "mean", True),
+    (64, 32, 100, False, "some", "mean", False), (32, 65, 300, True, "some", "mean", True), (33, 130, 1000, False, "all", "sum", True),
+    (17, 513, 4100, True, "some", "mean", False), (65, 33, 257, True, "some", "mean", True),
     (130, 100, 1001, True, "all", "sum", False), (257, 128, 512, False, "none", "mean", True),
     (300, 256, 4096, True, "some", "mean", False), (513, 96, 333, True, "some", "mean", True),
     (1024, 64, 2048, False, "some", "mean", False),
