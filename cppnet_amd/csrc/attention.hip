@@ -494,20 +494,19 @@ __global__ void __launch_bounds__(NT) att_dkv_kernel(AttArgs a) {
 // probabilities and their gradients are split into their two terms in the
 // registers and multiplied without leaving them.
 //
-// Scales.  Each operand has one power of two per head of a sample.
-// Probabilities are at most 1 and enter times 2^14.
-// dS = P (dP - delta) is bounded by 2 max ||dout_i|| max ||v_j||, whose power
-// of two scales it.
-struct Scale {
-  uint32_t largest;  // |x|, bits
-  float norm;        // largest row's Euclidean norm
-};
-
+// Scales.  Every block of 32 rows of an operand has a power of two of its own,
+// from its largest value.  A score takes the two of its operands out again.
+// Where blocks are summed, the sum is kept in the scale of the head's largest
+// block, and the other factor, P or dS, carries the difference.  Probabilities
+// are at most 1 and enter times 2^14; dS = P (dP - delta) is bounded by 2 max
+// ||dout_i|| max ||v_j||, whose power of two scales it.
 struct PackArgs {
   Seq<const float> x[4];  // q, k, v, dout
-  char* p[4];
-  Scale* part[4];         // [head of a sample][chunks]
-  int chunks[4], chunk_rows[4], blocks[4];
+  char* p[4];             // [head of a sample][block][fragments]
+  int* exp[4];            // [head of a sample][block]: a block's exponent,
+  float* norm[4];         // its largest row's Euclidean norm
+  int blocks[4];
+  int first;              // the operand of block z 0 of the packing launch
 };
 
 struct PairArgs {
@@ -516,51 +515,40 @@ struct PairArgs {
   float *dk_part, *dv_part;  // [B][heads][dh][Sk], where heads share keys
 };
 
-// The scale of a head (of a sample) over its chunks, the same in every lane.
-__device__ __forceinline__ Scale scale_of(const PackArgs& p, int which, int64_t bh) {
-  uint32_t m = 0;
-  float n = 0.f;
-  const int i = threadIdx.x & 63;
-  if (i < p.chunks[which]) {
-    const Scale s = p.part[which][bh * p.chunks[which] + i];
-    m = s.largest;
-    n = s.norm;
-  }
+// The exponent of a head's largest block, the same in every lane.
+__device__ __forceinline__ int least_exp(const PackArgs& p, int which, int64_t bh) {
+  int e = 126;
+  for (int i = threadIdx.x & 63; i < p.blocks[which]; i += 64) e = min(e, p.exp[which][bh * p.blocks[which] + i]);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-    n = fmaxf(n, __shfl_xor(n, o, 64));
-  }
-  return Scale{(uint32_t)__builtin_amdgcn_readfirstlane((int)m),
-               __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(n)))};
+  for (int o = 32; o > 0; o >>= 1) e = min(e, __shfl_xor(e, o, 64));
+  return __builtin_amdgcn_readfirstlane(e);
+}
+// A block's exponent by a vector load: a scalar load under way turns every wait
+// for LDS into one for all of it.
+__device__ __forceinline__ int exp_at(const int* p, int64_t i) {
+  int zero = 0;
+  asm("" : "+v"(zero));
+  return p[i + zero];
+}
+// The largest row norm of a head.
+__device__ __forceinline__ float most_norm(const PackArgs& p, int which, int64_t bh) {
+  float n = 0.f;
+  for (int i = threadIdx.x & 63; i < p.blocks[which]; i += 64) n = fmaxf(n, p.norm[which][bh * p.blocks[which] + i]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n = fmaxf(n, __shfl_xor(n, o, 64));
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(n)));
 }
 
-// Rows of operand `which` that a sample has (past them k and v count as zeros).
-__device__ __forceinline__ int rows_of(const AttArgs& a, int which, int b) {
-  return which == 1 || which == 2 ? keys_of(a, b) : a.Sq;
-}
-
-// The head of operand `which` that block (.., y, z) of a packing launch has;
-// false where the operand has fewer heads.
+// The head of an operand that a wave works on, and the rows that its sample has
+// (past them k and v count as zeros).
 struct Operand {
   int which, b, head;
   int64_t bh;  // head of a sample, counted through
   int rows;
 };
-__device__ __forceinline__ bool operand_of(const AttArgs& a, Operand& o) {
-  o.which = (int)blockIdx.z;
-  const int heads = o.which == 1 || o.which == 2 ? a.kv_heads : a.heads;
-  o.b = (int)blockIdx.y / a.heads;
-  o.head = (int)blockIdx.y % a.heads;
-  o.bh = (int64_t)o.b * heads + o.head;
-  o.rows = rows_of(a, o.which, o.b);
-  return o.head < heads;
-}
-
-// The norm of a row whose squares sum to n; where they leave the range, its
-// bound by the largest value.
-__device__ __forceinline__ float norm_of(float n, uint32_t largest, int dh) {
-  return n > 1e-30f && n < 1e37f ? sqrtf(n) : __uint_as_float(largest) * sqrtf((float)dh);
+__device__ __forceinline__ Operand operand(const AttArgs& a, int which, int b, int head) {
+  const bool kv = which == 1 || which == 2;
+  return Operand{which, b, head, (int64_t)b * (kv ? a.kv_heads : a.heads) + head, kv ? keys_of(a, b) : a.Sq};
 }
 
 // 32 rows of a head in a wave's registers: features 16 s + 8 (lane / 32) .. + 7 of
@@ -568,18 +556,17 @@ __device__ __forceinline__ float norm_of(float n, uint32_t largest, int dh) {
 template <int KS>
 struct RowBlock {
   float v[KS][8];
-  __device__ __forceinline__ void load(const AttArgs& a, const PackArgs& p, const Operand& o, int blk) {
+  __device__ __forceinline__ void load(const AttArgs& a, const Seq<const float>& x, const Operand& o, int blk) {
     const int lane = (int)threadIdx.x & 63, r = blk * 32 + (lane & 31), d0 = 8 * (lane >> 5);
     const bool held = r < o.rows;
-    const Seq<const float>& x = p.x[o.which];
     const float* q = x.at(o.b, held ? r : 0, (int64_t)o.head * a.dh);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[s][e] = held && 16 * s + d0 + e < a.dh ? q[(16 * s + d0 + e) * x.col] : 0.f;
   }
-  // the largest finite value, and the largest row's norm, of the whole wave
-  __device__ __forceinline__ Scale scale(int dh) const {
+  // the exponent of the wave's largest finite value, and the largest row's norm
+  __device__ __forceinline__ int exponent(float* norm, int dh) const {
     uint32_t m = 0;
     float n = 0.f;
 #pragma unroll
@@ -596,122 +583,64 @@ struct RowBlock {
       m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
       n = fmaxf(n, __shfl_xor(n, o, 64));
     }
-    return Scale{m, norm_of(n, m, dh)};
+    // squares that leave the range: the bound by the largest value
+    if (norm) *norm = n > 1e-30f && n < 1e37f ? sqrtf(n) : __uint_as_float(m) * sqrtf((float)dh);
+    return pr::scale_exp((uint32_t)__builtin_amdgcn_readfirstlane((int)m));
   }
-  __device__ __forceinline__ void pack(const PackArgs& p, const Operand& o, int blk, float f) const {
-    const int lane = (int)threadIdx.x & 63;
-    char* q = p.p[o.which] + (o.bh * p.blocks[o.which] + blk) * KS * (2 * pr::kFrag);
+  // step s times f in terms, as this lane's fragment
+  __device__ __forceinline__ void terms(int s, float f, pr::f16x8 (&x)[2]) const {
+    pr::u32x4 hi, lo;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      pr::u32x4 hi, lo;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t w0, w1;
-        pr::split2(v[s][2 * e] * f, v[s][2 * e + 1] * f, w0, w1);
-        hi[e] = w0;
-        lo[e] = w1;
-      }
-      char* at = q + s * (2 * pr::kFrag) + pr::slot(lane, s);
-      *reinterpret_cast<pr::u32x4*>(at) = hi;
-      *reinterpret_cast<pr::u32x4*>(at + pr::kFrag) = lo;
+    for (int e = 0; e < 4; ++e) {
+      uint32_t w0, w1;
+      pr::split2(v[s][2 * e] * f, v[s][2 * e + 1] * f, w0, w1);
+      hi[e] = w0;
+      lo[e] = w1;
     }
+    x[0] = __builtin_bit_cast(pr::f16x8, hi);
+    x[1] = __builtin_bit_cast(pr::f16x8, lo);
   }
   // delta of the rows, these being dout's
   __device__ __forceinline__ void delta(const AttArgs& a, const Operand& o, int blk) const {
-    const int lane = (int)threadIdx.x & 63, r = blk * 32 + (lane & 31), d0 = 8 * (lane >> 5);
-    const bool held = r < o.rows;
-    const float* q = a.o.at(o.b, held ? r : 0, (int64_t)o.head * a.dh);
-    float x[KS][8], d = 0.f;
+    const int lane = (int)threadIdx.x & 63, r = blk * 32 + (lane & 31);
+    RowBlock<KS> out;
+    out.load(a, a.o, o, blk);
+    float d = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[s][e] = held && 16 * s + d0 + e < a.dh ? q[(16 * s + d0 + e) * a.o.col] : 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d = fmaf(v[s][e], x[s][e], d);
+      for (int e = 0; e < 8; ++e) d = fmaf(v[s][e], out.v[s][e], d);
     d += other_half(d);
-    if (held && lane < 32) a.delta[o.bh * a.Sq + r] = d;
+    if (r < o.rows && lane < 32) a.delta[o.bh * a.Sq + r] = d;
   }
 };
 
-// Short sequences, up to 32 rows a wave in one block: scale and packing of a
-// head with one reading.
-template <int KS>
-__global__ void __launch_bounds__(1024) att_pack_head_kernel(PairArgs g) {
-  __shared__ Scale part[16];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
-  Operand o;
-  if (!operand_of(g.a, o)) return;
-  RowBlock<KS> x;
-  x.load(g.a, g.p, o, wave);
-  Scale s = x.scale(g.a.dh);
-  if (lane == 0) part[wave] = s;
-  __syncthreads();
-  for (int w = 0; w < waves; ++w) {
-    s.largest = max(s.largest, part[w].largest);
-    s.norm = fmaxf(s.norm, part[w].norm);
-  }
-  if (threadIdx.x == 0) g.p.part[o.which][o.bh] = s;
-  if (wave >= g.p.blocks[o.which]) return;
-  x.pack(g.p, o, wave, pr::exp2i(pr::scale_exp(s.largest)));
-  if (o.which == 3) x.delta(g.a, o, wave);
-}
-
-// Longer ones: the scale of a chunk of rows of a head (a lane per row, 256
-// adjacent bytes a load, the four waves a quarter of the features each), then
-// the packing, a wave per 32 rows.
-template <int KS>
-__global__ void __launch_bounds__(NT) att_scale_kernel(PairArgs g) {
-  __shared__ float squares[4][64];
-  __shared__ uint32_t part[4];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const AttArgs& a = g.a;
-  Operand o;
-  if (!operand_of(a, o) || (int)blockIdx.x >= g.p.chunks[o.which]) return;
-  const Seq<const float>& x = g.p.x[o.which];
-  const int rows = g.p.chunk_rows[o.which];
-  constexpr int U = 4 * KS;
-  uint32_t m = 0;
-  float norm = 0.f;
-  for (int r0 = (int)blockIdx.x * rows; r0 < ((int)blockIdx.x + 1) * rows && r0 < o.rows; r0 += 64) {
-    const int r = r0 + lane;
-    const float* p = x.at(o.b, r < o.rows ? r : 0, (int64_t)o.head * a.dh);
-    float v[U], n = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = r < o.rows && wave * U + u < a.dh ? p[(wave * U + u) * x.col] : 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t bits = pr::finite_bits(v[u]);
-      m = max(m, bits);
-      n = fmaf(__uint_as_float(bits), __uint_as_float(bits), n);
-    }
-    squares[wave][lane] = n;
-    __syncthreads();
-    norm = fmaxf(norm, (squares[0][lane] + squares[1][lane]) + (squares[2][lane] + squares[3][lane]));
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 32; i > 0; i >>= 1) {
-    m = max(m, (uint32_t)__shfl_xor((int)m, i, 64));
-    norm = fmaxf(norm, __shfl_xor(norm, i, 64));
-  }
-  if (lane == 0) part[wave] = m;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  m = max(max(part[0], part[1]), max(part[2], part[3]));
-  g.p.part[o.which][o.bh * g.p.chunks[o.which] + blockIdx.x] = Scale{m, norm_of(norm, m, a.dh)};
-}
-
+// A wave packs 32 rows of a head; of dout it also leaves delta.
 template <int KS>
 __global__ void __launch_bounds__(NT) att_pack_kernel(PairArgs g) {
-  Operand o;
-  const int blk = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
-  if (!operand_of(g.a, o) || blk >= g.p.blocks[o.which]) return;
+  const int lane = (int)threadIdx.x & 63, which = (int)blockIdx.z + g.p.first;
+  const int head = (int)blockIdx.y % g.a.heads, blk = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+  if (blk >= g.p.blocks[which] || ((which == 1 || which == 2) && head >= g.a.kv_heads)) return;
+  const Operand o = operand(g.a, which, (int)blockIdx.y / g.a.heads, head);
   RowBlock<KS> x;
-  x.load(g.a, g.p, o, blk);
-  x.pack(g.p, o, blk, pr::exp2i(pr::scale_exp(scale_of(g.p, o.which, o.bh).largest)));
-  if (o.which == 3) x.delta(g.a, o, blk);
+  x.load(g.a, g.p.x[which], o, blk);
+  float norm;
+  const int e = x.exponent(&norm, g.a.dh);
+  const int64_t at = o.bh * g.p.blocks[which] + blk;
+  if (lane == 0) {
+    g.p.exp[which][at] = e;
+    g.p.norm[which][at] = norm;
+  }
+  char* q = g.p.p[which] + at * KS * (2 * pr::kFrag);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    pr::f16x8 t[2];
+    x.terms(s, pr::exp2i(e), t);
+    char* to = q + s * (2 * pr::kFrag) + pr::slot(lane, s);
+    *reinterpret_cast<pr::f16x8*>(to) = t[0];
+    *reinterpret_cast<pr::f16x8*>(to + pr::kFrag) = t[1];
+  }
+  if (which == 3) x.delta(g.a, o, blk);
 }
 
 // This block's head of a sample and 128 rows of it.  The longest go first (a
@@ -896,17 +825,17 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   const int lim = held ? limit(a, n, start, i) : 0;
   const int row0 = tile * 128 + 32 * __builtin_amdgcn_readfirstlane(wave);
   const int mine = tiles_read(a, n, start, row0), all = (limit(a, n, start, min(tile * 128 + 127, a.Sq - 1)) + 31) / 32;
-  const int ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest), ev = pr::scale_exp(scale_of(g.p, 2, bkh).largest);
-  const int eq = pr::scale_exp(scale_of(g.p, 0, bh).largest);
-  // not zero, so that a masked score stays -inf
-  const float c = fmaxf(pr::times_exp2(fabsf(a.scale) * kLog2e, -eq - ek), 0x1p-126f);
+  const int ev = least_exp(g.p, 2, bkh);
+  const int *kexp = g.p.exp[1] + bkh * g.p.blocks[1], *vexp = g.p.exp[2] + bkh * g.p.blocks[2];
   RowFrags<KS> q;
-  q.load(g.p.p[0] + (int64_t)bh * g.p.blocks[0] * TILE, held ? i : 0, held);
-  if (a.scale < 0.f) {
+  int eq;
+  {
+    RowBlock<KS> x;
+    x.load(a, a.q, operand(a, 0, b, head), row0 / 32);
+    eq = x.exponent(nullptr, a.dh);
+    const float f = a.scale < 0.f ? -pr::exp2i(eq) : pr::exp2i(eq);  // the scale's sign enters here
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) q.x[s][u] = pr::flip(q.x[s][u], 0x80008000u);
+    for (int u = 0; u < KS; ++u) x.terms(u, f, q.x[u]);
   }
   const char* kp = g.p.p[1] + bkh * g.p.blocks[1] * TILE;
   const char* vp = g.p.p[2] + bkh * g.p.blocks[2] * TILE;
@@ -916,9 +845,12 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   // tile t - 1, which then multiply its values.
   f32x16 s[1] = {};
   TileFrags p;
-  float base = 0.f;
-  // tile t's scores masked, the maximum and what it rescales
-  auto top = [&](int t) {
+  float base = 0.f, c = 0.f, part = 0.f;
+  // tile t's scores masked, the maximum and what it rescales; ek, the exponents
+  // of the tile's keys, and dv, by how much that of its values is above ev
+  auto top = [&](int t, int ek, int dv) {
+    // not zero, so that a masked score stays -inf
+    c = fmaxf(pr::times_exp2(fabsf(a.scale) * kLog2e, -eq - ek), 0x1p-126f);
     if (!__all(lim >= 32 * t + 32)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -939,28 +871,39 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
         for (int e = 0; e < 16; ++e) o[d][e] *= f;
       m = mn;
     }
-    base = (m == -INFINITY ? 0.f : m) - kPExp;
+    base = (m == -INFINITY ? 0.f : m) - kPExp + (float)dv;
+    part = 0.f;
   };
   auto pair = [&](const f32x16& x, int e) {
     const float p0 = __builtin_amdgcn_exp2f(fmaf(x[2 * e], c, -base)), p1 = __builtin_amdgcn_exp2f(fmaf(x[2 * e + 1], c, -base));
-    l += p0 + p1;
+    part += p0 + p1;
     p.split(e, p0, p1);
   };
   const RowFrags<KS>* const rows[1] = {&q};
   const TileFrags* const probs[1] = {&p};
   f32x16 (*const sums[1])[KS / 2] = {&o};
   if (all > 0) copy_tile<KS>(kp, kbuf[0]);
+  int ek = 0, evt = ev;  // tile t - 1's
   for (int t = 0; t <= all; ++t) {
     pr::wait_and_meet<0>();
+    const int u = min(t, all - 1), ek_next = all > 0 ? exp_at(kexp, u) : 0, ev_next = all > 0 ? exp_at(vexp, u) : ev;
     if (t + 1 < all) copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, kbuf[(t + 1) & 1]);
     if (t < all) copy_tile<KS>(vp + (int64_t)t * TILE, vbuf[t & 1]);
     if (t > mine) continue;
     const char* const now[1] = {kbuf[t & 1]};
+    // values below 2^-60 of the head's largest add nothing that is kept
+    const int over = __builtin_amdgcn_readfirstlane(evt) - ev;
+    const bool adds = over <= 60;
+    const int dv = adds ? over : 0;
     if (t == 0) {
       if (mine > 0) dot_pairs<KS, 1>(now, rows, s, [](int) {});
+      ek = ek_next;
+      evt = ev_next;
       continue;
     }
-    top(t - 1);
+    top(t - 1, ek, dv);
+    ek = ek_next;
+    evt = ev_next;
     const char* const before[1] = {vbuf[(t - 1) & 1]};
     Adder<KS, 1> add;
     if (t < mine) {
@@ -978,7 +921,8 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
 #pragma unroll
       for (int e = 0; e < 8; ++e) pair(s[0], e);
     }
-    add.run(before, probs, sums, [](int) {});
+    l += pr::times_exp2(part, dv);
+    if (adds) add.run(before, probs, sums, [](int) {});
   }
   l += other_half(l);
   const float f = lim > 0 ? 1.f / l : 0.f;
@@ -1000,8 +944,8 @@ __device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
 }
 
 // The exponent of dS: 2 max ||dout|| max ||v|| bounds it.
-__device__ __forceinline__ int grad_exp(const Scale& g, const Scale& v) {
-  const float bound = 2.f * g.norm * v.norm;
+__device__ __forceinline__ int grad_exp(const PackArgs& p, int64_t bh, int64_t bkh) {
+  const float bound = 2.f * most_norm(p, 3, bh) * most_norm(p, 2, bkh);
   return pr::scale_exp(__float_as_uint(fminf(bound, 3e38f)));
 }
 
@@ -1024,16 +968,16 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   const int lim = held ? limit(a, n, start, i) : 0;
   const int row0 = tile * 128 + 32 * __builtin_amdgcn_readfirstlane(wave);
   const int mine = tiles_read(a, n, start, row0), all = (limit(a, n, start, min(tile * 128 + 127, a.Sq - 1)) + 31) / 32;
-  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bh);
-  const int eq = pr::scale_exp(scale_of(g.p, 0, bh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
-  const int eg = pr::scale_exp(sg.largest), ev = pr::scale_exp(sv.largest), ed = grad_exp(sg, sv);
-  const float c = score_factor(a, eq + ek), cd = pr::times_exp2(1.f, ed - eg - ev);
-  const float none = copysignf(INFINITY, -c);  // the score of a key that is not read
+  const int ed = grad_exp(g.p, bh, bkh), ek = least_exp(g.p, 1, bkh), own = min(row0 / 32, g.p.blocks[0] - 1);
+  const int eq = g.p.exp[0][(int64_t)bh * g.p.blocks[0] + own], eg = g.p.exp[3][(int64_t)bh * g.p.blocks[3] + own];
+  const int *kexp = g.p.exp[1] + bkh * g.p.blocks[1], *vexp = g.p.exp[2] + bkh * g.p.blocks[2];
+  const float none = a.scale < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not read
   RowFrags<KS> q, go;
   q.load(g.p.p[0] + (int64_t)bh * g.p.blocks[0] * TILE, held ? i : 0, held);
   go.load(g.p.p[3] + (int64_t)bh * g.p.blocks[3] * TILE, held ? i : 0, held);
   const float lse = held ? lse2_of(a, b, head, i) : INFINITY;
-  const float delta = held ? pr::times_exp2(a.delta[(int64_t)bh * a.Sq + i], ed) : 0.f;
+  const float delta0 = held ? pr::times_exp2(a.delta[(int64_t)bh * a.Sq + i], ed) : 0.f;
+  float c = 0.f, cd = 0.f, delta = 0.f;
   const char* kp = g.p.p[1] + bkh * g.p.blocks[1] * TILE;
   const char* vp = g.p.p[2] + bkh * g.p.blocks[2] * TILE;
   f32x16 acc[DHP / 32] = {};
@@ -1051,15 +995,24 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   const RowFrags<KS>* const rows[2] = {&q, &go};
   const TileFrags* const probs[1] = {&p};
   f32x16 (*const sums[1])[KS / 2] = {&acc};
+  int ekt = 0, evt = 0;  // the next tile's
   if (all > 0) {
     copy_tile<KS>(kp, kbuf[0]);
     copy_tile<KS>(vp, vbuf[0]);
+    ekt = exp_at(kexp, 0);
+    evt = exp_at(vexp, 0);
   }
   for (int t = 0; t < all; ++t) {
     pr::wait_and_meet<0>();
+    // dS carries by how much the keys' exponent is above the head's
+    c = score_factor(a, eq + ekt);
+    cd = pr::times_exp2(1.f, ed - eg - evt - (ekt - ek));
+    delta = pr::times_exp2(delta0, -(ekt - ek));
     if (t + 1 < all) {
       copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, kbuf[(t + 1) & 1]);
       copy_tile<KS>(vp + (int64_t)(t + 1) * TILE, vbuf[(t + 1) & 1]);
+      ekt = exp_at(kexp, t + 1);
+      evt = exp_at(vexp, t + 1);
     }
     if (t >= mine) continue;
     const char* const now[2] = {kbuf[t & 1], vbuf[t & 1]};
@@ -1100,11 +1053,12 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
   const int n = keys_of(a, b);
   const int64_t start = start_of(a, b);
   const bool held = key < n;
-  const Scale sv = scale_of(g.p, 2, bkh), sg = scale_of(g.p, 3, bh);
-  const int eq = pr::scale_exp(scale_of(g.p, 0, bh).largest), ek = pr::scale_exp(scale_of(g.p, 1, bkh).largest);
-  const int eg = pr::scale_exp(sg.largest), ev = pr::scale_exp(sv.largest), ed = grad_exp(sg, sv);
-  const float c = score_factor(a, eq + ek), cd = pr::times_exp2(1.f, ed - eg - ev - (int)kPExp);
-  const float none = copysignf(INFINITY, -c);  // the score of a key that is not read
+  const int ed = grad_exp(g.p, bh, bkh), eq = least_exp(g.p, 0, bh), eg = least_exp(g.p, 3, bh);
+  const int own = min(key0 / 32 + __builtin_amdgcn_readfirstlane(wave), g.p.blocks[1] - 1);
+  const int ek = g.p.exp[1][bkh * g.p.blocks[1] + own], ev = g.p.exp[2][bkh * g.p.blocks[2] + own];
+  const int *qexp = g.p.exp[0] + (int64_t)bh * g.p.blocks[0], *gexp = g.p.exp[3] + (int64_t)bh * g.p.blocks[3];
+  const float none = a.scale < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not read
+  float c = 0.f, cd = 0.f;
   RowFrags<KS> k, v;
   k.load(g.p.p[1] + bkh * g.p.blocks[1] * TILE, held ? key : 0, held);
   v.load(g.p.p[2] + bkh * g.p.blocks[2] * TILE, held ? key : 0, held);
@@ -1115,15 +1069,19 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
   const char* qp = g.p.p[0] + ((int64_t)bh * g.p.blocks[0] + first) * TILE;
   const char* gp = g.p.p[3] + ((int64_t)bh * g.p.blocks[3] + first) * TILE;
   f32x16 dk[DHP / 32] = {}, dv[DHP / 32] = {};
-  float st = 0.f;
-  auto copy = [&](int t, int buf) {
-    copy_tile<KS>(qp + (int64_t)t * TILE, qbuf[buf]);
-    copy_tile<KS>(gp + (int64_t)t * TILE, gbuf[buf]);
-    const int64_t i = (first + t) * 32 + (lane & 31);
-    if (wave != 0) return;
-    if (i >= a.Sq) st = lane < 32 ? INFINITY : 0.f;
-    else if (lane < 32) st = lse2_of(a, b, head, i) - kPExp;
-    else st = pr::times_exp2(a.delta[(int64_t)bh * a.Sq + i], ed - (int)kPExp);
+  // Of the next tile: its exponents, and a query's lse (lanes 0 .. 31) or delta,
+  // as loaded: they are on their way with the copies
+  int eqt = 0, egt = 0;
+  float raw = 0.f;
+  auto copy = [&](int t) {
+    copy_tile<KS>(qp + (int64_t)t * TILE, qbuf[t & 1]);
+    copy_tile<KS>(gp + (int64_t)t * TILE, gbuf[t & 1]);
+    eqt = exp_at(qexp, first + t);
+    egt = exp_at(gexp, first + t);
+    const int64_t i = min((first + t) * 32 + (lane & 31), (int64_t)a.Sq - 1);
+    const float* p = lane < 32 ? a.lse_in + b * a.lse_sample + i * a.lse_row + head * a.lse_col
+                               : a.delta + (int64_t)bh * a.Sq + i;
+    if (wave == 0) raw = *p;
   };
   // A wave's first tile is that of the first query that reads its first key.
   const int64_t skip = a.causal ? key0 + 32 * __builtin_amdgcn_readfirstlane(wave) - start - first * 32 : 0;
@@ -1144,11 +1102,24 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
   const RowFrags<KS>* const rows[2] = {&k, &v};
   const TileFrags* const probs[2] = {&p, &ds};
   f32x16 (*const sums[2])[KS / 2] = {&dv, &dk};
-  if (total > 0) copy(0, 0);
+  if (total > 0) copy(0);
   for (int t = 0; t < total; ++t) {
-    if (wave == 0) stat[t & 1][lane >> 5][lane & 31] = st;
+    // P carries by how much the exponent of the tile's output gradients is above
+    // the head's (by more than 60: they add nothing that is kept), and dS that of
+    // its queries; shift: the exponent of dS over that of P
+    const int over = egt - eg, shift = ed - (eqt - eq) - (int)kPExp + over;
+    const bool adds = over <= 60;
+    c = score_factor(a, eqt + ek);
+    cd = adds ? pr::times_exp2(1.f, shift - egt - ev) : 0.f;
+    if (wave == 0) {
+      const bool in = adds && (first + t) * 32 + (lane & 31) < a.Sq;
+      float st = lane < 32 ? INFINITY : 0.f;
+      if (in && lane >= 32) st = pr::times_exp2(raw, shift);
+      else if (in && raw != -INFINITY) st = raw * kLog2e - kPExp + (float)over;
+      stat[t & 1][lane >> 5][lane & 31] = st;
+    }
     pr::wait_and_meet<0>();
-    if (t + 1 < total) copy(t + 1, (t + 1) & 1);
+    if (t + 1 < total) copy(t + 1);
     if (t < from) continue;
     const char* const now[2] = {qbuf[t & 1], gbuf[t & 1]};
     dot_pairs<KS, 2>(now, rows, s, [](int) {});
@@ -1220,56 +1191,52 @@ void by_width(int dh, F&& f) {
   else f(std::integral_constant<int, 128>{});
 }
 
-// Lays out the workspace of the packed operands and packs them.  ops: 3 (q, k,
-// v) or 4; with dout's packing comes delta.
-int pack(PairArgs& g, int ops, hipStream_t st, const char* who) {
+// Lays out the workspace of the packed operands and packs them: k and v, and
+// for the backward q and dout too, with whose packing comes delta.
+int pack(PairArgs& g, bool backward, hipStream_t st, const char* who) {
   AttArgs& a = g.a;
   PackArgs& p = g.p;
   const int steps = a.dh <= 32 ? 2 : a.dh <= 64 ? 4 : a.dh <= 96 ? 6 : 8;
-  const int most = a.Sq > a.Sk ? a.Sq : a.Sk;
-  const bool one = most <= 512;  // 16 waves of 32 rows
-  size_t bytes = 0, part[4], data[4];
+  p.first = backward ? 0 : 1;
+  const int last = backward ? 3 : 2;
+  size_t bytes = 0, data[4], exps[4], norms[4];
   auto place_bytes = [&](size_t n) {
     const size_t at = bytes;
     bytes += (n + 255) / 256 * 256;
     return at;
   };
-  for (int w = 0; w < ops; ++w) {
+  int most = 0;
+  for (int w = p.first; w <= last; ++w) {
     const bool kv = w == 1 || w == 2;
-    const int64_t S = kv ? a.Sk : a.Sq, heads = kv ? a.kv_heads : a.heads;
-    p.blocks[w] = (int)((S + 31) / 32);
-    p.chunk_rows[w] = (int)((S + 64 * 64 - 1) / (64 * 64) * 64);  // 64 chunks at most
-    p.chunks[w] = one ? 1 : (int)((S + p.chunk_rows[w] - 1) / p.chunk_rows[w]);
-    part[w] = place_bytes((size_t)a.B * heads * p.chunks[w] * sizeof(Scale));
-    data[w] = place_bytes((size_t)a.B * heads * p.blocks[w] * steps * 2 * pr::kFrag);
+    p.blocks[w] = (int)(((kv ? a.Sk : a.Sq) + 31) / 32);
+    most = p.blocks[w] > most ? p.blocks[w] : most;
+    const size_t n = (size_t)a.B * (kv ? a.kv_heads : a.heads) * p.blocks[w];
+    data[w] = place_bytes(n * steps * 2 * pr::kFrag);
+    exps[w] = place_bytes(n * sizeof(int));
+    norms[w] = place_bytes(n * sizeof(float));
   }
-  const size_t delta = place_bytes(ops == 4 ? (size_t)a.B * a.heads * a.Sq * sizeof(float) : 0);
-  const size_t sums = ops == 4 && a.group > 1 ? (size_t)a.B * a.heads * a.dh * a.Sk * sizeof(float) : 0;
+  const size_t delta = place_bytes(backward ? (size_t)a.B * a.heads * a.Sq * sizeof(float) : 0);
+  const size_t sums = backward && a.group > 1 ? (size_t)a.B * a.heads * a.dh * a.Sk * sizeof(float) : 0;
   const size_t dk_part = place_bytes(sums), dv_part = place_bytes(sums);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, bytes, &ws, who));
   char* base = static_cast<char*>(ws);
   g.dk_part = reinterpret_cast<float*>(base + dk_part);
   g.dv_part = reinterpret_cast<float*>(base + dv_part);
-  for (int w = 0; w < ops; ++w) {
-    p.part[w] = reinterpret_cast<Scale*>(base + part[w]);
+  for (int w = p.first; w <= last; ++w) {
     p.p[w] = base + data[w];
+    p.exp[w] = reinterpret_cast<int*>(base + exps[w]);
+    p.norm[w] = reinterpret_cast<float*>(base + norms[w]);
   }
   a.delta = reinterpret_cast<float*>(base + delta);
   p.x[0] = a.q;
   p.x[1] = a.k;
   p.x[2] = a.v;
   p.x[3] = a.dout;
-  const unsigned bh = (unsigned)(a.B * a.heads), blocks = (unsigned)((most + 31) / 32);
   by_width(a.dh, [&](auto d) {
-    constexpr int KS = d() / 16;
-    if (one) {
-      hipLaunchKernelGGL(att_pack_head_kernel<KS>, dim3(1, bh, (unsigned)ops), dim3(64 * blocks), 0, st, g);
-    } else {
-      const int chunks = p.chunks[0] > p.chunks[1] ? p.chunks[0] : p.chunks[1];
-      hipLaunchKernelGGL(att_scale_kernel<KS>, dim3((unsigned)chunks, bh, (unsigned)ops), dim3(NT), 0, st, g);
-      hipLaunchKernelGGL(att_pack_kernel<KS>, dim3((blocks + 3) / 4, bh, (unsigned)ops), dim3(NT), 0, st, g);
-    }
+    hipLaunchKernelGGL(att_pack_kernel<d() / 16>,
+                       dim3((unsigned)((most + 3) / 4), (unsigned)(a.B * a.heads), (unsigned)(last - p.first + 1)), dim3(NT),
+                       0, st, g);
   });
   return check_launch(who);
 }
@@ -1360,7 +1327,7 @@ int cnhip_attention_forward(const float* q, const float* k, const float* v, floa
   a.lse = lse;
   if (cnhip::use_pairs(a)) {
     cnhip::PairArgs g{a, {}, nullptr, nullptr};
-    CNHIP_TRY(cnhip::pack(g, 3, st, who));
+    CNHIP_TRY(cnhip::pack(g, false, st, who));
     const int tiles = (int)((Sq + 127) / 128);
     cnhip::by_width(a.dh, [&](auto d) {
       hipLaunchKernelGGL((cnhip::att_fwd_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st,
@@ -1413,7 +1380,7 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
   a.lse_in = lse;
   if (cnhip::use_pairs(a)) {
     cnhip::PairArgs g{a, {}, nullptr, nullptr};
-    CNHIP_TRY(cnhip::pack(g, 4, st, who));
+    CNHIP_TRY(cnhip::pack(g, true, st, who));
     const int tiles = (int)((Sq + 127) / 128), key_tiles = (int)((Sk + 127) / 128);
     cnhip::by_width(a.dh, [&](auto d) {
       hipLaunchKernelGGL((cnhip::att_dkv_pair_kernel<d()>), dim3((unsigned)(key_tiles * B * heads)), dim3(cnhip::NT), 0,
