@@ -56,6 +56,8 @@ struct CeArgs {
   CeState* state;
   uint32_t *row_max, *w_part;  // largest finite |X| of each row, |W| of each block's part
   int w_blocks;
+  int *xe, *we;                // without gradients: the exponents of a row of X, of 32 rows of W^T
+  float* zt;                   // and the logit of a row's target
   char *xp, *wp, *gp;  // packed X [N x D], W^T [V x D], the piece's G [R x V]
   int steps_d, steps_v;
   float* db_part;      // [ceil(R / 256)][V], or null
@@ -238,6 +240,73 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(CeArgs a, int64_t w_frags,
   put_frag(a.xp, f % blocks, a.steps_d, step, x);
 }
 
+// Without gradients no sum runs over blocks of W or rows of X, and each is packed
+// with an exponent of its own: one launch, a block of eight waves for 32 rows,
+// which reads them twice (the second time from the L2).
+__global__ void __launch_bounds__(512) ce_pack_own_kernel(CeArgs a, int w_blocks) {
+  __shared__ uint32_t part[8][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+  const bool w = (int)blockIdx.x < w_blocks;
+  const int64_t blk = w ? blockIdx.x : (int64_t)blockIdx.x - w_blocks, row = blk * 32 + r;
+  const bool in = row < (w ? a.V : a.N), held = w || (in && has_target(a, row));
+  auto load = [&](int step, float (&x)[8]) {
+    const int64_t d0 = step * 16 + 8 * h;
+    if (w) {
+      const float* p = a.W + row * a.D + d0;
+      if (in && d0 + 8 <= a.D) {
+        const f32x4 lo = *reinterpret_cast<const f32x4u*>(p), hi = *reinterpret_cast<const f32x4u*>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = lo[e];
+          x[4 + e] = hi[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = in && d0 + e < a.D ? p[e] : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = in && d0 + e < a.D ? a.X[row + a.N * (d0 + e)] : 0.f;
+    }
+  };
+  uint32_t m = 0;
+  for (int s0 = wave; s0 < a.steps_d; s0 += 32) {
+    float x[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (s0 + 8 * u < a.steps_d) load(s0 + 8 * u, x[u]);
+      else
+        for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, pr::finite_bits(x[u][e]));
+  }
+  if (w) m = wave_max(m);
+  else m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+  if (lane < 32) part[wave][lane] = m;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) m = max(m, part[q][r]);
+  const int exp = pr::scale_exp(m);
+  const float f = pr::exp2i(exp);
+  if (wave == 0 && lane < 32) {
+    if (!w && in) a.xe[row] = exp;
+    if (w && lane == 0) a.we[blk] = exp;
+  }
+  for (int step = wave; step < a.steps_d; step += 8) {
+    float x[8];
+    load(step, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (!held) x[e] = x[e] - x[e] == 0.f ? x[e] : 0.f;
+      x[e] *= f;
+    }
+    put_frag(w ? a.wp : a.xp, blk, a.steps_d, step, x);
+  }
+}
+
 // ------------------------------------------------------------- the products
 // Element (m, n) of a product goes to out[n + ld m].
 struct Out {
@@ -290,8 +359,10 @@ __device__ __forceinline__ void put_tile(const pr::Acc& acc, int tm, int tn, int
   }
 }
 
-// Logits of a piece (M: classes, N: rows): stored, with each row's maximum and
-// sum of exponentials over the wave's 128 classes.
+// Logits of a piece (M: classes, N: rows) with each row's maximum and sum of
+// exponentials over the wave's 128 classes; stored for the gradients, else the
+// targets' alone.
+template <bool GRADS>
 __global__ void __launch_bounds__(pr::GNT, 2) ce_logits_kernel(pr::GemmArgs g, CeArgs a) {
   __shared__ __align__(16) char lds[pr::kGemmLds];
   int tm, tn;
@@ -299,14 +370,16 @@ __global__ void __launch_bounds__(pr::GNT, 2) ce_logits_kernel(pr::GemmArgs g, C
   pr::Acc acc;
   pr::gemm_tile<false, false>(g, tm, tn, 0, g.steps, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int ez[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
-    ez[j] = -pr::scale_exp(a.state->w_max) - x_exp(a, a.row0 + min(n, g.N - 1));
-  }
   const int m0 = tm * pr::TM + (wave >> 2) * 128;
   if (m0 >= g.M) return;
+  int ex[2], ew[4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t n = a.row0 + min(tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31), g.N - 1);
+    ex[j] = GRADS ? x_exp(a, n) : a.xe[n];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ew[i] = GRADS ? pr::scale_exp(a.state->w_max) : a.we[min(m0 / 32 + i, (g.M - 1) / 32)];
   const bool whole = m0 + 128 <= g.M;
   auto row = [&](int i, int e) { return m0 + 32 * i + 8 * (e / 4) + 4 * (lane >> 5) + e % 4; };
 #pragma unroll
@@ -315,7 +388,7 @@ __global__ void __launch_bounds__(pr::GNT, 2) ce_logits_kernel(pr::GemmArgs g, C
     for (int e = 0; e < 16; ++e) {
       const float b = a.b ? a.b[min(row(i, e), g.M - 1)] : 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc.x[i][j][e] = pr::times_exp2(acc.x[i][j][e], ez[j]) + b;
+      for (int j = 0; j < 2; ++j) acc.x[i][j][e] = pr::times_exp2(acc.x[i][j][e], -ex[j] - ew[i]) + b;
     }
   if (!whole) {
 #pragma unroll
@@ -344,8 +417,24 @@ __global__ void __launch_bounds__(pr::GNT, 2) ce_logits_kernel(pr::GemmArgs g, C
     sum += __shfl_xor(sum, 32, 64);
     if (n >= g.N) continue;
     if (lane < 32) a.stat[(int64_t)(tm * 2 + (wave >> 2)) * a.R + n] = float2{top, sum};
+    if (!GRADS) {
+      const int32_t t = a.t[a.row0 + n];
+      if (t < m0 || t >= min(m0 + 128, g.M)) continue;
+      const int at = t - row(0, 0);  // this lane has it where it is one of row(i, e) - row(0, 0)
+      float z = 0.f;
+      bool mine = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (at == 32 * i + 8 * (e / 4) + e % 4) {
+            z = acc.x[i][j][e];
+            mine = true;
+          }
+      if (mine) a.zt[a.row0 + n] = z;
+    }
   }
-  put_tile<false>(acc, tm, tn, g.M, g.N, a.Z, a.R, [](float x) { return x; });
+  if (GRADS) put_tile<false>(acc, tm, tn, g.M, g.N, a.Z, a.R, [](float x) { return x; });
 }
 
 // dX (A: W across its rows, B: G) and dW (A: G, B: X, both across their rows)
@@ -383,27 +472,47 @@ __global__ void __launch_bounds__(256) ce_reduce_kernel(CeArgs a, Out o, int M, 
 }
 
 // ------------------------------------------------------------- row by row
+// One row's statistics joined: this lane's parts q0, q0 + 16, ... of stat.
+__device__ __forceinline__ float2 join_stats(const CeArgs& a, int64_t q0, int64_t rows, int64_t r) {
+  float m = -INFINITY, s = 0.f;
+  constexpr int U = 8;  // loads under way
+  for (; q0 < a.stat_blocks; q0 += 16 * U) {
+    float2 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      x[u] = q0 + 16 * u < a.stat_blocks ? a.stat[(q0 + 16 * u) * rows + r] : float2{-INFINITY, 0.f};
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, x[u].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    s *= expf(m - base);
+#pragma unroll
+    for (int u = 0; u < U; ++u) s += x[u].y * expf(x[u].x - base);
+    m = top;
+  }
+  return float2{m, s};
+}
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
+  return float2{m, a.y * expf(a.x - base) + b.y * expf(b.x - base)};
+}
+
 // lse and loss of 64 rows a block; the 16 waves share the row's parts.
-__global__ void __launch_bounds__(1024) ce_row_kernel(CeArgs a) {
+__global__ void __launch_bounds__(1024) ce_row_kernel(CeArgs a, int grads) {
   __shared__ float2 part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = (int64_t)blockIdx.x * 64 + lane;
-  float m = -INFINITY, s = 0.f;
-  auto add = [&](float2 x) {
-    const float mn = fmaxf(m, x.x), base = mn == -INFINITY ? 0.f : mn;
-    s = s * expf(m - base) + x.y * expf(x.x - base);
-    m = mn;
-  };
-  if (r < a.R)
-    for (int64_t q = wave; q < a.stat_blocks; q += 16) add(a.stat[q * a.R + r]);
-  part[wave][lane] = float2{m, s};
+  float2 x = {-INFINITY, 0.f};
+  if (r < a.R) x = join_stats(a, wave, a.R, r);
+  part[wave][lane] = x;
   __syncthreads();
   if (wave || r >= a.R) return;
-  for (int w = 1; w < 16; ++w) add(part[w][lane]);
-  const float lse = m + logf(s);
+  for (int w = 1; w < 16; ++w) x = join(x, part[w][lane]);
+  const float lse = x.x + logf(x.y);
   const int64_t n = a.row0 + r;
+  const bool held = has_target(a, n);
   a.lse[n] = lse;
-  a.row_loss[n] = has_target(a, n) ? lse - a.Z[r + a.R * (int64_t)a.t[n]] : 0.f;
+  a.row_loss[n] = held ? lse - (grads ? a.Z[r + a.R * (int64_t)a.t[n]] : a.zt[n]) : 0.f;
 }
 
 // The piece's G packed, a wave for a step of 16 classes and eight blocks of 32
@@ -418,7 +527,6 @@ __global__ void __launch_bounds__(256) ce_grad_kernel(CeArgs a) {
   const int64_t v0 = (int64_t)step * 16 + 8 * h;
   const float one = pr::exp2i(kGExp);
   float sum[8] = {};
-#pragma unroll 2
   for (int64_t b = grp * 8; b < (grp * 8 + 8 < blocks ? grp * 8 + 8 : blocks); ++b) {
     const int64_t n = b * 32 + r;
     const bool in = n < a.R;
@@ -455,19 +563,48 @@ __global__ void __launch_bounds__(256) ce_db_kernel(CeArgs a, float* db, int acc
   db[v] = accumulate ? db[v] + s : s;
 }
 
-// the losses of the rows in a fixed order (one block)
-__global__ void __launch_bounds__(1024) ce_loss_kernel(CeArgs a, float* __restrict__ loss) {
-  __shared__ float part[1024];
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < a.N; i += 1024) s += a.row_loss[i];
-  part[threadIdx.x] = s;
+// The losses of the rows in a fixed order (one block); `count`: also the targets
+// past the last class, where no state kernel does.
+__global__ void __launch_bounds__(1024) ce_loss_kernel(CeArgs a, float* __restrict__ loss, int count) {
+  __shared__ float part[16];
+  __shared__ int total[2];
+  if (threadIdx.x < 2) total[threadIdx.x] = 0;
   __syncthreads();
-  for (int w = 512; w > 0; w >>= 1) {
-    if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
-    __syncthreads();
+  float s = 0.f;
+  int n = 0, past = 0;
+  constexpr int U = 8;  // loads under way
+  for (int64_t i0 = threadIdx.x; i0 < a.N; i0 += U * 1024) {
+    float l[U];
+    int32_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * 1024;
+      l[u] = i < a.N ? a.row_loss[i] : 0.f;
+      t[u] = i < a.N ? a.t[i] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s += l[u];
+      n += t[u] >= 0 && t[u] < a.V;
+      past += t[u] >= a.V;
+    }
   }
-  const int held = a.state->held;
-  if (threadIdx.x == 0) *loss = a.mean ? part[0] / (float)(held > 0 ? held : 1) : part[0];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    n += __shfl_xor(n, o, 64);
+    past += __shfl_xor(past, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    part[threadIdx.x >> 6] = s;
+    atomicAdd(&total[0], n);
+    atomicAdd(&total[1], past);
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 16; ++w) s += part[w];
+  *loss = a.mean ? s / (float)(total[0] > 0 ? total[0] : 1) : s;
+  if (count && a.oob && total[1]) atomicAdd(a.oob, total[1]);
 }
 
 // ------------------------------------------------------------ few rows
@@ -572,36 +709,15 @@ __global__ void __launch_bounds__(512) ce_few_logits_kernel(CeArgs a) {
 __global__ void __launch_bounds__(1024) ce_few_rows_kernel(CeArgs a, float* __restrict__ loss) {
   __shared__ float2 part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float m = -INFINITY, s = 0.f;
-  if (lane < a.N) {
-    constexpr int U = 8;
-    for (int64_t q0 = wave; q0 < a.stat_blocks; q0 += 16 * U) {
-      float2 x[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        x[u] = q0 + 16 * u < a.stat_blocks ? a.stat[(q0 + 16 * u) * a.N + lane] : float2{-INFINITY, 0.f};
-      float top = m;
-#pragma unroll
-      for (int u = 0; u < U; ++u) top = fmaxf(top, x[u].x);
-      const float base = top == -INFINITY ? 0.f : top;
-      s *= expf(m - base);
-#pragma unroll
-      for (int u = 0; u < U; ++u) s += x[u].y * expf(x[u].x - base);
-      m = top;
-    }
-  }
-  part[wave][lane] = float2{m, s};
+  float2 x = {-INFINITY, 0.f};
+  if (lane < a.N) x = join_stats(a, wave, a.N, lane);
+  part[wave][lane] = x;
   __syncthreads();
   if (wave) return;
-  for (int w = 1; w < 16; ++w) {
-    const float2 x = part[w][lane];
-    const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.f : top;
-    s = s * expf(m - base) + x.y * expf(x.x - base);
-    m = top;
-  }
+  for (int w = 1; w < 16; ++w) x = join(x, part[w][lane]);
   const int32_t t = lane < a.N ? a.t[lane] : -1;
   const bool held = t >= 0 && t < a.V;
-  const float lse = m + logf(s);
+  const float lse = x.x + logf(x.y);
   if (lane < a.N) a.lse[lane] = lse;
   float l = held ? lse - a.Z[lane + a.N * (int64_t)t] : 0.f;
 #pragma unroll
@@ -789,9 +905,10 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   a.steps_d = (int)((D + 31) / 32 * 2);
   a.steps_v = (int)((V + 31) / 32 * 2);
   a.stat_blocks = (V + 127) / 128;
-  // rows of a piece: 2^26 logits, but 1024 rows at least, so that the
-  // gradients of W are read and written once in 1024 rows at most
-  const int64_t most = ((int64_t)1 << 26) / V;
+  // Rows of a piece: 2^27 logits (half a GiB, and as much for G), but 1024 rows
+  // at least, so that the gradients of W are read and written once in 1024 rows
+  // at most.  8192 rows, 1024 -> 32000: 2^26 4.98 ms, 2^27 4.61, 2^28 4.46.
+  const int64_t most = ((int64_t)1 << 27) / V;
   int64_t R = most < 1024 ? 1024 : most / 256 * 256;
   if (R > N) R = N;
   const int64_t Rp = (R + 31) / 32 * 32, Np = (N + 31) / 32 * 32, Vp = (V + 31) / 32 * 32, Dp = (D + 31) / 32 * 32;
@@ -806,8 +923,9 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   };
   const size_t o_state = place(sizeof(CeState)), o_loss = place((size_t)N * 4), o_rows = place((size_t)N * 4),
                o_wpart = place((size_t)a.w_blocks * 4), o_x = place((size_t)(Np * Dp) * 4),
-               o_w = place((size_t)(Vp * Dp) * 4), o_z = place((size_t)R * (size_t)V * 4),
-               o_stat = place((size_t)a.stat_blocks * (size_t)R * 8);
+               o_w = place((size_t)(Vp * Dp) * 4), o_z = place(g ? (size_t)R * (size_t)V * 4 : 0),
+               o_stat = place((size_t)a.stat_blocks * (size_t)R * 8), o_xe = place(g ? 0 : (size_t)N * 4),
+               o_we = place(g ? 0 : (size_t)(Vp / 32) * 4), o_zt = place(g ? 0 : (size_t)N * 4);
   const size_t o_g = place(g ? (size_t)(Rp * Vp) * 4 : 0), o_db = place(g && g->db ? (size_t)((R + 255) / 256 * V) * 4 : 0);
   const size_t px = sx.splits > 1 ? (size_t)sx.splits * (size_t)(D * R) * 4 : 0,
                pw = sw.splits > 1 ? (size_t)sw.splits * (size_t)(V * D) * 4 : 0;
@@ -824,16 +942,24 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   a.Z = reinterpret_cast<float*>(base + o_z);
   a.stat = reinterpret_cast<float2*>(base + o_stat);
   a.gp = base + o_g;
+  a.xe = reinterpret_cast<int*>(base + o_xe);
+  a.we = reinterpret_cast<int*>(base + o_we);
+  a.zt = reinterpret_cast<float*>(base + o_zt);
   a.db_part = g && g->db ? reinterpret_cast<float*>(base + o_db) : nullptr;
   float* part = reinterpret_cast<float*>(base + o_part);
 
-  hipLaunchKernelGGL(ce_max_kernel, dim3((unsigned)(a.w_blocks + (N + 63) / 64)), dim3(1024), 0, st, a);
-  CNHIP_TRY(check_launch(who));
-  hipLaunchKernelGGL(ce_state_kernel, dim3(1), dim3(1024), 0, st, a);
-  CNHIP_TRY(check_launch(who));
-  const int64_t w_frags = Vp / 32 * a.steps_d, x_frags = Np / 32 * a.steps_d;
-  hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)((w_frags + x_frags + 3) / 4)), dim3(256), 0, st, a, w_frags, x_frags);
-  CNHIP_TRY(check_launch(who));
+  if (g) {
+    hipLaunchKernelGGL(ce_max_kernel, dim3((unsigned)(a.w_blocks + (N + 63) / 64)), dim3(1024), 0, st, a);
+    CNHIP_TRY(check_launch(who));
+    hipLaunchKernelGGL(ce_state_kernel, dim3(1), dim3(1024), 0, st, a);
+    CNHIP_TRY(check_launch(who));
+    const int64_t w_frags = Vp / 32 * a.steps_d, x_frags = Np / 32 * a.steps_d;
+    hipLaunchKernelGGL(ce_pack_kernel, dim3((unsigned)((w_frags + x_frags + 3) / 4)), dim3(256), 0, st, a, w_frags, x_frags);
+    CNHIP_TRY(check_launch(who));
+  } else {
+    hipLaunchKernelGGL(ce_pack_own_kernel, dim3((unsigned)((Vp + Np) / 32)), dim3(512), 0, st, a, (int)(Vp / 32));
+    CNHIP_TRY(check_launch(who));
+  }
 
   const pr::Packed pw_{a.wp, (int)(Vp / 32), a.steps_d};
   auto tiles = [](int64_t M, int64_t Nn) { return (M + pr::TM - 1) / pr::TM * ((Nn + pr::TN - 1) / pr::TN); };
@@ -845,10 +971,12 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
     const pr::Packed pg_{a.gp, rb, a.steps_v};
     {
       const pr::GemmArgs ga{pw_, px_, (int)V, (int)a.R, a.steps_d, a.steps_d, a.steps_d / 2};
-      hipLaunchKernelGGL(ce_logits_kernel, dim3((unsigned)tiles(V, a.R)), dim3(pr::GNT), 0, st, ga, a);
+      const dim3 grid((unsigned)tiles(V, a.R));
+      if (g) hipLaunchKernelGGL(ce_logits_kernel<true>, grid, dim3(pr::GNT), 0, st, ga, a);
+      else hipLaunchKernelGGL(ce_logits_kernel<false>, grid, dim3(pr::GNT), 0, st, ga, a);
       CNHIP_TRY(check_launch(who));
     }
-    hipLaunchKernelGGL(ce_row_kernel, dim3((unsigned)((a.R + 63) / 64)), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(ce_row_kernel, dim3((unsigned)((a.R + 63) / 64)), dim3(1024), 0, st, a, g ? 1 : 0);
     CNHIP_TRY(check_launch(who));
     if (!g) continue;
     const int add = g->accumulate || r0 > 0;
@@ -874,7 +1002,7 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
                     Out{g->dX + r0, N, nullptr, 0, 1, 2}));
     CNHIP_TRY(grads(ce_grads_kernel<true, true>, pg_, px_, V, D, 2 * rb, sw, Out{g->dW, D, nullptr, add, 0, 2}));
   }
-  hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(1024), 0, st, a, loss);
+  hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(1024), 0, st, a, loss, g ? 0 : 1);
   return check_launch(who);
 }
 
