@@ -7,19 +7,20 @@
 //   dq = dS k,  dk = dS^T q,  dv = P^T dout   (dk, dv summed over the query
 //   heads that share a key head).
 //
-// The products run on fp32 MFMAs (v_mfma_f32_32x32x2f32) whose accumulators
-// feed the next product without leaving the registers.  An accumulator holds
-// for its column (lane & 31) the rows 8 (r / 4) + 4 (lane / 32) + r % 4, and a
-// B operand holds for its column one k per half-wave: register r of a score
-// tile is the B operand of the k pair {8 (r / 4) + r % 4, the same + 4}.  So the
-// scores are formed with the contraction of the product that follows along
-// their rows: S^T = k q^T for out and dq (keys along the rows, a query per
-// lane, whose maximum, sum and rescaling are the lane's own), S = q k^T for dk
-// and dv (queries along the rows, a key per lane).  The features of a row lie
-// a whole column apart in memory, so a [feature][row] tile in LDS is staged
-// with float4s along the rows as it stands, and serves both as the operand
-// whose lanes are rows (one float per lane) and as the one whose lanes are
-// features (four rows per float4).
+// Three ways, by rules whose comments measure both sides: single tokens on the
+// vector ALUs (att_few_kernel), a forward of few queries on fp32 MFMAs with the
+// keys split over blocks (att_fwd_kernel), everything else, the backward above
+// all, on the fp16 matrix cores over operands packed as pairs.
+//
+// On either matrix core a product's accumulators feed the next one without
+// leaving the registers.  An accumulator of 32 x 32 holds for its column (lane &
+// 31) the rows 8 (r / 4) + 4 (lane / 32) + r % 4, and a B operand holds for its
+// column some k's per half-wave, so the order in which the other operand's k's are
+// taken can be that of the accumulator.  So the scores are formed with the
+// contraction of the product that follows along their rows: S^T = k q^T for out
+// and dq (keys along the rows, a query per lane, whose maximum, sum and rescaling
+// are the lane's own), S = q k^T for dk and dv (queries along the rows, a key per
+// lane).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -59,12 +60,15 @@ struct AttArgs {
   const int32_t *k_len, *q_start;
 };
 
-// Keys of sample b, and the position of its first query.
-__device__ __forceinline__ int keys_of(const AttArgs& a, int b) {
-  return a.k_len ? min(max(a.k_len[b], 0), a.Sk) : a.Sk;
-}
+// The position of the first query of sample b, and the sample's keys: those past
+// its last query's are not among them, so a cache may hold anything there.
 __device__ __forceinline__ int64_t start_of(const AttArgs& a, int b) {
   return a.q_start ? (int64_t)a.q_start[b] : (int64_t)a.Sk - a.Sq;
+}
+__device__ __forceinline__ int keys_of(const AttArgs& a, int b) {
+  int64_t n = a.k_len ? min(a.k_len[b], a.Sk) : a.Sk;
+  if (a.causal) n = min(n, start_of(a, b) + a.Sq);
+  return (int)max(n, (int64_t)0);
 }
 // Keys that query i reads: the first limit(..) of the sample's n.
 __device__ __forceinline__ int limit(const AttArgs& a, int n, int64_t start, int64_t i) {
@@ -75,39 +79,7 @@ __device__ __forceinline__ int limit(const AttArgs& a, int n, int64_t start, int
 
 constexpr int RT = 32;       // rows of a streamed tile
 constexpr int LS = RT + 4;   // floats between features of a tile in LDS
-constexpr int NT = 256;      // threads of a block: four waves of 32 rows each
-
-// A [DHP][RT] tile on its way to LDS: RT rows from `row0` on, of which
-// `valid` exist; others, and features past dh, become zeros.
-template <int DHP, bool UNIT>
-struct TileLoad {
-  static constexpr int U = DHP / 32;  // float4s per thread
-  f32x4 v[U];
-  __device__ __forceinline__ void load(const float* base, int64_t row, int64_t col, int valid, int dh) {
-    const int r = 4 * ((int)threadIdx.x & 7), d0 = (int)threadIdx.x >> 3;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int d = d0 + 32 * u;
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      if (d < dh) {
-        const float* p = base + r * row + d * col;
-        if (UNIT && r + 3 < valid) {
-          x = *reinterpret_cast<const f32x4u*>(p);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (r + e < valid) x[e] = p[e * row];
-        }
-      }
-      v[u] = x;
-    }
-  }
-  __device__ __forceinline__ void store(float* lds) const {
-    const int r = 4 * ((int)threadIdx.x & 7), d0 = (int)threadIdx.x >> 3;
-#pragma unroll
-    for (int u = 0; u < U; ++u) *reinterpret_cast<f32x4*>(lds + (d0 + 32 * u) * LS + r) = v[u];
-  }
-};
+constexpr int NT = 256;      // threads of a block
 
 // The operand of this lane's row for a contraction over the features: feature
 // 2 s + lane / 32 in register s, zeros past dh or where there is no row.
@@ -166,11 +138,17 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 
 
 // Forward of few queries.  A block owns 32 rows of a key head's queries (row
 // g Sq + i is query i of the g-th of the query heads that share the key head,
-// so that single queries of a group fill a wave together) and a run of keys,
+// so that the queries of a group fill a wave together) and a run of keys,
 // whose tiles its four waves take in turn, each staging its own through its
 // own part of LDS: no wave waits for another before the end.  There the four
 // join their sums, and where the keys are shared out over several blocks
-// att_join_kernel joins theirs.
+// att_join_kernel joins theirs.  The features of a row lie a whole column apart in
+// memory, so a [feature][row] tile in LDS is staged with float4s along the rows as
+// it stands, and serves both as the operand whose lanes are rows (one float per
+// lane) and as the one whose lanes are features (four rows per float4).  In v_mfma_
+// f32_32x32x2f32 register r of a score tile is the B operand of the k pair {8 (r /
+// 4) + r % 4, the same + 4}.  Bound by latency at its sizes: 4 samples, 4 heads, 63
+// x 63, head_dim 32: 9 us.
 struct SplitArgs {
   int splits, tiles_per_split;  // of 32 keys
   float* o;                     // [split][B kv_heads][row tile][feature][32]
@@ -312,6 +290,236 @@ __global__ void __launch_bounds__(NT) att_fwd_kernel(AttArgs a, SplitArgs p) {
   else if (a.lse && held) a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = lim > 0 ? (top + log2f(total)) * kLn2 : -INFINITY;
 }
 
+// Forward of a key head with up to R query rows (4 or 8), single tokens above
+// all: half a flop a byte of the cache and row, which the vector ALUs keep up with,
+// where a matrix instruction would fill 32 rows for them.  A wave takes tiles of
+// 32 keys as they lie in memory: lane l has keys 4 (l % 8) .. + 3 of features l / 8
+// + 8 i, so every load is a float4 and nothing is staged.  The lanes' parts of the
+// scores are summed so that each ends with one row's four, whose softmax is its
+// part; the probabilities reach the other lanes through LDS, and each lane sums
+// its own keys' share of its own features of out until the end.  The loads run a
+// chunk of C features ahead.
+//
+// Bound by the cache's bytes.  16 samples of 4096 keys, head_dim 128 (268 MB),
+// with the joining launch: 16 heads on 4 47 us (5.6 TB/s; the kernel of 32 rows
+// 94), 32 on 4 72 (95); one sample of 16384, 64 on 8 (134 MB) 50 (126); 64 samples
+// of 1024, 8 on 8, head_dim 64 (268 MB) 42 (70).
+// x[0 .. N) summed over LANES lanes: of N /
+// LANES sums each, the q-th lane has those from q N / LANES on, in
+// x[0 ..).  UNIT: the distance of those lanes.
+template <int N, int LANES, int UNIT, int SIZE>
+__device__ __forceinline__ void sum_scatter(float (&x)[SIZE]) {
+  if constexpr (LANES > 1) {
+    constexpr int at = LANES / 2 * UNIT;
+    const bool up = (int)threadIdx.x & at;
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      const float keep = up ? x[e + N / 2] : x[e], give = up ? x[e] : x[e + N / 2];
+      x[e] = keep + __shfl_xor(give, at, 64);
+      if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // few in flight, for the registers
+    }
+    sum_scatter<N / 2, LANES / 2, UNIT>(x);
+  }
+}
+
+// out of feature d of row r of a key head from its sums, with feature 0 the lse.
+__device__ __forceinline__ void put_few(const AttArgs& a, int n, int b, int kh, int r, int d, float x, float top, float total) {
+  const int head = kh * a.group + r / a.Sq, i = r % a.Sq;
+  const bool reads = limit(a, n, start_of(a, b), i) > 0;
+  *a.out.at(b, i, (int64_t)head * a.dh + d) = reads ? x / total : 0.f;
+  if (d == 0 && a.lse)
+    a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = reads ? (top + log2f(total)) * kLn2 : -INFINITY;
+}
+
+// waves of a SIMD that the registers allow
+constexpr int few_waves(int dhp, int r) { return dhp * r > 512 ? 1 : 2; }
+
+template <int DHP, int R, bool UNIT>
+__global__ void __launch_bounds__(NT, few_waves(DHP, R)) att_few_kernel(AttArgs a, SplitArgs p) {
+  constexpr int G = 8, L = 64 / G, TK = 4 * L, NF = DHP / G, C = 4, NC = NF / C, OWN = R * NF / L;
+  __shared__ __align__(16) float qs[DHP][R];       // the rows, scaled by nothing
+  __shared__ __align__(16) f32x4 ps[4][R][L];     // a wave's probabilities of a row and 4 keys
+  __shared__ __align__(16) float fs[4][R];         // and its rows' rescaling
+  __shared__ float os[4][R][DHP];
+  __shared__ float2 stat[4][R];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, kq = lane % L, fg = lane / L;
+  const int row = fg / (G / R);  // whose softmax this lane does
+  const int b = (int)blockIdx.x / a.kv_heads, kh = (int)blockIdx.x % a.kv_heads;
+  const int rows = a.group * a.Sq;
+  for (int e = (int)threadIdx.x; e < DHP * R; e += NT) {
+    const int r = e % R, d = e / R;
+    qs[d][r] = r < rows && d < a.dh ? *a.q.at(b, r % a.Sq, (int64_t)(kh * a.group + r / a.Sq) * a.dh + d) : 0.f;
+  }
+  __syncthreads();
+  const int n = keys_of(a, b);
+  const int lim = row < rows ? limit(a, n, start_of(a, b), row % a.Sq) : 0;
+  const int t1 = min((n + TK - 1) / TK, ((int)blockIdx.y + 1) * p.tiles_per_split);
+  const float c = a.scale * kLog2e;
+  const float* kp = a.k.at(b, 4 * kq, (int64_t)kh * a.dh + fg);
+  const float* vp = a.v.at(b, 4 * kq, (int64_t)kh * a.dh + fg);
+
+  f32x4 x[2][C];
+  auto load = [&](f32x4 (&to)[C], int part, int t) {  // parts 0 .. NC - 1 of k, then of v
+    int64_t key = part < NC ? a.k.row : a.v.row, col = part < NC ? a.k.col : a.v.col;
+    asm volatile("" : "+s"(key), "+s"(col));  // no address is carried from tile to tile
+    const int i0 = part % NC * C, valid = n - t * TK - 4 * kq;
+    const float* at = (part < NC ? kp : vp) + (t * TK * key + G * i0 * col);
+    const bool whole = UNIT && (t + 1) * TK <= n;
+#pragma unroll
+    for (int u = 0; u < C; ++u, at += G * col) {
+      // of the padding there are fewer than 32
+      const bool in = G * (i0 + u + 1) <= DHP - 31 || fg + G * (i0 + u) < a.dh;
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+      if (whole) {
+        if (in) y = *reinterpret_cast<const f32x4u*>(at);
+      } else if (in) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < valid) y[e] = at[e * key];
+      }
+      to[u] = y;
+    }
+  };
+  float o[R * NF] = {};  // [row][feature fg + G i]
+  float m = -INFINITY, l = 0.f;  // of the row; l of this lane's keys
+  int t = (int)blockIdx.y * p.tiles_per_split + wave;
+  if (t < t1) load(x[0], 0, t);
+  for (; t < t1; t += 4) {
+    float s[R * 4] = {};
+    f32x4 pr[R];
+#pragma unroll
+    for (int part = 0; part < 2 * NC; ++part) {
+      if (part + 1 < 2 * NC) load(x[(part + 1) & 1], part + 1, t);
+      else if (t + 4 < t1) load(x[0], 0, t + 4);
+      __builtin_amdgcn_sched_barrier(0);  // one chunk ahead, no more
+      const f32x4(&y)[C] = x[part & 1];
+      if (part < NC) {
+#pragma unroll
+        for (int u = 0; u < C; ++u) {
+          asm volatile("" ::: "memory");  // q stays in LDS until it is used
+          float q[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r) q[r] = qs[fg + G * (part * C + u)][r];
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * r + e] = fmaf(y[u][e], q[r], s[4 * r + e]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float& z = o[r * NF + (part - NC) * C + u];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z = fmaf(y[u][e], pr[r][e], z);
+          }
+      }
+      if (part != NC - 1) continue;
+      sum_scatter<4 * R, R, L * (G / R)>(s);  // s[0 .. 4): the row's scores of this lane's keys
+      if (R < G) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += __shfl_xor(s[e], L, 64);
+      }
+      float mn = m;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[e] = t * TK + 4 * kq + e < lim ? s[e] * c : -INFINITY;
+        mn = fmaxf(mn, s[e]);
+      }
+#pragma unroll
+      for (int w = L / 2; w > 0; w /= 2) mn = fmaxf(mn, __shfl_xor(mn, w, 64));
+      const float base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m - base);
+      f32x4 e4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) e4[e] = __builtin_amdgcn_exp2f(s[e] - base);
+      l = l * f + ((e4[0] + e4[1]) + (e4[2] + e4[3]));
+      const bool moved = __ballot(mn != m) != 0;
+      m = mn;
+      own_lds();
+      ps[wave][row][kq] = e4;  // by G / R lanes alike
+      if (kq == 0) fs[wave][row] = f;
+      own_lds();
+#pragma unroll
+      for (int r = 0; r < R; ++r) pr[r] = ps[wave][r][kq];
+      if (moved) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float fr = fs[wave][r];
+#pragma unroll
+          for (int i = 0; i < NF; ++i) o[r * NF + i] *= fr;
+        }
+      }
+    }
+  }
+  sum_scatter<R * NF, L, 1>(o);
+#pragma unroll
+  for (int w = L / 2; w > 0; w /= 2) l += __shfl_xor(l, w, 64);
+#pragma unroll
+  for (int e = 0; e < OWN; ++e) {
+    const int at = kq * OWN + e;
+    os[wave][at / NF][fg + G * (at % NF)] = o[e];
+  }
+  if (kq == 0) stat[wave][row] = float2{m, l};
+  __syncthreads();
+  const int64_t heads = gridDim.x, at = (int64_t)blockIdx.y * heads + blockIdx.x;
+  for (int e = (int)threadIdx.x; e < rows * a.dh; e += NT) {
+    const int r = e / a.dh, d = e % a.dh;
+    float top = -INFINITY, total = 0.f, z = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][r].x);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(stat[w][r].x - base);
+      total = fmaf(stat[w][r].y, f, total);
+      z = fmaf(os[w][r][d], f, z);
+    }
+    if (p.splits > 1) {
+      p.o[at * rows * a.dh + e] = z;
+      if (d == 0) p.ml[at * rows + r] = float2{top, total};
+    } else {
+      put_few(a, n, b, kh, r, d, z, top, total);
+    }
+  }
+}
+
+// Joins the sums of a key head's runs of keys, in their order; a thread per row
+// and feature.
+__global__ void __launch_bounds__(NT) att_few_join_kernel(AttArgs a, SplitArgs p) {
+  const int b = (int)blockIdx.x / a.kv_heads, kh = (int)blockIdx.x % a.kv_heads, rows = a.group * a.Sq;
+  const int e = (int)(blockIdx.y * NT + threadIdx.x);
+  if (e >= rows * a.dh) return;
+  const int r = e / a.dh, d = e % a.dh;
+  float top = -INFINITY, total = 0.f, z = 0.f;
+  const int64_t heads = gridDim.x;
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+    float2 ml[8];
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t at = (int64_t)(s0 + u) * heads + blockIdx.x;
+      const bool in = s0 + u < p.splits;
+      ml[u] = in ? p.ml[at * rows + r] : float2{-INFINITY, 0.f};
+      x[u] = in ? p.o[at * rows * a.dh + e] : 0.f;
+    }
+    float mn = top;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) mn = fmaxf(mn, ml[u].x);
+    const float base = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(top - base);
+    total *= f;
+    z *= f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float fu = __builtin_amdgcn_exp2f(ml[u].x - base);
+      total = fmaf(ml[u].y, fu, total);
+      z = fmaf(x[u], fu, z);
+    }
+    top = mn;
+  }
+  put_few(a, keys_of(a, b), b, kh, r, d, z, top, total);
+}
+
 // Joins the sums of a row tile's runs of keys, in their order; 32 features a
 // block, a thread per row and four of them.
 __global__ void __launch_bounds__(NT) att_join_kernel(AttArgs a, SplitArgs p) {
@@ -351,139 +559,6 @@ __device__ __forceinline__ float lse2_of(const AttArgs& a, int b, int head, int6
   return l == -INFINITY ? INFINITY : l * kLog2e;  // a row that reads no key: every 2^(t - inf) is 0
 }
 
-// dq: a block owns 128 rows as in the forward and streams keys and values; it
-// leaves delta for the kernel of dk and dv.
-template <int DHP, bool UNIT>
-__global__ void __launch_bounds__(NT) att_dq_kernel(AttArgs a) {
-  __shared__ __align__(16) float lds[2][DHP * LS];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const int b = (int)blockIdx.y / a.kv_heads, kh = (int)blockIdx.y % a.kv_heads;
-  const int64_t rows = (int64_t)a.group * a.Sq;
-  const int64_t r = (int64_t)blockIdx.x * 128 + 32 * wave + (lane & 31);
-  const bool held = r < rows;
-  const int head = kh * a.group + (int)(held ? r / a.Sq : 0);
-  const int64_t i = held ? r % a.Sq : 0;
-  const int n = keys_of(a, b);
-  const int lim = held ? limit(a, n, start_of(a, b), i) : 0;
-  float q[DHP / 2], g[DHP / 2];
-  load_row<DHP>(a.q.at(b, i, (int64_t)head * a.dh), a.q.col, held, a.dh, q);
-  load_row<DHP>(a.dout.at(b, i, (int64_t)head * a.dh), a.dout.col, held, a.dh, g);
-  const float lse = held ? lse2_of(a, b, head, i) : INFINITY;
-  float delta = 0.f;
-  {
-    float out[DHP / 2];
-    load_row<DHP>(a.o.at(b, i, (int64_t)head * a.dh), a.o.col, held, a.dh, out);
-#pragma unroll
-    for (int s = 0; s < DHP / 2; ++s) delta = fmaf(g[s], out[s], delta);
-    delta += other_half(delta);
-    if (held && lane < 32) a.delta[((int64_t)b * a.heads + head) * a.Sq + i] = delta;
-  }
-  __shared__ int most;
-  if (threadIdx.x == 0) most = 0;
-  __syncthreads();
-  atomicMax(&most, lim);
-  __syncthreads();
-  const int end = most;
-  const float c = a.scale * kLog2e;
-  const float* kp = a.k.at(b, 0, (int64_t)kh * a.dh);
-  const float* vp = a.v.at(b, 0, (int64_t)kh * a.dh);
-  f32x16 acc[DHP / 32] = {};
-  TileLoad<DHP, UNIT> tk, tv;
-  if (end > 0) {
-    tk.load(kp, a.k.row, a.k.col, n, a.dh);
-    tv.load(vp, a.v.row, a.v.col, n, a.dh);
-  }
-  for (int j0 = 0; j0 < end; j0 += RT) {
-    __syncthreads();
-    tk.store(lds[0]);
-    tv.store(lds[1]);
-    __syncthreads();
-    if (j0 + RT < end) {
-      tk.load(kp + (j0 + RT) * a.k.row, a.k.row, a.k.col, n - j0 - RT, a.dh);
-      tv.load(vp + (j0 + RT) * a.v.row, a.v.row, a.v.col, n - j0 - RT, a.dh);
-    }
-    if (!__any(lim > j0)) continue;
-    f32x16 s = dot_rows<DHP>(lds[0], q);
-    const f32x16 dp = dot_rows<DHP>(lds[1], g);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int j = j0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-      s[e] = j < lim ? __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (dp[e] - delta) : 0.f;
-    }
-    add_rows<DHP>(lds[0], s, acc);
-  }
-  store_row<DHP>(a.dq.at(b, i, (int64_t)head * a.dh), a.dq.col, held, a.dh, a.scale, acc);
-}
-
-// dk, dv: a block owns 128 keys of a key head and streams the queries and
-// output gradients of the heads that share it, one head after the other.
-template <int DHP, bool UNIT>
-__global__ void __launch_bounds__(NT) att_dkv_kernel(AttArgs a) {
-  __shared__ __align__(16) float lds[2][DHP * LS];
-  __shared__ __align__(16) float stat[2][RT];  // lse (base 2), delta of the tile's queries
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-  const int b = (int)blockIdx.y / a.kv_heads, kh = (int)blockIdx.y % a.kv_heads;
-  const int key0 = (int)blockIdx.x * 128;
-  const int key = key0 + 32 * wave + (lane & 31);
-  const int n = keys_of(a, b);
-  const int64_t start = start_of(a, b);
-  const bool held = key < n;
-  float k[DHP / 2], v[DHP / 2];
-  const int at = key < a.Sk ? key : 0;
-  load_row<DHP>(a.k.at(b, at, (int64_t)kh * a.dh), a.k.col, held, a.dh, k);
-  load_row<DHP>(a.v.at(b, at, (int64_t)kh * a.dh), a.v.col, held, a.dh, v);
-  const float c = a.scale * kLog2e;
-  // the first query that reads the block's first key
-  int64_t first = a.causal ? key0 - start : 0;
-  first = first < 0 ? 0 : first / RT * RT;
-  const int tiles = key0 < n && first < a.Sq ? (int)((a.Sq - first + RT - 1) / RT) : 0;
-  f32x16 dk[DHP / 32] = {}, dv[DHP / 32] = {};
-  TileLoad<DHP, UNIT> tq, tg;
-  float st = 0.f;
-  auto load = [&](int t) {
-    const int head = kh * a.group + t / tiles;
-    const int64_t i0 = first + (int64_t)(t % tiles) * RT;
-    const int valid = (int)(a.Sq - i0 < RT ? a.Sq - i0 : RT);
-    tq.load(a.q.at(b, i0, (int64_t)head * a.dh), a.q.row, a.q.col, valid, a.dh);
-    tg.load(a.dout.at(b, i0, (int64_t)head * a.dh), a.dout.row, a.dout.col, valid, a.dh);
-    const int r = (int)threadIdx.x & 31;
-    if (threadIdx.x < RT) st = r < valid ? lse2_of(a, b, head, i0 + r) : INFINITY;
-    else if (threadIdx.x < 2 * RT) st = r < valid ? a.delta[((int64_t)b * a.heads + head) * a.Sq + i0 + r] : 0.f;
-  };
-  const int total = tiles * a.group;
-  if (total > 0) load(0);
-  for (int t = 0; t < total; ++t) {
-    __syncthreads();
-    tq.store(lds[0]);
-    tg.store(lds[1]);
-    if (threadIdx.x < 2 * RT) stat[threadIdx.x / RT][threadIdx.x & 31] = st;
-    __syncthreads();
-    if (t + 1 < total) load(t + 1);
-    const int64_t i0 = first + (int64_t)(t % tiles) * RT;
-    if (a.causal && start + i0 + RT - 1 < key0 + 32 * wave) continue;  // no query of the tile reads this wave's keys
-    f32x16 s = dot_rows<DHP>(lds[0], k);
-    f32x16 dp = dot_rows<DHP>(lds[1], v);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int r = 8 * q + 4 * (lane >> 5);
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[0][r]);
-      const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[1][r]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool reads = held && (!a.causal || key <= start + i0 + r + e);
-        s[4 * q + e] = reads ? __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], c, -lse[e])) : 0.f;
-        dp[4 * q + e] = s[4 * q + e] * (dp[4 * q + e] - delta[e]);
-      }
-    }
-    add_rows<DHP>(lds[1], s, dv);
-    add_rows<DHP>(lds[0], dp, dk);
-  }
-  // keys past the sample's last are nobody's: their gradients are zeros
-  const bool stored = key < a.Sk;
-  store_row<DHP>(a.dk.at(b, at, (int64_t)kh * a.dh), a.dk.col, stored, a.dh, a.scale, dk);
-  store_row<DHP>(a.dv.at(b, at, (int64_t)kh * a.dh), a.dv.col, stored, a.dh, 1.f, dv);
-}
-
 // ------------------------------------------------------- packed operands
 // Long sequences run on the fp16 matrix cores: q, k, v and dout are packed as
 // pairs (mfma_pair.hpp), 32 steps x 16 features a fragment, once for each pass,
@@ -496,10 +571,11 @@ __global__ void __launch_bounds__(NT) att_dkv_kernel(AttArgs a) {
 //
 // Scales.  Every block of 32 rows of an operand has a power of two of its own,
 // from its largest value.  A score takes the two of its operands out again.
-// Where blocks are summed, the sum is kept in the scale of the head's largest
-// block, and the other factor, P or dS, carries the difference.  Probabilities
-// are at most 1 and enter times 2^14; dS = P (dP - delta) is bounded by 2 max
-// ||dout_i|| max ||v_j||, whose power of two scales it.
+// Where blocks are summed, the sum is kept in the scale of the largest block so
+// far: a larger one rescales the sum, of a smaller one the other factor, P or dS,
+// carries the difference.  Probabilities are at most 1 and enter times 2^14; dS =
+// P (dP - delta) of a block of queries is bounded by 2 max ||dout_i|| max ||v_j||,
+// i in the block, whose power of two scales it.
 struct PackArgs {
   Seq<const float> x[4];  // q, k, v, dout
   char* p[4];             // [head of a sample][block][fragments]
@@ -515,20 +591,29 @@ struct PairArgs {
   float *dk_part, *dv_part;  // [B][heads][dh][Sk], where heads share keys
 };
 
-// The exponent of a head's largest block, the same in every lane.
-__device__ __forceinline__ int least_exp(const PackArgs& p, int which, int64_t bh) {
-  int e = 126;
-  for (int i = threadIdx.x & 63; i < p.blocks[which]; i += 64) e = min(e, p.exp[which][bh * p.blocks[which] + i]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) e = min(e, __shfl_xor(e, o, 64));
-  return __builtin_amdgcn_readfirstlane(e);
-}
 // A block's exponent by a vector load: a scalar load under way turns every wait
 // for LDS into one for all of it.
-__device__ __forceinline__ int exp_at(const int* p, int64_t i) {
+template <class T>
+__device__ __forceinline__ T exp_at(const T* p, int64_t i) {
   int zero = 0;
   asm("" : "+v"(zero));
   return p[i + zero];
+}
+// A sum kept with an exponent, before a block of exponent `next` is added: the
+// larger of the two becomes the sum's.  Returns by how much the block's is above
+// it.
+constexpr int kNoExp = 400;  // of a sum that nothing has been added to
+template <int N>
+__device__ __forceinline__ int meet_exp(f32x16 (&sum)[N], int& exp, int next) {
+  next = __builtin_amdgcn_readfirstlane(next);
+  if (next < exp) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum[d][e] = pr::times_exp2(sum[d][e], next - exp);
+    exp = next;
+  }
+  return next - exp;
 }
 // The largest row norm of a head.
 __device__ __forceinline__ float most_norm(const PackArgs& p, int which, int64_t bh) {
@@ -825,7 +910,6 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   const int lim = held ? limit(a, n, start, i) : 0;
   const int row0 = tile * 128 + 32 * __builtin_amdgcn_readfirstlane(wave);
   const int mine = tiles_read(a, n, start, row0), all = (limit(a, n, start, min(tile * 128 + 127, a.Sq - 1)) + 31) / 32;
-  const int ev = least_exp(g.p, 2, bkh);
   const int *kexp = g.p.exp[1] + bkh * g.p.blocks[1], *vexp = g.p.exp[2] + bkh * g.p.blocks[2];
   RowFrags<KS> q;
   int eq;
@@ -846,6 +930,7 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   f32x16 s[1] = {};
   TileFrags p;
   float base = 0.f, c = 0.f, part = 0.f;
+  int ev = kNoExp;  // the exponent of o
   // tile t's scores masked, the maximum and what it rescales; ek, the exponents
   // of the tile's keys, and dv, by how much that of its values is above ev
   auto top = [&](int t, int ek, int dv) {
@@ -883,24 +968,24 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   const TileFrags* const probs[1] = {&p};
   f32x16 (*const sums[1])[KS / 2] = {&o};
   if (all > 0) copy_tile<KS>(kp, kbuf[0]);
-  int ek = 0, evt = ev;  // tile t - 1's
+  int ek = 0, evt = 0;  // tile t - 1's
   for (int t = 0; t <= all; ++t) {
     pr::wait_and_meet<0>();
-    const int u = min(t, all - 1), ek_next = all > 0 ? exp_at(kexp, u) : 0, ev_next = all > 0 ? exp_at(vexp, u) : ev;
+    const int u = min(t, all - 1), ek_next = all > 0 ? exp_at(kexp, u) : 0, ev_next = all > 0 ? exp_at(vexp, u) : 0;
     if (t + 1 < all) copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, kbuf[(t + 1) & 1]);
     if (t < all) copy_tile<KS>(vp + (int64_t)t * TILE, vbuf[t & 1]);
     if (t > mine) continue;
     const char* const now[1] = {kbuf[t & 1]};
-    // values below 2^-60 of the head's largest add nothing that is kept
-    const int over = __builtin_amdgcn_readfirstlane(evt) - ev;
-    const bool adds = over <= 60;
-    const int dv = adds ? over : 0;
     if (t == 0) {
       if (mine > 0) dot_pairs<KS, 1>(now, rows, s, [](int) {});
       ek = ek_next;
       evt = ev_next;
       continue;
     }
+    // values below 2^-60 of the largest add nothing that is kept
+    const int over = meet_exp(o, ev, evt);
+    const bool adds = over <= 60;
+    const int dv = adds ? over : 0;
     top(t - 1, ek, dv);
     ek = ek_next;
     evt = ev_next;
@@ -943,10 +1028,9 @@ __device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
   return copysignf(fmaxf(fabsf(c), 0x1p-126f), c);
 }
 
-// The exponent of dS: 2 max ||dout|| max ||v|| bounds it.
-__device__ __forceinline__ int grad_exp(const PackArgs& p, int64_t bh, int64_t bkh) {
-  const float bound = 2.f * most_norm(p, 3, bh) * most_norm(p, 2, bkh);
-  return pr::scale_exp(__float_as_uint(fminf(bound, 3e38f)));
+// The exponent of dS of a block of queries: 2 max ||dout|| max ||v|| bounds it.
+__device__ __forceinline__ int grad_exp(float dout_norm, float v_norm) {
+  return pr::scale_exp(__float_as_uint(fminf(2.f * dout_norm * v_norm, 3e38f)));
 }
 
 // dq: a wave holds 32 queries of one head and streams keys and values.
@@ -968,7 +1052,8 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   const int lim = held ? limit(a, n, start, i) : 0;
   const int row0 = tile * 128 + 32 * __builtin_amdgcn_readfirstlane(wave);
   const int mine = tiles_read(a, n, start, row0), all = (limit(a, n, start, min(tile * 128 + 127, a.Sq - 1)) + 31) / 32;
-  const int ed = grad_exp(g.p, bh, bkh), ek = least_exp(g.p, 1, bkh), own = min(row0 / 32, g.p.blocks[0] - 1);
+  const int own = min(row0 / 32, g.p.blocks[0] - 1);
+  const int ed = grad_exp(g.p.norm[3][(int64_t)bh * g.p.blocks[3] + own], most_norm(g.p, 2, bkh));
   const int eq = g.p.exp[0][(int64_t)bh * g.p.blocks[0] + own], eg = g.p.exp[3][(int64_t)bh * g.p.blocks[3] + own];
   const int *kexp = g.p.exp[1] + bkh * g.p.blocks[1], *vexp = g.p.exp[2] + bkh * g.p.blocks[2];
   const float none = a.scale < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not read
@@ -981,6 +1066,7 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   const char* kp = g.p.p[1] + bkh * g.p.blocks[1] * TILE;
   const char* vp = g.p.p[2] + bkh * g.p.blocks[2] * TILE;
   f32x16 acc[DHP / 32] = {};
+  int ek = kNoExp;  // the exponent of acc, less that of dS
   // dS of a tile's first 16 keys is formed, then that of the others beside the
   // product of the first
   f32x16 s[2];
@@ -1004,10 +1090,10 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
   }
   for (int t = 0; t < all; ++t) {
     pr::wait_and_meet<0>();
-    // dS carries by how much the keys' exponent is above the head's
+    const int over = meet_exp(acc, ek, ekt);
     c = score_factor(a, eq + ekt);
-    cd = pr::times_exp2(1.f, ed - eg - evt - (ekt - ek));
-    delta = pr::times_exp2(delta0, -(ekt - ek));
+    cd = pr::times_exp2(1.f, ed - eg - evt - over);
+    delta = pr::times_exp2(delta0, -over);
     if (t + 1 < all) {
       copy_tile<KS>(kp + (int64_t)(t + 1) * TILE, kbuf[(t + 1) & 1]);
       copy_tile<KS>(vp + (int64_t)(t + 1) * TILE, vbuf[(t + 1) & 1]);
@@ -1053,10 +1139,11 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
   const int n = keys_of(a, b);
   const int64_t start = start_of(a, b);
   const bool held = key < n;
-  const int ed = grad_exp(g.p, bh, bkh), eq = least_exp(g.p, 0, bh), eg = least_exp(g.p, 3, bh);
+  const float v_norm = most_norm(g.p, 2, bkh);
   const int own = min(key0 / 32 + __builtin_amdgcn_readfirstlane(wave), g.p.blocks[1] - 1);
   const int ek = g.p.exp[1][bkh * g.p.blocks[1] + own], ev = g.p.exp[2][bkh * g.p.blocks[2] + own];
   const int *qexp = g.p.exp[0] + (int64_t)bh * g.p.blocks[0], *gexp = g.p.exp[3] + (int64_t)bh * g.p.blocks[3];
+  const float* gnorm = g.p.norm[3] + (int64_t)bh * g.p.blocks[3];
   const float none = a.scale < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not read
   float c = 0.f, cd = 0.f;
   RowFrags<KS> k, v;
@@ -1072,12 +1159,14 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
   // Of the next tile: its exponents, and a query's lse (lanes 0 .. 31) or delta,
   // as loaded: they are on their way with the copies
   int eqt = 0, egt = 0;
-  float raw = 0.f;
+  float raw = 0.f, norm = 0.f;
+  int edk = kNoExp, edv = kNoExp;  // the exponents of dk and dv
   auto copy = [&](int t) {
     copy_tile<KS>(qp + (int64_t)t * TILE, qbuf[t & 1]);
     copy_tile<KS>(gp + (int64_t)t * TILE, gbuf[t & 1]);
     eqt = exp_at(qexp, first + t);
     egt = exp_at(gexp, first + t);
+    norm = exp_at(gnorm, first + t);
     const int64_t i = min((first + t) * 32 + (lane & 31), (int64_t)a.Sq - 1);
     const float* p = lane < 32 ? a.lse_in + b * a.lse_sample + i * a.lse_row + head * a.lse_col
                                : a.delta + (int64_t)bh * a.Sq + i;
@@ -1105,10 +1194,12 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
   if (total > 0) copy(0);
   for (int t = 0; t < total; ++t) {
     // P carries by how much the exponent of the tile's output gradients is above
-    // the head's (by more than 60: they add nothing that is kept), and dS that of
-    // its queries; shift: the exponent of dS over that of P
-    const int over = egt - eg, shift = ed - (eqt - eq) - (int)kPExp + over;
-    const bool adds = over <= 60;
+    // that of dv (by more than 100: they add nothing that is kept), and dS the same
+    // of dk; shift: the exponent of dS over that of P
+    const int ed = grad_exp(norm, v_norm);
+    const int over = meet_exp(dv, edv, egt), over_k = meet_exp(dk, edk, ed + eqt);
+    const int shift = ed - over_k - (int)kPExp + over;
+    const bool adds = over <= 100;
     c = score_factor(a, eqt + ek);
     cd = adds ? pr::times_exp2(1.f, shift - egt - ev) : 0.f;
     if (wave == 0) {
@@ -1143,8 +1234,8 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
   for (int d = 0; d < DHP / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      dk[d][e] = pr::times_exp2(dk[d][e], -eq - ed);
-      dv[d][e] = pr::times_exp2(dv[d][e], -eg - (int)kPExp);
+      dk[d][e] = pr::times_exp2(dk[d][e], -edk);
+      dv[d][e] = pr::times_exp2(dv[d][e], -edv - (int)kPExp);
     }
   const bool stored = key < a.Sk;
   const int at = stored ? key : 0;
@@ -1241,10 +1332,16 @@ int pack(PairArgs& g, bool backward, hipStream_t st, const char* who) {
   return check_launch(who);
 }
 
-// Whether a pass runs on packed operands.
-bool use_pairs(const AttArgs& a) { return a.Sq >= 64 && a.Sk >= 64; }
+// Whether the forward runs on packed operands.  The kernel of few queries splits
+// the keys over blocks too, and wins where the queries alone are too few blocks of
+// 128: 4 samples, 4 heads, 128 x 128, head_dim 32 7 us against 13 on packed
+// operands, 8 x 8, 64 x 1024, 64 36 (56); 32 x 8, 128 x 128, 64 37 (31), 8 x 8, 1024
+// x 63, 64 109 (21).
+bool pairs_forward(const AttArgs& a) { return a.Sq >= 64 && (int64_t)a.B * a.heads * a.Sq >= 8192; }
 
 constexpr int kMaxHeadDim = 128;
+constexpr int64_t kFewRows = 8;  // query rows of a key head that att_few_kernel takes, whose comment measures both sides
+
 
 template <class T>
 Seq<T> seq(T* p, int64_t B, int64_t S, int rows) {
@@ -1325,7 +1422,7 @@ int cnhip_attention_forward(const float* q, const float* k, const float* v, floa
       cnhip::base_args(q, k, v, B, Sq, Sk, heads, kv_heads, head_dim, scale, causal, k_len, q_start, rows);
   a.out = cnhip::seq(out, B, Sq, rows);
   a.lse = lse;
-  if (cnhip::use_pairs(a)) {
+  if (cnhip::pairs_forward(a)) {
     cnhip::PairArgs g{a, {}, nullptr, nullptr};
     CNHIP_TRY(cnhip::pack(g, false, st, who));
     const int tiles = (int)((Sq + 127) / 128);
@@ -1333,6 +1430,36 @@ int cnhip_attention_forward(const float* q, const float* k, const float* v, floa
       hipLaunchKernelGGL((cnhip::att_fwd_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st,
                          g, tiles);
     });
+    return cnhip::check_launch(who);
+  }
+  if (a.group * Sq <= cnhip::kFewRows) {
+    const int R = a.group * Sq <= 4 ? 4 : 8, rows = (int)(a.group * Sq);
+    const int64_t tiles = (Sk + 31) / 32;
+    // Runs of keys: as many blocks as the CUs hold, at least one tile a wave.
+    const int width = (int)((head_dim + 31) / 32 * 32);
+    int64_t splits = 256 * cnhip::few_waves(width, R) / (B * kv_heads);
+    if (splits > tiles / 4) splits = tiles / 4;
+    if (splits < 1) splits = 1;
+    cnhip::SplitArgs p{};
+    p.tiles_per_split = (int)((tiles + splits - 1) / splits);
+    p.splits = (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
+    if (p.splits > 1) {
+      const size_t all = (size_t)(p.splits * B * kv_heads * rows);
+      void* ws = nullptr;
+      CNHIP_TRY(cnhip::scratch(st, cnhip::kScratchLayer, all * (sizeof(float2) + head_dim * sizeof(float)), &ws, who));
+      p.ml = static_cast<float2*>(ws);
+      p.o = reinterpret_cast<float*>(p.ml + all);
+    }
+    const dim3 grid((unsigned)(B * kv_heads), (unsigned)p.splits);
+    cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
+      if (R == 4) hipLaunchKernelGGL((cnhip::att_few_kernel<d(), 4, unit()>), grid, dim3(cnhip::NT), 0, st, a, p);
+      else hipLaunchKernelGGL((cnhip::att_few_kernel<d(), 8, unit()>), grid, dim3(cnhip::NT), 0, st, a, p);
+    });
+    CNHIP_TRY(cnhip::check_launch(who));
+    if (p.splits == 1) return CNHIP_OK;
+    hipLaunchKernelGGL(cnhip::att_few_join_kernel,
+                       dim3((unsigned)(B * kv_heads), (unsigned)((rows * head_dim + cnhip::NT - 1) / cnhip::NT)),
+                       dim3(cnhip::NT), 0, st, a, p);
     return cnhip::check_launch(who);
   }
   // Runs of keys: enough blocks for two on every CU, at least two tiles a wave.
@@ -1378,39 +1505,23 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
   a.dk = cnhip::seq(dk, B, Sk, rows);
   a.dv = cnhip::seq(dv, B, Sk, rows);
   a.lse_in = lse;
-  if (cnhip::use_pairs(a)) {
-    cnhip::PairArgs g{a, {}, nullptr, nullptr};
-    CNHIP_TRY(cnhip::pack(g, true, st, who));
-    const int tiles = (int)((Sq + 127) / 128), key_tiles = (int)((Sk + 127) / 128);
-    cnhip::by_width(a.dh, [&](auto d) {
-      hipLaunchKernelGGL((cnhip::att_dkv_pair_kernel<d()>), dim3((unsigned)(key_tiles * B * heads)), dim3(cnhip::NT), 0,
-                         st, g);
-    });
-    CNHIP_TRY(cnhip::check_launch(who));
-    if (a.group > 1) {
-      hipLaunchKernelGGL(cnhip::att_share_kernel,
-                         dim3((unsigned)((Sk + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * kv_heads), (unsigned)((head_dim + 3) / 4 * 2)),
-                         dim3(cnhip::NT), 0, st, g);
-      CNHIP_TRY(cnhip::check_launch(who));
-    }
-    cnhip::by_width(a.dh, [&](auto d) {
-      hipLaunchKernelGGL((cnhip::att_dq_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st, g,
-                         tiles);
-    });
-    return cnhip::check_launch(who);
-  }
-  void* ws = nullptr;
-  CNHIP_TRY(cnhip::scratch(st, cnhip::kScratchLayer, (size_t)(B * heads * Sq) * sizeof(float), &ws, who));
-  a.delta = static_cast<float*>(ws);
-  cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
-    hipLaunchKernelGGL((cnhip::att_dq_kernel<d(), unit()>),
-                       dim3((unsigned)((a.group * Sq + 127) / 128), (unsigned)(B * kv_heads)), dim3(cnhip::NT), 0, st,
-                       a);
+  cnhip::PairArgs g{a, {}, nullptr, nullptr};
+  CNHIP_TRY(cnhip::pack(g, true, st, who));
+  const int tiles = (int)((Sq + 127) / 128), key_tiles = (int)((Sk + 127) / 128);
+  cnhip::by_width(a.dh, [&](auto d) {
+    hipLaunchKernelGGL((cnhip::att_dkv_pair_kernel<d()>), dim3((unsigned)(key_tiles * B * heads)), dim3(cnhip::NT), 0,
+                       st, g);
   });
   CNHIP_TRY(cnhip::check_launch(who));
-  cnhip::dispatch(a.dh, a.k.row == 1, [&](auto d, auto unit) {
-    hipLaunchKernelGGL((cnhip::att_dkv_kernel<d(), unit()>),
-                       dim3((unsigned)((Sk + 127) / 128), (unsigned)(B * kv_heads)), dim3(cnhip::NT), 0, st, a);
+  if (a.group > 1) {
+    hipLaunchKernelGGL(cnhip::att_share_kernel,
+                       dim3((unsigned)((Sk + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * kv_heads), (unsigned)((head_dim + 3) / 4 * 2)),
+                       dim3(cnhip::NT), 0, st, g);
+    CNHIP_TRY(cnhip::check_launch(who));
+  }
+  cnhip::by_width(a.dh, [&](auto d) {
+    hipLaunchKernelGGL((cnhip::att_dq_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st, g,
+                       tiles);
   });
   return cnhip::check_launch(who);
 }

@@ -779,14 +779,15 @@ int cnhip_token_embedding_backward(const int32_t* ids, const float* dY, float* g
  * are cut to [0, Sk]), and with causal != 0 only those with j <= q_start[b] + i
  * (device int32 [B], the position of the sample's first query among the keys;
  * NULL: Sk - Sq).  So a padded batch passes its lengths, and a decoding step
- * over a cache of capacity Sk passes k_len = the tokens held and q_start =
- * k_len - Sq.  Keys and values at and past k_len are never used, whatever they
- * hold; a query that reads no key gives a zero row and lse = -inf.  A NaN or
- * infinity in a key or value that only some queries of the batch may read can
- * reach the causal rows just before it.
+ * over a cache of capacity Sk passes q_start = the tokens held before it.
+ * Keys and values that no query of their sample reads (at and past k_len; with
+ * causal at and past q_start + Sq) are never used, whatever they hold; a query
+ * that reads no key gives a zero row and lse = -inf.  A NaN or infinity in a key
+ * or value that only some queries of the sample read can reach the causal rows
+ * just before it.
  * lse [B*Sq, heads] has q's rows; it may be NULL in the forward.
- * backward: gradients of q, k and v (overwritten; zeros for keys at and past
- * k_len) from out, lse and dout; the probabilities are formed again, dk and dv
+ * backward: gradients of q, k and v (overwritten; zeros for keys that no query
+ * reads) from out, lse and dout; the probabilities are formed again, dk and dv
  * are summed over the heads that share a key head.  head_dim <= 128,
  * B * heads <= 65535. */
 int cnhip_attention_forward(const float* q, const float* k, const float* v, float* out,

@@ -13,10 +13,20 @@ Where an operand is held as a pair of fp16 terms (cppnet_amd/csrc/mfma_pair.hpp)
 a value is kept to 2^-22 of itself, which the 8 more in g cover (2 * 8 u =
 2^-20), but not closer than F = 2^-39 of the operand's largest: the largest is
 scaled to at least 2^14, and the second term is rounded on fp16's subnormal grid
-of 2^-24, so by 2^-25 at most.  Probabilities are scaled by 2^14 exactly, the
-cross-entropy's gradient by 2^15, and dS by the power of two that takes its
-bound 2 max ||dout_i|| max ||v_j|| to 2^14 at least; maxima are those of a
-sample and key head."""
+of 2^-24, so by 2^-25 at most.  The cross-entropy's gradient is scaled by 2^15.
+
+In the attention, operands are blocks of 32 rows of a sample and head.
+Probabilities are scaled by 2^14, and dS by the power of two that takes its
+block's bound 2 max ||dout_i|| max ||v_j|| (i in the block) to 2^14 at least.
+In sums over blocks, P and dS also carry by how much the other factor's block,
+x, is smaller than the largest block up to there, X: by 2^-d, the quotient of the
+two blocks' powers of two.  Scaled, x and X both lie in [2^14, 2^15), so 2^d < 2 X
+/ x.  P and dS are off by F at most (times dS's bound), so their product with a
+value |y| <= x by F 2^d |y| < 2 F X.  A pair of a query and a key is off by at most
+2 F max |v| in out, 2 F bound_i max |k| in dq, 2 F max |dout| in dv, 2 F max (bound
+|q|) in dk (2^-25 2^15 in scaled units, of which bound and |q| each are 2^14 or
+more), where the last two are over the blocks of queries from that on which the
+first of the 128 keys around it is read by."""
 import numpy as np
 
 U = 2.0 ** -24
@@ -81,20 +91,22 @@ def attention(q, k, v, ok, scale, dout=None):
     # scores: the contraction, and the roundings of scale * log2(e) and of the
     # exponent's difference; from the score's and the maximum's size
     es = np.where(m, g(dh) * abs(scale) * (np.abs(q) @ T(np.abs(K))) + 6 * U * np.abs(np.where(m, s, 0)), 0.0)
-    def most(x):  # the largest of a sample and key head, for every query head
-        x = x.max((2, 3))
-        if x.shape[1] == H:
-            x = x.reshape(B, KH, G).max(2)
-        return np.repeat(x, G, 1)[:, :, None, None]
+
+    def block(x):  # every row's block's largest
+        x = np.abs(x).max(3)
+        top = np.maximum.reduceat(x, np.arange(0, x.shape[2], 32), 2)
+        return np.repeat(top, 32, 2)[:, :, :x.shape[2], None]
 
     aq, aK = np.abs(q), np.abs(K)
-    mq, mk, mv = most(aq), most(np.abs(k0)), most(np.abs(v0))
+    mq, mk, mv = block(q), block(K), block(Vv)
     row = lambda x: x.sum(3, keepdims=True)  # noqa: E731
-    es = es + np.where(m, abs(scale) * F * (mq * T(row(aK)) + mk * row(aq)), 0.0)
+    most = lambda x: x.max(2, keepdims=True)  # noqa: E731
+    reads = m.sum(3, keepdims=True)
+    es = es + np.where(m, abs(scale) * F * (mq * T(row(aK)) + T(mk) * row(aq)), 0.0)
     es = es.max(3, keepdims=True) + 6 * U * np.abs(top)
     eP = 2 * es + g(Sk)  # relative, of every probability of a row
     aV = P @ np.abs(Vv)
-    eo = eP * aV + g(Sk) * aV + F * (m @ np.abs(Vv)) + F * mv
+    eo = eP * aV + g(Sk) * aV + F * (P @ mv) + 2 * F * reads * most(mv)
     el = (es + g(Sk) + 4 * U * np.abs(np.where(np.isfinite(lse), lse, 0))[..., None])[..., 0]
     res = {"out": (out, 1.05 * eo), "lse": (lse, 1.05 * el)}
     if dout is None:
@@ -102,22 +114,30 @@ def attention(q, k, v, ok, scale, dout=None):
     do, ado = dout, np.abs(dout)
     dP = do @ T(Vv)
     norm = lambda x: np.sqrt((x * x).sum(3, keepdims=True))  # noqa: E731
-    mdo, bound = most(ado), 2 * most(norm(do)) * most(norm(v0))
-    edP = g(dh) * (ado @ T(np.abs(Vv))) + F * (mdo * T(row(np.abs(Vv))) + mv * row(ado))
+    mdo, bound = block(do), 2 * block(norm(do)) * most(norm(Vv))
+    edP = g(dh) * (ado @ T(np.abs(Vv))) + F * (mdo * T(row(np.abs(Vv))) + T(mv) * row(ado))
     delta = (do * out).sum(3, keepdims=True)
     edelta = g(dh) * (ado * np.abs(out)).sum(3, keepdims=True) + (ado * eo).sum(3, keepdims=True)
     dS = P * (dP - delta) * scale
     eb = 2 * es + el[..., None] + g(0)  # of the probability formed again from lse
     edS = abs(scale) * P * (edP + edelta + (eb + g(0)) * (np.abs(dP) + np.abs(delta)))
-    edS = np.where(m, edS + abs(scale) * F * bound, 0.0)
+    edS = np.where(m, edS, 0.0)
     aS = np.abs(dS)
-    dq, eq = dS @ K, edS @ np.abs(K) + g(Sk) * (aS @ np.abs(K)) + F * mk * row(aS)
+    dq, eq = dS @ K, edS @ np.abs(K) + g(Sk) * (aS @ np.abs(K)) + F * (aS @ mk)
+    eq = eq + 2 * abs(scale) * F * bound * most(mk) * reads
+    # the first of the queries' blocks for each key, and the largest from there on
+    read = ok.reshape(B, Sq, Sk).any(1)
+    lead = np.arange(Sk) // 128 * 128
+    first = np.where(read, ok.argmax(1), Sq - 1)[:, lead] // 32 * 32
+    after = lambda x: np.take_along_axis(np.maximum.accumulate(x[:, :, ::-1], 2)[:, :, ::-1],  # noqa: E731
+                                         np.broadcast_to(first[:, None, :, None], (B, H, Sk, 1)), 2)
+    taken = np.broadcast_to(T(m).sum(3, keepdims=True), (B, H, Sk, 1))
     share = lambda x: x.reshape(B, KH, G, Sk, dh).sum(2)  # noqa: E731
     n = Sq * G
     dk = share(T(dS) @ q)
-    ek = share(T(edS) @ np.abs(q) + g(n) * (T(aS) @ np.abs(q)) + F * mq * row(T(aS)))
+    ek = share(T(edS) @ np.abs(q) + g(n) * (T(aS) @ np.abs(q)) + F * (T(aS) @ mq) + 2 * abs(scale) * F * taken * after(bound * mq))
     dv = share(T(P) @ do)
-    ev = share(T(P * eb + F * m) @ ado + g(n) * (T(P) @ ado) + F * mdo * row(T(P)))
+    ev = share(T(P * eb) @ ado + g(n) * (T(P) @ ado) + F * (T(P) @ mdo) + 2 * F * taken * after(mdo))
     res.update(dq=(dq, 1.05 * eq), dk=(dk, 1.05 * ek), dv=(dv, 1.05 * ev))
     return res
 

@@ -1,0 +1,260 @@
+"""GPU tests of the language-model operators where their paths and their data
+end: every path of the attention over caches that hold anything past the read
+keys, blocks of very different size, row pieces of the cross-entropy, rows
+without a target that hold anything, captured calls.  Forms and bounds are
+those of lm_ops_ref.py."""
+import numpy as np
+import pytest
+import torch
+
+import lm_ops_ref as ref
+from cppnet_amd import ops
+from test_gpu_lm_ops import REF, SAMPLE, Buffers, att_run, host, per_head
+
+pytestmark = pytest.mark.gpu
+
+
+def wide(x, h):
+    return per_head(x.astype(np.float64), h)
+
+
+def att_check(dims, causal, k_len, q_start, rows, scale, q, k, v, do):
+    B, Sq, Sk, H, KH, dh = dims
+    ok = ref.allowed(B, Sq, Sk, causal, k_len, q_start)
+    buf = Buffers()
+    got = att_run(buf, (q, k, v), dict(causal=causal, k_len=k_len, q_start=q_start, rows=rows), dims, do, scale)
+    read = ok.any(1)[:, :, None]
+    want = ref.attention(wide(q, H), wide(np.where(read, k, 0), KH), wide(np.where(read, v, 0), KH), ok,
+                         dh ** -0.5 if scale is None else scale, None if do is None else wide(do, H))
+    for name, (w, lim) in want.items():
+        x = got[name].transpose(0, 2, 1) if name == "lse" else per_head(got[name], KH if name in ("dk", "dv") else H)
+        print("  ", name, ref.check(name, x, w, lim))
+    buf.intact()
+    return got
+
+
+FEW = [  # B, Sq, Sk, H, KH, dh, causal, rows: one to nine query rows a key head
+    (1, 1, 1, 1, 1, 1, False, SAMPLE), (2, 1, 31, 3, 1, 8, True, REF), (3, 1, 32, 4, 1, 32, False, SAMPLE),
+    (1, 1, 33, 5, 1, 33, True, SAMPLE), (2, 2, 127, 2, 2, 64, True, SAMPLE), (1, 4, 129, 2, 1, 80, True, REF),
+    (2, 1, 257, 8, 1, 96, False, SAMPLE), (1, 8, 300, 1, 1, 97, True, SAMPLE), (2, 1, 3001, 4, 1, 128, True, SAMPLE),
+    (1, 3, 2050, 4, 2, 128, True, REF), (1, 1, 5000, 8, 1, 128, False, SAMPLE), (2, 7, 40, 2, 2, 100, True, SAMPLE),
+    (2, 3, 90, 3, 1, 64, True, SAMPLE), (5, 1, 700, 6, 6, 40, True, SAMPLE), (2, 5, 3, 1, 1, 16, True, SAMPLE),
+]
+
+
+@pytest.mark.parametrize("B,Sq,Sk,H,KH,dh,causal,rows", FEW)
+def test_attention_of_few_rows(gpu, B, Sq, Sk, H, KH, dh, causal, rows):
+    print(f"[attention] B={B} {Sq}x{Sk} heads {H}/{KH} dh={dh} causal={causal} rows={rows}", flush=True)
+    rng = np.random.default_rng(B + Sk + dh)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    q, k, v = f(B, Sq, H * dh), f(B, Sk, KH * dh), f(B, Sk, KH * dh)
+    k_len = [int(n) for n in rng.integers(0, Sk + 1, B)]
+    k_len[-1] = Sk
+    for b in range(B):
+        k[b, k_len[b]:], v[b, k_len[b]:] = np.nan, np.inf
+    start = [n - Sq for n in k_len] if causal else None
+    att_check((B, Sq, Sk, H, KH, dh), causal, k_len, start, rows, None, q, k, v, None)
+
+
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+@pytest.mark.parametrize("Sq,H,KH,dh", [(1, 4, 2, 64), (3, 2, 1, 128), (20, 4, 2, 32), (70, 2, 1, 64), (130, 2, 2, 96)])
+def test_attention_over_a_cache_with_anything_past_its_last_query(gpu, Sq, H, KH, dh, rows):
+    print(f"[attention] cache {Sq} heads {H}/{KH} dh={dh} rows={rows}", flush=True)
+    rng = np.random.default_rng(Sq)
+    B, Sk = 4, 300
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    q, k, v, do = f(B, Sq, H * dh), f(B, Sk, KH * dh), f(B, Sk, KH * dh), f(B, Sq, H * dh)
+    start = [0, 299 - Sq, -Sq, 101]  # the third sample reads nothing
+    for b in range(B):
+        k[b, start[b] + Sq:], v[b, start[b] + Sq:] = np.inf, np.nan
+    got = att_check((B, Sq, Sk, H, KH, dh), True, None, start, rows, None, q, k, v, do)
+    for name in ("dk", "dv"):
+        for b in range(B):
+            assert (got[name][b, start[b] + Sq:] == 0).all()
+    assert (got["out"][2] == 0).all() and (got["lse"][2] == -np.inf).all() and (got["dq"][2] == 0).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("S,H,KH,dh", [(160, 2, 1, 64), (200, 1, 1, 128), (40, 2, 2, 32)])
+def test_attention_of_blocks_of_very_different_size(gpu, S, H, KH, dh, causal):
+    print(f"[attention] blocks {S} heads {H}/{KH} dh={dh} causal={causal}", flush=True)
+    rng = np.random.default_rng(S + dh)
+    size = lambda *e: np.array(e)[np.arange(S) // 32 % len(e)].astype(np.float32)[None, :, None]  # noqa: E731
+    f = lambda h: rng.standard_normal((2, S, h * dh)).astype(np.float32)  # noqa: E731
+    q = f(H) * size(1.0, 2.0 ** -30, 4.0, 0.0, 2.0 ** -70)
+    k = f(KH) * size(2.0 ** -20, 1.0, 0.0, 2.0)
+    v = f(KH) * size(2.0 ** 40, 2.0 ** -40, 1.0, 0.0, 2.0 ** 20)
+    do = f(H) * size(2.0 ** -50, 1.0, 2.0 ** 30, 0.0)
+    att_check((2, S, S, H, KH, dh), causal, None, None, SAMPLE, None, q, k, v, do)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout", "all"])
+@pytest.mark.parametrize("S", [5, 40, 100])
+def test_attention_of_zeros(gpu, S, which):
+    rng = np.random.default_rng(S)
+    x = {n: rng.standard_normal((2, S, 64)).astype(np.float32) for n in ("q", "k", "v", "dout")}
+    for n in x:
+        if which in (n, "all"):
+            x[n][:] = 0
+    att_check((2, S, S, 2, 2, 32), True, None, None, REF, None, x["q"], x["k"], x["v"], x["dout"])
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0 ** -60, 1.5])
+@pytest.mark.parametrize("S", [6, 45, 97])
+def test_attention_gradients_at_any_scale(gpu, S, scale):
+    rng = np.random.default_rng(S)
+    q, k, v, do = (rng.standard_normal((2, S, 96)).astype(np.float32) for _ in range(4))
+    att_check((2, S, S, 2, 2, 48), True, [S, S // 2], None, SAMPLE, scale, q, k, v, do)
+
+
+@pytest.mark.parametrize("Sq", [1, 2, 20, 70])
+def test_attention_gradient_is_the_slope(gpu, Sq):
+    """Along a direction u, f = sum(out * dout) in 64 bits moves by the gradients.
+    A step h of the central difference leaves h^2 / 6 of the third derivative.
+    That of a row of out is a fourth joint cumulant of v and s' three times, s'
+    = scale u k or scale q u: at most 2^4 + 3 * 2^4 of |v| |s'|^3, for values
+    off their mean by twice their largest."""
+    rng = np.random.default_rng(Sq)
+    B, Sk, H, KH, dh, h = 1, 90, 2, 1, 32, 2.0 ** -14
+    f = lambda s, h: rng.standard_normal((B, s, h * dh)).astype(np.float32)  # noqa: E731
+    x, do = [f(Sq, H), f(Sk, KH), f(Sk, KH)], f(Sq, H)
+    dims, kw = (B, Sq, Sk, H, KH, dh), dict(causal=True, k_len=None, q_start=None, rows=SAMPLE)
+    got = att_run(Buffers(), x, kw, dims, do)
+    ok = ref.allowed(B, Sq, Sk, True, None, None)
+    wq, wk, wv = (wide(a, n) for a, n in zip(x, (H, KH, KH)))
+    want = ref.attention(wq, wk, wv, ok, dh ** -0.5, wide(do, H))
+    longest = max(np.linalg.norm(wq, axis=3).max(), np.linalg.norm(wk, axis=3).max())
+    third = 64 * np.abs(do).sum() * np.abs(wv).max() * (dh ** -0.5 * longest) ** 3
+    for i, name in enumerate(("dq", "dk", "dv")):
+        u = rng.standard_normal((wq, wk, wv)[i].shape)
+        u /= np.linalg.norm(u)
+        def value(step):
+            y = [wq, wk, wv]
+            y[i] = y[i] + step * u
+            return (ref.attention(*y, ok, dh ** -0.5)["out"][0] * wide(do, H)).sum()
+        slope = (value(h) - value(-h)) / (2 * h)
+        along = (wide(got[name], (H, KH, KH)[i]) * u).sum()
+        lim = (want[name][1] * np.abs(u)).sum() + h * h / 6 * third + 1e-12 * np.abs(do).sum() / h
+        assert abs(along - slope) <= lim, (name, along, slope, lim)
+
+
+def ce_run(buf, X, W, b, t, reduction, base=None):
+    N, D = X.shape
+    V = W.shape[1]
+    x, w, tt = buf.new(X.T), buf.new(W.T), buf.new(t, np.int32)
+    loss, lse, dX = buf.empty(1), buf.empty(N), buf.empty(N * D)
+    dW = buf.empty(D * V) if base is None else base
+    bb, db = (None, None) if b is None else (buf.new(b), buf.empty(V))
+    ops.linear_ce_head(x, w, bb, tt, loss, lse, dX, dW, db, N, D, V, reduction, base is not None)
+    return {"loss": host(loss), "lse": host(lse), "dX": host(dX).reshape(D, N).T, "dW": host(dW).reshape(V, D).T,
+            **({} if b is None else {"db": host(db)})}, dW, (x, w, bb, tt)
+
+
+@pytest.mark.parametrize("N", [40, 100, 600])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf, 1e30, 3e38])
+def test_linear_ce_rows_without_a_target_may_hold_anything(gpu, N, what):
+    print(f"[linear ce] N={N} {what} in rows without a target", flush=True)
+    rng = np.random.default_rng(N)
+    D, V = 70, 700
+    X, W = rng.standard_normal((N, D)).astype(np.float32), (rng.standard_normal((D, V)) / 8).astype(np.float32)
+    b, t = rng.standard_normal(V).astype(np.float32), rng.integers(0, V, N).astype(np.int32)
+    t[rng.random(N) < 0.4] = -1
+    held = t >= 0
+    plain = np.where(held[:, None], X, 0)
+    X[~held, 3:9] = what
+    buf = Buffers()
+    got, _, (x, w, bb, tt) = ce_run(buf, X, W, b, t, "mean")
+    d = lambda a: a.astype(np.float64)  # noqa: E731
+    want = ref.linear_ce(d(plain), d(W), d(b), t, True)
+    for name in ("loss", "dX", "dW", "db"):
+        print("  ", name, ref.check(name, got[name], *want[name]))
+    ref.check("lse", got["lse"][held], *(a[held] for a in want["lse"]))
+    loss, lse = buf.empty(1), buf.empty(N)
+    ops.linear_ce_forward(x, w, bb, tt, loss, lse, N, D, V)
+    ref.check("loss of the forward", host(loss), *want["loss"])
+    ref.check("lse of the forward", host(lse)[held], *(a[held] for a in want["lse"]))
+    if not np.isfinite(what):  # such values count as zeros
+        zeroed = ref.linear_ce(d(np.where(np.isfinite(X), X, 0)), d(W), d(b), t, True)["lse"]
+        ref.check("lse of all", got["lse"], *zeroed)
+        ref.check("lse of all, forward", host(lse), *zeroed)
+    buf.intact()
+
+
+def test_linear_ce_in_pieces_of_rows(gpu):
+    """1100 rows of 131080 classes go through as 1024 and 76, as two calls over
+    those rows do, the second adding to the first's gradient.  The parts that dX
+    is summed in may be others where a call's largest piece is another."""
+    rng = np.random.default_rng(8)
+    N, D, V, R = 1100, 20, 131080, 1024
+    X, W = rng.standard_normal((N, D)).astype(np.float32), (rng.standard_normal((D, V)) / 4).astype(np.float32)
+    X[[0, R]] = 5.0  # the same largest value in both
+    t = rng.integers(0, V, N).astype(np.int32)
+    t[[3, 500, 1050]] = -1
+    buf = Buffers()
+    whole, _, (x, w, _, tt) = ce_run(buf, X, W, None, t, "sum")
+    one, dW, _ = ce_run(buf, X[:R], W, None, t[:R], "sum")
+    two, _, _ = ce_run(buf, X[R:], W, None, t[R:], "sum", dW)
+    np.testing.assert_array_equal(whole["lse"], np.concatenate([one["lse"], two["lse"]]))
+    np.testing.assert_array_equal(whole["dX"][:R], one["dX"])
+    d = lambda a: a.astype(np.float64)  # noqa: E731
+    sample = np.concatenate([np.arange(20), [3, 500], np.arange(R, R + 20), [1050]])
+    want = ref.linear_ce(d(X[sample]), d(W), None, t[sample], False)
+    ref.check("lse", whole["lse"][sample], *want["lse"])
+    ref.check("dX", whole["dX"][sample], *want["dX"])
+    ref.check("dX of two calls", np.concatenate([one["dX"], two["dX"]])[sample], *want["dX"])
+    lse = np.concatenate([np.log(np.exp(d(X[i:i + 100]) @ d(W)).sum(1)) for i in range(0, N, 100)])
+    held = t >= 0
+    loss = (lse - (d(X) * d(W)[:, np.where(held, t, 0)].T).sum(1))[held].sum()
+    bound = ref.g(D + V + N) * (np.abs(lse) + np.abs(d(X)).sum(1) * np.abs(W).max()).sum()
+    assert abs(whole["loss"][0] - loss) <= bound and abs(one["loss"][0] + two["loss"][0] - loss) <= bound
+    cols = np.unique(np.concatenate([t[held][:50], rng.integers(0, V, 50), [0, V - 1]]))
+    z = d(X) @ d(W)[:, cols]
+    P = np.exp(z - lse[:, None])
+    G = np.where(held[:, None], P - (t[:, None] == cols), 0)
+    # errors of z, lse and G as in the reference, with the rows' largest values
+    ez = ref.g(D) * (np.abs(d(X)) @ np.abs(d(W)[:, cols])) + 2 * D * ref.F * np.abs(X).max() * np.abs(W).max()
+    el = ref.g(D) * (np.abs(d(X)).sum(1) * np.abs(W).max()) + ref.g(V) + 16 * ref.U * np.abs(lse)
+    eG = held[:, None] * (P * (ez + el[:, None] + ref.g(0)) + 4 * ref.U * np.abs(G) + ref.F)
+    lim = np.abs(d(X)).T @ eG + ref.g(N) * (np.abs(d(X)).T @ np.abs(G)) + ref.F * 5.0 * np.abs(G).sum(0)
+    for a in (whole, two):
+        ref.check("dW", a["dW"][:, cols], d(X).T @ G, 1.05 * lim)
+    loss, lse32 = buf.empty(1), buf.empty(N)
+    ops.linear_ce_forward(x, w, None, tt, loss, lse32, N, D, V, "sum")
+    ref.check("lse of the forward", host(lse32), lse, 1.05 * el)
+    buf.intact()
+
+
+@pytest.mark.parametrize("Sq,N", [(1, 30), (40, 70), (96, 300)])
+def test_captured_calls_replayed_over_new_data(gpu, Sq, N):
+    """Attention and cross-entropy forward in one graph, replayed with eager
+    calls of other sizes between the replays."""
+    rng = np.random.default_rng(Sq)
+    B, Sk, H, KH, dh, D, V = 2, 640, 4, 2, 64, 48, 900
+    f = lambda n: torch.from_numpy(rng.standard_normal(n).astype(np.float32)).cuda()  # noqa: E731
+    q, k, v = f(B * Sq * H * dh), f(B * Sk * KH * dh), f(B * Sk * KH * dh)
+    X, W, t = f(N * D), f(D * V), torch.from_numpy(rng.integers(-1, V, N).astype(np.int32)).cuda()
+    new = lambda: [torch.empty(n, device="cuda") for n in (q.numel(), B * Sq * H, 1, N)]  # noqa: E731
+    got, want = new(), new()
+
+    def run(out):
+        ops.attention_forward(q, k, v, out[0], out[1], B, Sq, Sk, H, KH, dh, True)
+        ops.linear_ce_forward(X, W, None, t, out[2], out[3], N, D, V)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(got)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run(got)
+    for _ in range(4):
+        for x in (q, k, v, X):
+            x.copy_(f(x.numel()))
+        for x in got:
+            x.fill_(float("nan"))
+        run(want)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
