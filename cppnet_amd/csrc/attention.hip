@@ -733,8 +733,7 @@ __global__ void __launch_bounds__(NT) att_pack_kernel(PairArgs g) {
 // heads of a tile before the next.  Where the heads divide by the eight XCDs,
 // to which consecutive blocks go in turn, each takes a run of them, whose keys
 // then stay in its L2.
-__device__ __forceinline__ void place(int heads, int& tile, int& bh) {
-  const int bid = (int)blockIdx.x;
+__device__ __forceinline__ void place(int bid, int heads, int& tile, int& bh) {
   if (heads % 8 == 0) {
     const int per = heads / 8, local = bid >> 3;
     tile = local / per;
@@ -886,11 +885,6 @@ __device__ __forceinline__ int tiles_read(const AttArgs& a, int n, int64_t start
 
 constexpr float kPExp = 14.f;  // probabilities enter times 2^14
 
-template <int DHP>
-constexpr int pair_waves() { return DHP <= 64 ? 2 : 1; }
-template <int DHP>
-constexpr int dkv_waves() { return DHP <= 64 ? 2 : 1; }
-
 // Forward: a wave holds 32 queries of one head.
 template <int DHP>
 __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int tiles) {
@@ -899,7 +893,7 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
-  place(a.B * a.heads, tile, bh);
+  place((int)blockIdx.x, a.B * a.heads, tile, bh);
   tile = tiles - 1 - tile;
   const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
   const int64_t bkh = (int64_t)b * a.kv_heads + kh;
@@ -1033,15 +1027,23 @@ __device__ __forceinline__ int grad_exp(float dout_norm, float v_norm) {
   return pr::scale_exp(__float_as_uint(fminf(2.f * dout_norm * v_norm, 3e38f)));
 }
 
+// LDS of a block of the backward: two tiles of each of two operands.
+template <int DHP>
+struct GradLds {
+  __align__(16) char buf[2][2][DHP / 16 * 2 * pr::kFrag];
+  __align__(16) float stat[2][2][32];  // lse (base 2) - 14, scaled delta of the tiles' queries
+};
+
 // dq: a wave holds 32 queries of one head and streams keys and values.
 template <int DHP>
-__global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(PairArgs g, int tiles) {
+__device__ __forceinline__ void dq_block(const PairArgs& g, int bid, int tiles, GradLds<DHP>& lds) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
-  __shared__ __align__(16) char kbuf[2][TILE], vbuf[2][TILE];
+  auto& kbuf = lds.buf[0];
+  auto& vbuf = lds.buf[1];
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
-  place(a.B * a.heads, tile, bh);
+  place(bid, a.B * a.heads, tile, bh);
   tile = tiles - 1 - tile;
   const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
   const int64_t bkh = (int64_t)b * a.kv_heads + kh;
@@ -1125,14 +1127,15 @@ __global__ void __launch_bounds__(NT, pair_waves<DHP>()) att_dq_pair_kernel(Pair
 // one query head; where heads share the keys, into sums of their own
 // ([head of a sample][feature][key], att_share_kernel adds them).
 template <int DHP>
-__global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(PairArgs g) {
+__device__ __forceinline__ void dkv_block(const PairArgs& g, int bid, GradLds<DHP>& lds) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
-  __shared__ __align__(16) char qbuf[2][TILE], gbuf[2][TILE];
-  __shared__ __align__(16) float stat[2][2][32];  // lse (base 2) - 14, scaled delta of the tiles' queries
+  auto& qbuf = lds.buf[0];
+  auto& gbuf = lds.buf[1];
+  auto& stat = lds.stat;
   const AttArgs& a = g.a;
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   int tile, bh;
-  place(a.B * a.heads, tile, bh);  // the first keys are read by the most queries
+  place(bid, a.B * a.heads, tile, bh);  // the first keys are read by the most queries
   const int b = bh / a.heads, head = bh % a.heads, kh = head / a.group;
   const int64_t bkh = (int64_t)b * a.kv_heads + kh;
   const int key0 = tile * 128, key = key0 + 32 * wave + (lane & 31);
@@ -1247,6 +1250,18 @@ __global__ void __launch_bounds__(NT, dkv_waves<DHP>()) att_dkv_pair_kernel(Pair
     store_row<DHP>(g.dk_part + o, a.Sk, stored, a.dh, a.scale, dk);
     store_row<DHP>(g.dv_part + o, a.Sk, stored, a.dh, 1.f, dv);
   }
+}
+
+// Both in one launch, so that the blocks of one fill what those of the other leave
+// (head_dim 96 then holds dq to one block on a CU).  Backward, two launches and
+// one: 4 samples, 4 heads, 63 x 63, head_dim 32 18 and 13 us, 1 x 8, 1024 x 1024,
+// 128 178 and 117, 5 x 6, 1001 x 1001, 80 158 and 117, 8 x 8, 1024 x 1024, 128 312
+// and 308; 16 x 8, 2048 x 2048, 96 1377 and 1431.
+template <int DHP>
+__global__ void __launch_bounds__(NT, DHP <= 64 ? 2 : 1) att_grads_pair_kernel(PairArgs g, int dkv_blocks, int tiles) {
+  __shared__ GradLds<DHP> lds;
+  if ((int)blockIdx.x < dkv_blocks) dkv_block<DHP>(g, (int)blockIdx.x, lds);
+  else dq_block<DHP>(g, (int)blockIdx.x - dkv_blocks, tiles, lds);
 }
 
 // dk, dv of a key head: the sums of the heads that share it, in their order; a
@@ -1373,7 +1388,7 @@ int check_args(const char* who, int64_t B, int64_t Sq, int64_t Sk, int64_t heads
   CNHIP_REQUIRE(causal || !q_start, "%s: q_start needs causal", who);
   CNHIP_REQUIRE(std::isfinite(scale), "%s: scale is not finite", who);
   CNHIP_REQUIRE(B <= 65535 && heads <= 65535 && B * heads <= 65535, "%s: B * heads exceeds 65535", who);
-  CNHIP_REQUIRE(B * heads * ((Sq > Sk ? Sq : Sk) / 128 + 1) < (int64_t)1 << 31, "%s: too many rows", who);
+  CNHIP_REQUIRE(B * heads * (Sq / 128 + Sk / 128 + 2) < (int64_t)1 << 31, "%s: too many rows", who);
   CNHIP_REQUIRE(Sq < (1 << 30) && Sk < (1 << 30) && Sq * (heads / kv_heads) < (int64_t)1 << 31,
                 "%s: sequence too long", who);
   return CNHIP_OK;
@@ -1507,22 +1522,17 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
   a.lse_in = lse;
   cnhip::PairArgs g{a, {}, nullptr, nullptr};
   CNHIP_TRY(cnhip::pack(g, true, st, who));
-  const int tiles = (int)((Sq + 127) / 128), key_tiles = (int)((Sk + 127) / 128);
+  const int tiles = (int)((Sq + 127) / 128);
+  const unsigned dkv_blocks = (unsigned)((Sk + 127) / 128 * B * heads), dq_blocks = (unsigned)(tiles * B * heads);
   cnhip::by_width(a.dh, [&](auto d) {
-    hipLaunchKernelGGL((cnhip::att_dkv_pair_kernel<d()>), dim3((unsigned)(key_tiles * B * heads)), dim3(cnhip::NT), 0,
-                       st, g);
+    hipLaunchKernelGGL((cnhip::att_grads_pair_kernel<d()>), dim3(dkv_blocks + dq_blocks), dim3(cnhip::NT), 0, st, g,
+                       (int)dkv_blocks, tiles);
   });
   CNHIP_TRY(cnhip::check_launch(who));
-  if (a.group > 1) {
-    hipLaunchKernelGGL(cnhip::att_share_kernel,
-                       dim3((unsigned)((Sk + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * kv_heads), (unsigned)((head_dim + 3) / 4 * 2)),
-                       dim3(cnhip::NT), 0, st, g);
-    CNHIP_TRY(cnhip::check_launch(who));
-  }
-  cnhip::by_width(a.dh, [&](auto d) {
-    hipLaunchKernelGGL((cnhip::att_dq_pair_kernel<d()>), dim3((unsigned)(tiles * B * heads)), dim3(cnhip::NT), 0, st, g,
-                       tiles);
-  });
+  if (a.group == 1) return CNHIP_OK;
+  hipLaunchKernelGGL(cnhip::att_share_kernel,
+                     dim3((unsigned)((Sk + cnhip::NT - 1) / cnhip::NT), (unsigned)(B * kv_heads), (unsigned)((head_dim + 3) / 4 * 2)),
+                     dim3(cnhip::NT), 0, st, g);
   return cnhip::check_launch(who);
 }
 

@@ -224,6 +224,44 @@ def test_linear_ce_in_pieces_of_rows(gpu):
     buf.intact()
 
 
+@pytest.mark.parametrize("N", [65, 70, 257])
+@pytest.mark.parametrize("D,V", [(1, 1), (1, 2), (2, 1), (17, 3), (3, 129), (700, 1), (33, 32)])
+def test_linear_ce_of_few_features_and_classes(gpu, N, D, V):
+    rng = np.random.default_rng(N + D)
+    X, W = rng.standard_normal((N, D)).astype(np.float32), rng.standard_normal((D, V)).astype(np.float32)
+    b, t = rng.standard_normal(V).astype(np.float32), rng.integers(-1, V + 1, N).astype(np.int32)
+    buf = Buffers()
+    got, _, (x, w, bb, tt) = ce_run(buf, X, W, b, t, "mean")
+    want = ref.linear_ce(*(a.astype(np.float64) for a in (X, W, b)), t, True)
+    for name, a in got.items():
+        ref.check(name, a, *want[name])
+    loss, lse, oob = buf.empty(1), buf.empty(N), buf.new([5], np.int32)
+    ops.linear_ce_forward(x, w, bb, tt, loss, lse, N, D, V, "mean", oob)
+    ref.check("loss of the forward", host(loss), *want["loss"])
+    ref.check("lse of the forward", host(lse), *want["lse"])
+    assert host(oob)[0] == 5 + (t == V).sum()
+    buf.intact()
+
+
+@pytest.mark.parametrize("scale", [-1.5, 0.0, 2.0 ** -130])
+def test_token_embedding_at_any_scale(gpu, scale):
+    rng = np.random.default_rng(3)
+    B, S, V, D = 3, 70, 40, 33
+    ids = rng.integers(-1, V + 1, B * S).astype(np.int32)
+    W, dY = rng.standard_normal((V, D)).astype(np.float32), rng.standard_normal((B * S, D)).astype(np.float32)
+    W[~np.isin(np.arange(V), ids)] = np.nan  # rows that no id names are not read
+    buf = Buffers()
+    tid, out, gW = buf.new(ids, np.int32), buf.empty(B * S * D), buf.empty(V * D)
+    ops.token_embedding_forward(tid, buf.new(W), out, B, S, V, D, scale)
+    held = (ids >= 0) & (ids < V)
+    want = np.where(held[:, None], W[np.clip(ids, 0, V - 1)] * np.float32(scale), np.float32(0))
+    np.testing.assert_array_equal(host(out).reshape(D, B * S).T, want)
+    ops.token_embedding_backward(tid, buf.new(dY.T), gW, B, S, V, D, scale)
+    want, lim = ref.embedding_grad(ids, dY.astype(np.float64), V, scale)
+    ref.check("gW", host(gW).reshape(V, D), want, lim + 2.0 ** -149)  # below 2^-126 a rounding is to 2^-149
+    buf.intact()
+
+
 @pytest.mark.parametrize("Sq,N", [(1, 30), (40, 70), (96, 300)])
 def test_captured_calls_replayed_over_new_data(gpu, Sq, N):
     """Attention and cross-entropy forward in one graph, replayed with eager
