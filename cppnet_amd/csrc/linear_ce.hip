@@ -174,9 +174,14 @@ __global__ void __launch_bounds__(1024) ce_state_kernel(CeArgs a) {
   for (int i = threadIdx.x; i < a.w_blocks; i += 1024) w = max(w, a.w_part[i]);
   x = wave_max(x);
   w = wave_max(w);
-  atomicAdd(&total[0], (uint32_t)n);
-  atomicAdd(&total[1], (uint32_t)past);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    n += __shfl_xor(n, o, 64);
+    past += __shfl_xor(past, o, 64);
+  }
   if ((threadIdx.x & 63) == 0) {
+    atomicAdd(&total[0], (uint32_t)n);
+    atomicAdd(&total[1], (uint32_t)past);
     atomicMax(&total[2], x);
     atomicMax(&total[3], w);
   }

@@ -753,6 +753,12 @@ int cnhip_rnn_backward(const float* X, const float* W_ih, const float* W_hh, con
  * the same sizes first.  Calls on different streams may overlap; calls on one
  * stream from several host threads at once are not supported.  Every sum runs
  * in an order fixed by the arguments, so equal calls give equal bits.
+ * A graph captured by other means holds the stream's workspace as well, but
+ * does not freeze it.  No output may overlap an input.
+ * Large products run on pairs of fp16 terms: a value is kept to 2^-22 of
+ * itself, but no closer than 2^-39 of its operand's largest finite value (X's
+ * rows with a target, W, the gradient of the logits; 32 rows of a head of q, k,
+ * v and dout, whose sums' scale is that of the largest block so far).
  *
  * Token embedding: out[p, d] = scale * Wt[d + D id_p], ids ColMajor [B, S],
  * out a [B, S, D] sequence in either row order.  Ids outside [0, V) give zero
