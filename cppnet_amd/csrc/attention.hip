@@ -700,7 +700,8 @@ struct RowBlock {
   }
 };
 
-// A wave packs 32 rows of a head; of dout it also leaves delta.
+// A wave packs 32 rows of a head; of dout it also leaves delta.  Bound by memory:
+// 32 x 256, 8 heads of 64, forward and backward 40 us for 218 MB (5.4 TB/s).
 template <int KS>
 __global__ void __launch_bounds__(NT) att_pack_kernel(PairArgs g) {
   const int lane = (int)threadIdx.x & 63, which = (int)blockIdx.z + g.p.first;
@@ -885,7 +886,11 @@ __device__ __forceinline__ int tiles_read(const AttArgs& a, int n, int64_t start
 
 constexpr float kPExp = 14.f;  // probabilities enter times 2^14
 
-// Forward: a wave holds 32 queries of one head.
+// Forward: a wave holds 32 queries of one head and streams the keys and values,
+// which a block's four waves share through LDS.  Scores of the next tile are formed
+// beside the probabilities of this one.  Bound by the fp16 matrix cores, whose
+// sustained rate is 341 TFLOP/s of fp32 products: 2 x 4096 causal, 16 heads of 128,
+// 454 us (303 TFLOP/s).
 template <int DHP>
 __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int tiles) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;
@@ -1252,6 +1257,9 @@ __device__ __forceinline__ void dkv_block(const PairArgs& g, int bid, GradLds<DH
   }
 }
 
+// Seven products, of which the scores and dP are formed for dq and again for dk and
+// dv: summing dq over blocks of keys instead would take partial sums or an order
+// that changes.  2 x 4096 causal, 16 heads of 128 on 4: 1618 us (297 TFLOP/s).
 // Both in one launch, so that the blocks of one fill what those of the other leave
 // (head_dim 96 then holds dq to one block on a CU).  Backward, two launches and
 // one: 4 samples, 4 heads, 63 x 63, head_dim 32 18 and 13 us, 1 x 8, 1024 x 1024,
@@ -1265,7 +1273,7 @@ __global__ void __launch_bounds__(NT, DHP <= 64 ? 2 : 1) att_grads_pair_kernel(P
 }
 
 // dk, dv of a key head: the sums of the heads that share it, in their order; a
-// thread per key and four features.
+// thread per key and four features.  2 x 4096, 16 heads of 128 on 4: 168 MB, 50 us.
 __global__ void __launch_bounds__(NT) att_share_kernel(PairArgs g) {
   const AttArgs& a = g.a;
   const int key = (int)blockIdx.x * NT + (int)threadIdx.x, widths = (a.dh + 3) / 4;
