@@ -296,3 +296,103 @@ def test_captured_calls_replayed_over_new_data(gpu, Sq, N):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_attention_over_a_cache_past_32_bits(gpu):
+    """One query over a cache of more than 2^31 values: 17 GB of keys and
+    values.  Sums run in lanes, waves and blocks, 1024 tiles of 32 keys a block
+    at most, so no chain of additions is longer than 2^12 and g(2^12) bounds
+    them; out, lse, and dk and dv of the first and last keys, each a product of
+    the one query."""
+    dh, Sk = 128, 2 ** 24 + 77
+    torch.manual_seed(1)
+    k, v = torch.randn(dh, Sk, device="cuda"), torch.randn(dh, Sk, device="cuda")
+    q, do = torch.randn(dh, device="cuda"), torch.randn(dh, device="cuda")
+    out, lse = torch.full_like(q, float("nan")), torch.full((1,), float("nan"), device="cuda")
+    dims, kw = (1, 1, Sk, 1, 1, dh), dict(causal=True, rows=SAMPLE)
+    ops.attention_forward(q, k, v, out, lse, *dims, **kw)
+    scale = dh ** -0.5
+    s, es = [], 0.0
+    for j in range(0, Sk, 1 << 20):
+        part = k[:, j:j + (1 << 20)].double()
+        s.append(q.double() @ part * scale)
+        es = max(es, float((q.double().abs() @ part.abs()).max()) * ref.g(dh) * scale + 6 * ref.U * float(s[-1].abs().max()))
+    s = torch.cat(s)
+    es += 6 * ref.U * float(s.max())
+    want_lse = torch.logsumexp(s, 0)
+    P = torch.exp(s - want_lse)
+    want, mag = torch.zeros(dh, device="cuda", dtype=torch.float64), torch.zeros(dh, device="cuda", dtype=torch.float64)
+    for j in range(0, Sk, 1 << 20):
+        part = v[:, j:j + (1 << 20)].double()
+        want += part @ P[j:j + (1 << 20)]
+        mag += part.abs() @ P[j:j + (1 << 20)]
+    n = 2 ** 12
+    el = es + ref.g(n) + 4 * ref.U * abs(float(want_lse))
+    eo = (2 * es + 2 * ref.g(n)) * mag
+    num = lambda t: t.cpu().double().numpy()  # noqa: E731
+    ref.check("lse", num(lse), num(want_lse[None]), 1.05 * el)
+    ref.check("out", num(out), num(want), num(1.05 * eo))
+    dq, dk, dv = torch.empty_like(q), torch.full_like(k, float("nan")), torch.full_like(v, float("nan"))
+    ops.attention_backward(q, k, v, out, lse, do, dq, dk, dv, *dims, **kw)
+    delta = float((do.double() * want).sum())
+    edelta = float((do.double().abs() * want.abs()).sum()) * ref.g(dh) + float((do.double().abs() * eo).sum())
+    eb = 2 * es + el + ref.g(0)
+    top = lambda x: float(x.abs().max())  # noqa: E731
+    bound = 2 * float(do.double().norm()) * float(v.norm(dim=0).max())
+    for at in (slice(0, 300), slice(Sk - 300, Sk)):
+        p, part = P[at], v[:, at].double()
+        dP = do.double() @ part
+        dS = p * (dP - delta) * scale
+        edP = ref.g(dh) * (do.double().abs() @ part.abs()) + 2 * dh * ref.F * top(do) * top(v)
+        edS = scale * p * (edP + edelta + (eb + ref.g(0)) * (dP.abs() + abs(delta)))
+        aq, ado = q.double().abs()[:, None], do.double().abs()[:, None]
+        ek = aq * edS + ref.g(1) * aq * dS.abs() + 2 * scale * ref.F * bound * top(q) + ref.F * top(q) * dS.abs()
+        ev = ado * p * (eb + ref.g(1)) + 3 * ref.F * top(do)
+        ref.check("dk", num(dk[:, at]), num(q.double()[:, None] * dS), num(1.05 * ek))
+        ref.check("dv", num(dv[:, at]), num(do.double()[:, None] * p), num(1.05 * ev))
+    assert torch.isfinite(dq).all() and torch.isfinite(dk[:, ::1009]).all() and torch.isfinite(dv[:, ::1009]).all()
+
+
+@pytest.mark.parametrize("N", [5, 70])
+def test_tied_table_past_32_bits(gpu, N):
+    """A table of more than 2^31 values, 9 GB, as the embedding's and as the
+    Linear's weight.  Exponentials are summed over 128 classes at once, then in
+    chains of 2^11 in sixteen waves: g(2^12) bounds them."""
+    V, D = 2 ** 22 + 5, 520
+    torch.manual_seed(2)
+    W = torch.randn(V, D, device="cuda") / D ** 0.5
+    X = torch.randn(D, N, device="cuda")
+    t = torch.randint(0, V, (N,), device="cuda", dtype=torch.int32)
+    t[0], t[1], t[2] = V - 1, 0, V
+    loss, lse, dX = (torch.full((n,), float("nan"), device="cuda") for n in (1, N, N * D))
+    dW = torch.full_like(W, float("nan"))
+    ops.linear_ce_head(X, W, None, t, loss, lse, dX, dW, None, N, D, V, "sum")
+    x, step = X.double().t(), 1 << 18
+    z = torch.cat([x @ W[v:v + step].double().t() for v in range(0, V, step)], 1)
+    mag = max(float((x.abs() @ W[v:v + step].double().abs().t()).max()) for v in range(0, V, step))
+    want = torch.logsumexp(z, 1)
+    top = lambda a: float(a.abs().max())  # noqa: E731
+    ez = ref.g(D) * mag + 2 * D * ref.F * top(X) * top(W)
+    el = ez + 12 * ref.U * top(z) + ref.g(2 ** 12) + 4 * ref.U * top(want)
+    num = lambda a: a.cpu().double().numpy()  # noqa: E731
+    ref.check("lse", num(lse), num(want), 1.05 * el)
+    held = t < V
+    at = torch.where(held, t, 0).long()
+    rows = torch.where(held, want - z.gather(1, at[:, None])[:, 0], 0.0)
+    ref.check("loss", num(loss), num(rows.sum()[None]), 1.05 * N * (el + ez + 4 * ref.U * top(rows)) + ref.g(N) * float(rows.sum()))
+    for cols in (slice(0, 300), slice(V - 300, V)):
+        P = torch.exp(z[:, cols] - want[:, None])
+        G = torch.where(held[:, None], P - (t[:, None] == torch.arange(V, device="cuda")[cols]).double(), 0.0)
+        eG = held[:, None] * (P * (ez + el + ref.g(0)) + 4 * ref.U * G.abs() + ref.F)
+        lim = eG.t() @ x.abs() + ref.g(N) * (G.abs().t() @ x.abs()) + ref.F * top(X) * G.abs().sum(0)[:, None]
+        ref.check("dW", num(dW[cols]), num(G.t() @ x), num(1.05 * lim))
+    assert torch.isfinite(dX).all() and torch.isfinite(dW.view(-1)[::1009]).all()
+    # the embedding of the same table, its gradient added to the Linear's
+    ids = torch.tensor([V - 1, 0, V - 2, V - 1, V, -1], device="cuda", dtype=torch.int32)
+    out, dY = torch.full((D, 6), float("nan"), device="cuda"), torch.randn(D, 6, device="cuda")
+    ops.token_embedding_forward(ids, W, out, 1, 6, V, D)
+    assert torch.equal(out[:, :4].t(), W[ids[:4].long()]) and (out[:, 4:] == 0).all()
+    before = dW[[V - 1, V - 2, 0, V - 3]].clone()
+    ops.token_embedding_backward(ids, dY, dW, 1, 6, V, D, 1.0, True)
+    assert torch.equal(dW[[V - 1, V - 2, 0, V - 3]],
+                       before + torch.stack([dY[:, 0] + dY[:, 3], dY[:, 2], dY[:, 1], torch.zeros_like(dY[:, 0])]))
