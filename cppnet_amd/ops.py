@@ -487,7 +487,12 @@ def _held(device_of, *operands) -> list:
     Each has to be a contiguous tensor of that many values on device_of's device."""
     ptrs = []
     device = getattr(device_of, "device", None)
+    index = device_of.get_device() if isinstance(device_of, torch.Tensor) else -1
     for t, name, n, dtype in operands:
+        if (index >= 0 and isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype
+                and t.numel() == n and t.is_contiguous()):
+            ptrs.append(t.data_ptr())  # as it has to be; what is not is told apart below
+            continue
         ptrs.append(_p(t, name))
         if t is None:
             continue
@@ -502,11 +507,14 @@ def _held(device_of, *operands) -> list:
 
 def _call_on(t, name: str, *args) -> None:
     """Calls an entry point on t's device, on that device's current stream."""
-    if t.device.index == torch.cuda.current_device():
-        _capi.call(name, *args, _stream())
+    index = t.get_device()
+    # torch.cuda.current_stream() makes an object of it: 2.5 us, of 9 for a small call
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch.cuda.current_device():
+        _capi.call(name, *args, stream)
         return
-    with torch.cuda.device(t.device):
-        _capi.call(name, *args, _stream())
+    with torch.cuda.device(index):
+        _capi.call(name, *args, stream)
 
 
 def _positive(**sizes) -> None:
