@@ -545,13 +545,14 @@ __global__ void __launch_bounds__(NT) att_join_kernel(AttArgs a, SplitArgs p) {
     for (int e = 0; e < 4; ++e)
       if (d0 + e < a.dh) x[e] = fmaf(p.o[((at + s * step) * a.dh + d0 + e) * 32 + lane], f, x[e]);
   }
-  const float inv = total > 0.f ? 1.f / total : top == -INFINITY ? 0.f : NAN;
+  const bool reads = limit(a, keys_of(a, b), start_of(a, b), i) > 0;
+  const float inv = reads ? 1.f / total : 0.f;
   float* out = a.out.at(b, i, (int64_t)head * a.dh);
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (d0 + e < a.dh) out[(d0 + e) * a.out.col] = x[e] * inv;
   if (a.lse && part == 0 && blockIdx.z == 0)
-    a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+    a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = reads ? (top + log2f(total)) * kLn2 : -INFINITY;
 }
 
 __device__ __forceinline__ float lse2_of(const AttArgs& a, int b, int head, int64_t i) {

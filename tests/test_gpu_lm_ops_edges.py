@@ -99,6 +99,25 @@ def test_attention_of_zeros(gpu, S, which):
     att_check((2, S, S, 2, 2, 32), True, None, None, REF, None, x["q"], x["k"], x["v"], x["dout"])
 
 
+@pytest.mark.parametrize("B,Sq,Sk", [(1, 1, 40), (1, 1, 4000), (2, 20, 30), (2, 20, 900), (64, 130, 140)])
+def test_attention_of_scores_past_the_range(gpu, B, Sq, Sk):
+    """Where every score that a query reads is -inf, its softmax is 0 / 0 in
+    every path; other queries keep theirs, but for those packed with it, whose
+    scale is that query's."""
+    rng = np.random.default_rng(Sk)
+    q, k, v = (np.abs(rng.standard_normal((B, s, 32))).astype(np.float32) + np.float32(0.5) for s in (Sq, Sk, Sk))
+    k *= np.float32(-1e25)
+    q *= np.float32(1e-25)
+    q[:, 0] *= np.float32(1e38)
+    q[:, 0] *= np.float32(1e7)  # scores below -1e43
+    got = att_run(Buffers(), (q, k, v), dict(causal=False, k_len=None, q_start=None, rows=SAMPLE), (B, Sq, Sk, 1, 1, 32))
+    assert np.isnan(got["out"][:, 0]).all() and not np.isfinite(got["lse"][:, 0]).any()
+    want = ref.attention(wide(q[:, 1:], 1), wide(k, 1), wide(v, 1), np.ones((B, Sq - 1, Sk), bool), 32 ** -0.5) if 1 < Sq < 64 else {}
+    for name, (w, lim) in want.items():
+        x = got[name].transpose(0, 2, 1) if name == "lse" else per_head(got[name], 1)
+        ref.check(name, x[:, :, 1:], w, lim)
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0 ** -60, 1.5])
 @pytest.mark.parametrize("S", [6, 45, 97])
 def test_attention_gradients_at_any_scale(gpu, S, scale):
