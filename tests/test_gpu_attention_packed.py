@@ -1,0 +1,91 @@
+"""GPU tests of the attention's forward on packed operands, which takes over
+from 64 queries and 8192 query rows over all samples and heads on: values of out
+and lse, and the gradients that follow from them, against the 64-bit form and
+the bounds of lm_ops_ref.py."""
+import numpy as np
+import pytest
+
+import lm_ops_ref as ref
+from test_gpu_lm_ops import REF, SAMPLE, Buffers, att_run, per_head
+from test_gpu_lm_ops_edges import att_check, wide
+
+pytestmark = pytest.mark.gpu
+
+
+def packed(B, Sq, H):
+    return Sq >= 64 and B * H * Sq >= 8192
+
+
+PACKED = [  # B, Sq, Sk, H, KH, dh, causal, k_len, q_start, rows, scale
+    (8, 128, 128, 8, 8, 64, True, None, None, SAMPLE, None),
+    (8, 130, 140, 8, 4, 32, True, None, None, SAMPLE, None),
+    (7, 147, 147, 8, 8, 96, True, None, None, REF, None),
+    (9, 129, 129, 8, 2, 128, False, None, None, SAMPLE, None),
+    (33, 64, 64, 4, 4, 128, True, None, None, REF, None),
+    (4, 260, 33, 8, 8, 40, False, None, None, SAMPLE, None),         # keys of one tile and one more
+    (4, 260, 31, 8, 1, 64, True, None, None, SAMPLE, None),          # 229 queries read nothing
+    (3, 700, 1, 4, 4, 17, False, None, None, REF, None),             # one key
+    (2, 1100, 257, 4, 2, 100, True, None, [0, 100], SAMPLE, None),
+    (6, 200, 300, 8, 4, 64, False, [300, 0, 1, 31, 32, 33], None, SAMPLE, None),
+    (6, 200, 300, 8, 2, 33, True, [300, 0, 3, 64, 299, 129], None, REF, None),
+    (6, 200, 300, 8, 8, 128, True, [300, 300, 70, 0, 5, 400], [100, -150, 60, 7, 299, -300], SAMPLE, None),
+    (5, 300, 200, 6, 3, 80, False, [200, 199, 128, 97, 65], None, REF, None),
+    (8, 150, 150, 8, 8, 64, True, None, None, SAMPLE, -0.3),
+    (8, 150, 150, 8, 4, 48, False, None, None, REF, -1.5),
+    (8, 150, 150, 8, 8, 1, True, None, None, SAMPLE, 0.0),
+    (8, 150, 150, 8, 8, 32, True, None, None, SAMPLE, 2.0 ** -60),
+    (1, 1200, 1300, 7, 1, 128, True, None, None, SAMPLE, None),      # seven heads on one, rows past a tile
+    (1, 2049, 65, 4, 4, 66, True, None, [-1], REF, None),
+]
+BORDER = [  # B, Sq, H: just below the rule and just on it
+    (64, 64, 2), (65, 63, 2), (43, 95, 2), (64, 127, 1), (64, 128, 1), (1, 8191, 1), (1, 8192, 1),
+]
+
+
+def test_the_cases_run_packed():
+    assert all(packed(c[0], c[1], c[3]) for c in PACKED)
+    assert [packed(*c) for c in BORDER] == [True, False, False, False, True, False, True]
+
+
+def data(rng, B, Sq, Sk, H, KH, dh, causal, k_len, q_start):
+    """Operands with NaN and infinities at every key that no query of its sample reads."""
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    q, k, v, do = f(B, Sq, H * dh), f(B, Sk, KH * dh), f(B, Sk, KH * dh), f(B, Sq, H * dh)
+    unread = ~ref.allowed(B, Sq, Sk, causal, k_len, q_start).any(1)
+    k[unread], v[unread] = np.nan, np.inf
+    return q, k, v, do
+
+
+@pytest.mark.parametrize("B,Sq,Sk,H,KH,dh,causal,k_len,q_start,rows,scale", PACKED)
+def test_values(gpu, B, Sq, Sk, H, KH, dh, causal, k_len, q_start, rows, scale):
+    print(f"[attention] B={B} {Sq}x{Sk} heads {H}/{KH} dh={dh} causal={causal} {k_len} {q_start} rows={rows} {scale}", flush=True)
+    rng = np.random.default_rng(Sq + 7 * Sk + dh)
+    x = data(rng, B, Sq, Sk, H, KH, dh, causal, k_len, q_start)
+    att_check((B, Sq, Sk, H, KH, dh), causal, k_len, q_start, rows, scale, *x)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,Sq,H", BORDER)
+def test_values_on_both_sides_of_the_rule(gpu, B, Sq, H, causal):
+    print(f"[attention] B={B} {Sq}x50 heads {H} causal={causal}", flush=True)
+    rng = np.random.default_rng(Sq)
+    x = data(rng, B, Sq, 50, H, 1, 32, causal, None, [50 - Sq] * B if causal else None)
+    att_check((B, Sq, 50, H, 1, 32), causal, None, None, SAMPLE, None, *x)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,S,H,KH,dh", [(16, 160, 4, 2, 64), (11, 200, 4, 4, 128), (30, 70, 4, 1, 32)])
+def test_blocks_of_very_different_size(gpu, B, S, H, KH, dh, causal):
+    """The sums' scale follows the largest block of values so far."""
+    print(f"[attention] blocks {B}x{S} heads {H}/{KH} dh={dh} causal={causal}", flush=True)
+    rng = np.random.default_rng(S + dh)
+    size = lambda *e: np.array(e)[np.arange(S) // 32 % len(e)].astype(np.float32)[None, :, None]  # noqa: E731
+    f = lambda h: rng.standard_normal((B, S, h * dh)).astype(np.float32)  # noqa: E731
+    q = f(H) * size(1.0, 2.0 ** -30, 4.0, 0.0, 2.0 ** -70)
+    k = f(KH) * size(2.0 ** -20, 1.0, 0.0, 2.0)
+    v = f(KH) * size(2.0 ** 40, 2.0 ** -40, 1.0, 0.0, 2.0 ** 20)
+    do = f(H) * size(2.0 ** -50, 1.0, 2.0 ** 30, 0.0)
+    assert packed(B, S, H)
+    att_check((B, S, S, H, KH, dh), causal, None, None, SAMPLE, None, q, k, v, do)
+    v = f(KH) * size(2.0 ** -40, 2.0 ** 20, 2.0 ** -45, 1.0, 2.0 ** 40)  # growing, and far below what came before
+    att_check((B, S, S, H, KH, dh), causal, None, None, REF, None, q, k, v, do)
