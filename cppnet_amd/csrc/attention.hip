@@ -956,7 +956,17 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
         for (int e = 0; e < 16; ++e) o[d][e] *= f;
       m = mn;
     }
-    base = (m == -INFINITY ? 0.f : m) - kPExp + (float)dv;
+    base = m == -INFINITY ? 0.f : m;
+    if (__any(fabsf(base) >= 0x1p23f)) {
+      // The 14 is lost in a maximum of 2^24 and more, and c times a score there is
+      // rounded by as much as it: the difference is taken first, of the product as
+      // it was rounded for the maximum, so that the largest gives 0.
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[0][e] = pr::opaque(s[0][e] * c) - base;
+      c = 1.f;
+      base = 0.f;
+    }
+    base = base - kPExp + (float)dv;
     part = 0.f;
   };
   auto pair = [&](const f32x16& x, int e) {

@@ -89,3 +89,41 @@ def test_blocks_of_very_different_size(gpu, B, S, H, KH, dh, causal):
     att_check((B, S, S, H, KH, dh), causal, None, None, SAMPLE, None, q, k, v, do)
     v = f(KH) * size(2.0 ** -40, 2.0 ** 20, 2.0 ** -45, 1.0, 2.0 ** 40)  # growing, and far below what came before
     att_check((B, S, S, H, KH, dh), causal, None, None, REF, None, q, k, v, do)
+
+
+def sharp(rng, B, Sq, Sk, H, KH, dh, level):
+    """Operands whose scores lie around `level` and vary by some 1e7: 64 exact
+    units in feature 0 carry the level, the other features the variation."""
+    q, k = (rng.standard_normal((B, s, h * dh)).astype(np.float32) * np.float32(2e3) for s, h in ((Sq, H), (Sk, KH)))
+    q[:, :, ::dh], k[:, :, ::dh] = np.float32(8192), np.float32(level / 8192)
+    return q, k
+
+
+@pytest.mark.parametrize("level", [0.0, 7e7, -7e7, 1e9, -1e9])
+@pytest.mark.parametrize("B,Sq,Sk,H,KH,dh,causal", [(2, 1, 300, 4, 2, 32, False), (2, 20, 300, 4, 2, 64, True),
+                                                    (8, 130, 200, 8, 4, 64, True), (9, 128, 100, 8, 8, 128, False)])
+def test_scores_far_from_zero(gpu, B, Sq, Sk, H, KH, dh, causal, level):
+    """Where a query's largest score leads by more than the scores' errors, out
+    is that key's value; no finite score gives anything that is not finite.  A
+    probability of another key is below e^-40."""
+    print(f"[attention] B={B} {Sq}x{Sk} heads {H}/{KH} dh={dh} causal={causal} level {level}", flush=True)
+    rng = np.random.default_rng(Sk + dh)
+    q, k = sharp(rng, B, Sq, Sk, H, KH, dh, level)
+    v = rng.standard_normal((B, Sk, KH * dh)).astype(np.float32)
+    got = att_run(Buffers(), (q, k, v), dict(causal=causal, k_len=None, q_start=None, rows=SAMPLE), (B, Sq, Sk, H, KH, dh), None, 1.0)
+    assert np.isfinite(got["out"]).all() and np.isfinite(got["lse"]).all()
+    wq, wk, wv = wide(q, H), np.repeat(wide(k, KH), H // KH, 1), np.repeat(wide(v, KH), H // KH, 1)
+    ok = ref.allowed(B, Sq, Sk, causal, None, None)[:, None]
+    s = np.where(ok, wq @ wk.transpose(0, 1, 3, 2), -np.inf)
+    es = ref.g(dh) * np.where(ok, np.abs(wq) @ np.abs(wk).transpose(0, 1, 3, 2), 0).max(3)
+    es += 2 * dh * ref.F * np.abs(wq).max() * np.abs(wk).max() + 12 * ref.U * np.abs(s.max(3))
+    best = s.argmax(3)
+    others = np.where(np.arange(Sk) == best[..., None], -np.inf, s).max(3)
+    leads = s.max(3) - others > 2 * es + 40
+    assert leads.mean() > 0.5, leads.mean()
+    want = np.take_along_axis(wv, best[..., None], 2)
+    lim = (ref.g(Sk) + Sk * np.exp(-40.0)) * np.abs(wv).max()
+    off = np.abs(per_head(got["out"], H) - want).max(3)[leads]
+    assert off.max() <= lim, (off.max(), lim)
+    off = np.abs(got["lse"].transpose(0, 2, 1) - s.max(3))
+    assert (off <= es + 4 * ref.U * np.abs(s.max(3)) + np.log(Sk)).all()
