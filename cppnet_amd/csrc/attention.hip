@@ -1038,6 +1038,14 @@ __device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
   return copysignf(fmaxf(fabsf(c), 0x1p-126f), c);
 }
 
+// A probability times 2^top from its score and its row's lse (base 2) less top.
+// The score's and the lse's own errors may take it above 1, by any power of two
+// where scores or the products that cancel in them are 2^22 and more: it is held
+// to 1, which the scales of P and dS rely on (a NaN stays one).
+__device__ __forceinline__ float prob(float s, float c, float lse, float top) {
+  return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(fmaf(s, c, -lse), top));
+}
+
 // The exponent of dS of a block of queries: 2 max ||dout|| max ||v|| bounds it.
 __device__ __forceinline__ int grad_exp(float dout_norm, float v_norm) {
   return pr::scale_exp(__float_as_uint(fminf(2.f * dout_norm * v_norm, 3e38f)));
@@ -1093,7 +1101,7 @@ __device__ __forceinline__ void dq_block(const PairArgs& g, int bid, int tiles, 
     float d[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      d[u] = __builtin_amdgcn_exp2f(fmaf(s[0][2 * e + u], c, -lse)) * fmaf(s[1][2 * e + u], cd, -delta);
+      d[u] = prob(s[0][2 * e + u], c, lse, 0.f) * fmaf(s[1][2 * e + u], cd, -delta);
     p.split(e, d[0], d[1]);
   };
   const RowFrags<KS>* const rows[2] = {&q, &go};
@@ -1164,7 +1172,7 @@ __device__ __forceinline__ void dkv_block(const PairArgs& g, int bid, GradLds<DH
   const int *qexp = g.p.exp[0] + (int64_t)bh * g.p.blocks[0], *gexp = g.p.exp[3] + (int64_t)bh * g.p.blocks[3];
   const float* gnorm = g.p.norm[3] + (int64_t)bh * g.p.blocks[3];
   const float none = a.scale < 0.f ? INFINITY : -INFINITY;  // the score of a key that is not read
-  float c = 0.f, cd = 0.f;
+  float c = 0.f, cd = 0.f, top = 0.f;
   RowFrags<KS> k, v;
   k.load(g.p.p[1] + bkh * g.p.blocks[1] * TILE, held ? key : 0, held);
   v.load(g.p.p[2] + bkh * g.p.blocks[2] * TILE, held ? key : 0, held);
@@ -1202,7 +1210,7 @@ __device__ __forceinline__ void dkv_block(const PairArgs& g, int bid, GradLds<DH
     const int r = 8 * (e / 2) + 4 * (lane >> 5) + 2 * (e & 1);
     const float2 lse = *reinterpret_cast<const float2*>(&st[0][r]);
     const float2 delta = *reinterpret_cast<const float2*>(&st[1][r]);
-    float w[2] = {__builtin_amdgcn_exp2f(fmaf(s[0][2 * e], c, -lse.x)), __builtin_amdgcn_exp2f(fmaf(s[0][2 * e + 1], c, -lse.y))};
+    float w[2] = {prob(s[0][2 * e], c, lse.x, top), prob(s[0][2 * e + 1], c, lse.y, top)};
     float d[2] = {w[0] * fmaf(s[1][2 * e], cd, -delta.x), w[1] * fmaf(s[1][2 * e + 1], cd, -delta.y)};
     p.split(e, w[0], w[1]);
     ds.split(e, d[0], d[1]);
@@ -1221,6 +1229,7 @@ __device__ __forceinline__ void dkv_block(const PairArgs& g, int bid, GradLds<DH
     const bool adds = over <= 100;
     c = score_factor(a, eqt + ek);
     cd = adds ? pr::times_exp2(1.f, shift - egt - ev) : 0.f;
+    top = kPExp - (float)over;
     if (wave == 0) {
       const bool in = adds && (first + t) * 32 + (lane & 31) < a.Sq;
       float st = lane < 32 ? INFINITY : 0.f;
@@ -1238,11 +1247,11 @@ __device__ __forceinline__ void dkv_block(const PairArgs& g, int bid, GradLds<DH
     add.read(turned, 0);
     const int64_t i0 = start + (first + t) * 32;  // the position of the tile's first query
     if (!(__all(held) && (!a.causal || key0 + 32 * wave + 31 <= i0))) {
+      // the first of the tile's queries that reads this lane's key
+      const int64_t behind = a.causal ? key - i0 : 0;
+      const int lead = !held ? 32 : (int)(behind < 0 ? 0 : behind < 32 ? behind : 32);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const bool reads = held && (!a.causal || key <= i0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4);
-        s[0][e] = reads ? s[0][e] : none;
-      }
+      for (int e = 0; e < 16; ++e) s[0][e] = 8 * (e / 4) + 4 * (lane >> 5) + e % 4 >= lead ? s[0][e] : none;
     }
     const float (*const st_now)[32] = stat[t & 1];
     auto work = [&](int e) { pair(st_now, e); };

@@ -127,3 +127,31 @@ def test_scores_far_from_zero(gpu, B, Sq, Sk, H, KH, dh, causal, level):
     assert off.max() <= lim, (off.max(), lim)
     off = np.abs(got["lse"].transpose(0, 2, 1) - s.max(3))
     assert (off <= es + 4 * ref.U * np.abs(s.max(3)) + np.log(Sk)).all()
+
+
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+@pytest.mark.parametrize("level", [0.0, 7e7, -1e9])
+@pytest.mark.parametrize("Sq,Sk,H,KH,dh,causal", [(1, 1, 2, 2, 32, False), (40, 70, 4, 2, 64, True), (200, 150, 2, 1, 128, False), (70, 70, 3, 3, 96, True)])
+def test_gradients_of_scores_far_from_zero(gpu, Sq, Sk, H, KH, dh, causal, level, rows):
+    """The probabilities formed again from lse are off by 2^-22 |lse| of
+    themselves and the like of the scores' own errors, which at scores of 1e7 and
+    more says little about them; but each is held to 1, so dv of a key is at most
+    the sum of |dout| over the queries that read it, and the other gradients are
+    finite.  Level 0: scores of moderate size whose terms cancel."""
+    print(f"[attention] {Sq}x{Sk} heads {H}/{KH} dh={dh} causal={causal} level {level} rows={rows}", flush=True)
+    rng = np.random.default_rng(Sk + dh)
+    B = 2
+    q, k = sharp(rng, B, Sq, Sk, H, KH, dh, level)
+    if level == 0.0:
+        half = dh // 2
+        for x, h, sign in ((q, H, 1), (k, KH, -1)):
+            y = x.reshape(B, -1, h, dh)
+            y[..., half:] = sign * y[..., :half]
+    v, do = (rng.standard_normal((B, s, h * dh)).astype(np.float32) for s, h in ((Sk, KH), (Sq, H)))
+    got = att_run(Buffers(), (q, k, v), dict(causal=causal, k_len=None, q_start=None, rows=rows), (B, Sq, Sk, H, KH, dh), do, 1.0)
+    for name, x in got.items():
+        assert np.isfinite(x).all(), name
+    ok = ref.allowed(B, Sq, Sk, causal, None, None)[:, None]
+    most = (ok.transpose(0, 1, 3, 2) @ np.abs(wide(do, H))).reshape(B, KH, H // KH, Sk, dh).sum(2)
+    dv = np.abs(per_head(got["dv"], KH).astype(np.float64))
+    assert (dv <= most * (1 + ref.g(Sq * H)) + 4 * Sq * ref.F * np.abs(do).max()).all(), (dv - most).max()
