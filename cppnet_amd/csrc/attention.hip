@@ -992,10 +992,9 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
       evt = ev_next;
       continue;
     }
-    // values below 2^-60 of the largest add nothing that is kept
-    const int over = meet_exp(o, ev, evt);
-    const bool adds = over <= 60;
-    const int dv = adds ? over : 0;
+    // Values below 2^-60 of the largest are multiplied by probabilities that the
+    // terms hold as zeros: they add nothing, but for those that are not finite.
+    const int dv = min(meet_exp(o, ev, evt), 60);
     top(t - 1, ek, dv);
     ek = ek_next;
     evt = ev_next;
@@ -1017,7 +1016,7 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
       for (int e = 0; e < 8; ++e) pair(s[0], e);
     }
     l += pr::times_exp2(part, dv);
-    if (adds) add.run(before, probs, sums, [](int) {});
+    add.run(before, probs, sums, [](int) {});
   }
   l += other_half(l);
   const float f = lim > 0 ? 1.f / l : 0.f;

@@ -155,3 +155,30 @@ def test_gradients_of_scores_far_from_zero(gpu, Sq, Sk, H, KH, dh, causal, level
     most = (ok.transpose(0, 1, 3, 2) @ np.abs(wide(do, H))).reshape(B, KH, H // KH, Sk, dh).sum(2)
     dv = np.abs(per_head(got["dv"], KH).astype(np.float64))
     assert (dv <= most * (1 + ref.g(Sq * H)) + 4 * Sq * ref.F * np.abs(do).max()).all(), (dv - most).max()
+
+
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("B,Sq,Sk,H,KH,dh", [(2, 1, 100, 2, 2, 32), (2, 20, 100, 2, 1, 64), (8, 130, 100, 8, 4, 64), (16, 128, 70, 4, 4, 32)])
+def test_values_that_are_not_finite_among_small_ones(gpu, B, Sq, Sk, H, KH, dh, what):
+    """A block of values that are zeros but for one that is not finite: its
+    feature of out is not finite either, however small the block's others are
+    beside those of the blocks before; other features are as without it."""
+    print(f"[attention] B={B} {Sq}x{Sk} heads {H}/{KH} dh={dh} {what}", flush=True)
+    rng = np.random.default_rng(Sk + dh)
+    f = lambda s, h: rng.standard_normal((B, s, h * dh)).astype(np.float32)  # noqa: E731
+    q, k, v = f(Sq, H), f(Sk, KH), f(Sk, KH)
+    v[:, 32:64] = 0
+    v[:, 40, 3] = what  # feature 3 of the first key head
+    dims, kw = (B, Sq, Sk, H, KH, dh), dict(causal=False, k_len=None, q_start=None, rows=SAMPLE)
+    got = att_run(Buffers(), (q, k, v), kw, dims)
+    out = per_head(got["out"], H)
+    readers = slice(0, H // KH)
+    assert not np.isfinite(out[:, readers, :, 3]).any()
+    v[:, 40, 3] = 0
+    want = ref.attention(wide(q, H), wide(k, KH), wide(v, KH), ref.allowed(B, Sq, Sk, False, None, None), dh ** -0.5)
+    hit = np.zeros(out.shape, bool)
+    hit[:, readers, :, 3] = True
+    ref.check("out", np.where(hit, 0, out), np.where(hit, 0, want["out"][0]), want["out"][1])
+    ref.check("lse", got["lse"].transpose(0, 2, 1), *want["lse"])
+    v[:, 32:64] = what  # and a block of nothing else
+    assert not np.isfinite(att_run(Buffers(), (q, k, v), kw, dims)["out"]).any()
