@@ -887,6 +887,14 @@ __device__ __forceinline__ int tiles_read(const AttArgs& a, int n, int64_t start
 
 constexpr float kPExp = 14.f;  // probabilities enter times 2^14
 
+// scale log2(e) over the packed operands' scales.  Neither zero, so that times the
+// score of a key that is not read it stays infinite, nor infinite, so that times a
+// score of zero it stays zero.
+__device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
+  const float c = pr::times_exp2(a.scale * kLog2e, -exps);
+  return copysignf(fminf(fmaxf(fabsf(c), 0x1p-126f), 0x1p127f), c);
+}
+
 // Forward: a wave holds 32 queries of one head and streams the keys and values,
 // which a block's four waves share through LDS.  Scores of the next tile are formed
 // beside the probabilities of this one.  Bound by the fp16 matrix cores, whose
@@ -934,8 +942,8 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   // tile t's scores masked, the maximum and what it rescales; ek, the exponents
   // of the tile's keys, and dv, by how much that of its values is above ev
   auto top = [&](int t, int ek, int dv) {
-    // not zero, so that a masked score stays -inf
-    c = fmaxf(pr::times_exp2(fabsf(a.scale) * kLog2e, -eq - ek), 0x1p-126f);
+    // of no sign: it is in q
+    c = fabsf(score_factor(a, eq + ek));
     if (!__all(lim >= 32 * t + 32)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -1028,13 +1036,6 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
   if (a.lse && held && lane < 32)
     a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] =
         lim > 0 ? (m + log2f(pr::times_exp2(l, -(int)kPExp))) * kLn2 : -INFINITY;
-}
-
-// scale log2(e) over the packed operands' scales; not zero, so that times the
-// score of a key that is not read it stays infinite
-__device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
-  const float c = pr::times_exp2(a.scale * kLog2e, -exps);
-  return copysignf(fmaxf(fabsf(c), 0x1p-126f), c);
 }
 
 // A probability times 2^top from its score and its row's lse (base 2) less top.

@@ -182,3 +182,24 @@ def test_values_that_are_not_finite_among_small_ones(gpu, B, Sq, Sk, H, KH, dh, 
     ref.check("lse", got["lse"].transpose(0, 2, 1), *want["lse"])
     v[:, 32:64] = what  # and a block of nothing else
     assert not np.isfinite(att_run(Buffers(), (q, k, v), kw, dims)["out"]).any()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,Sq,Sk,H,KH,dh", [(2, 1, 100, 2, 2, 32), (2, 20, 100, 2, 1, 64), (2, 70, 90, 2, 1, 64), (8, 130, 100, 8, 4, 64)])
+def test_large_operands_that_do_not_meet(gpu, B, Sq, Sk, H, KH, dh, causal):
+    """Queries of 2^80 in one feature and keys of 2^80 in another: every score is
+    an exact 0.  Values and gradients are those of the same operands at 1, dq and
+    dk times 2^80."""
+    print(f"[attention] B={B} {Sq}x{Sk} heads {H}/{KH} dh={dh} causal={causal}", flush=True)
+    rng = np.random.default_rng(Sk + dh)
+    q, k = np.zeros((B, Sq, H, dh), np.float32), np.zeros((B, Sk, KH, dh), np.float32)
+    q[..., 1], k[..., 2] = 1, 1
+    q, k = q.reshape(B, Sq, H * dh), k.reshape(B, Sk, KH * dh)
+    v, do = (rng.standard_normal((B, s, h * dh)).astype(np.float32) for s, h in ((Sk, KH), (Sq, H)))
+    big = np.float32(2.0 ** 80)
+    dims, kw = (B, Sq, Sk, H, KH, dh), dict(causal=causal, k_len=None, q_start=None, rows=SAMPLE)
+    got = att_run(Buffers(), (q * big, k * big, v), kw, dims, do)
+    want = ref.attention(wide(q, H), wide(k, KH), wide(v, KH), ref.allowed(B, Sq, Sk, causal, None, None), dh ** -0.5, wide(do, H))
+    for name, (w, lim) in want.items():
+        x = got[name].transpose(0, 2, 1) if name == "lse" else per_head(got[name], KH if name in ("dk", "dv") else H)
+        print("  ", name, ref.check(name, x * 2.0 ** -80 if name in ("dq", "dk") else x, w, lim))
