@@ -891,8 +891,8 @@ constexpr float kPExp = 14.f;  // probabilities enter times 2^14
 // score of a key that is not read it stays infinite, nor infinite, so that times a
 // score of zero it stays zero.
 __device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
-  const float c = pr::times_exp2(a.scale * kLog2e, -exps);
-  return copysignf(fminf(fmaxf(fabsf(c), 0x1p-126f), 0x1p127f), c);
+  const float c = fminf(fmaxf(pr::times_exp2(fabsf(a.scale) * kLog2e, -exps), 0x1p-126f), 0x1p127f);
+  return a.scale < 0.f ? -c : c;  // as unread keys' scores have it, also at a scale of -0
 }
 
 // Forward: a wave holds 32 queries of one head and streams the keys and values,

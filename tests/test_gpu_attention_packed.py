@@ -203,3 +203,13 @@ def test_large_operands_that_do_not_meet(gpu, B, Sq, Sk, H, KH, dh, causal):
     for name, (w, lim) in want.items():
         x = got[name].transpose(0, 2, 1) if name == "lse" else per_head(got[name], KH if name in ("dk", "dv") else H)
         print("  ", name, ref.check(name, x * 2.0 ** -80 if name in ("dq", "dk") else x, w, lim))
+
+
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+@pytest.mark.parametrize("B,Sq,Sk,H,KH,dh", [(2, 3, 50, 2, 2, 32), (2, 40, 70, 2, 1, 64), (8, 130, 100, 8, 4, 64)])
+def test_scale_of_minus_zero(gpu, B, Sq, Sk, H, KH, dh, rows):
+    rng = np.random.default_rng(Sk)
+    k_len, start = [Sk - 9] * B, [Sk - Sq - 9] * B
+    x = data(rng, B, Sq, Sk, H, KH, dh, True, k_len, start)
+    got = att_check((B, Sq, Sk, H, KH, dh), True, k_len, start, rows, -0.0, *x)
+    assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
