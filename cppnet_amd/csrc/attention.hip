@@ -891,7 +891,7 @@ constexpr float kPExp = 14.f;  // probabilities enter times 2^14
 // score of a key that is not read it stays infinite, nor infinite, so that times a
 // score of zero it stays zero.
 __device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
-  const float c = fminf(fmaxf(pr::times_exp2(fabsf(a.scale) * kLog2e, -exps), 0x1p-126f), 0x1p127f);
+  const float c = __builtin_amdgcn_fmed3f(pr::times_exp2(fabsf(a.scale) * kLog2e, -exps), 0x1p-126f, 0x1p127f);
   return a.scale < 0.f ? -c : c;  // as unread keys' scores have it, also at a scale of -0
 }
 
