@@ -276,14 +276,14 @@ __global__ void __launch_bounds__(NT) att_fwd_kernel(AttArgs a, SplitArgs p) {
       own[(32 * d + 8 * (e / 4) + 4 * (lane >> 5) + e % 4) * 32 + (lane & 31)] = o[d][e] * f;
   __syncthreads();
   const int64_t at = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-  const float inv = p.splits > 1 ? 1.f : lim > 0 ? 1.f / total : 0.f;
+  const float inv = 1.f / total;
   float* out = a.out.at(b, i, (int64_t)head * a.dh);
   for (int d = 2 * wave + (lane >> 5); d < a.dh; d += 8) {
     float x = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) x += lds[w][0][d * 32 + (lane & 31)];
     if (p.splits > 1) p.o[(at * a.dh + d) * 32 + (lane & 31)] = x;
-    else if (held) out[d * a.out.col] = x * inv;
+    else if (held) out[d * a.out.col] = lim > 0 ? x * inv : 0.f;
   }
   if (wave != 0 || lane >= 32) return;
   if (p.splits > 1) p.ml[at * 32 + lane] = float2{top, total};
@@ -546,11 +546,11 @@ __global__ void __launch_bounds__(NT) att_join_kernel(AttArgs a, SplitArgs p) {
       if (d0 + e < a.dh) x[e] = fmaf(p.o[((at + s * step) * a.dh + d0 + e) * 32 + lane], f, x[e]);
   }
   const bool reads = limit(a, keys_of(a, b), start_of(a, b), i) > 0;
-  const float inv = reads ? 1.f / total : 0.f;
+  const float inv = 1.f / total;
   float* out = a.out.at(b, i, (int64_t)head * a.dh);
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (d0 + e < a.dh) out[(d0 + e) * a.out.col] = x[e] * inv;
+    if (d0 + e < a.dh) out[(d0 + e) * a.out.col] = reads ? x[e] * inv : 0.f;
   if (a.lse && part == 0 && blockIdx.z == 0)
     a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = reads ? (top + log2f(total)) * kLn2 : -INFINITY;
 }
@@ -625,16 +625,19 @@ __device__ __forceinline__ float most_norm(const PackArgs& p, int which, int64_t
   return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(n)));
 }
 
-// The head of an operand that a wave works on, and the rows that its sample has
-// (past them k and v count as zeros).
+// The head of an operand that a wave works on, and the rows of its sample that
+// count, first .. rows - 1: keys that the sample has, queries that read a key.
+// Others are zeros, whatever they hold.
 struct Operand {
   int which, b, head;
   int64_t bh;  // head of a sample, counted through
-  int rows;
+  int first, rows;
 };
 __device__ __forceinline__ Operand operand(const AttArgs& a, int which, int b, int head) {
-  const bool kv = which == 1 || which == 2;
-  return Operand{which, b, head, (int64_t)b * (kv ? a.kv_heads : a.heads) + head, kv ? keys_of(a, b) : a.Sq};
+  const int n = keys_of(a, b);
+  if (which == 1 || which == 2) return Operand{which, b, head, (int64_t)b * a.kv_heads + head, 0, n};
+  const int64_t before = a.causal ? -start_of(a, b) : 0;  // queries before the first key
+  return Operand{which, b, head, (int64_t)b * a.heads + head, (int)(before < 0 ? 0 : min(before, (int64_t)a.Sq)), n > 0 ? a.Sq : 0};
 }
 
 // 32 rows of a head in a wave's registers: features 16 s + 8 (lane / 32) .. + 7 of
@@ -644,7 +647,7 @@ struct RowBlock {
   float v[KS][8];
   __device__ __forceinline__ void load(const AttArgs& a, const Seq<const float>& x, const Operand& o, int blk) {
     const int lane = (int)threadIdx.x & 63, r = blk * 32 + (lane & 31), d0 = 8 * (lane >> 5);
-    const bool held = r < o.rows;
+    const bool held = r >= o.first && r < o.rows;
     const float* q = x.at(o.b, held ? r : 0, (int64_t)o.head * a.dh);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -697,7 +700,7 @@ struct RowBlock {
 #pragma unroll
       for (int e = 0; e < 8; ++e) d = fmaf(v[s][e], out.v[s][e], d);
     d += other_half(d);
-    if (r < o.rows && lane < 32) a.delta[o.bh * a.Sq + r] = d;
+    if (r < a.Sq && lane < 32) a.delta[o.bh * a.Sq + r] = d;
   }
 };
 
@@ -1027,11 +1030,11 @@ __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int til
     add.run(before, probs, sums, [](int) {});
   }
   l += other_half(l);
-  const float f = lim > 0 ? 1.f / l : 0.f;
+  const float f = 1.f / l;
 #pragma unroll
   for (int d = 0; d < DHP / 32; ++d)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[d][e] = pr::times_exp2(o[d][e] * f, -ev);
+    for (int e = 0; e < 16; ++e) o[d][e] = lim > 0 ? pr::times_exp2(o[d][e] * f, -ev) : 0.f;
   store_row<DHP>(a.out.at(b, held ? i : 0, (int64_t)head * a.dh), a.out.col, held, a.dh, 1.f, o);
   if (a.lse && held && lane < 32)
     a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] =
@@ -1143,7 +1146,7 @@ __device__ __forceinline__ void dq_block(const PairArgs& g, int bid, int tiles, 
 #pragma unroll
   for (int d = 0; d < DHP / 32; ++d)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[d][e] = pr::times_exp2(acc[d][e], -ek - ed);
+    for (int e = 0; e < 16; ++e) acc[d][e] = lim > 0 ? pr::times_exp2(acc[d][e], -ek - ed) : 0.f;
   store_row<DHP>(a.dq.at(b, held ? i : 0, (int64_t)head * a.dh), a.dq.col, held, a.dh, a.scale, acc);
 }
 

@@ -213,3 +213,39 @@ def test_scale_of_minus_zero(gpu, B, Sq, Sk, H, KH, dh, rows):
     x = data(rng, B, Sq, Sk, H, KH, dh, True, k_len, start)
     got = att_check((B, Sq, Sk, H, KH, dh), True, k_len, start, rows, -0.0, *x)
     assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
+
+
+@pytest.mark.parametrize("what", [np.nan, np.inf, 1e30])
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+@pytest.mark.parametrize("B,Sq,Sk,H,KH,dh", [(3, 4, 60, 2, 2, 32), (3, 40, 600, 2, 1, 64), (3, 70, 90, 2, 1, 64), (9, 130, 100, 8, 4, 64),
+                                             (9, 257, 140, 4, 4, 128)])
+def test_queries_that_read_nothing_may_hold_anything(gpu, B, Sq, Sk, H, KH, dh, rows, what):
+    """The first queries of a sample that begins before its keys, and all of a
+    sample without keys, give zero rows and reach no gradient."""
+    print(f"[attention] B={B} {Sq}x{Sk} heads {H}/{KH} dh={dh} rows={rows} {what}", flush=True)
+    rng = np.random.default_rng(Sk + dh)
+    f = lambda s, h: rng.standard_normal((B, s, h * dh)).astype(np.float32)  # noqa: E731
+    q, k, v, do = f(Sq, H), f(Sk, KH), f(Sk, KH), f(Sq, H)
+    start = [(-(Sq // 2), 3, -1)[b % 3] for b in range(B)]
+    k_len = [(Sk, 0, Sk - 5)[b % 3] for b in range(B)]
+    ok = ref.allowed(B, Sq, Sk, True, k_len, start)
+    reads = ok.any(2)[:, :, None]
+    assert not reads.all() and reads.any()
+    dims, kw = (B, Sq, Sk, H, KH, dh), dict(causal=True, k_len=k_len, q_start=start, rows=rows)
+    buf = Buffers()
+    got = att_run(buf, (np.where(reads, q, np.float32(what)), k, v), kw, dims, np.where(reads, do, np.float32(what)))
+    read = ok.any(1)[:, :, None]
+    want = ref.attention(wide(np.where(reads, q, 0), H), wide(np.where(read, k, 0), KH), wide(np.where(read, v, 0), KH), ok,
+                         dh ** -0.5, wide(np.where(reads, do, 0), H))
+    for name, (w, lim) in want.items():
+        x = got[name].transpose(0, 2, 1) if name == "lse" else per_head(got[name], KH if name in ("dk", "dv") else H)
+        print("  ", name, ref.check(name, x, w, lim))
+    for name in ("out", "dq"):
+        assert (got[name][~reads[:, :, 0]] == 0).all()
+    buf.intact()
+    # nor does a key or value that only the others read reach their rows
+    k[:, 0], v[:, 0] = what, what
+    got = att_run(Buffers(), (q, k, v), kw, dims, do)
+    for name in ("out", "dq"):
+        assert (got[name][~reads[:, :, 0]] == 0).all()
+    assert (got["lse"][~reads[:, :, 0]] == -np.inf).all()
