@@ -1,6 +1,7 @@
 // Runtime services of the C ABI: errors, devices, memory, streams, events.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdint>
@@ -44,6 +45,7 @@ struct ScratchEntry {
   void* p;
   size_t cap;
   uint64_t gen;  // which allocation p is (unique over the process)
+  bool held;     // a graph that was captured by other means than cnhip_graph_* refers to p
 };
 uint64_t g_scratch_gens = 0;
 std::mutex g_scratch_mu;
@@ -51,6 +53,8 @@ std::vector<ScratchEntry> g_scratch;
 // Streams whose scratch slots a captured graph refers to: their buffers
 // must keep their addresses, so a request that would grow one fails.
 std::vector<std::pair<int, hipStream_t>> g_frozen;
+// Streams that cnhip_graph_begin_capture captures (they are frozen afterwards).
+std::vector<hipStream_t> g_capturing;
 
 bool frozen(int dev, hipStream_t stream) {
   for (auto& f : g_frozen)
@@ -159,12 +163,13 @@ int scratch(hipStream_t stream, int slot, size_t bytes, void** ptr, uint64_t* ge
   for (auto& x : g_scratch)
     if (x.dev == dev && x.stream == stream && x.slot == slot) e = &x;
   if (!e) {
-    g_scratch.push_back(ScratchEntry{dev, stream, slot, nullptr, 0, 0});
+    g_scratch.push_back(ScratchEntry{dev, stream, slot, nullptr, 0, 0, false});
     e = &g_scratch.back();
   }
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  // the default stream cannot be captured, and is not asked for nothing while another is
+  if (stream || e->cap < bytes) CNHIP_TRY(check_hip(hipStreamIsCapturing(stream, &cs), where));
   if (e->cap < bytes) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    CNHIP_TRY(check_hip(hipStreamIsCapturing(stream, &cs), where));
     if (cs != hipStreamCaptureStatusNone || frozen(dev, stream)) {
       set_error("%s: scratch slot %d of this stream must grow to %zu bytes (has %zu) while a "
                 "captured graph uses it; run the work once uncaptured before capturing it",
@@ -173,9 +178,12 @@ int scratch(hipStream_t stream, int slot, size_t bytes, void** ptr, uint64_t* ge
     }
     if (e->p) {
       void* old = e->p;
+      const bool held = e->held;
       e->p = nullptr;
       e->cap = 0;
-      CNHIP_TRY(check_hip(hipFreeAsync(old, stream), where));
+      e->held = false;
+      // nobody tells when such a graph is gone: its replays keep their workspace
+      if (!held) CNHIP_TRY(check_hip(hipFreeAsync(old, stream), where));
     }
     // grow with headroom, in 2 MiB steps, so slowly rising sizes settle
     size_t cap = bytes + bytes / 4;
@@ -184,6 +192,9 @@ int scratch(hipStream_t stream, int slot, size_t bytes, void** ptr, uint64_t* ge
     e->cap = cap;
     e->gen = ++g_scratch_gens;
   }
+  if (cs != hipStreamCaptureStatusNone &&
+      std::find(g_capturing.begin(), g_capturing.end(), stream) == g_capturing.end())
+    e->held = true;
   *ptr = e->p;
   if (gen) *gen = e->gen;
   if (cap_out) *cap_out = e->cap;
@@ -348,7 +359,10 @@ int cnhip_graph_begin_capture(cnhip_stream_t stream) {
   CNHIP_REQUIRE(!cnhip::timing_on(), "%s: per-launch kernel timing is enabled; disable it first", who);
   // Relaxed: allocations of not-yet-cached buffers by the host layer may
   // call hipMalloc while the capture is open (that is not stream work).
-  return check_hip(hipStreamBeginCapture(as_stream(stream), hipStreamCaptureModeRelaxed), who);
+  CNHIP_TRY(check_hip(hipStreamBeginCapture(as_stream(stream), hipStreamCaptureModeRelaxed), who));
+  std::lock_guard<std::mutex> lock(cnhip::g_scratch_mu);
+  cnhip::g_capturing.push_back(as_stream(stream));
+  return CNHIP_OK;
 }
 
 int cnhip_graph_end_capture(cnhip_stream_t stream, int ok, cnhip_graph_t* graph) {
@@ -357,6 +371,11 @@ int cnhip_graph_end_capture(cnhip_stream_t stream, int ok, cnhip_graph_t* graph)
   if (graph) *graph = nullptr;
   hipGraph_t g = nullptr;
   const hipError_t e = hipStreamEndCapture(as_stream(stream), &g);
+  {
+    std::lock_guard<std::mutex> lock(cnhip::g_scratch_mu);
+    auto& open = cnhip::g_capturing;
+    open.erase(std::remove(open.begin(), open.end(), as_stream(stream)), open.end());
+  }
   if (e != hipSuccess || !ok || !graph) {
     if (g) (void)hipGraphDestroy(g);
     if (e != hipSuccess) return check_hip(e, who);

@@ -753,8 +753,11 @@ int cnhip_rnn_backward(const float* X, const float* W_ih, const float* W_hh, con
  * the same sizes first.  Calls on different streams may overlap; calls on one
  * stream from several host threads at once are not supported.  Every sum runs
  * in an order fixed by the arguments, so equal calls give equal bits.
- * A graph captured by other means holds the stream's workspace as well, but
- * does not freeze it.  No output may overlap an input.
+ * A graph captured by other means holds the stream's workspace as well, without
+ * freezing it: a later call that needs more takes a new one and leaves the
+ * graph's as it is until the process ends.  Graphs captured on one stream share
+ * its workspace, so their replays must follow each other and the stream's other
+ * calls.  No output may overlap an input.
  * Large products run on pairs of fp16 terms: a value is kept to 2^-22 of
  * itself, but no closer than 2^-39 of its operand's largest finite value (X's
  * rows with a target, W, the gradient of the logits; 32 rows of a head of q, k,
