@@ -290,23 +290,8 @@ __global__ void __launch_bounds__(NT) att_fwd_kernel(AttArgs a, SplitArgs p) {
   else if (a.lse && held) a.lse[b * a.lse_sample + i * a.lse_row + head * a.lse_col] = lim > 0 ? (top + log2f(total)) * kLn2 : -INFINITY;
 }
 
-// Forward of a key head with up to R query rows (4 or 8), single tokens above
-// all: half a flop a byte of the cache and row, which the vector ALUs keep up with,
-// where a matrix instruction would fill 32 rows for them.  A wave takes tiles of
-// 32 keys as they lie in memory: lane l has keys 4 (l % 8) .. + 3 of features l / 8
-// + 8 i, so every load is a float4 and nothing is staged.  The lanes' parts of the
-// scores are summed so that each ends with one row's four, whose softmax is its
-// part; the probabilities reach the other lanes through LDS, and each lane sums
-// its own keys' share of its own features of out until the end.  The loads run a
-// chunk of C features ahead.
-//
-// Bound by the cache's bytes.  16 samples of 4096 keys, head_dim 128 (268 MB),
-// with the joining launch: 16 heads on 4 47 us (5.6 TB/s; the kernel of 32 rows
-// 94), 32 on 4 72 (95); one sample of 16384, 64 on 8 (134 MB) 50 (126); 64 samples
-// of 1024, 8 on 8, head_dim 64 (268 MB) 42 (70).
-// x[0 .. N) summed over LANES lanes: of N /
-// LANES sums each, the q-th lane has those from q N / LANES on, in
-// x[0 ..).  UNIT: the distance of those lanes.
+// x[0 .. N) summed over LANES lanes that are UNIT apart.  Of the N sums each ends
+// with N / LANES in x[0 ..): the q-th lane with those from q N / LANES on.
 template <int N, int LANES, int UNIT, int SIZE>
 __device__ __forceinline__ void sum_scatter(float (&x)[SIZE]) {
   if constexpr (LANES > 1) {
@@ -334,6 +319,20 @@ __device__ __forceinline__ void put_few(const AttArgs& a, int n, int b, int kh, 
 // waves of a SIMD that the registers allow
 constexpr int few_waves(int dhp, int r) { return dhp * r > 512 ? 1 : 2; }
 
+// Forward of a key head with up to R query rows (4 or 8), single tokens above
+// all: half a flop a byte of the cache and row, which the vector ALUs keep up with,
+// where a matrix instruction would fill 32 rows for them.  A wave takes tiles of
+// 32 keys as they lie in memory: lane l has keys 4 (l % 8) .. + 3 of features l / 8
+// + 8 i, so every load is a float4 and nothing is staged.  The lanes' parts of the
+// scores are summed so that each ends with one row's four, whose softmax is its
+// part; the probabilities reach the other lanes through LDS, and each lane sums
+// its own keys' share of its own features of out until the end.  The loads run a
+// chunk of C features ahead.
+//
+// Bound by the cache's bytes.  16 samples of 4096 keys, head_dim 128 (268 MB),
+// with the joining launch: 16 heads on 4 47 us (5.6 TB/s; the kernel of 32 rows
+// 94), 32 on 4 72 (95); one sample of 16384, 64 on 8 (134 MB) 50 (126); 64 samples
+// of 1024, 8 on 8, head_dim 64 (268 MB) 42 (70).
 template <int DHP, int R, bool UNIT>
 __global__ void __launch_bounds__(NT, few_waves(DHP, R)) att_few_kernel(AttArgs a, SplitArgs p) {
   constexpr int G = 8, L = 64 / G, TK = 4 * L, NF = DHP / G, C = 4, NC = NF / C, OWN = R * NF / L;
@@ -1387,7 +1386,6 @@ bool pairs_forward(const AttArgs& a) { return a.Sq >= 64 && (int64_t)a.B * a.hea
 
 constexpr int kMaxHeadDim = 128;
 constexpr int64_t kFewRows = 8;  // query rows of a key head that att_few_kernel takes, whose comment measures both sides
-
 
 template <class T>
 Seq<T> seq(T* p, int64_t B, int64_t S, int rows) {

@@ -30,11 +30,6 @@
 #include "mfma_pair.hpp"
 
 namespace cnhip {
-
-int gemm_f32(int trans_a, int trans_b, int64_t M, int64_t N, int64_t K, float alpha, const float* A, int64_t lda,
-             const float* B, int64_t ldb, float beta, float* C, int64_t ldc, const float* bias, int epilogue,
-             hipStream_t st, const char* who);
-
 namespace {
 
 using pr::f32x16;
