@@ -37,6 +37,8 @@ using pr::f32x4;
 using pr::f32x4u;
 using pr::u32x4;
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 // What the kernels of a call share, at the head of its workspace.
 struct CeState {
   int held;        // rows of the batch with a target
@@ -53,6 +55,7 @@ struct CeArgs {
   float2* stat;        // [stat_blocks][R]: maximum and sum of exp(z - maximum)
   int64_t stat_blocks;
   float *lse, *row_loss;
+  float2* top;         // of the piece's rows: largest logit, log of the sum of exp(z - largest)
   CeState* state;
   uint32_t *row_max, *w_part;  // largest finite |X| of each row, |W| of each block's part
   int w_blocks;
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(pr::GNT, 2) ce_logits_kernel(pr::GemmArgs g, C
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        sum += __builtin_amdgcn_exp2f((acc.x[i][j][e] - base) * 1.4426950408889634f);
+        sum += __builtin_amdgcn_exp2f((acc.x[i][j][e] - base) * kLog2e);
     sum += __shfl_xor(sum, 32, 64);
     if (n >= g.N) continue;
     if (lane < 32) a.stat[(int64_t)(tm * 2 + (wave >> 2)) * a.R + n] = float2{top, sum};
@@ -513,15 +516,18 @@ __global__ void __launch_bounds__(1024) ce_row_kernel(CeArgs a, int grads) {
   __syncthreads();
   if (wave || r >= a.R) return;
   for (int w = 1; w < 16; ++w) x = join(x, part[w][lane]);
-  const float lse = x.x + logf(x.y);
+  const float log_sum = logf(x.y);
   const int64_t n = a.row0 + r;
   const bool held = has_target(a, n);
-  a.lse[n] = lse;
-  a.row_loss[n] = held ? lse - (grads ? a.Z[r + a.R * (int64_t)a.t[n]] : a.zt[n]) : 0.f;
+  a.lse[n] = x.x + log_sum;
+  if (grads) a.top[r] = float2{x.x, log_sum};
+  a.row_loss[n] = held ? (x.x - (grads ? a.Z[r + a.R * (int64_t)a.t[n]] : a.zt[n])) + log_sum : 0.f;
 }
 
 // The piece's G packed, a wave for a step of 16 classes and eight blocks of 32
-// rows; with its column sums where they are wanted.
+// rows; with its column sums where they are wanted.  The softmax is taken from the
+// row's largest logit and log sum apart: their sum, the lse, is rounded to 2^-24 of
+// itself, which logits of 10^5 and more would feel.
 __global__ void __launch_bounds__(256) ce_grad_kernel(CeArgs a) {
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -537,13 +543,14 @@ __global__ void __launch_bounds__(256) ce_grad_kernel(CeArgs a) {
     const bool in = n < a.R;
     const int32_t t = in ? a.t[a.row0 + n] : -1;
     const bool held = t >= 0 && t < a.V;
-    const float lse = in ? a.lse[a.row0 + n] : 0.f;
+    const float2 top = in ? a.top[n] : float2{0.f, 0.f};
+    const float log2_sum = top.y * kLog2e;
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = in && v0 + e < a.V ? a.Z[n + a.R * (v0 + e)] : -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      x[e] = __builtin_amdgcn_exp2f((x[e] - lse) * 1.4426950408889634f) - (v0 + e == t ? 1.f : 0.f);
+      x[e] = __builtin_amdgcn_exp2f(fmaf(x[e] - top.x, kLog2e, -log2_sum)) - (v0 + e == t ? 1.f : 0.f);
       x[e] = held && v0 + e < a.V ? x[e] * one : 0.f;
       sum[e] += x[e];
     }
@@ -725,9 +732,12 @@ __global__ void __launch_bounds__(1024) ce_few_rows_kernel(CeArgs a, float* __re
   for (int w = 1; w < 16; ++w) x = join(x, part[w][lane]);
   const int32_t t = lane < a.N ? a.t[lane] : -1;
   const bool held = t >= 0 && t < a.V;
-  const float lse = x.x + logf(x.y);
-  if (lane < a.N) a.lse[lane] = lse;
-  float l = held ? lse - a.Z[lane + a.N * (int64_t)t] : 0.f;
+  const float log_sum = logf(x.y);
+  if (lane < a.N) {
+    a.lse[lane] = x.x + log_sum;
+    a.top[lane] = float2{x.x, log_sum};
+  }
+  float l = held ? (x.x - a.Z[lane + a.N * (int64_t)t]) + log_sum : 0.f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
   const int count = __popcll(__ballot(held)), past = __popcll(__ballot(t >= a.V));
@@ -759,7 +769,7 @@ __global__ void __launch_bounds__(256) ce_few_grads_kernel(CeArgs a, float* dW, 
     const int n = threadIdx.x % NR;
     const int32_t t = n < N ? a.t[n] : -1;
     const bool held = t >= 0 && t < a.V;
-    const float lse = held ? a.lse[n] : 0.f;
+    const float2 top = held ? a.top[n] : float2{0.f, 0.f};
     constexpr int STEP = 256 / NR, UG = kFewSlice / STEP, UX = kFewWidth / STEP;
     float z[UG], x[UX];
 #pragma unroll
@@ -776,7 +786,7 @@ __global__ void __launch_bounds__(256) ce_few_grads_kernel(CeArgs a, float* dW, 
     for (int u = 0; u < UG; ++u) {
       const int c = threadIdx.x / NR + u * STEP;
       const int64_t v = v0 + c;
-      G[c * LD + n] = held && v < a.V ? (expf(z[u] - lse) - (v == t ? 1.f : 0.f)) * f : 0.f;
+      G[c * LD + n] = held && v < a.V ? (expf((z[u] - top.x) - top.y) - (v == t ? 1.f : 0.f)) * f : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < UX; ++u) xs[(threadIdx.x / NR + u * STEP) * LD + n] = x[u];
@@ -865,9 +875,11 @@ int run_few(CeArgs& a, float* loss, const CeGrads* g, hipStream_t st, const char
   a.stat_blocks = (V + kFewClasses - 1) / kFewClasses;
   const size_t z = (size_t)(N * V) * 4, stat = (size_t)(a.stat_blocks * N) * 8, part = g ? (size_t)(slices * D * N) * 4 : 0;
   void* ws = nullptr;
-  CNHIP_TRY(scratch(st, kScratchLayer, 256 + stat + z + part, &ws, who));
+  constexpr size_t head = 256 + kFewRows * sizeof(float2);  // the state, the rows' statistics
+  CNHIP_TRY(scratch(st, kScratchLayer, head + stat + z + part, &ws, who));
   a.state = static_cast<CeState*>(ws);
-  a.stat = reinterpret_cast<float2*>(static_cast<char*>(ws) + 256);
+  a.top = reinterpret_cast<float2*>(static_cast<char*>(ws) + 256);
+  a.stat = reinterpret_cast<float2*>(static_cast<char*>(ws) + head);
   a.Z = reinterpret_cast<float*>(a.stat + a.stat_blocks * N);
   float* dx_part = a.Z + N * V;
   const dim3 logits((unsigned)a.stat_blocks), grads((unsigned)slices, (unsigned)((D + kFewWidth - 1) / kFewWidth));
@@ -934,6 +946,7 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
                o_w = place((size_t)(Vp * Dp) * 4), o_z = place(g ? (size_t)R * (size_t)V * 4 : 0),
                o_stat = place((size_t)a.stat_blocks * (size_t)R * 8), o_xe = place(g ? 0 : (size_t)N * 4),
                o_we = place(g ? 0 : (size_t)(Vp / 32) * 4), o_zt = place(g ? 0 : (size_t)N * 4);
+  const size_t o_top = place(g ? (size_t)R * sizeof(float2) : 0);
   const size_t o_g = place(g ? (size_t)(Rp * Vp) * 4 : 0), o_db = place(g && g->db ? (size_t)((R + 255) / 256 * V) * 4 : 0);
   const size_t px = sx.splits > 1 ? (size_t)sx.splits * (size_t)(D * R) * 4 : 0,
                pw = sw.splits > 1 ? (size_t)sw.splits * (size_t)(V * D) * 4 : 0;
@@ -953,6 +966,7 @@ int run(const float* X, const float* W, const float* b, const int32_t* targets, 
   a.xe = reinterpret_cast<int*>(base + o_xe);
   a.we = reinterpret_cast<int*>(base + o_we);
   a.zt = reinterpret_cast<float*>(base + o_zt);
+  a.top = reinterpret_cast<float2*>(base + o_top);
   a.db_part = g && g->db ? reinterpret_cast<float*>(base + o_db) : nullptr;
   float* part = reinterpret_cast<float*>(base + o_part);
 
