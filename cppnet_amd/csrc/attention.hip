@@ -899,9 +899,9 @@ __device__ __forceinline__ float score_factor(const AttArgs& a, int exps) {
 
 // Forward: a wave holds 32 queries of one head and streams the keys and values,
 // which a block's four waves share through LDS.  Scores of the next tile are formed
-// beside the probabilities of this one.  Bound by the fp16 matrix cores, whose
-// sustained rate is 341 TFLOP/s of fp32 products: 2 x 4096 causal, 16 heads of 128,
-// 454 us (303 TFLOP/s).
+// beside the probabilities of this one.  Bound by the fp16 matrix cores (341
+// TFLOP/s of fp32 products at a large library product's rate): 2 x 4096 causal, 16
+// heads of 128, 452 us (304 TFLOP/s).
 template <int DHP>
 __global__ void __launch_bounds__(NT, 2) att_fwd_pair_kernel(PairArgs g, int tiles) {
   constexpr int KS = DHP / 16, TILE = KS * 2 * pr::kFrag;

@@ -18,10 +18,11 @@
 // leaves each row's maximum and sum of exponentials over the 128 columns that
 // a wave holds, so the logits are read once more only, to become G.
 //
-// Bound by the fp16 matrix cores: a third of their sustained rate (1023 TFLOP/s
-// in a large library product) is 341 TFLOP/s of fp32 products.  8192 rows, 1024 ->
-// 32000: logits 1.61 ms (333 TFLOP/s), dX 1.45 ms (371), dW 1.59 ms (338), G formed
-// and packed 0.38 ms (5.6 TB/s), everything else 0.15 ms.
+// Bound by the fp16 matrix cores at the clock that the power limit leaves: a large
+// library fp16 product reaches 1023 TFLOP/s, a third of which is 341 of fp32
+// products.  8192 rows, 1024 -> 32000: logits 1.56 ms (344 TFLOP/s), dX 1.40 ms
+// (383), dW 1.56 ms (344), G formed and packed 0.42 ms (5.0 TB/s), everything else
+// 0.15 ms; on another card 333, 371 and 338 TFLOP/s.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(1024) ce_loss_kernel(CeArgs a, float* __restri
 // those parts.  64 rows, 512 -> 8192 with gradients: 49 us (15, 7, 26 and 5), of
 // which the fp32 products alone take 10 and the memory 7; 64 against 65 rows, this
 // way and packed: forward 21 and 55 us, with gradients 52 and 110; 1024 -> 32000 95
-// and 140, 277 and 256.
+// and 140, 277 and 256, where the parts of dX are as many bytes as W.
 constexpr int kFewRows = 64;
 constexpr int kFewClasses = 32;   // classes a block of the first launch
 constexpr int kFewSlice = 64;     // classes a block of the third

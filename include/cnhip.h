@@ -761,7 +761,10 @@ int cnhip_rnn_backward(const float* X, const float* W_ih, const float* W_hh, con
  * Large products run on pairs of fp16 terms: a value is kept to 2^-22 of
  * itself, but no closer than 2^-39 of its operand's largest finite value (X's
  * rows with a target, W, the gradient of the logits; 32 rows of a head of q, k,
- * v and dout, whose sums' scale is that of the largest block so far).
+ * v and dout, whose sums' scale is that of the largest block so far).  So a
+ * probability enters the cross-entropy's gradients to within 2^-40, and one that
+ * stays below that in every row gives its class a gradient of zero; an infinity in
+ * such an operand comes out as NaN.
  *
  * Token embedding: out[p, d] = scale * Wt[d + D id_p], ids ColMajor [B, S],
  * out a [B, S, D] sequence in either row order.  Ids outside [0, V) give zero
@@ -793,11 +796,14 @@ int cnhip_token_embedding_backward(const int32_t* ids, const float* dY, float* g
  * causal at and past q_start + Sq) are never used, whatever they hold; a query
  * that reads no key gives a zero row and lse = -inf.  A NaN or infinity in a key
  * or value that only some queries of the sample read can reach the causal rows
- * just before it.
+ * just before it, and one in a row of q or dout the gradients of the keys just
+ * behind those that it reads; a row that reads none reaches nothing.
  * lse [B*Sq, heads] has q's rows; it may be NULL in the forward.
  * backward: gradients of q, k and v (overwritten; zeros for keys that no query
- * reads) from out, lse and dout; the probabilities are formed again, dk and dv
- * are summed over the heads that share a key head.  head_dim <= 128,
+ * reads) from out, lse and dout; dk and dv are summed over the heads that share a
+ * key head.  The probabilities are formed again from lse, to about 2^-22 |lse| of
+ * themselves beside the scores' own errors, and held to 1: scores of 10^5 and more
+ * leave the gradients few right digits, but finite.  head_dim <= 128,
  * B * heads <= 65535. */
 int cnhip_attention_forward(const float* q, const float* k, const float* v, float* out,
                             float* lse, int64_t B, int64_t Sq, int64_t Sk, int64_t heads,
@@ -821,7 +827,10 @@ int cnhip_attention_backward(const float* q, const float* k, const float* v, con
  * finite count as zeros.
  * head: also dX [batch, in_features] (overwritten), dW and db (added to with
  * accumulate, else overwritten; db NULL exactly where b is).  No logits
- * outlive the call; the rows go through in pieces that bound the workspace. */
+ * outlive the call: the rows go through in pieces of up to 2^27 logits (1024 rows
+ * where that is more).  The stream's scratch holds and keeps a piece's logits and
+ * their gradients (1 GiB at 2^27), X and W as packed, and where a product is split
+ * its parts; up to 64 rows, the logits and a part of dX for every 64 classes. */
 int cnhip_linear_ce_forward(const float* X, const float* W, const float* b,
                             const int32_t* targets, float* loss, float* lse, int64_t batch,
                             int64_t in_features, int64_t classes, int reduction,
