@@ -167,7 +167,7 @@ int scratch(hipStream_t stream, int slot, size_t bytes, void** ptr, uint64_t* ge
     e = &g_scratch.back();
   }
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  // the default stream cannot be captured, and is not asked for nothing while another is
+  // the default stream cannot be captured: it is asked only where its buffer has to grow
   if (stream || e->cap < bytes) CNHIP_TRY(check_hip(hipStreamIsCapturing(stream, &cs), where));
   if (e->cap < bytes) {
     if (cs != hipStreamCaptureStatusNone || frozen(dev, stream)) {
