@@ -1,7 +1,9 @@
 """GPU tests of the attention's forward on packed operands, which takes over
 from 64 queries and 8192 query rows over all samples and heads on: values of out
 and lse, and the gradients that follow from them, against the 64-bit form and
-the bounds of lm_ops_ref.py."""
+the bounds of lm_ops_ref.py.  Then, in every path, operands at the ends of the
+range: scores far from zero, values that are not finite, operands whose sizes
+multiply past it, queries that read nothing."""
 import numpy as np
 import pytest
 
