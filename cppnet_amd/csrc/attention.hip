@@ -1249,11 +1249,11 @@ __device__ __forceinline__ void dkv_block(const PairArgs& g, int bid, GradLds<DH
     add.read(turned, 0);
     const int64_t i0 = start + (first + t) * 32;  // the position of the tile's first query
     if (!(__all(held) && (!a.causal || key0 + 32 * wave + 31 <= i0))) {
-      // the first of the tile's queries that reads this lane's key
-      const int64_t behind = a.causal ? key - i0 : 0;
-      const int lead = !held ? 32 : (int)(behind < 0 ? 0 : behind < 32 ? behind : 32);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[0][e] = 8 * (e / 4) + 4 * (lane >> 5) + e % 4 >= lead ? s[0][e] : none;
+      for (int e = 0; e < 16; ++e) {
+        const bool reads = held && (!a.causal || key <= i0 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4);
+        s[0][e] = reads ? s[0][e] : none;
+      }
     }
     const float (*const st_now)[32] = stat[t & 1];
     auto work = [&](int e) { pair(st_now, e); };
