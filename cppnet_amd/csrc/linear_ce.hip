@@ -36,7 +36,11 @@ namespace {
 using pr::f32x16;
 using pr::f32x4;
 using pr::f32x4u;
-using pr::u32x4;
+using pr::put_frag;
+using pr::put_tile;
+using pr::Split;
+using pr::split_of;
+using pr::wave_max;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -83,12 +87,6 @@ constexpr int kGExp = 15;
 __device__ __forceinline__ float grad_factor(const CeArgs& a) {
   const int held = a.state->held;
   return a.mean ? 1.f / (float)(held > 0 ? held : 1) : 1.f;
-}
-
-__device__ __forceinline__ uint32_t wave_max(uint32_t m) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-  return m;
 }
 
 // The largest finite |W| of each of the first w_blocks blocks' parts, then of
@@ -189,20 +187,6 @@ __global__ void __launch_bounds__(1024) ce_state_kernel(CeArgs a) {
     *a.state = CeState{(int)total[0], total[2], total[3]};
     if (a.oob && total[1]) atomicAdd(a.oob, (int)total[1]);
   }
-}
-
-__device__ __forceinline__ void put_frag(char* p, int64_t block, int steps, int step, const float (&x)[8]) {
-  u32x4 hi, lo;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    uint32_t h, l;
-    pr::split2(x[2 * e], x[2 * e + 1], h, l);
-    hi[e] = h;
-    lo[e] = l;
-  }
-  char* q = p + (block * steps + step) * (2 * pr::kFrag) + pr::slot(threadIdx.x & 63, step);
-  *reinterpret_cast<u32x4*>(q) = hi;
-  *reinterpret_cast<u32x4*>(q + pr::kFrag) = lo;
 }
 
 // X and W^T packed, a wave per fragment of 32 rows x 16 k.  Of rows without a
@@ -329,45 +313,6 @@ struct Out {
 __device__ __forceinline__ int scale_of(const CeState& s, int which) {
   return which == 0 ? pr::scale_exp(s.x_max) : which == 1 ? pr::scale_exp(s.w_max) : kGExp;
 }
-// p[n + ld m] = value(element), or += for ADD, for the elements of a tile that
-// this lane holds and that exist.  ADD reads all of a column before it writes
-// one, so the reads are under way together.
-template <bool ADD, class F>
-__device__ __forceinline__ void put_tile(const pr::Acc& acc, int tm, int tn, int M, int N, float* __restrict__ p,
-                                         int64_t ld, F&& value) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = tm * pr::TM + (wave >> 2) * 128, m1 = m0 + 4 * (lane >> 5);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
-    if (n >= N) continue;
-    float* q = p + n + ld * m1;
-    auto row = [](int i, int e) { return 32 * i + 8 * (e / 4) + e % 4; };
-    if (m0 + 128 <= M) {
-      float old[4][16];
-      if (ADD) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) old[i][e] = q[ld * row(i, e)];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) q[ld * row(i, e)] = ADD ? old[i][e] + value(acc.x[i][j][e]) : value(acc.x[i][j][e]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (m1 + row(i, e) < M) {
-            float* at = q + ld * row(i, e);
-            *at = ADD ? *at + value(acc.x[i][j][e]) : value(acc.x[i][j][e]);
-          }
-    }
-  }
-}
-
 // Logits of a piece (M: classes, N: rows) with each row's maximum and sum of
 // exponentials over the wave's 128 classes; stored for the gradients, else the
 // targets' alone.
@@ -855,21 +800,6 @@ struct CeGrads {
   float *dX, *dW, *db;
   int accumulate;
 };
-
-struct Split {
-  int splits, steps;
-};
-// Splits of a contraction so that the tiles fill the 256 CUs, each at least 16
-// steps (256 k) long.
-Split split_of(int64_t M, int64_t N, int steps) {
-  const int64_t tiles = (M + pr::TM - 1) / pr::TM * ((N + pr::TN - 1) / pr::TN);
-  int64_t s = tiles >= 224 ? 1 : 256 / tiles;
-  if (s > steps / 16) s = steps / 16;
-  if (s < 1) s = 1;
-  int per = (int)((steps + s - 1) / s);
-  per = (per + 1) / 2 * 2;
-  return Split{(steps + per - 1) / per, per};
-}
 
 int run_few(CeArgs& a, float* loss, const CeGrads* g, hipStream_t st, const char* who) {
   const int64_t N = a.N, D = a.D, V = a.V, slices = (V + kFewSlice - 1) / kFewSlice;

@@ -93,6 +93,27 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& w0, uint32_t&
   w1 = __builtin_bit_cast(uint32_t, l);
 }
 
+__device__ __forceinline__ uint32_t wave_max(uint32_t m) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+  return m;
+}
+
+// This lane's eight k of fragment (block, step) of an operand of `steps` steps.
+__device__ __forceinline__ void put_frag(char* p, int64_t block, int steps, int step, const float (&x)[8]) {
+  u32x4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t h, l;
+    split2(x[2 * e], x[2 * e + 1], h, l);
+    hi[e] = h;
+    lo[e] = l;
+  }
+  char* q = p + (block * steps + step) * (2 * kFrag) + slot(threadIdx.x & 63, step);
+  *reinterpret_cast<u32x4*>(q) = hi;
+  *reinterpret_cast<u32x4*>(q + kFrag) = lo;
+}
+
 // ----------------------------------------------------------- global -> LDS
 // 16 bytes a lane from `src` (the lane's own address) to lds + 16 lane; lds is
 // wave-uniform.  Counted by vmcnt.  Written out because the compiler, where it
@@ -293,6 +314,60 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
 #pragma unroll
       for (int j = 0; j < 2; ++j) acc.x[i][j] = -acc.x[i][j];
   }
+}
+
+// p[n + ld m] = value(element), or += for ADD, for the elements of a tile that
+// this lane holds and that exist.  ADD reads all of a column before it writes
+// one, so the reads are under way together.
+template <bool ADD, class F>
+__device__ __forceinline__ void put_tile(const Acc& acc, int tm, int tn, int M, int N, float* __restrict__ p,
+                                         int64_t ld, F&& value) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m0 = tm * TM + (wave >> 2) * 128, m1 = m0 + 4 * (lane >> 5);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = tn * TN + (wave & 3) * 64 + 32 * j + (lane & 31);
+    if (n >= N) continue;
+    float* q = p + n + ld * m1;
+    auto row = [](int i, int e) { return 32 * i + 8 * (e / 4) + e % 4; };
+    if (m0 + 128 <= M) {
+      float old[4][16];
+      if (ADD) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) old[i][e] = q[ld * row(i, e)];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) q[ld * row(i, e)] = ADD ? old[i][e] + value(acc.x[i][j][e]) : value(acc.x[i][j][e]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (m1 + row(i, e) < M) {
+            float* at = q + ld * row(i, e);
+            *at = ADD ? *at + value(acc.x[i][j][e]) : value(acc.x[i][j][e]);
+          }
+    }
+  }
+}
+
+struct Split {
+  int splits, steps;
+};
+// Splits of a contraction so that the tiles fill the 256 CUs, each at least 16
+// steps (256 k) long.
+inline Split split_of(int64_t M, int64_t N, int steps) {
+  const int64_t tiles = (M + TM - 1) / TM * ((N + TN - 1) / TN);
+  int64_t s = tiles >= 224 ? 1 : 256 / tiles;
+  if (s > steps / 16) s = steps / 16;
+  if (s < 1) s = 1;
+  int per = (int)((steps + s - 1) / s);
+  per = (per + 1) / 2 * 2;
+  return Split{(steps + per - 1) / per, per};
 }
 
 }  // namespace pr
