@@ -157,6 +157,14 @@ SIGNATURES: dict[str, tuple] = {
     "cnhip_attention_backward": (i32, [vp] * 9 + [i64] * 6 + [f32, i32, vp, vp, i32, vp]),
     "cnhip_linear_ce_forward": (i32, [vp] * 6 + [i64] * 3 + [i32, vp, vp]),
     "cnhip_linear_ce_head": (i32, [vp] * 9 + [i64] * 3 + [i32, i32, vp, vp]),
+    "cnhip_dropout_seeded": (i32, [vp, vp, i64, f32, C.c_uint64, C.c_uint64, vp, vp]),
+    "cnhip_dropout_advance": (i32, [vp, C.c_uint64, vp]),
+    "cnhip_rms_norm_forward": (i32, [vp] * 6 + [i64, i64, f32, f32, C.c_uint64, C.c_uint64, vp, vp]),
+    "cnhip_rms_norm_backward": (i32, [vp] * 8 + [i64, i64, f32, C.c_uint64, C.c_uint64, vp, i32, vp]),
+    "cnhip_linear_recurrence_forward": (i32, [vp] * 6 + [i64] * 3 + [vp, i32, vp]),
+    "cnhip_linear_recurrence_backward": (i32, [vp] * 11 + [i64] * 3 + [vp, i32, vp]),
+    "cnhip_gated_ffn_forward": (i32, [vp] * 5 + [i64] * 3 + [i32, vp]),
+    "cnhip_gated_ffn_backward": (i32, [vp] * 7 + [i64] * 3 + [i32, i32, vp]),
     "cnhip_rnn_forward": (i32, [vp] * 5 + [i64] * 4 + [vp]),
     "cnhip_rnn_backward": (i32, [vp] * 9 + [i64] * 4 + [vp]),
 }

@@ -22,6 +22,7 @@
 #include <cmath>
 
 #include "common.hpp"
+#include "dropout_rng.hpp"
 
 namespace cnhip {
 namespace {
@@ -226,11 +227,7 @@ __global__ void __launch_bounds__(256) huber_bwd_kernel(const float* __restrict_
 // u = (top 24 bits of splitmix64(seed + (offset + i) * golden)) / 2^24, so a
 // mask is reproducible from (seed, offset) and needs no state.
 __device__ __forceinline__ float dropout_u(uint64_t seed, uint64_t idx) {
-  uint64_t z = seed + idx * 0x9E3779B97F4A7C15ull;
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  z ^= z >> 31;
-  return (float)(z >> 40) * (1.0f / 16777216.0f);
+  return (float)dropout_top24(seed + idx * kDropoutStep) * (1.0f / 16777216.0f);
 }
 __global__ void __launch_bounds__(256) dropout_fwd_kernel(const float* __restrict__ x,
                                                           float* __restrict__ y,

@@ -23,12 +23,12 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def _p(t: torch.Tensor | None, name: str = "tensor") -> int | None:
+def _p(t: torch.Tensor | None, name: str = "tensor", also: torch.dtype | None = None) -> int | None:
     if t is None:
         return None
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name}: expected a device tensor (the HIP path has no host fallback)")
-    if t.dtype not in (torch.float32, torch.int32, torch.uint8):
+    if t.dtype not in (torch.float32, torch.int32, torch.uint8) and t.dtype is not also:
         raise TypeError(f"{name}: expected float32/int32/uint8, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor")
@@ -493,7 +493,7 @@ def _held(device_of, *operands) -> list:
                 and t.numel() == n and t.is_contiguous()):
             ptrs.append(t.data_ptr())  # as it has to be; what is not is told apart below
             continue
-        ptrs.append(_p(t, name))
+        ptrs.append(_p(t, name, dtype))
         if t is None:
             continue
         if t.dtype is not dtype:
@@ -588,3 +588,90 @@ def linear_ce_head(X, W, b, targets, loss, lse, dX, dW, db, batch: int, in_featu
               (dX, "dX", batch * in_features, f), (dW, "dW", in_features * classes, f), (db, "db", classes, f),
               (oob, "oob", 1, i))
     _call_on(loss, "cnhip_linear_ce_head", *p[:9], batch, in_features, classes, _red(reduction), int(accumulate), p[9])
+
+
+# ---- a recurrent language model's block ----
+def dropout_seeded(x, y, p: float, seed: int, offset: int = 0, counter=None) -> None:
+    """y = dropout(x) with no stored mask; also its backward, on the gradient.
+    counter: int64 [1] on the device, added to offset (advance it for every step of a captured graph)."""
+    n = x.numel()
+    q = _held(y, (x, "x", n, torch.float32), (y, "y", n, torch.float32), (counter, "counter", 1, torch.int64))
+    _call_on(y, "cnhip_dropout_seeded", q[0], q[1], n, p, seed, offset, q[2])
+
+
+def dropout_advance(counter, n: int) -> None:
+    """counter += n."""
+    q = _held(counter, (counter, "counter", 1, torch.int64))
+    _call_on(counter, "cnhip_dropout_advance", q[0], n)
+
+
+def rms_norm_forward(x, residual, gamma, y, sum, rstd, N, F, eps: float = 1e-5, p: float = 0.0, seed: int = 0,
+                     offset: int = 0, counter=None) -> None:
+    """sum = residual + dropout(x), y = sum * rstd * gamma over the features of [N, F]; residual, sum and rstd may be
+    None."""
+    _positive(N=N, F=F)
+    f = torch.float32
+    q = _held(y, (x, "x", N * F, f), (residual, "residual", N * F, f), (gamma, "gamma", F, f), (y, "y", N * F, f),
+              (sum, "sum", N * F, f), (rstd, "rstd", N, f), (counter, "counter", 1, torch.int64))
+    _call_on(y, "cnhip_rms_norm_forward", *q[:6], N, F, eps, p, seed, offset, q[6])
+
+
+def rms_norm_backward(sum, rstd, gamma, dy, dsum, dx, dresidual, dgamma, N, F, p: float = 0.0, seed: int = 0,
+                      offset: int = 0, counter=None, accumulate: bool = False) -> None:
+    """dx, dresidual (None: not wanted) and dgamma from dy and dsum (None: nothing passes the norm)."""
+    _positive(N=N, F=F)
+    f = torch.float32
+    q = _held(dx, (sum, "sum", N * F, f), (rstd, "rstd", N, f), (gamma, "gamma", F, f), (dy, "dy", N * F, f),
+              (dsum, "dsum", N * F, f), (dx, "dx", N * F, f), (dresidual, "dresidual", N * F, f),
+              (dgamma, "dgamma", F, f), (counter, "counter", 1, torch.int64))
+    _call_on(dx, "cnhip_rms_norm_backward", *q[:8], N, F, p, seed, offset, q[8], int(accumulate))
+
+
+def linear_recurrence_forward(x, f, i, h0, h, h_last, B, S, D, seq_len=None, rows=ROWS_REF) -> None:
+    """h_t = sigmoid(f_t) h_{t-1} + w_t x_t, w = sigmoid(i) (i None: 1 - sigmoid(f)); h0, h_last [B, D] may be None.
+    seq_len: steps of each sample, int32 [B]."""
+    _positive(B=B, S=S, D=D)
+    t, n, m = torch.float32, B * S * D, B * D
+    q = _held(h, (x, "x", n, t), (f, "f", n, t), (i, "i", n, t), (h0, "h0", m, t), (h, "h", n, t),
+              (h_last, "h_last", m, t), (seq_len, "seq_len", B, torch.int32))
+    _call_on(h, "cnhip_linear_recurrence_forward", *q[:6], B, S, D, q[6], rows)
+
+
+def linear_recurrence_backward(x, f, i, h0, h, dh, dh_last, dx, df, di, dh0, B, S, D, seq_len=None,
+                               rows=ROWS_REF) -> None:
+    """Gradients from the forward's inputs and h, dh and dh_last (None: zeros); di goes with i, dh0 may be None."""
+    _positive(B=B, S=S, D=D)
+    t, n, m = torch.float32, B * S * D, B * D
+    q = _held(dx, (x, "x", n, t), (f, "f", n, t), (i, "i", n, t), (h0, "h0", m, t), (h, "h", n, t), (dh, "dh", n, t),
+              (dh_last, "dh_last", m, t), (dx, "dx", n, t), (df, "df", n, t), (di, "di", n, t), (dh0, "dh0", m, t),
+              (seq_len, "seq_len", B, torch.int32))
+    _call_on(dx, "cnhip_linear_recurrence_backward", *q[:11], B, S, D, q[11], rows)
+
+
+_GATES = {"silu": 0, "gelu": 1, "sigmoid": 2, "relu": 3}
+
+
+def _gate(act: str) -> int:
+    if act not in _GATES:
+        raise ValueError(f"act must be one of {', '.join(_GATES)}, got {act!r}")
+    return _GATES[act]
+
+
+def gated_ffn_forward(X, W, b, H, Z, batch: int, in_features: int, hidden: int, act: str = "silu") -> None:
+    """H = act(gate) * up, [gate up] = X W + b (W [in_features, 2 hidden]); Z keeps both for the backward (None: not)."""
+    _positive(batch=batch, in_features=in_features, hidden=hidden)
+    f = torch.float32
+    q = _held(H, (X, "X", batch * in_features, f), (W, "W", 2 * in_features * hidden, f), (b, "b", 2 * hidden, f),
+              (H, "H", batch * hidden, f), (Z, "Z", 2 * batch * hidden, f))
+    _call_on(H, "cnhip_gated_ffn_forward", *q, batch, in_features, hidden, _gate(act))
+
+
+def gated_ffn_backward(X, W, Z, dH, dX, dW, db, batch: int, in_features: int, hidden: int, act: str = "silu",
+                       accumulate: bool = False) -> None:
+    """dX overwritten, dW and db (None without a bias) overwritten or added to."""
+    _positive(batch=batch, in_features=in_features, hidden=hidden)
+    f = torch.float32
+    q = _held(dX, (X, "X", batch * in_features, f), (W, "W", 2 * in_features * hidden, f),
+              (Z, "Z", 2 * batch * hidden, f), (dH, "dH", batch * hidden, f), (dX, "dX", batch * in_features, f),
+              (dW, "dW", 2 * in_features * hidden, f), (db, "db", 2 * hidden, f))
+    _call_on(dX, "cnhip_gated_ffn_backward", *q, batch, in_features, hidden, _gate(act), int(accumulate))

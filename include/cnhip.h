@@ -840,6 +840,95 @@ int cnhip_linear_ce_head(const float* X, const float* W, const float* b, const i
                          int64_t in_features, int64_t classes, int reduction, int accumulate,
                          int32_t* oob_count, cnhip_stream_t stream);
 
+/* ---- a recurrent language model's block -----------------------------------
+ * A norm of the residual's sum, dropout that stores no mask, a gated linear
+ * recurrence and a gated feed-forward layer.  The reference has none of them in
+ * this form; they stand beside its BatchNorm (batch_norm.cpp:25-401), Dropout
+ * (dropout.cpp:140-270), GRU (gru.cpp:30-322) and Linear (linear.cpp:108-358).
+ * Streams, workspace, capture and overlap are as for the language-model operators
+ * above; sums run in an order fixed by the arguments.
+ *
+ * Dropout without a mask: y = x / (1 - p) where element j of the call is kept,
+ * +0 where it is not, whatever x holds there.  Element j is kept as
+ * cnhip_dropout_forward of the same seed keeps the element at position
+ * offset + *counter + j (counter: a device uint64, NULL: 0).  The backward is the
+ * same call on the gradient.  y may be x.  A captured graph reads the counter at
+ * every replay: advance it by the positions that a step used, behind the step's
+ * backward, and every replay draws new masks. */
+int cnhip_dropout_seeded(const float* x, float* y, int64_t n, float p, uint64_t seed,
+                         uint64_t offset, const uint64_t* counter, cnhip_stream_t stream);
+/* *counter += n, modulo 2^64 */
+int cnhip_dropout_advance(uint64_t* counter, uint64_t n, cnhip_stream_t stream);
+/* Root-mean-square norm of a residual's sum over the features of [N, F]:
+ *   s = residual + dropout(x),  rstd_n = 1 / sqrt(mean_f s_nf^2 + eps),
+ *   y_nf = s_nf rstd_n gamma_f
+ * residual NULL: s = dropout(x).  p = 0: x enters whole.  Element (n, f) is at
+ * position n + N f of the mask, so s has the bits of cnhip_dropout_seeded
+ * followed by an addition.  sum (s; it may be the residual itself) and rstd [N]
+ * are what the backward reads; either may be NULL where it is not wanted.  A row
+ * with a NaN or infinity gives NaN in that row alone.
+ * backward, n = s rstd, d = gamma dy:
+ *   ds = dsum + rstd (d - n mean_f(d n)),  dresidual = ds,  dx = dropout(ds),
+ *   dgamma_f (+)= sum_n dy_nf n_nf
+ * sum: the forward's (x itself where there was no residual and p = 0).  dsum: the
+ * gradient that reaches s past the norm, NULL: none.  dresidual may be NULL; with
+ * p = 0 it equals dx.  dx and dresidual are overwritten, dgamma is added to with
+ * accumulate 1.  eps > 0, N < 2^28, F < 2^31. */
+int cnhip_rms_norm_forward(const float* x, const float* residual, const float* gamma, float* y,
+                           float* sum, float* rstd, int64_t N, int64_t F, float eps, float p,
+                           uint64_t seed, uint64_t offset, const uint64_t* counter,
+                           cnhip_stream_t stream);
+int cnhip_rms_norm_backward(const float* sum, const float* rstd, const float* gamma,
+                            const float* dy, const float* dsum, float* dx, float* dresidual,
+                            float* dgamma, int64_t N, int64_t F, float p, uint64_t seed,
+                            uint64_t offset, const uint64_t* counter, int accumulate,
+                            cnhip_stream_t stream);
+/* Gated linear recurrence over x, f, i, h [B, S, D] in either row order:
+ *   a = sigmoid(f), w = sigmoid(i), or 1 - a with i NULL (as the GRU's gate),
+ *   h_t = a_t h_{t-1} + w_t x_t, h_{-1} = h0 [B, D] (NULL: zeros).
+ * seq_len: steps of each sample (device int32 [B]; NULL: all S; values are cut to
+ * [0, S]).  Steps at and past it give zero rows and reach nothing, whatever they
+ * hold.  h_last [B, D] (may be NULL, or h0 itself): the state after the last step,
+ * h0 where there is none; so S = 1 with h0 and h_last is a decoding step.
+ * f may be +-infinity: a gate that keeps or drops everything.  1 - a keeps its
+ * relative precision however near a is to 1.  A state that is not finite stays so,
+ * or turns to NaN, to the end of its sequence and reaches no other.
+ * backward, from the last step to the first, u_S = dh_last (NULL: zeros):
+ *   g_t = dh_t + u_{t+1},  u_t = a_t g_t,  dx = w g,  dh0 = u_0,
+ *   df = a (1 - a) g (h_{t-1} - x_t); with i: a (1 - a) g h_{t-1}, di = w (1 - w) g x
+ * from the forward's inputs and h; gradients are overwritten (zeros past seq_len),
+ * di goes with i, dh0 may be NULL or dh_last itself. */
+int cnhip_linear_recurrence_forward(const float* x, const float* f, const float* i,
+                                    const float* h0, float* h, float* h_last, int64_t B, int64_t S,
+                                    int64_t D, const int32_t* seq_len, int rows,
+                                    cnhip_stream_t stream);
+int cnhip_linear_recurrence_backward(const float* x, const float* f, const float* i,
+                                     const float* h0, const float* h, const float* dh,
+                                     const float* dh_last, float* dx, float* df, float* di,
+                                     float* dh0, int64_t B, int64_t S, int64_t D,
+                                     const int32_t* seq_len, int rows, cnhip_stream_t stream);
+/* Gated feed-forward layer: Z = X W + b with X [batch, in_features], W
+ * [in_features, 2 hidden] (the gate's columns, then the up projection's), b [2
+ * hidden] or NULL;  H [batch, hidden] = act(Z[:, :hidden]) * Z[:, hidden:].
+ * Z [batch, 2 hidden] is what the backward reads; NULL: not wanted.
+ * backward: dX (overwritten), dW and db (added to with accumulate 1, else
+ * overwritten; db NULL exactly where b was) from X, W, Z and dH.
+ * Products of more than 64 rows, and the backward's, run on pairs of fp16 terms
+ * as above; the operands with a largest value of their own are a row of X and 32
+ * columns of W in the forward; W, the rows of X and those of Z's gradient that go
+ * through together in the backward (2^27 / hidden / 2, at least 1024).  An infinity
+ * in such an operand comes out as NaN. */
+#define CNHIP_GATE_SILU 0     /* z sigmoid(z) */
+#define CNHIP_GATE_GELU 1     /* z Phi(z), as CNHIP_ACT_GELU */
+#define CNHIP_GATE_SIGMOID 2
+#define CNHIP_GATE_RELU 3
+int cnhip_gated_ffn_forward(const float* X, const float* W, const float* b, float* H, float* Z,
+                            int64_t batch, int64_t in_features, int64_t hidden, int act,
+                            cnhip_stream_t stream);
+int cnhip_gated_ffn_backward(const float* X, const float* W, const float* Z, const float* dH,
+                             float* dX, float* dW, float* db, int64_t batch, int64_t in_features,
+                             int64_t hidden, int act, int accumulate, cnhip_stream_t stream);
+
 /* ---- DataLoader batch assembly (ref: dataloader.cpp:68-88) ----
  * src: the dataset sample-major (sample n's F values at src + n*F), N
  * samples; idx: B int32 sample indices (one outside [0, N) yields zeros);
