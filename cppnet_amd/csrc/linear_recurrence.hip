@@ -107,16 +107,19 @@ __device__ __forceinline__ Map from_lane(const Map& m, int lane) {
 //   kRun: the steps of a chain lie side by side (rows by sample, or one sample).
 //     A lane takes 4 in a row, U times 256 steps further.
 //   kShort: the same for sequences of up to 128 steps; a wave takes several chains.
-//   kStrided: rows in the reference's order, a step's samples side by side.  A wave
-//     takes the samples (up to 64) of one feature and, of fewer than 33, several
-//     steps of them, U times.
+//   kStrided: rows in the reference's order, a step's samples side by side.  The lanes
+//     of a wave take the samples (up to 64) of one feature and, of fewer than 33, 4
+//     steps in a row of each, U times.  A load then reads every fourth step's line, and
+//     the four loads read them whole (a step a lane, so that each load runs along
+//     memory, joins maps across lanes for every step and not for every fourth: 5 x
+//     1001, width 333, with its gradients, 61 us for 39).
 enum Layout { kRun, kShort, kStrided };
 
 // PASS 0: everything.  Where few chains have many steps these are cut in segments:
 // PASS 1 leaves each segment's map, PASS 2 runs it from the segments before.
 template <Layout LAY, bool BWD, bool IG, int U, int PASS>
 __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
-  constexpr int E = LAY == kStrided ? 1 : 4;
+  constexpr int E = 4;
   __shared__ Map totals[2][kMostWaves][LAY == kStrided ? 64 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int seat = wave % a.waves;  // of the waves that share a chain
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
   const int64_t q_begin = PASS ? seg * a.segment : 0;
   const int64_t q_end = PASS ? (q_begin + a.segment < a.S ? q_begin + a.segment : a.S) : a.S;
   // steps of a wave and of all that share a chain, in a round
-  const int span = LAY == kStrided ? U * width : U * 4 * width;
+  const int span = U * E * width;
   const int64_t round = (int64_t)span * a.waves;
 
   float state = 0.f;  // what enters the round
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
   };
   // position q0 + e in the order of the maps is step t
   auto first_q = [&](int64_t r0, int u) {
-    return r0 + (int64_t)seat * span + (LAY == kStrided ? u * width + at : u * 4 * width + 4 * at);
+    return r0 + (int64_t)seat * span + (u * width + at) * E;
   };
   auto load = [&](int64_t r0, Raw& v) {
 #pragma unroll
@@ -192,7 +195,7 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
       const int64_t lo = BWD ? a.S - E - q0 : q0;
       const bool any = mine && q0 < q_end && lo < len;
       auto get = [&](const float* p, float (&to)[E], int back) {
-        if (E == 4 && any && q0 + 4 <= a.S && lo >= back) {
+        if (LAY != kStrided && any && q0 + 4 <= a.S && lo >= back) {
           const f32x4 w = *reinterpret_cast<const f32x4u*>(p + base + lo - back);
 #pragma unroll
           for (int e = 0; e < E; ++e) to[e] = w[BWD ? E - 1 - e : e];
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
       }
       if (!mine || q0 >= q_end) continue;
       auto put = [&](float* to, const float (&v)[E]) {
-        if (E == 4 && q0 + 4 <= q_end) {
+        if (LAY != kStrided && q0 + 4 <= q_end) {
           f32x4 w4;
 #pragma unroll
           for (int e = 0; e < E; ++e) w4[BWD ? E - 1 - e : e] = v[e];
@@ -382,9 +385,9 @@ int run(RecArgs& a, int rows, hipStream_t st, const char* who) {
   // many as fill the chip several times over and as there are steps for.
   const int64_t teams = side ? a.chains : a.D * ((a.B + 63) / 64);
   const int width = side ? 64 : a.B > 32 ? 1 : (int)(64 / a.B);
-  const int u = side ? (BWD || a.S <= 256 ? 1 : 2) : 4;
-  const int64_t span = (int64_t)u * (side ? 4 : 1) * width;
-  while (a.waves < kMostWaves && teams * a.waves < 4096 && span * a.waves < a.S) a.waves *= 2;
+  const int u = BWD || (side && a.S <= 256) ? 1 : 2;
+  const int64_t span = (int64_t)u * 4 * width;
+  while (a.waves < kMostWaves && teams * a.waves * 2 <= 4096 && span * a.waves < a.S) a.waves *= 2;
   const int64_t round = span * a.waves;
   if (a.waves == kMostWaves && teams * a.waves < 2048 && a.S >= 2 * round) {
     int64_t n = 2048 / (teams * a.waves), most = a.S / round;
@@ -403,10 +406,11 @@ int run(RecArgs& a, int rows, hipStream_t st, const char* who) {
     a.start = reinterpret_cast<float*>(static_cast<char*>(ws) + parts);
   }
   const dim3 grid((unsigned)blocks, (unsigned)a.segments);
-  if (!side) return launch<kStrided, BWD, IG, 4>(a, grid, 64 * block_waves, st, who);
-  if (u == 1) return launch<kRun, BWD, IG, 1>(a, grid, 64 * block_waves, st, who);
-  if constexpr (!BWD) return launch<kRun, BWD, IG, 2>(a, grid, 64 * block_waves, st, who);
-  return CNHIP_OK;
+  if (!side) return launch<kStrided, BWD, IG, BWD ? 1 : 2>(a, grid, 64 * block_waves, st, who);
+  if constexpr (!BWD) {
+    if (u == 2) return launch<kRun, BWD, IG, 2>(a, grid, 64 * block_waves, st, who);
+  }
+  return launch<kRun, BWD, IG, 1>(a, grid, 64 * block_waves, st, who);
 }
 
 int check_shape(int64_t B, int64_t S, int64_t D, int rows, const char* who) {
