@@ -7,11 +7,15 @@
 //   ds = dsum + rstd (d - n mean_f(d n)),  dresidual = ds, dx = drop(ds),
 //   dgamma_f (+)= sum_n dy_nf n_nf
 //
-// Matrices are ColMajor [N, F]: the features of a row lie N apart, so a block
-// takes a few rows side by side and all of their features, and holds them in
-// registers between the sum over the features and the result.  Everything is
-// read once and written once.  The sums over a row are kept in 64 bits, which
-// neither overflow nor vanish for any finite fp32 row.
+// Matrices are ColMajor [N, F]: the features of a row lie N apart.  A block that held
+// whole rows would read a line or two of every column, each on a page of its own:
+// 4097 x 4099, forward, 203 us in blocks of 16 rows for 81 here.  So the matrix goes
+// through in tiles of 256 rows x 64 or 128 columns, a KiB in a row of every column,
+// twice: the first launch leaves each tile's sums over its columns, the second joins
+// them and reads s (and dy) again, for the most part from the caches.  Where a few
+// rows are all there is, one launch does both and holds them in registers.  The sums
+// over a row are kept in 64 bits, which neither overflow nor vanish for any finite
+// fp32 row.
 //
 // Element j of the [N, F] storage is kept where the generator's word for
 // position + j says so; the backward draws the same words again.
@@ -65,29 +69,18 @@ struct NormArgs {
   const float *x, *residual, *gamma;
   float *y, *sum, *rstd;
   const float *s, *dy, *dsum;
-  float *dx, *dresidual, *dgamma, *part;
+  float *dx, *dresidual, *dgamma;
   int64_t N, F;
-  int shift;       // log2 of the rows of a block
-  int64_t tiles;   // of that many rows
   double eps, inv_f;
   Drop drop;
   int accumulate;
+  int shift;          // few rows: log2 of the rows of a block; tiles: of the lanes along the rows
+  int row_tiles, col_tiles;
+  double* part;       // [col_tiles][N]: sums over a tile's columns
+  float* gamma_part;  // [row_tiles][F]: sums over a tile's rows
 };
 
 constexpr int kNormThreads = 1024, kNormWaves = kNormThreads / 64;
-
-// The sum over a block's threads with the same row (thread % rows), in every one of them.
-__device__ __forceinline__ double row_sum(double v, int shift, double (*part)[64]) {
-  const int rows = 1 << shift, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int o = rows; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-  if (lane < rows) part[wave][lane] = v;
-  __syncthreads();
-  double t = 0.0;
-  const int r = lane & (rows - 1);
-#pragma unroll
-  for (int w = 0; w < kNormWaves; ++w) t += part[w][r];
-  return t;
-}
 
 // 1 / sqrt(v) to fp32's precision and range.
 __device__ __forceinline__ float inv_sqrt(double v) {
@@ -96,6 +89,7 @@ __device__ __forceinline__ float inv_sqrt(double v) {
   return (float)r;
 }
 
+// ---- few rows
 // Where a thread's elements lie: feature `first` + k cols of its row for k = 0, 1, ...,
 // at[j] of a matrix's part(k).  What the lanes of a wave share is kept apart, so that an
 // element costs one 32-bit address and not one of 64 bits in every matrix.
@@ -118,198 +112,413 @@ struct Seat {
   __device__ __forceinline__ bool has(int k, int64_t F) const { return first0 + (int64_t)k * cols + lane_f < F; }
 };
 
-// K: a thread's features at a time.  ONCE: they are all of its features; otherwise s is
-// read again for the result.
-template <int K, bool ONCE, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_fwd_kernel(NormArgs a) {
+// The sum over a block's threads with the same row (thread % rows), in every one of them.
+__device__ __forceinline__ double row_sum(double v, int shift, double (*part)[64]) {
+  const int rows = 1 << shift, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int o = rows; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  if (lane < rows) part[wave][lane] = v;
+  __syncthreads();
+  double t = 0.0;
+  const int r = lane & (rows - 1);
+#pragma unroll
+  for (int w = 0; w < kNormWaves; ++w) t += part[w][r];
+  return t;
+}
+
+// K: a thread's features at most.
+template <int K, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_few_fwd_kernel(NormArgs a) {
 #pragma clang fp contract(off)
   __shared__ double part[kNormWaves][64];
   const Seat w(a.N, a.shift);
   const int64_t n0 = (int64_t)blockIdx.x << a.shift;
   const bool in = n0 + w.r < a.N;
   const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)w.j * kDropoutStep : 0;
-  const int rounds = (int)((a.F + w.cols - 1) / w.cols);  // of all the columns of threads
-  auto get = [&](int k) {
+  float s[K];
+  double q = 0.0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    s[k] = 0.f;
+    if (!in || !w.has(k, a.F)) continue;
     const int64_t o = n0 + w.part(k);
     float v = (a.x + o)[w.j];
     if (DROP) v = dropped(a.drop, z0 + (uint64_t)o * kDropoutStep, v);
-    return a.residual ? (a.residual + o)[w.j] + v : v;
-  };
-  float s[K];
-  double q = 0.0;
-  for (int k0 = 0; k0 < rounds; k0 += K) {
+    s[k] = a.residual ? (a.residual + o)[w.j] + v : v;
+  }
 #pragma unroll
-    for (int k = 0; k < K; ++k) s[k] = in && w.has(k0 + k, a.F) ? get(k0 + k) : 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      q = fma((double)s[k], (double)s[k], q);
-      if (a.sum && in && w.has(k0 + k, a.F)) (a.sum + n0 + w.part(k0 + k))[w.j] = s[k];
-    }
-    if (ONCE) break;
+  for (int k = 0; k < K; ++k) {
+    q = fma((double)s[k], (double)s[k], q);
+    if (a.sum && in && w.has(k, a.F)) (a.sum + n0 + w.part(k))[w.j] = s[k];
   }
   const float rstd = inv_sqrt(row_sum(q, a.shift, part) * a.inv_f + a.eps);
   if (!in) return;
   if (a.rstd && threadIdx.x < (unsigned)w.rows) a.rstd[n0 + w.r] = rstd;
-  for (int k0 = 0; k0 < rounds; k0 += K) {
-    if (!ONCE) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        s[k] = w.has(k0 + k, a.F) ? (a.sum ? (a.sum + n0 + w.part(k0 + k))[w.j] : get(k0 + k)) : 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (w.has(k0 + k, a.F))
-        (a.y + n0 + w.part(k0 + k))[w.j] = (s[k] * rstd) * (a.gamma + w.first0 + (int64_t)(k0 + k) * w.cols)[w.lane_f];
-    if (ONCE) break;
-  }
+  for (int k = 0; k < K; ++k)
+    if (w.has(k, a.F)) (a.y + n0 + w.part(k))[w.j] = (s[k] * rstd) * (a.gamma + w.first0 + (int64_t)k * w.cols)[w.lane_f];
 }
 
-// A block takes every gridDim.x-th tile of rows and sums its part of dgamma over
-// them: in registers where a thread's features are all at hand (ONCE).
-template <int K, bool ONCE, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_bwd_kernel(NormArgs a) {
-  __shared__ double part[2][kNormWaves][64];
+template <int K, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_few_bwd_kernel(NormArgs a) {
+  __shared__ double part[kNormWaves][64];
   const Seat w(a.N, a.shift);
+  const int64_t n0 = (int64_t)blockIdx.x << a.shift;
+  const bool in = n0 + w.r < a.N;
   const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)w.j * kDropoutStep : 0;
-  const int rounds = (int)((a.F + w.cols - 1) / w.cols);
-  float dg[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) dg[k] = 0.f;
-  int parity = 0;
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, parity ^= 1) {
-    const int64_t n0 = tile << a.shift;
-    const bool in = n0 + w.r < a.N;
-    const float rstd = in ? a.rstd[n0 + w.r] : 0.f;
-    float u[K], d[K];  // the normed row, and the gradient at it
-    double q = 0.0;
-    auto gamma = [&](int k) { return (a.gamma + w.first0 + (int64_t)k * w.cols)[w.lane_f]; };
-    auto get = [&](int k0) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const bool on = in && w.has(k0 + k, a.F);
-        const int64_t o = n0 + w.part(k0 + k);
-        u[k] = on ? (a.s + o)[w.j] * rstd : 0.f;
-        d[k] = on ? (a.dy + o)[w.j] : 0.f;
-      }
-    };
-    for (int k0 = 0; k0 < rounds; k0 += K) {
-      get(k0);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (ONCE) dg[k] = fmaf(d[k], u[k], dg[k]);
-        d[k] *= w.has(k0 + k, a.F) ? gamma(k0 + k) : 0.f;
-        q = fma((double)d[k], (double)u[k], q);
-      }
-      if (ONCE) break;
-    }
-    const float c = (float)(row_sum(q, a.shift, part[parity]) * a.inv_f);
-    for (int k0 = 0; k0 < rounds; k0 += K) {
-      if (!ONCE) {
-        get(k0);
-#pragma unroll
-        for (int k = 0; k < K; ++k) d[k] *= w.has(k0 + k, a.F) ? gamma(k0 + k) : 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!in || !w.has(k0 + k, a.F)) continue;
-        const int64_t o = n0 + w.part(k0 + k);
-        float g = rstd * fmaf(-u[k], c, d[k]);
-        if (a.dsum) g += (a.dsum + o)[w.j];
-        if (a.dresidual) (a.dresidual + o)[w.j] = g;
-        (a.dx + o)[w.j] = DROP ? dropped(a.drop, z0 + (uint64_t)o * kDropoutStep, g) : g;
-      }
-      if (ONCE) break;
-    }
-  }
-  if (!ONCE) return;
-  // over the rows of the block: lanes side by side
+  const float rstd = in ? a.rstd[n0 + w.r] : 0.f;
+  float u[K], d[K];  // the normed row, and the gradient at it
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    for (int o = w.rows >> 1; o > 0; o >>= 1) dg[k] += __shfl_xor(dg[k], o, 64);
-    if (w.r == 0 && w.has(k, a.F)) (a.part + (int64_t)blockIdx.x * a.F + w.first0 + (int64_t)k * w.cols)[w.lane_f] = dg[k];
+    const bool on = in && w.has(k, a.F);
+    const int64_t o = n0 + w.part(k);
+    u[k] = on ? (a.s + o)[w.j] * rstd : 0.f;
+    d[k] = on ? (a.dy + o)[w.j] : 0.f;
+  }
+  double q = 0.0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    // dgamma's part: over the rows of the block, lanes side by side
+    float dg = d[k] * u[k];
+    for (int o = w.rows >> 1; o > 0; o >>= 1) dg += __shfl_xor(dg, o, 64);
+    if (w.has(k, a.F)) {
+      const int64_t f = w.first0 + (int64_t)k * w.cols;
+      if (w.r == 0) (a.gamma_part + blockIdx.x * a.F + f)[w.lane_f] = dg;
+      d[k] *= (a.gamma + f)[w.lane_f];
+    }
+    q = fma((double)d[k], (double)u[k], q);
+  }
+  const float c = (float)(row_sum(q, a.shift, part) * a.inv_f);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (!in || !w.has(k, a.F)) continue;
+    const int64_t o = n0 + w.part(k);
+    float g = rstd * fmaf(-u[k], c, d[k]);
+    if (a.dsum) g += (a.dsum + o)[w.j];
+    if (a.dresidual) (a.dresidual + o)[w.j] = g;
+    (a.dx + o)[w.j] = DROP ? dropped(a.drop, z0 + (uint64_t)o * kDropoutStep, g) : g;
   }
 }
 
-// dgamma (+)= the blocks' parts, in order: 64 features a block, its waves share the parts.
-__global__ void __launch_bounds__(1024) rms_norm_gamma_kernel(const float* __restrict__ part, float* dgamma, int64_t F,
-                                                              int blocks, int accumulate) {
-  __shared__ float sum[16][64];
+// dgamma (+)= the tiles' parts, in order: 64 features a block, its waves share the parts.
+__device__ __forceinline__ void join_gamma(const NormArgs& a, int64_t block, float (*sum)[64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t f = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t f = block * 64 + lane;
   float t = 0.f;
-  if (f < F) {
+  if (f < a.F) {
 #pragma unroll 8
-    for (int b = wave; b < blocks; b += 16) t += part[(int64_t)b * F + f];
+    for (int b = wave; b < a.row_tiles; b += kNormWaves) t += a.gamma_part[(int64_t)b * a.F + f];
   }
   sum[wave][lane] = t;
   __syncthreads();
-  if (wave || f >= F) return;
-  for (int w = 1; w < 16; ++w) t += sum[w][lane];
-  dgamma[f] = accumulate ? dgamma[f] + t : t;
-}
-
-// dgamma of wide rows, from dy, s and rstd once more: a wave for a feature's rows.
-__global__ void __launch_bounds__(256) rms_norm_gamma_wide_kernel(NormArgs a) {
-  __shared__ float sum[4];
-  const int64_t f = blockIdx.x;
-  const float *s = a.s + a.N * f, *dy = a.dy + a.N * f;
-  float t = 0.f;
-#pragma unroll 4
-  for (int64_t n = threadIdx.x; n < a.N; n += 256) t = fmaf(dy[n], s[n] * a.rstd[n], t);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = t;
-  __syncthreads();
-  if (threadIdx.x) return;
-  t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  if (wave || f >= a.F) return;
+  for (int w = 1; w < kNormWaves; ++w) t += sum[w][lane];
   a.dgamma[f] = a.accumulate ? a.dgamma[f] + t : t;
 }
-
-constexpr int kNormHeld = 32, kNormHeldBack = 16;  // features of a thread that are kept between the passes
-constexpr int kNormBlocks = 512;    // of the backward, and so parts of dgamma at most
-
-// Rows of a block, as a power of two: 32 are whole lines of memory.  Fewer where there
-// are fewer rows, or where 32 rows are more than a block holds.
-int rows_shift(int64_t N, int64_t F, int held) {
-  int shift = 5;
-  while (shift > 0 && ((int64_t)1 << (shift - 1)) >= N) --shift;
-  while (shift > 4 && (F << shift) > (int64_t)kNormThreads * held) --shift;
-  return shift;
+__global__ void __launch_bounds__(kNormThreads) rms_norm_gamma_kernel(NormArgs a) {
+  __shared__ float sum[kNormWaves][64];
+  join_gamma(a, blockIdx.x, sum);
 }
 
-template <bool BWD, bool DROP>
-int run_norm(NormArgs& a, hipStream_t st, const char* who) {
-  constexpr int held = BWD ? kNormHeldBack : kNormHeld;
-  a.shift = rows_shift(a.N, a.F, held);
-  a.tiles = (a.N + ((int64_t)1 << a.shift) - 1) >> a.shift;
-  const int64_t cols = kNormThreads >> a.shift, per = (a.F + cols - 1) / cols;
-  const bool once = per <= held;
-  if constexpr (!BWD) {
-    const dim3 grid((unsigned)a.tiles), threads(kNormThreads);
-    if (per <= 4) hipLaunchKernelGGL((rms_norm_fwd_kernel<4, true, DROP>), grid, threads, 0, st, a);
-    else if (per <= 16) hipLaunchKernelGGL((rms_norm_fwd_kernel<16, true, DROP>), grid, threads, 0, st, a);
-    else if (once) hipLaunchKernelGGL((rms_norm_fwd_kernel<kNormHeld, true, DROP>), grid, threads, 0, st, a);
-    else hipLaunchKernelGGL((rms_norm_fwd_kernel<16, false, DROP>), grid, threads, 0, st, a);
-    return check_launch(who);
-  } else {
-    const int blocks = (int)(a.tiles < kNormBlocks ? a.tiles : kNormBlocks);
-    const dim3 grid((unsigned)blocks), threads(kNormThreads);
-    if (once) {
-      void* ws = nullptr;
-      CNHIP_TRY(scratch(st, kScratchLayer, (size_t)blocks * (size_t)a.F * sizeof(float), &ws, who));
-      a.part = static_cast<float*>(ws);
+// ---- tiles
+// 2^shift lanes along the rows, 4 rows each, and K times (1024 >> shift) columns.
+// Row tiles lie side by side in the order of the blocks.
+template <int K>
+struct TileSeat {
+  int64_t n, f0, base;  // the lane's first row; the wave's first column, its first element
+  int64_t step;
+  uint32_t lane_f, j;
+  int cols, row, tile_r, tile_c, left;  // rows of this lane's 4 that exist
+  __device__ __forceinline__ TileSeat(const NormArgs& a, int bid) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    tile_r = bid % a.row_tiles;
+    tile_c = bid / a.row_tiles;
+    cols = kNormThreads >> a.shift;
+    row = 4 * (lane & ((1 << a.shift) - 1));
+    lane_f = lane >> a.shift;
+    const int64_t n0 = (int64_t)tile_r << (a.shift + 2);
+    f0 = (int64_t)tile_c * (K * cols) + (int64_t)wave * (64 >> a.shift);
+    n = n0 + row;
+    base = n0 + a.N * f0;
+    step = a.N * cols;
+    j = (uint32_t)row + (uint32_t)a.N * lane_f;
+    left = n + 4 <= a.N ? 4 : n < a.N ? (int)(a.N - n) : 0;
+  }
+  __device__ __forceinline__ bool has(int k, int64_t F) const { return f0 + (int64_t)k * cols + lane_f < F; }
+  __device__ __forceinline__ int64_t at(int k) const { return base + k * step; }
+  __device__ __forceinline__ f32x4 get(const float* p, int k, int64_t F) const {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (!has(k, F)) return v;
+    const float* q = p + at(k) + j;
+    if (left == 4) return f32x4(*reinterpret_cast<const f32x4u*>(q));
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < left) v[e] = q[e];
+    return v;
+  }
+  __device__ __forceinline__ void put(float* p, int k, int64_t F, const f32x4& v) const {
+    if (!has(k, F)) return;
+    float* q = p + at(k) + j;
+    if (left == 4) {
+      *reinterpret_cast<f32x4u*>(q) = v;
+      return;
     }
-    if (per <= 4) hipLaunchKernelGGL((rms_norm_bwd_kernel<4, true, DROP>), grid, threads, 0, st, a);
-    else if (once) hipLaunchKernelGGL((rms_norm_bwd_kernel<kNormHeldBack, true, DROP>), grid, threads, 0, st, a);
-    else hipLaunchKernelGGL((rms_norm_bwd_kernel<16, false, DROP>), grid, threads, 0, st, a);
-    CNHIP_TRY(check_launch(who));
-    if (once)
-      hipLaunchKernelGGL(rms_norm_gamma_kernel, dim3((unsigned)((a.F + 63) / 64)), dim3(1024), 0, st, a.part, a.dgamma,
-                         a.F, blocks, a.accumulate);
-    else
-      hipLaunchKernelGGL(rms_norm_gamma_wide_kernel, dim3((unsigned)a.F), dim3(256), 0, st, a);
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < left) q[e] = v[e];
+  }
+  __device__ __forceinline__ float of_column(const float* p, int k, int64_t F) const {
+    return has(k, F) ? (p + f0 + (int64_t)k * cols)[lane_f] : 0.f;
+  }
+  // dropout of the lane's 4 elements in column k; z0: the word of the lane's own offset
+  __device__ __forceinline__ f32x4 drop(const Drop& d, uint64_t z0, int k, f32x4 v) const {
+    const uint64_t z = z0 + (uint64_t)at(k) * kDropoutStep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = dropped(d, z + (uint64_t)e * kDropoutStep, v[e]);
+    return v;
+  }
+};
+
+// The tile's sums over its columns -> part; q: of the thread's rows.
+template <class Seat_>
+__device__ __forceinline__ void leave_sums(const NormArgs& a, const Seat_& t, double (&q)[4], double (*lds)[256]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lanes = 1 << a.shift;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    for (int o = lanes; o < 64; o <<= 1) q[e] += __shfl_xor(q[e], o, 64);
+    if (lane < lanes) lds[wave][4 * lane + e] = q[e];
+  }
+  __syncthreads();
+  const int r = threadIdx.x;
+  const int64_t n = ((int64_t)t.tile_r << (a.shift + 2)) + r;
+  if (r >= 4 * lanes || n >= a.N) return;
+  double v = 0.0;
+#pragma unroll
+  for (int w = 0; w < kNormWaves; ++w) v += lds[w][r];
+  a.part[(int64_t)t.tile_c * a.N + n] = v;
+}
+// The sums over all columns of the thread's 4 rows; 1024 threads share them.
+template <class Seat_>
+__device__ __forceinline__ void all_sums(const NormArgs& a, const Seat_& t, double (&q)[4], double (*lds)[256]) {
+  const int rows = 4 << a.shift, r = threadIdx.x & (rows - 1), g = threadIdx.x >> (a.shift + 2),
+            groups = kNormThreads >> (a.shift + 2);
+  const int64_t n = ((int64_t)t.tile_r << (a.shift + 2)) + r;
+  double v = 0.0;
+  if (n < a.N) {
+#pragma unroll 4
+    for (int c = g; c < a.col_tiles; c += groups) v += a.part[(int64_t)c * a.N + n];
+  }
+  // groups of fewer rows than a line of lds share one: [groups rows / 256][256]
+  (&lds[0][0])[threadIdx.x] = v;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    q[e] = 0.0;
+    for (int k = 0; k < min(groups, a.col_tiles); ++k) q[e] += (&lds[0][0])[k * rows + t.row + e];
+  }
+}
+
+template <int K, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_sum_kernel(NormArgs a) {
+#pragma clang fp contract(off)
+  __shared__ double lds[kNormWaves][256];
+  const TileSeat<K> t(a, (int)blockIdx.x);
+  const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
+  f32x4 s[K], r[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    s[k] = t.get(a.x, k, a.F);
+    if (a.residual) r[k] = t.get(a.residual, k, a.F);
+  }
+  double q[4] = {};
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (DROP) s[k] = t.drop(a.drop, z0, k, s[k]);
+    if (a.residual) s[k] = r[k] + s[k];
+    if (a.sum) t.put(a.sum, k, a.F, s[k]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = fma((double)s[k][e], (double)s[k][e], q[e]);
+  }
+  leave_sums(a, t, q, lds);
+}
+
+template <int K, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_apply_kernel(NormArgs a) {
+#pragma clang fp contract(off)
+  __shared__ double lds[4][256];
+  const TileSeat<K> t(a, (int)blockIdx.x);
+  f32x4 s[K];
+  if (a.sum) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = t.get(a.sum, k, a.F);
+  } else {
+    const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      s[k] = t.get(a.x, k, a.F);
+      if (DROP) s[k] = t.drop(a.drop, z0, k, s[k]);
+      if (a.residual) s[k] = t.get(a.residual, k, a.F) + s[k];
+    }
+  }
+  double q[4];
+  all_sums(a, t, q, lds);
+  f32x4 rstd;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) rstd[e] = inv_sqrt(q[e] * a.inv_f + a.eps);
+  if (a.rstd && t.tile_c == 0 && threadIdx.x < (1u << a.shift)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < t.left) a.rstd[t.n + e] = rstd[e];
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const float g = t.of_column(a.gamma, k, a.F);
+    t.put(a.y, k, a.F, (s[k] * rstd) * g);
+  }
+}
+
+// First of the backward: the sums of d n over a tile's columns and of dy n over its rows.
+template <int K>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_dots_kernel(NormArgs a) {
+  __shared__ double lds[kNormWaves][256];
+  const TileSeat<K> t(a, (int)blockIdx.x);
+  f32x4 u[K], d[K], rstd = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    u[k] = t.get(a.s, k, a.F);
+    d[k] = t.get(a.dy, k, a.F);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < t.left) rstd[e] = a.rstd[t.n + e];
+  double q[4] = {};
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const float g = t.of_column(a.gamma, k, a.F);
+    float dg = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float n = u[k][e] * rstd[e];
+      if (e < t.left) dg = fmaf(d[k][e], n, dg);
+      q[e] = fma((double)(d[k][e] * g), (double)n, q[e]);
+    }
+    for (int o = (1 << a.shift) >> 1; o > 0; o >>= 1) dg += __shfl_xor(dg, o, 64);
+    if (t.row == 0 && t.has(k, a.F)) (a.gamma_part + (int64_t)t.tile_r * a.F + t.f0 + (int64_t)k * t.cols)[t.lane_f] = dg;
+  }
+  leave_sums(a, t, q, lds);
+}
+
+// Second: dx and dresidual; the blocks behind the tiles join dgamma.
+template <int K, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_grad_kernel(NormArgs a) {
+  __shared__ double lds[4][256];
+  const int tiles = a.row_tiles * a.col_tiles;
+  if ((int)blockIdx.x >= tiles) {
+    join_gamma(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
+    return;
+  }
+  const TileSeat<K> t(a, (int)blockIdx.x);
+  const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
+  f32x4 u[K], d[K], p[K], rstd = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    u[k] = t.get(a.s, k, a.F);
+    d[k] = t.get(a.dy, k, a.F);
+    if (a.dsum) p[k] = t.get(a.dsum, k, a.F);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < t.left) rstd[e] = a.rstd[t.n + e];
+  double q[4];
+  all_sums(a, t, q, lds);
+  float c[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] = (float)(q[e] * a.inv_f);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const float gamma = t.of_column(a.gamma, k, a.F);
+    f32x4 g;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      g[e] = rstd[e] * fmaf(-(u[k][e] * rstd[e]), c[e], d[k][e] * gamma);
+      if (a.dsum) g[e] += p[k][e];
+    }
+    if (a.dresidual) t.put(a.dresidual, k, a.F, g);
+    t.put(a.dx, k, a.F, DROP ? t.drop(a.drop, z0, k, g) : g);
+  }
+}
+
+constexpr int kFewHeld = 16;  // features of a thread that a block of few rows holds
+constexpr int kTileCols = 4;  // columns of a thread in a tile (8 in the forward of many tiles)
+
+// Few rows: up to 32, as many as a block holds.
+bool few_rows(NormArgs& a) {
+  int shift = 0;
+  while (((int64_t)1 << shift) < a.N && shift < 6) ++shift;
+  if (a.N > 32 || (a.F << shift) > (int64_t)kNormThreads * kFewHeld) return false;
+  a.shift = shift;
+  return true;
+}
+
+// The tiles of K columns a thread; their number is checked by the caller.
+int64_t set_tiles(NormArgs& a, int K) {
+  a.shift = 0;
+  while (((int64_t)4 << a.shift) < a.N && a.shift < 6) ++a.shift;
+  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)K * (kNormThreads >> a.shift);
+  a.row_tiles = (int)((a.N + rows - 1) / rows);
+  const int64_t c = (a.F + cols - 1) / cols;
+  a.col_tiles = (int)c;
+  return a.row_tiles * c;
+}
+
+template <bool DROP>
+int run_forward(NormArgs& a, hipStream_t st, const char* who) {
+  const dim3 threads(kNormThreads);
+  if (few_rows(a)) {
+    const int64_t per = ((a.F << a.shift) + kNormThreads - 1) / kNormThreads;
+    if (per <= 4) hipLaunchKernelGGL((rms_norm_few_fwd_kernel<4, DROP>), dim3(1), threads, 0, st, a);
+    else hipLaunchKernelGGL((rms_norm_few_fwd_kernel<kFewHeld, DROP>), dim3(1), threads, 0, st, a);
     return check_launch(who);
   }
+  int K = 2 * kTileCols;
+  if (set_tiles(a, K) < 512) set_tiles(a, K = kTileCols);
+  const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles;
+  CNHIP_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too large", who);
+  void* ws = nullptr;
+  CNHIP_TRY(scratch(st, kScratchLayer, (size_t)a.col_tiles * (size_t)a.N * sizeof(double), &ws, who));
+  a.part = static_cast<double*>(ws);
+  const dim3 grid((unsigned)tiles);
+  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_sum_kernel<kTileCols, DROP>), grid, threads, 0, st, a);
+  else hipLaunchKernelGGL((rms_norm_sum_kernel<2 * kTileCols, DROP>), grid, threads, 0, st, a);
+  CNHIP_TRY(check_launch(who));
+  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_apply_kernel<kTileCols, DROP>), grid, threads, 0, st, a);
+  else hipLaunchKernelGGL((rms_norm_apply_kernel<2 * kTileCols, DROP>), grid, threads, 0, st, a);
+  return check_launch(who);
+}
+
+template <bool DROP>
+int run_backward(NormArgs& a, hipStream_t st, const char* who) {
+  const dim3 threads(kNormThreads);
+  const bool few = few_rows(a);
+  a.row_tiles = a.col_tiles = 1;
+  const int64_t tiles = few ? 1 : set_tiles(a, kTileCols), gamma_blocks = (a.F + 63) / 64;
+  CNHIP_REQUIRE(tiles + gamma_blocks < ((int64_t)1 << 31), "%s: too large", who);
+  const size_t sums = few ? 0 : (size_t)a.col_tiles * (size_t)a.N * sizeof(double);
+  void* ws = nullptr;
+  CNHIP_TRY(scratch(st, kScratchLayer, sums + (size_t)a.row_tiles * (size_t)a.F * sizeof(float), &ws, who));
+  a.part = static_cast<double*>(ws);
+  a.gamma_part = reinterpret_cast<float*>(static_cast<char*>(ws) + sums);
+  if (few) {
+    const int64_t per = ((a.F << a.shift) + kNormThreads - 1) / kNormThreads;
+    if (per <= 4) hipLaunchKernelGGL((rms_norm_few_bwd_kernel<4, DROP>), dim3(1), threads, 0, st, a);
+    else hipLaunchKernelGGL((rms_norm_few_bwd_kernel<kFewHeld, DROP>), dim3(1), threads, 0, st, a);
+    CNHIP_TRY(check_launch(who));
+    hipLaunchKernelGGL(rms_norm_gamma_kernel, dim3((unsigned)gamma_blocks), threads, 0, st, a);
+    return check_launch(who);
+  }
+  hipLaunchKernelGGL(rms_norm_dots_kernel<kTileCols>, dim3((unsigned)tiles), threads, 0, st, a);
+  CNHIP_TRY(check_launch(who));
+  hipLaunchKernelGGL((rms_norm_grad_kernel<kTileCols, DROP>), dim3((unsigned)(tiles + gamma_blocks)), threads, 0, st, a);
+  return check_launch(who);
 }
 
 int check_drop(float p, const char* who) {
@@ -374,7 +583,7 @@ int cnhip_rms_norm_forward(const float* x, const float* residual, const float* g
   const hipStream_t st = cnhip::as_stream(stream);
   cnhip::HbmTimer timer("rms_norm_fwd_kernel", 4.0 * (double)N * (double)F * (2 + (residual != nullptr) + (sum != nullptr)),
                         st);
-  return p > 0.f ? cnhip::run_norm<false, true>(a, st, who) : cnhip::run_norm<false, false>(a, st, who);
+  return p > 0.f ? cnhip::run_forward<true>(a, st, who) : cnhip::run_forward<false>(a, st, who);
 }
 
 int cnhip_rms_norm_backward(const float* sum, const float* rstd, const float* gamma, const float* dy, const float* dsum,
@@ -402,7 +611,7 @@ int cnhip_rms_norm_backward(const float* sum, const float* rstd, const float* ga
   const hipStream_t st = cnhip::as_stream(stream);
   cnhip::HbmTimer timer("rms_norm_bwd_kernel",
                         4.0 * (double)N * (double)F * (3 + (dsum != nullptr) + (dresidual != nullptr)), st);
-  return p > 0.f ? cnhip::run_norm<true, true>(a, st, who) : cnhip::run_norm<true, false>(a, st, who);
+  return p > 0.f ? cnhip::run_backward<true>(a, st, who) : cnhip::run_backward<false>(a, st, who);
 }
 
 }  // extern "C"
