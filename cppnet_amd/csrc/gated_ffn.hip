@@ -25,10 +25,13 @@ using pr::f32x16;
 using pr::f32x4;
 using pr::f32x4u;
 
-// Largest finite values, as bits: of W, and of a piece's X and dZ.
+// Largest finite values, as bits: of W, of a piece's X and a bound of its dZ.
 struct FfnScales {
-  uint32_t x, z;
+  uint32_t w, x, z;
 };
+// What the blocks that look for them found: of W, X and dZ.
+constexpr int kMaxBlocks[3] = {256, 256, 512};
+constexpr int kMaxAt[3] = {0, 256, 512}, kMaxParts = 1024;
 
 struct FfnArgs {
   const float *X, *W, *b, *Z, *dH;
@@ -40,9 +43,11 @@ struct FfnArgs {
   int *xe, *we;        // forward: the exponents of a row of X, of 32 rows of W^T
   int steps_d;         // of 16 features of D
   int steps_f;         // of 16 of the hidden features
-  uint32_t* w_max;
-  FfnScales* scales;   // the piece's
-  float* db_part;      // [ceil(R / 256)][2 F], or null
+  uint32_t* max_part;  // [kMaxParts]
+  int max_blocks[3];
+  FfnScales* scales;
+  int z_blocks;        // blocks of 32 rows that a wave packs of dZ
+  float* db_part;      // [ceil(R / 32 / z_blocks)][2 F], or null
 };
 
 // Column of W that row m of the packed W^T holds; -1 for padding.
@@ -152,12 +157,17 @@ __global__ void __launch_bounds__(512) ffn_pack_own_kernel(FfnArgs a, int w_bloc
 }
 
 // A: W^T (M: packed columns), B: X (N: rows); H and, where it is kept, Z.
-__global__ void __launch_bounds__(pr::GNT, 2) ffn_forward_kernel(pr::GemmArgs g, FfnArgs a) {
+__global__ void __launch_bounds__(pr::GNT, 2) ffn_forward_kernel(pr::GemmArgs g, FfnArgs a, float* part) {
   __shared__ __align__(16) char lds[pr::kGemmLds];
   int tm, tn;
   pr::tile_of((int)blockIdx.x, (g.M + pr::TM - 1) / pr::TM, (g.N + pr::TN - 1) / pr::TN, tm, tn);
   pr::Acc acc;
-  pr::gemm_tile<false, false>(g, tm, tn, 0, g.steps, lds, acc);
+  const int t0 = (int)blockIdx.y * g.steps_per_split;
+  pr::gemm_tile<false, false>(g, tm, tn, t0, min(g.steps, t0 + g.steps_per_split), lds, acc);
+  if (part) {
+    pr::put_tile<false>(acc, tm, tn, g.M, g.N, part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float x) { return x; });
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int block0 = tm * (pr::TM / 32) + (wave >> 2) * 4;  // the wave's first of 32 packed columns: a gate's
   int64_t n[2];
@@ -190,6 +200,28 @@ __global__ void __launch_bounds__(pr::GNT, 2) ffn_forward_kernel(pr::GemmArgs g,
       }
     }
   }
+}
+
+// The same from split sums, [splits][M][N].
+__global__ void __launch_bounds__(256) ffn_join_kernel(FfnArgs a, const float* __restrict__ part, int64_t M, int splits) {
+  const int64_t total = M * a.N;
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, f = blockIdx.y;
+  if (n >= a.N) return;
+  const int64_t at = ((f >> 5) * 64 + (f & 31)) * a.N + n;
+  float gate = 0.f, up = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    gate += part[s * total + at];
+    up += part[s * total + at + 32 * a.N];
+  }
+  const int ex = a.xe[n], blk = (int)(f >> 5) * 2;
+  gate = pr::times_exp2(gate, -ex - a.we[blk]) + (a.b ? a.b[f] : 0.f);
+  up = pr::times_exp2(up, -ex - a.we[blk + 1]) + (a.b ? a.b[a.F + f] : 0.f);
+  if (a.Zout) {
+    a.Zout[n + a.N * f] = gate;
+    a.Zout[n + a.N * (a.F + f)] = up;
+  }
+  a.H[n + a.N * f] = gate_f(a.act, gate) * up;
 }
 
 // Few rows: W is read once and each value used for a handful of products, so the
@@ -268,82 +300,180 @@ __device__ __forceinline__ void grads_of(const FfnArgs& a, float gate, float up,
   du = dh * y;
 }
 
-// The largest finite |W| (the first w_blocks blocks, with the first piece), |X| (x_blocks)
-// and |dZ| of a piece's rows.
-__global__ void __launch_bounds__(256) ffn_max_kernel(FfnArgs a, int w_blocks, int x_blocks) {
-  uint32_t m = 0;
-  uint32_t* to;
-  int bid = (int)blockIdx.x;
-  const int64_t chunks = (a.R + 1023) / 1024;  // of rows
-  if (bid < w_blocks) {
-    to = a.w_max;
-    const int64_t n = a.D * 2 * a.F, step = (int64_t)w_blocks * 1024;
-    for (int64_t i = ((int64_t)bid * 256 + threadIdx.x) * 4; i < n; i += step) {
-      if (i + 4 <= n) {
-        const f32x4 x = *reinterpret_cast<const f32x4u*>(a.W + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = max(m, pr::finite_bits(x[e]));
-      } else {
-        for (int64_t e = i; e < n; ++e) m = max(m, pr::finite_bits(a.W[e]));
-      }
-    }
-  } else if ((bid -= w_blocks) < x_blocks) {
-    to = &a.scales->x;
-    for (int64_t t = bid; t < a.D * chunks; t += x_blocks) {
-      const int64_t n = t % chunks * 1024 + 4 * threadIdx.x;
-      const float* p = a.X + a.row0 + n + a.N * (t / chunks);
-      if (n + 4 <= a.R) {
-        const f32x4 x = *reinterpret_cast<const f32x4u*>(p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = max(m, pr::finite_bits(x[e]));
-      } else {
-        for (int e = 0; n + e < a.R; ++e) m = max(m, pr::finite_bits(p[e]));
-      }
-    }
+// An upper bound of |dgate| and |dup|, a few times their size at most but next to a zero
+// of act': an operand's scale need not be closer, and the functions themselves would
+// make the pass over Z and dH half as long again (8192 x 4096, GELU: 122 us for 116).
+//   z >= 0: |act| <= z (sigmoid: 1), |act'| <= 1.13
+//   z < 0:  with r = e^z, or e^(-z^2 / 2) for GELU, |act| <= r |z|, |act'| <= r (1 + |z|);
+//   sigmoid: act <= r, and act' <= e^-|z| everywhere.  ReLU: as they are.
+__device__ __forceinline__ uint32_t grad_bound(int act, float gate, float up, float dh) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  const float m = fabsf(gate);
+  float y, d;
+  if (act == CNHIP_GATE_RELU) {
+    y = relu_f(gate);
+    d = relu_mask(y);
   } else {
-    bid -= x_blocks;
-    to = &a.scales->z;
-    const int z_blocks = (int)gridDim.x - w_blocks - x_blocks;
-    for (int64_t t = bid; t < a.F * chunks; t += z_blocks) {
-      const int64_t n = t % chunks * 1024 + 4 * threadIdx.x, at = a.row0 + n + a.N * (t / chunks);
-      f32x4 zg = {0.f, 0.f, 0.f, 0.f}, zu = zg, dh = zg;
-      if (n + 4 <= a.R) {
-        zg = *reinterpret_cast<const f32x4u*>(a.Z + at);
-        zu = *reinterpret_cast<const f32x4u*>(a.Z + a.N * a.F + at);
-        dh = *reinterpret_cast<const f32x4u*>(a.dH + at);
-      } else {
+    const float r = __builtin_amdgcn_exp2f(-kLog2e * (act == CNHIP_GATE_GELU ? 0.5f * m * m : m));
+    if (act == CNHIP_GATE_SIGMOID) {
+      y = gate < 0.f ? r : 1.f;
+      d = r;
+    } else {
+      y = gate < 0.f ? r * m : gate;
+      d = gate < 0.f ? fmaf(r, m, r) : 1.13f;
+    }
+  }
+  return max(pr::finite_bits(dh * up * d), pr::finite_bits(dh * y));
+}
+
+// The largest finite |W|, |X| and bound of |dZ| of a piece's rows, by blocks.
+__global__ void __launch_bounds__(1024) ffn_max_kernel(FfnArgs a) {
+  __shared__ uint32_t part[16];
+  uint32_t m = 0;
+  int bid = (int)blockIdx.x, kind = 2;  // the most work first
+  while (kind > 0 && bid >= a.max_blocks[kind]) bid -= a.max_blocks[kind--];
+  const int blocks = a.max_blocks[kind];
+  constexpr int U = 4;  // loads of each operand under way
+  if (kind == 0) {
+    const int64_t n = a.D * 2 * a.F, step = (int64_t)blocks * 4096;
+    for (int64_t i0 = ((int64_t)bid * 1024 + threadIdx.x) * 4; i0 < n; i0 += U * step) {
+      f32x4 x[U];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (n + e >= a.R) continue;
-          zg[e] = a.Z[at + e];
-          zu[e] = a.Z[a.N * a.F + at + e];
-          dh[e] = a.dH[at + e];
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = i0 + u * step;
+        x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (i + 4 <= n) {
+          x[u] = *reinterpret_cast<const f32x4u*>(a.W + i);
+        } else {
+          for (int e = 0; e < 4; ++e)
+            if (i + e < n) x[u][e] = a.W[i + e];
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float dg, du;
-        grads_of(a, zg[e], zu[e], dh[e], dg, du);
-        m = max(m, max(pr::finite_bits(dg), pr::finite_bits(du)));
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max(m, pr::finite_bits(x[u][e]));
+    }
+  } else {
+    // items of 256 rows of a column, a wave each: item t is chunk t % chunks of column
+    // t / chunks, kept up by additions
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int chunks = (int)((a.R + 255) / 256), step = blocks * 16;
+    const int64_t cols = kind == 1 ? a.D : a.F;
+    const int step_cols = step / chunks, step_chunks = step % chunks;
+    int64_t col = (bid * 16 + wave) / chunks;
+    int chunk = (bid * 16 + wave) % chunks;
+    auto get = [&](const float* p, int n) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (n + 4 <= a.R) return f32x4(*reinterpret_cast<const f32x4u*>(p + n));
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.R) x[e] = p[n + e];
+      return x;
+    };
+    while (col < cols) {
+      f32x4 x[U], y[U], z[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int n = chunk * 256 + 4 * lane;
+        x[u] = y[u] = z[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (col < cols) {
+          const int64_t at = a.row0 + a.N * col;
+          x[u] = get((kind == 1 ? a.X : a.Z) + at, n);
+          if (kind == 2) {
+            y[u] = get(a.Z + a.N * a.F + at, n);
+            z[u] = get(a.dH + at, n);
+          }
+        }
+        col += step_cols;
+        chunk += step_chunks;
+        if (chunk >= chunks) {
+          chunk -= chunks;
+          ++col;
+        }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          m = max(m, kind == 1 ? pr::finite_bits(x[u][e]) : grad_bound(a.act, x[u][e], y[u][e], z[u][e]));
     }
   }
-  __shared__ uint32_t part[4];
   m = pr::wave_max(m);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x) return;
-  m = max(max(part[0], part[1]), max(part[2], part[3]));
-  if (m) atomicMax(to, m);  // a maximum is the same in any order
+  for (int w = 1; w < 16; ++w) m = max(m, part[w]);
+  a.max_part[kMaxAt[kind] + bid] = m;
 }
 
-// W^T (with the first piece) and the piece's rows of X packed, a wave per fragment.
-__global__ void __launch_bounds__(256) ffn_pack_kernel(FfnArgs a, int64_t w_frags, int64_t x_frags) {
+// Of all the blocks that looked at operand `kind`, in every lane.
+__device__ __forceinline__ uint32_t max_of(const FfnArgs& a, int kind) {
+  uint32_t m = 0;
+  for (int i = threadIdx.x & 63; i < a.max_blocks[kind]; i += 64) m = max(m, a.max_part[kMaxAt[kind] + i]);
+  return pr::wave_max(m);
+}
+
+// What the products of the backward read, packed; a wave for
+//   - a step of 16 hidden features of dZ and z_blocks blocks of 32 rows, with its column
+//     sums where they are wanted (the first z_waves waves),
+//   - a fragment of W^T, of X.
+__global__ void __launch_bounds__(256) ffn_pack_kernel(FfnArgs a, int64_t z_waves, int64_t w_frags, int64_t x_frags) {
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-  int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t blocks = (a.R + 31) / 32;
+  int64_t f = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (f == 0) {  // for the products
+    const FfnScales s{max_of(a, 0), max_of(a, 1), max_of(a, 2)};
+    if (lane == 0) *a.scales = s;
+  }
+  if (f < z_waves) {
+    const int64_t groups = (blocks + a.z_blocks - 1) / a.z_blocks, grp = f % groups;
+    const int step = (int)(f / groups);
+    const int64_t f0 = (int64_t)step * 16 + 8 * h;
+    const float s = pr::exp2i(pr::scale_exp(max_of(a, 2)));
+    float sg[8] = {}, su[8] = {};
+    for (int64_t b = grp * a.z_blocks; b < (grp + 1) * a.z_blocks && b < blocks; ++b) {
+      const int64_t n = b * 32 + r;
+      float zg[8], zu[8], dh[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = n < a.R && f0 + e < a.F;
+        const int64_t at = a.row0 + n + a.N * (f0 + e);
+        zg[e] = in ? a.Z[at] : 0.f;
+        zu[e] = in ? a.Z[a.N * a.F + at] : 0.f;
+        dh[e] = in ? a.dH[at] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float dg, du;
+        grads_of(a, zg[e], zu[e], dh[e], dg, du);
+        sg[e] += dg;
+        su[e] += du;
+        zg[e] = dg * s;
+        zu[e] = du * s;
+      }
+      const int at = 4 * (step >> 1) + (step & 1);  // the gate's step of the packed columns; the up's is two on
+      pr::put_frag(a.zp, b, 2 * a.steps_f, at, zg);
+      pr::put_frag(a.zp, b, 2 * a.steps_f, at + 2, zu);
+    }
+    if (!a.db_part) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        sg[e] += __shfl_xor(sg[e], o, 64);
+        su[e] += __shfl_xor(su[e], o, 64);
+      }
+      if (r == 0 && f0 + e < a.F) {
+        a.db_part[grp * 2 * a.F + f0 + e] = sg[e];
+        a.db_part[grp * 2 * a.F + a.F + f0 + e] = su[e];
+      }
+    }
+    return;
+  }
+  f -= z_waves;
   float x[8];
   if (f < w_frags) {
-    const float s = pr::exp2i(pr::scale_exp(*a.w_max));
     const int64_t col = column_of(f / a.steps_d * 32 + r, a.F);
     const int step = (int)(f % a.steps_d);
     const int64_t d0 = step * 16 + 8 * h;
@@ -352,89 +482,33 @@ __global__ void __launch_bounds__(256) ffn_pack_kernel(FfnArgs a, int64_t w_frag
       const f32x4 u = *reinterpret_cast<const f32x4u*>(p), w = *reinterpret_cast<const f32x4u*>(p + 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = u[e] * s;
-        x[4 + e] = w[e] * s;
+        x[e] = u[e];
+        x[4 + e] = w[e];
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = col >= 0 && d0 + e < a.D ? p[e] * s : 0.f;
+      for (int e = 0; e < 8; ++e) x[e] = col >= 0 && d0 + e < a.D ? p[e] : 0.f;
     }
+    const float s = pr::exp2i(pr::scale_exp(max_of(a, 0)));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= s;
     pr::put_frag(a.wp, f / a.steps_d, a.steps_d, step, x);
     return;
   }
   f -= w_frags;
   if (f >= x_frags) return;
   // neighbouring waves take neighbouring row blocks: their reads run along a column
-  const int64_t blocks = (a.R + 31) / 32, n = f % blocks * 32 + r;
+  const int64_t n = f % blocks * 32 + r;
   const int step = (int)(f / blocks);
-  const float s = pr::exp2i(pr::scale_exp(a.scales->x));
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int64_t d = step * 16 + 8 * h + e;
-    x[e] = n < a.R && d < a.D ? a.X[a.row0 + n + a.N * d] * s : 0.f;
+    x[e] = n < a.R && d < a.D ? a.X[a.row0 + n + a.N * d] : 0.f;
   }
+  const float s = pr::exp2i(pr::scale_exp(max_of(a, 1)));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= s;
   pr::put_frag(a.xp, f % blocks, a.steps_d, step, x);
-}
-
-// The piece's dZ packed, a wave for a step of 16 hidden features and eight blocks of
-// 32 rows; with its column sums where they are wanted.
-__global__ void __launch_bounds__(256) ffn_grad_kernel(FfnArgs a) {
-  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t groups = (a.R + 255) / 256, blocks = (a.R + 31) / 32;
-  const int64_t grp = w % groups;
-  const int step = (int)(w / groups);
-  if (step >= a.steps_f) return;
-  const int64_t f0 = (int64_t)step * 16 + 8 * h;
-  const float s = pr::exp2i(pr::scale_exp(a.scales->z));
-  float sg[8] = {}, su[8] = {};
-  for (int64_t b = grp * 8; b < (grp * 8 + 8 < blocks ? grp * 8 + 8 : blocks); ++b) {
-    const int64_t n = b * 32 + r;
-    float zg[8], zu[8], dh[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool in = n < a.R && f0 + e < a.F;
-      const int64_t at = a.row0 + n + a.N * (f0 + e);
-      zg[e] = in ? a.Z[at] : 0.f;
-      zu[e] = in ? a.Z[a.N * a.F + at] : 0.f;
-      dh[e] = in ? a.dH[at] : 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float dg, du;
-      grads_of(a, zg[e], zu[e], dh[e], dg, du);
-      sg[e] += dg;
-      su[e] += du;
-      zg[e] = dg * s;
-      zu[e] = du * s;
-    }
-    const int at = 4 * (step >> 1) + (step & 1);  // the gate's step of the packed columns; the up's is two on
-    pr::put_frag(a.zp, b, 2 * a.steps_f, at, zg);
-    pr::put_frag(a.zp, b, 2 * a.steps_f, at + 2, zu);
-  }
-  if (!a.db_part) return;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      sg[e] += __shfl_xor(sg[e], o, 64);
-      su[e] += __shfl_xor(su[e], o, 64);
-    }
-    if (r == 0 && f0 + e < a.F) {
-      a.db_part[grp * 2 * a.F + f0 + e] = sg[e];
-      a.db_part[grp * 2 * a.F + a.F + f0 + e] = su[e];
-    }
-  }
-}
-
-// db (+)= the sums of the groups of rows, in order
-__global__ void __launch_bounds__(256) ffn_db_kernel(FfnArgs a, float* db, int accumulate) {
-  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (v >= 2 * a.F) return;
-  float s = 0.f;
-#pragma unroll 8
-  for (int64_t q = 0; q < (a.R + 255) / 256; ++q) s += a.db_part[q * 2 * a.F + v];
-  db[v] = accumulate ? db[v] + s : s;
 }
 
 struct FfnOut {
@@ -446,21 +520,30 @@ struct FfnOut {
 // COLS: row m of the product is column_of(m) of the output.
 template <bool COLS>
 __device__ __forceinline__ int scale_out(const FfnArgs& a) {
-  return -pr::scale_exp(a.scales->z) - pr::scale_exp(COLS ? a.scales->x : *a.w_max);
+  return -pr::scale_exp(a.scales->z) - pr::scale_exp(COLS ? a.scales->x : a.scales->w);
 }
+
+// A product of the backward as blocks [tile][split].
+struct FfnProduct {
+  pr::GemmArgs g;
+  FfnOut o;
+  int tiles, splits;
+};
 
 // dX (A: W across its rows, B: dZ), COLS false, and dW (A: dZ, B: X, both across
 // their rows), COLS true.
 template <bool TA, bool TB, bool COLS>
-__global__ void __launch_bounds__(pr::GNT, 2) ffn_grads_kernel(pr::GemmArgs g, FfnArgs a, FfnOut o) {
-  __shared__ __align__(16) char lds[pr::kGemmLds];
+__device__ __forceinline__ void ffn_product(const FfnProduct& p, const FfnArgs& a, int bid, char* lds) {
+  const pr::GemmArgs& g = p.g;
+  const FfnOut& o = p.o;
   int tm, tn;
-  pr::tile_of((int)blockIdx.x, (g.M + pr::TM - 1) / pr::TM, (g.N + pr::TN - 1) / pr::TN, tm, tn);
-  const int t0 = (int)blockIdx.y * g.steps_per_split, t1 = min(g.steps, t0 + g.steps_per_split);
+  const int split = bid / p.tiles;
+  pr::tile_of(bid % p.tiles, (g.M + pr::TM - 1) / pr::TM, (g.N + pr::TN - 1) / pr::TN, tm, tn);
+  const int t0 = split * g.steps_per_split, t1 = min(g.steps, t0 + g.steps_per_split);
   pr::Acc acc;
   pr::gemm_tile<TA, TB>(g, tm, tn, t0, t1, lds, acc);
   if (o.part) {
-    pr::put_tile<false>(acc, tm, tn, g.M, g.N, o.part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float x) { return x; });
+    pr::put_tile<false>(acc, tm, tn, g.M, g.N, o.part + (int64_t)split * g.M * g.N, g.N, [](float x) { return x; });
     return;
   }
   const int eo = scale_out<COLS>(a);
@@ -498,19 +581,52 @@ __global__ void __launch_bounds__(pr::GNT, 2) ffn_grads_kernel(pr::GemmArgs g, F
   }
 }
 
+// Both products, and db (+)= the sums of the groups of rows, in order, in the blocks
+// behind them.
+__global__ void __launch_bounds__(pr::GNT, 2) ffn_grads_kernel(FfnArgs a, FfnProduct x, FfnProduct w, float* db, int add) {
+  __shared__ __align__(16) char lds[pr::kGemmLds];
+  int bid = (int)blockIdx.x;
+  if (bid < x.tiles * x.splits) {
+    ffn_product<true, false, false>(x, a, bid, lds);
+    return;
+  }
+  bid -= x.tiles * x.splits;
+  if (bid < w.tiles * w.splits) {
+    ffn_product<true, true, true>(w, a, bid, lds);
+    return;
+  }
+  bid -= w.tiles * w.splits;
+  const int64_t v = (int64_t)bid * pr::GNT + threadIdx.x, blocks = (a.R + 31) / 32;
+  if (v >= 2 * a.F) return;
+  float s = 0.f;
+#pragma unroll 16
+  for (int64_t q = 0; q < (blocks + a.z_blocks - 1) / a.z_blocks; ++q) s += a.db_part[q * 2 * a.F + v];
+  db[v] = add ? db[v] + s : s;
+}
+
 template <bool COLS>
-__global__ void __launch_bounds__(256) ffn_reduce_kernel(FfnArgs a, FfnOut o, int M, int N, int splits) {
-  const int64_t total = (int64_t)M * N;
+__device__ __forceinline__ void ffn_reduce(const FfnProduct& p, const FfnArgs& a, int64_t first, int64_t step) {
+  const int64_t total = (int64_t)p.g.M * p.g.N;
   const int eo = scale_out<COLS>(a);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / N, to = COLS ? column_of(m, a.F) : m;
+  for (int64_t i = first; i < total; i += step) {
+    const int64_t m = i / p.g.N, to = COLS ? column_of(m, a.F) : m;
     if (to < 0) continue;
     float x = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) x += o.part[s * total + i];
-    float* p = o.p + i % N + o.ld * to;
+    for (int s = 0; s < p.splits; ++s) x += p.o.part[s * total + i];
+    float* q = p.o.p + i % p.g.N + p.o.ld * to;
     x = pr::times_exp2(x, eo);
-    *p = o.accumulate ? *p + x : x;
+    *q = p.o.accumulate ? *q + x : x;
+  }
+}
+// The products that were split, each over the blocks of its half of the grid.
+__global__ void __launch_bounds__(256) ffn_reduce_kernel(FfnArgs a, FfnProduct x, FfnProduct w) {
+  const int64_t half = gridDim.x / 2, bid = blockIdx.x % half;
+  const int64_t first = bid * 256 + threadIdx.x;
+  if (blockIdx.x < half) {
+    if (x.o.part) ffn_reduce<false>(x, a, first, half * 256);
+  } else {
+    if (w.o.part) ffn_reduce<true>(w, a, first, half * 256);
   }
 }
 
@@ -534,6 +650,37 @@ int check_shape(int64_t N, int64_t D, int64_t F, int act, const char* who) {
   return CNHIP_OK;
 }
 
+// Steps of a block of a product that runs beside another one, so that all blocks
+// together are done soonest: rounds of 256 blocks, a block's own time and about 8 steps
+// for its beginning and end, and what the split sums move.
+struct Job {
+  int64_t M, N;
+  int steps;
+};
+int steps_of(const Job* jobs, int n) {
+  constexpr double kStepUs = 1.55, kBytesUs = 5e6;
+  int longest = 2, best = 0;
+  for (int i = 0; i < n; ++i) longest = jobs[i].steps > longest ? jobs[i].steps : longest;
+  double least = 0;
+  for (int parts = 1; parts <= 64; ++parts) {
+    const int per = ((longest + parts - 1) / parts + 1) / 2 * 2;
+    if (parts > 1 && per < 6) break;
+    int64_t blocks = 0;
+    double moved = 0;
+    for (int i = 0; i < n; ++i) {
+      const int64_t splits = (jobs[i].steps + per - 1) / per;
+      blocks += tiles_of(jobs[i].M, jobs[i].N) * splits;
+      if (splits > 1) moved += 8.0 * (double)splits * (double)jobs[i].M * (double)jobs[i].N;
+    }
+    const double us = (double)((blocks + 255) / 256) * (per + 8) * kStepUs + moved / kBytesUs + (moved > 0 ? 3.0 : 0.0);
+    if (best == 0 || us < least) {
+      least = us;
+      best = per;
+    }
+  }
+  return best;
+}
+
 int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
   const int64_t N = a.N, D = a.D, F = a.F, Fp = pad32(F);
   if (N <= kFewRows) {
@@ -548,6 +695,9 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
   Places w;
   const size_t o_x = w.place((size_t)(pad32(N) * pad32(D)) * 4), o_w = w.place((size_t)(2 * Fp * pad32(D)) * 4),
                o_xe = w.place((size_t)N * 4), o_we = w.place((size_t)(2 * Fp / 32) * 4);
+  const Job job{2 * Fp, N, a.steps_d};
+  const int per = F < 65536 ? steps_of(&job, 1) : a.steps_d, splits = (a.steps_d + per - 1) / per;
+  const size_t o_part = w.place(splits > 1 ? (size_t)(splits * 2 * Fp * N) * 4 : 0);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, w.at, &ws, who));
   char* base = static_cast<char*>(ws);
@@ -559,8 +709,14 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
                      (int)(2 * Fp / 32));
   CNHIP_TRY(check_launch(who));
   const pr::GemmArgs g{pr::Packed{a.wp, (int)(2 * Fp / 32), a.steps_d}, pr::Packed{a.xp, (int)(pad32(N) / 32), a.steps_d},
-                       (int)(2 * Fp), (int)N, a.steps_d, a.steps_d, a.steps_d / 2};
-  hipLaunchKernelGGL(ffn_forward_kernel, dim3((unsigned)tiles_of(2 * Fp, N)), dim3(pr::GNT), 0, st, g, a);
+                       (int)(2 * Fp), (int)N, a.steps_d, per, a.steps_d / 2};
+  float* part = splits > 1 ? reinterpret_cast<float*>(base + o_part) : nullptr;
+  hipLaunchKernelGGL(ffn_forward_kernel, dim3((unsigned)tiles_of(2 * Fp, N), (unsigned)splits), dim3(pr::GNT), 0, st, g, a,
+                     part);
+  CNHIP_TRY(check_launch(who));
+  if (!part) return CNHIP_OK;
+  hipLaunchKernelGGL(ffn_join_kernel, dim3((unsigned)((N + 255) / 256), (unsigned)F), dim3(256), 0, st, a, part, 2 * Fp,
+                     splits);
   return check_launch(who);
 }
 
@@ -573,63 +729,69 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
   const int64_t most = ((int64_t)1 << 27) / (2 * Fp);
   int64_t R = most < 1024 ? 1024 : most / 256 * 256;
   if (R > N) R = N;
-  const int64_t Rp = pad32(R), pieces = (N + R - 1) / R;
-  const pr::Split sx = pr::split_of(D, R, 2 * a.steps_f), sw = pr::split_of(2 * Fp, D, (int)(Rp / 16));
-  const size_t px = sx.splits > 1 ? (size_t)sx.splits * (size_t)(D * R) * 4 : 0,
-               pw = sw.splits > 1 ? (size_t)sw.splits * (size_t)(2 * Fp * D) * 4 : 0;
+  const int64_t Rp = pad32(R);
+  const Job jobs[2] = {{D, R, 2 * a.steps_f}, {2 * Fp, D, (int)(Rp / 16)}};
+  const int per = steps_of(jobs, 2);
+  auto parts = [&](const Job& j) {
+    const int64_t splits = (j.steps + per - 1) / per;
+    return splits > 1 ? (size_t)(splits * j.M * j.N) * 4 : 0;
+  };
+  CNHIP_REQUIRE(tiles_of(D, R) * ((2 * a.steps_f + per - 1) / per) + tiles_of(2 * Fp, D) * ((Rp / 16 + per - 1) / per) <
+                    ((int64_t)1 << 30),
+                "%s: too large", who);
+  // blocks of 32 rows of dZ a wave: as many as leave 4096 waves, so that a wave that has
+  // several keeps its loads going
+  a.z_blocks = 8;
+  while (a.z_blocks > 1 && Rp / 32 / a.z_blocks * a.steps_f < 4096) a.z_blocks /= 2;
   Places w;
-  const size_t words = 256 + (size_t)pieces * sizeof(FfnScales);
-  const size_t o_max = w.place(words), o_x = w.place((size_t)(Rp * Dp) * 4), o_w = w.place((size_t)(2 * Fp * Dp) * 4),
-               o_z = w.place((size_t)(Rp * 2 * Fp) * 4),
-               o_db = w.place(db ? (size_t)((R + 255) / 256 * 2 * F) * 4 : 0), o_part = w.place(px > pw ? px : pw);
+  const size_t o_max = w.place(kMaxParts * 4 + sizeof(FfnScales)), o_x = w.place((size_t)(Rp * Dp) * 4),
+               o_w = w.place((size_t)(2 * Fp * Dp) * 4), o_z = w.place((size_t)(Rp * 2 * Fp) * 4),
+               o_db = w.place(db ? (size_t)((Rp / 32 + a.z_blocks - 1) / a.z_blocks * 2 * F) * 4 : 0),
+               o_px = w.place(parts(jobs[0])), o_pw = w.place(parts(jobs[1]));
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, w.at, &ws, who));
   char* base = static_cast<char*>(ws);
-  a.w_max = reinterpret_cast<uint32_t*>(base + o_max);
-  FfnScales* scales = reinterpret_cast<FfnScales*>(base + o_max + 256);
+  a.max_part = reinterpret_cast<uint32_t*>(base + o_max);
+  a.scales = reinterpret_cast<FfnScales*>(base + o_max + kMaxParts * 4);
   a.xp = base + o_x;
   a.wp = base + o_w;
   a.zp = base + o_z;
   a.db_part = db ? reinterpret_cast<float*>(base + o_db) : nullptr;
-  float* part = reinterpret_cast<float*>(base + o_part);
-  CNHIP_TRY(fill_bytes(a.w_max, 0, words, st, who));
   const pr::Packed pw_{a.wp, (int)(2 * Fp / 32), a.steps_d};
-  for (int64_t r0 = 0, piece = 0; r0 < N; r0 += R, ++piece) {
+  auto product = [&](const pr::Packed& A, const pr::Packed& B, int64_t M, int64_t Nn, int steps, float* p, int64_t ld,
+                     float* part, int add) {
+    const int splits = (steps + per - 1) / per;
+    return FfnProduct{pr::GemmArgs{A, B, (int)M, (int)Nn, steps, per, steps / 2},
+                      FfnOut{p, ld, splits > 1 ? part : nullptr, add}, (int)tiles_of(M, Nn), splits};
+  };
+  for (int64_t r0 = 0; r0 < N; r0 += R) {
     a.row0 = r0;
     a.R = N - r0 < R ? N - r0 : R;
-    a.scales = scales + piece;
     const int rb = (int)((a.R + 31) / 32);
-    auto clip = [](int64_t n, int64_t most_blocks) { return (int)(n < 1 ? 1 : n > most_blocks ? most_blocks : n); };
-    const int64_t chunks = (a.R + 1023) / 1024;
-    const int wb = piece ? 0 : clip(2 * D * F / 16384, 512), xb = clip(D * chunks / 4, 512), zb = clip(F * chunks / 2, 2048);
-    hipLaunchKernelGGL(ffn_max_kernel, dim3((unsigned)(wb + xb + zb)), dim3(256), 0, st, a, wb, xb);
+    // with loads for every thread, as far as there are any
+    const int64_t wanted[3] = {r0 ? a.max_blocks[0] : 2 * D * F / 16384, D * ((a.R + 255) / 256) / 64,
+                               F * ((a.R + 255) / 256) / 32};
+    for (int k = 0; k < 3; ++k)
+      a.max_blocks[k] = (int)(wanted[k] < 1 ? 1 : wanted[k] > kMaxBlocks[k] ? kMaxBlocks[k] : wanted[k]);
+    hipLaunchKernelGGL(ffn_max_kernel, dim3((unsigned)(a.max_blocks[0] + a.max_blocks[1] + a.max_blocks[2])), dim3(1024), 0,
+                       st, a);
     CNHIP_TRY(check_launch(who));
-    const int64_t wf = piece ? 0 : 2 * Fp / 32 * a.steps_d, xf = (int64_t)rb * a.steps_d;
-    hipLaunchKernelGGL(ffn_pack_kernel, dim3((unsigned)((wf + xf + 3) / 4)), dim3(256), 0, st, a, wf, xf);
+    const int64_t zw = (int64_t)((rb + a.z_blocks - 1) / a.z_blocks) * a.steps_f, wf = r0 ? 0 : 2 * Fp / 32 * a.steps_d,
+                  xf = (int64_t)rb * a.steps_d;
+    CNHIP_REQUIRE(zw + wf + xf < ((int64_t)1 << 32), "%s: too large", who);
+    hipLaunchKernelGGL(ffn_pack_kernel, dim3((unsigned)((zw + wf + xf + 3) / 4)), dim3(256), 0, st, a, zw, wf, xf);
     CNHIP_TRY(check_launch(who));
-    hipLaunchKernelGGL(ffn_grad_kernel, dim3((unsigned)(((a.R + 255) / 256 * a.steps_f + 3) / 4)), dim3(256), 0, st, a);
-    CNHIP_TRY(check_launch(who));
-    const int add = accumulate || piece > 0;
-    if (db) {
-      hipLaunchKernelGGL(ffn_db_kernel, dim3((unsigned)((2 * F + 255) / 256)), dim3(256), 0, st, a, db, add);
-      CNHIP_TRY(check_launch(who));
-    }
+    const int add = accumulate || r0 > 0;
     const pr::Packed px_{a.xp, rb, a.steps_d}, pz_{a.zp, rb, 2 * a.steps_f};
-    auto product = [&](auto kernel, auto reduce, const pr::Packed& A, const pr::Packed& B, int64_t M, int64_t Nn, int steps,
-                       pr::Split sp, FfnOut o) -> int {
-      const pr::GemmArgs g{A, B, (int)M, (int)Nn, steps, sp.steps, steps / 2};
-      const int splits = (steps + sp.steps - 1) / sp.steps;
-      o.part = splits > 1 ? part : nullptr;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)tiles_of(M, Nn), (unsigned)splits), dim3(pr::GNT), 0, st, g, a, o);
-      CNHIP_TRY(check_launch(who));
-      if (splits == 1) return CNHIP_OK;
-      hipLaunchKernelGGL(reduce, dim3(elementwise_grid(M * Nn, 256)), dim3(256), 0, st, a, o, (int)M, (int)Nn, splits);
-      return check_launch(who);
-    };
-    CNHIP_TRY(product(ffn_grads_kernel<true, false, false>, ffn_reduce_kernel<false>, pw_, pz_, D, a.R, 2 * a.steps_f, sx,
-                      FfnOut{dX + r0, N, nullptr, 0}));
-    CNHIP_TRY(product(ffn_grads_kernel<true, true, true>, ffn_reduce_kernel<true>, pz_, px_, 2 * Fp, D, 2 * rb, sw,
-                      FfnOut{dW, D, nullptr, add}));
+    const FfnProduct x = product(pw_, pz_, D, a.R, 2 * a.steps_f, dX + r0, N, reinterpret_cast<float*>(base + o_px), 0),
+                     y = product(pz_, px_, 2 * Fp, D, 2 * rb, dW, D, reinterpret_cast<float*>(base + o_pw), add);
+    const int64_t blocks = (int64_t)x.tiles * x.splits + (int64_t)y.tiles * y.splits + (db ? (2 * F + pr::GNT - 1) / pr::GNT : 0);
+    hipLaunchKernelGGL(ffn_grads_kernel, dim3((unsigned)blocks), dim3(pr::GNT), 0, st, a, x, y, db, add);
+    CNHIP_TRY(check_launch(who));
+    if (!x.o.part && !y.o.part) continue;
+    const int64_t most_out = (x.o.part ? D * a.R : 0) > (y.o.part ? 2 * Fp * D : 0) ? D * a.R : 2 * Fp * D;
+    hipLaunchKernelGGL(ffn_reduce_kernel, dim3(2 * elementwise_grid(most_out, 256)), dim3(256), 0, st, a, x, y);
+    CNHIP_TRY(check_launch(who));
   }
   return CNHIP_OK;
 }

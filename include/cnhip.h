@@ -916,8 +916,9 @@ int cnhip_linear_recurrence_backward(const float* x, const float* f, const float
  * Products of more than 64 rows, and the backward's, run on pairs of fp16 terms
  * as above; the operands with a largest value of their own are a row of X and 32
  * columns of W in the forward; W, the rows of X and those of Z's gradient that go
- * through together in the backward (2^27 / hidden / 2, at least 1024).  An infinity
- * in such an operand comes out as NaN. */
+ * through together in the backward (2^26 / hidden, at least 1024).  For Z's gradient
+ * a bound stands for the largest value, a few times it unless every gate lies next
+ * to a zero of act'.  An infinity in such an operand comes out as NaN. */
 #define CNHIP_GATE_SILU 0     /* z sigmoid(z) */
 #define CNHIP_GATE_GELU 1     /* z Phi(z), as CNHIP_ACT_GELU */
 #define CNHIP_GATE_SIGMOID 2

@@ -162,7 +162,9 @@ def ffn_backward(X, W, Z, dH, act, baseW=None, baseb=None):
     far = LOW * (1 + np.abs(Z[:, :Fh]))
     eZ = np.concatenate([np.abs(dH * up) * (16 * U * md + far), np.abs(dH) * (16 * U * np.abs(y) + far)], 1)
     aX, aW, aZ = np.abs(X), np.abs(W), np.abs(dZ)
-    mx, mw, mz = aX.max(), aW.max(), aZ.max()
+    # dZ's scale is that of a bound of its largest, up to 8 times it here: |act| and |act'| are bounded by
+    # max(z, 1) and 1.13 (z >= 0) and by (1 + |z|) e^z or (1 + |z|) e^(-z^2 / 2) (z < 0)
+    mx, mw, mz = aX.max(), aW.max(), 8 * aZ.max()
     eX = G(2 * Fh) * (aZ @ aW.T) + eZ @ aW.T + F * (mz * aW.sum(1)[None, :] + mw * aZ.sum(1)[:, None])
     eW = G(X.shape[0]) * (aX.T @ aZ) + aX.T @ eZ + F * (mx * aZ.sum(0)[None, :] + mz * aX.sum(0)[:, None])
     bW = 0.0 if baseW is None else baseW.astype(np.float64)

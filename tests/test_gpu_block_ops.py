@@ -491,17 +491,19 @@ def test_ffn_in_pieces(gpu):
     dX, dW, db = torch.empty(N * D, device="cuda"), torch.empty(D * 2 * F, device="cuda"), torch.empty(2 * F, device="cuda")
     ops.gated_ffn_backward(X, W, Z, dH, dX, dW, db, N, D, F, act=act)
     cut = lambda t, cols, a, b: t.view(cols, N)[:, a:b].contiguous().view(-1)  # noqa: E731
-    sW, sb = torch.zeros_like(dW), torch.zeros_like(db)
+    sW, sb, parts = torch.zeros_like(dW), torch.zeros_like(db), []
     for a, b in ((0, piece), (piece, N)):
-        part = torch.empty((b - a) * D, device="cuda")
-        ops.gated_ffn_backward(cut(X, D, a, b), W, cut(Z, 2 * F, a, b), cut(dH, F, a, b), part, sW, sb, b - a, D, F, act=act,
+        parts.append(torch.empty((b - a) * D, device="cuda"))
+        ops.gated_ffn_backward(cut(X, D, a, b), W, cut(Z, 2 * F, a, b), cut(dH, F, a, b), parts[-1], sW, sb, b - a, D, F, act=act,
                                accumulate=True)
-        assert torch.equal(part, cut(dX, D, a, b))
-    assert torch.equal(sb, db)
+    assert torch.equal(parts[0], cut(dX, D, 0, piece))
     # the last rows' sums may be split otherwise in a call of their own: both are off by their bound
     x, z, dh = (host(cut(t, k, piece, N)).reshape(k, last).T for t, k in ((X, D), (Z, 2 * F), (dH, F)))
-    lim = 2 * ref.ffn_backward(x, host(W).reshape(2 * F, D).T, z, dh, act)["dW"][1] + 2 * U * np.abs(host(dW).reshape(2 * F, D).T)
-    assert (np.abs((host(sW).astype(np.float64) - host(dW)).reshape(2 * F, D).T) <= lim).all()
+    want = ref.ffn_backward(x, host(W).reshape(2 * F, D).T, z, dh, act)
+    ref.check("dX", host(cut(dX, D, piece, N)).reshape(D, last).T, *want["dX"])
+    for one, other, bound in ((sW, dW, want["dW"][1].T), (sb, db, want["db"][1])):
+        one, other = host(one).astype(np.float64), host(other).astype(np.float64)
+        assert (np.abs(one - other) <= 2 * bound.ravel() + 2 * U * np.abs(other)).all()
 
 
 # ------------------------------------------------------------- differences
