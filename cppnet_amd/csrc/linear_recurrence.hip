@@ -22,6 +22,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "act_math.hpp"
 #include "common.hpp"
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
     mine = d < a.D && b < a.B && at < width;
   }
   const int stride = LAY == kStrided ? (int)(a.B < 64 ? a.B : 64) : 1;  // lanes from one step to the next
-  if (!mine) c = 0;
+  if (!mine) c = at = 0;  // reads what exists, writes nothing
   if (LAY != kStrided) b = c % a.B;
   else if (!mine) b = 0;
   const int64_t base = LAY == kStrided ? b + BS * (c / a.B) : a.S * c;  // the chain's first step
@@ -184,44 +185,65 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
     float f[U][E], x[U][E], i[U][E], hp[U][E], dh[U][E];
   };
   // position q0 + e in the order of the maps is step t
-  auto first_q = [&](int64_t r0, int u) {
-    return r0 + (int64_t)seat * span + (u * width + at) * E;
+  auto first_q = [&](int64_t r0, int u) { return r0 + (int64_t)seat * span + (u * width + at) * E; };
+  // Whether all of the wave's steps of a round exist and are within their lengths.  Its
+  // loads then go out one after the other; behind tests of their own each would be
+  // waited for.
+  auto is_whole = [&](int64_t r0) {
+    const int64_t w0 = r0 + (int64_t)seat * span;
+    return w0 + span <= q_end && __all(!mine || (BWD ? a.S - w0 <= len : w0 + span <= len));
   };
-  auto load = [&](int64_t r0, Raw& v) {
+  auto load = [&](int64_t r0, Raw& v, auto whole_tag) {
+    constexpr bool WHOLE = decltype(whole_tag)::value;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t q0 = first_q(r0, u);
       // the steps of these positions, [lo, lo + E)
       const int64_t lo = BWD ? a.S - E - q0 : q0;
-      const bool any = mine && q0 < q_end && lo < len;
-      auto get = [&](const float* p, float (&to)[E], int back) {
-        if (LAY != kStrided && any && q0 + 4 <= a.S && lo >= back) {
-          const f32x4 w = *reinterpret_cast<const f32x4u*>(p + base + lo - back);
+      const bool any = WHOLE || (mine && q0 < q_end && lo < len);
+      auto get = [&](const float* p, float (&to)[E], auto back_tag) {
+        constexpr int back = decltype(back_tag)::value;
+        if (LAY != kStrided && (WHOLE || (any && q0 + 4 <= a.S && lo >= back))) {
+          // (the state before step 0 is not read from here: the first chain's would lie before h)
+          const int64_t o = base + lo - back;
+          const bool edge = back && o < 0;
+          const f32x4 w = *reinterpret_cast<const f32x4u*>(p + (edge ? 0 : o));
 #pragma unroll
-          for (int e = 0; e < E; ++e) to[e] = w[BWD ? E - 1 - e : e];
+          for (int e = 0; e < E; ++e) to[e] = !BWD ? w[e] : edge && e + 1 < E ? w[E - 2 - e] : w[E - 1 - e];
         } else {
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const int64_t t = BWD ? a.S - 1 - (q0 + e) : q0 + e;
-            to[e] = any && t >= back && t < a.S ? p[base + step * (t - back)] : 0.f;
+            const int64_t t = BWD ? a.S - 1 - (q0 + e) : q0 + e, o = base + step * (t - back);
+            if (WHOLE) to[e] = p[back && o < 0 ? 0 : o];
+            else to[e] = any && t >= back && t < a.S ? p[o] : 0.f;
           }
         }
       };
-      get(a.f, v.f[u], 0);
-      if (!BWD || PASS != 1) get(a.x, v.x[u], 0);
-      if (IG && (!BWD || PASS != 1)) get(a.i, v.i[u], 0);
+      constexpr std::integral_constant<int, 0> now;
+      constexpr std::integral_constant<int, 1> before;
+      get(a.f, v.f[u], now);
+      if (!BWD || PASS != 1) get(a.x, v.x[u], now);
+      if (IG && (!BWD || PASS != 1)) get(a.i, v.i[u], now);
       if constexpr (BWD) {
-        get(a.dh, v.dh[u], 0);
-        if (PASS != 1) get(a.h, v.hp[u], 1);
+        get(a.dh, v.dh[u], now);
+        if (PASS != 1) get(a.h, v.hp[u], before);
       }
     }
   };
 
   Raw raw;
-  load(q_begin, raw);
+  bool whole_now = false, whole_next = false;
+  auto load_any = [&](int64_t r0) {
+    whole_next = is_whole(r0);
+    if (whole_next) load(r0, raw, std::true_type{});
+    else load(r0, raw, std::false_type{});
+  };
+  load_any(q_begin);
   Map whole = identity();  // PASS 1: of the rounds so far
+  const float first = BWD && PASS != 1 && a.h0 && mine ? a.h0[c] : 0.f;
   int parity = 0;
   for (int64_t r0 = q_begin; r0 < q_end; r0 += round, parity ^= 1) {
+    whole_now = whole_next;
     // forward: b = w x.  backward: b = dh, entered before the factor
     float p[U][E], l[U][E], y[U][E], w[U][E], off[U][E], wo[U][E], x[U][E], hp[U][E];
     Map m[U];
@@ -231,7 +253,7 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int64_t q = first_q(r0, u) + e, t = BWD ? a.S - 1 - q : q;
-        const bool in = q < q_end && t < len;
+        const bool in = whole_now || (q < q_end && t < len);
         gate(raw.f[u][e], p[u][e], off[u][e], l[u][e]);
         if (IG) {
           float none;
@@ -256,7 +278,7 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
         }
       }
     }
-    if (r0 + round < q_end) load(r0 + round, raw);
+    if (r0 + round < q_end) load_any(r0 + round);
     // m: of the lane's own steps -> of the chain's lanes up to this one; before: without it
     Map before[U], total[U];
 #pragma unroll
@@ -299,50 +321,55 @@ __global__ void __launch_bounds__(1024) recurrence_kernel(RecArgs a) {
       else state = apply(wave_map, state);
     }
     if constexpr (PASS == 1) continue;
+    auto finish = [&](auto whole_tag) {
+      constexpr bool WHOLE = decltype(whole_tag)::value;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float s = apply(before[u], enter);
-      enter = apply(total[u], enter);
-      const int64_t q0 = first_q(r0, u);
-      float o0[E], o1[E], o2[E];
+      for (int u = 0; u < U; ++u) {
+        float s = apply(before[u], enter);
+        enter = apply(total[u], enter);
+        const int64_t q0 = first_q(r0, u);
+        float o0[E], o1[E], o2[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int64_t q = q0 + e, t = BWD ? a.S - 1 - q : q;
-        const bool in = t < len;
+        for (int e = 0; e < E; ++e) {
+          const int64_t q = q0 + e, t = BWD ? a.S - 1 - q : q;
+          const bool in = WHOLE || t < len;
+          if constexpr (BWD) {
+            const float g = y[u][e] + s;
+            const float prev = t == 0 ? first : hp[u][e];
+            const float df = p[u][e] * off[u][e] * g;
+            o0[e] = in ? w[u][e] * g : 0.f;
+            o1[e] = in ? df * (IG ? prev : prev - x[u][e]) : 0.f;
+            if (IG) o2[e] = in ? w[u][e] * wo[u][e] * g * x[u][e] : 0.f;
+            s = fmaf(p[u][e], g, l[u][e] * g);
+          } else {
+            s = fmaf(p[u][e], s, fmaf(l[u][e], s, y[u][e]));
+            o0[e] = in ? s : 0.f;
+          }
+        }
+        if (!mine || (!WHOLE && q0 >= q_end)) continue;
+        auto put = [&](float* to, const float (&v)[E]) {
+          if (LAY != kStrided && (WHOLE || q0 + 4 <= q_end)) {
+            f32x4 w4;
+#pragma unroll
+            for (int e = 0; e < E; ++e) w4[BWD ? E - 1 - e : e] = v[e];
+            *reinterpret_cast<f32x4u*>(to + base + (BWD ? a.S - 4 - q0 : q0)) = w4;
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (WHOLE || q0 + e < q_end) to[base + step * (BWD ? a.S - 1 - (q0 + e) : q0 + e)] = v[e];
+          }
+        };
         if constexpr (BWD) {
-          const float g = y[u][e] + s;
-          const float prev = t == 0 ? (a.h0 && mine ? a.h0[c] : 0.f) : hp[u][e];
-          const float df = p[u][e] * off[u][e] * g;
-          o0[e] = in ? w[u][e] * g : 0.f;
-          o1[e] = in ? df * (IG ? prev : prev - x[u][e]) : 0.f;
-          if (IG) o2[e] = in ? w[u][e] * wo[u][e] * g * x[u][e] : 0.f;
-          s = fmaf(p[u][e], g, l[u][e] * g);
+          put(a.dx, o0);
+          put(a.df, o1);
+          if (IG) put(a.di, o2);
         } else {
-          s = fmaf(p[u][e], s, fmaf(l[u][e], s, y[u][e]));
-          o0[e] = in ? s : 0.f;
+          put(a.out, o0);
         }
       }
-      if (!mine || q0 >= q_end) continue;
-      auto put = [&](float* to, const float (&v)[E]) {
-        if (LAY != kStrided && q0 + 4 <= q_end) {
-          f32x4 w4;
-#pragma unroll
-          for (int e = 0; e < E; ++e) w4[BWD ? E - 1 - e : e] = v[e];
-          *reinterpret_cast<f32x4u*>(to + base + (BWD ? a.S - 4 - q0 : q0)) = w4;
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (q0 + e < q_end) to[base + step * (BWD ? a.S - 1 - (q0 + e) : q0 + e)] = v[e];
-        }
-      };
-      if constexpr (BWD) {
-        put(a.dx, o0);
-        put(a.df, o1);
-        if (IG) put(a.di, o2);
-      } else {
-        put(a.out, o0);
-      }
-    }
+    };
+    if (whole_now) finish(std::true_type{});
+    else finish(std::false_type{});
   }
   if (!mine || seat || at) return;
   if (PASS == 1) {

@@ -221,8 +221,10 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_gamma_kernel(NormArgs a
 
 // ---- tiles
 // 2^shift lanes along the rows, 4 rows each, and K times (1024 >> shift) columns.
-// Row tiles lie side by side in the order of the blocks.
-template <int K>
+// Row tiles lie side by side in the order of the blocks.  WHOLE: all of the tile's rows
+// and columns exist, and every thread's loads go out one after the other (behind the
+// tests of a ragged tile each would be waited for).
+template <int K, bool WHOLE>
 struct TileSeat {
   int64_t n, f0, base;  // the lane's first row; the wave's first column, its first element
   int64_t step;
@@ -241,15 +243,15 @@ struct TileSeat {
     base = n0 + a.N * f0;
     step = a.N * cols;
     j = (uint32_t)row + (uint32_t)a.N * lane_f;
-    left = n + 4 <= a.N ? 4 : n < a.N ? (int)(a.N - n) : 0;
+    left = WHOLE || n + 4 <= a.N ? 4 : n < a.N ? (int)(a.N - n) : 0;
   }
-  __device__ __forceinline__ bool has(int k, int64_t F) const { return f0 + (int64_t)k * cols + lane_f < F; }
+  __device__ __forceinline__ bool has(int k, int64_t F) const { return WHOLE || f0 + (int64_t)k * cols + lane_f < F; }
   __device__ __forceinline__ int64_t at(int k) const { return base + k * step; }
   __device__ __forceinline__ f32x4 get(const float* p, int k, int64_t F) const {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (!has(k, F)) return v;
     const float* q = p + at(k) + j;
-    if (left == 4) return f32x4(*reinterpret_cast<const f32x4u*>(q));
+    if (WHOLE || left == 4) return f32x4(*reinterpret_cast<const f32x4u*>(q));
 #pragma unroll
     for (int e = 0; e < 3; ++e)
       if (e < left) v[e] = q[e];
@@ -258,7 +260,7 @@ struct TileSeat {
   __device__ __forceinline__ void put(float* p, int k, int64_t F, const f32x4& v) const {
     if (!has(k, F)) return;
     float* q = p + at(k) + j;
-    if (left == 4) {
+    if (WHOLE || left == 4) {
       *reinterpret_cast<f32x4u*>(q) = v;
       return;
     }
@@ -317,11 +319,16 @@ __device__ __forceinline__ void all_sums(const NormArgs& a, const Seat_& t, doub
   }
 }
 
-template <int K, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_sum_kernel(NormArgs a) {
+template <int K>
+__device__ __forceinline__ bool whole_tile(const NormArgs& a, int bid) {
+  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)K * (kNormThreads >> a.shift);
+  return (bid % a.row_tiles + 1) * rows <= a.N && (bid / a.row_tiles + 1) * cols <= a.F;
+}
+
+template <int K, bool DROP, bool WHOLE>
+__device__ __forceinline__ void rms_norm_sum_tile(const NormArgs& a, double (*lds)[256]) {
 #pragma clang fp contract(off)
-  __shared__ double lds[kNormWaves][256];
-  const TileSeat<K> t(a, (int)blockIdx.x);
+  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
   const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
   f32x4 s[K], r[K];
 #pragma unroll
@@ -340,12 +347,17 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_sum_kernel(NormArgs a) 
   }
   leave_sums(a, t, q, lds);
 }
-
 template <int K, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_apply_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads) rms_norm_sum_kernel(NormArgs a) {
+  __shared__ double lds[kNormWaves][256];
+  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_sum_tile<K, DROP, true>(a, lds);
+  else rms_norm_sum_tile<K, DROP, false>(a, lds);
+}
+
+template <int K, bool DROP, bool WHOLE>
+__device__ __forceinline__ void rms_norm_apply_tile(const NormArgs& a, double (*lds)[256]) {
 #pragma clang fp contract(off)
-  __shared__ double lds[4][256];
-  const TileSeat<K> t(a, (int)blockIdx.x);
+  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
   f32x4 s[K];
   if (a.sum) {
 #pragma unroll
@@ -375,12 +387,17 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_apply_kernel(NormArgs a
     t.put(a.y, k, a.F, (s[k] * rstd) * g);
   }
 }
+template <int K, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_apply_kernel(NormArgs a) {
+  __shared__ double lds[4][256];
+  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_apply_tile<K, DROP, true>(a, lds);
+  else rms_norm_apply_tile<K, DROP, false>(a, lds);
+}
 
 // First of the backward: the sums of d n over a tile's columns and of dy n over its rows.
-template <int K>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_dots_kernel(NormArgs a) {
-  __shared__ double lds[kNormWaves][256];
-  const TileSeat<K> t(a, (int)blockIdx.x);
+template <int K, bool WHOLE>
+__device__ __forceinline__ void rms_norm_dots_tile(const NormArgs& a, double (*lds)[256]) {
+  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
   f32x4 u[K], d[K], rstd = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -406,17 +423,17 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_dots_kernel(NormArgs a)
   }
   leave_sums(a, t, q, lds);
 }
+template <int K>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_dots_kernel(NormArgs a) {
+  __shared__ double lds[kNormWaves][256];
+  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_dots_tile<K, true>(a, lds);
+  else rms_norm_dots_tile<K, false>(a, lds);
+}
 
 // Second: dx and dresidual; the blocks behind the tiles join dgamma.
-template <int K, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_grad_kernel(NormArgs a) {
-  __shared__ double lds[4][256];
-  const int tiles = a.row_tiles * a.col_tiles;
-  if ((int)blockIdx.x >= tiles) {
-    join_gamma(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
-    return;
-  }
-  const TileSeat<K> t(a, (int)blockIdx.x);
+template <int K, bool DROP, bool WHOLE>
+__device__ __forceinline__ void rms_norm_grad_tile(const NormArgs& a, double (*lds)[256]) {
+  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
   const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
   f32x4 u[K], d[K], p[K], rstd = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -445,6 +462,17 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_grad_kernel(NormArgs a)
     if (a.dresidual) t.put(a.dresidual, k, a.F, g);
     t.put(a.dx, k, a.F, DROP ? t.drop(a.drop, z0, k, g) : g);
   }
+}
+template <int K, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_grad_kernel(NormArgs a) {
+  __shared__ double lds[4][256];
+  const int tiles = a.row_tiles * a.col_tiles;
+  if ((int)blockIdx.x >= tiles) {
+    join_gamma(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
+    return;
+  }
+  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_grad_tile<K, DROP, true>(a, lds);
+  else rms_norm_grad_tile<K, DROP, false>(a, lds);
 }
 
 constexpr int kFewHeld = 16;  // features of a thread that a block of few rows holds
