@@ -10,7 +10,7 @@
 // Matrices are ColMajor [N, F]: the features of a row lie N apart.  A block that held
 // whole rows would read a line or two of every column, each on a page of its own:
 // 4097 x 4099, forward, 203 us in blocks of 16 rows for 81 here.  So the matrix goes
-// through in tiles of 256 rows x 64 or 128 columns, a KiB in a row of every column,
+// through in tiles of 256 rows x 32 or 64 columns, a KiB in a row of every column,
 // twice: the first launch leaves each tile's sums over its columns, the second joins
 // them and reads s (and dy) again, for the most part from the caches.  Where a few
 // rows are all there is, one launch does both and holds them in registers.  The sums
@@ -81,6 +81,7 @@ struct NormArgs {
 };
 
 constexpr int kNormThreads = 1024, kNormWaves = kNormThreads / 64;
+constexpr int kTileThreads = 512, kTileWaves = kTileThreads / 64;
 
 // 1 / sqrt(v) to fp32's precision and range.
 __device__ __forceinline__ float inv_sqrt(double v) {
@@ -200,27 +201,28 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_few_bwd_kernel(NormArgs
 }
 
 // dgamma (+)= the tiles' parts, in order: 64 features a block, its waves share the parts.
+template <int WAVES>
 __device__ __forceinline__ void join_gamma(const NormArgs& a, int64_t block, float (*sum)[64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t f = block * 64 + lane;
   float t = 0.f;
   if (f < a.F) {
 #pragma unroll 8
-    for (int b = wave; b < a.row_tiles; b += kNormWaves) t += a.gamma_part[(int64_t)b * a.F + f];
+    for (int b = wave; b < a.row_tiles; b += WAVES) t += a.gamma_part[(int64_t)b * a.F + f];
   }
   sum[wave][lane] = t;
   __syncthreads();
   if (wave || f >= a.F) return;
-  for (int w = 1; w < kNormWaves; ++w) t += sum[w][lane];
+  for (int w = 1; w < WAVES; ++w) t += sum[w][lane];
   a.dgamma[f] = a.accumulate ? a.dgamma[f] + t : t;
 }
 __global__ void __launch_bounds__(kNormThreads) rms_norm_gamma_kernel(NormArgs a) {
   __shared__ float sum[kNormWaves][64];
-  join_gamma(a, blockIdx.x, sum);
+  join_gamma<kNormWaves>(a, blockIdx.x, sum);
 }
 
 // ---- tiles
-// 2^shift lanes along the rows, 4 rows each, and K times (1024 >> shift) columns.
+// 2^shift lanes along the rows, 4 rows each, and K times (kTileThreads >> shift) columns.
 // Row tiles lie side by side in the order of the blocks.  WHOLE: all of the tile's rows
 // and columns exist, and every thread's loads go out one after the other (behind the
 // tests of a ragged tile each would be waited for).
@@ -234,7 +236,7 @@ struct TileSeat {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     tile_r = bid % a.row_tiles;
     tile_c = bid / a.row_tiles;
-    cols = kNormThreads >> a.shift;
+    cols = kTileThreads >> a.shift;
     row = 4 * (lane & ((1 << a.shift) - 1));
     lane_f = lane >> a.shift;
     const int64_t n0 = (int64_t)tile_r << (a.shift + 2);
@@ -295,14 +297,14 @@ __device__ __forceinline__ void leave_sums(const NormArgs& a, const Seat_& t, do
   if (r >= 4 * lanes || n >= a.N) return;
   double v = 0.0;
 #pragma unroll
-  for (int w = 0; w < kNormWaves; ++w) v += lds[w][r];
+  for (int w = 0; w < kTileWaves; ++w) v += lds[w][r];
   a.part[(int64_t)t.tile_c * a.N + n] = v;
 }
-// The sums over all columns of the thread's 4 rows; 1024 threads share them.
+// The sums over all columns of the thread's 4 rows; the threads share them out.
 template <class Seat_>
 __device__ __forceinline__ void all_sums(const NormArgs& a, const Seat_& t, double (&q)[4], double (*lds)[256]) {
   const int rows = 4 << a.shift, r = threadIdx.x & (rows - 1), g = threadIdx.x >> (a.shift + 2),
-            groups = kNormThreads >> (a.shift + 2);
+            groups = kTileThreads >> (a.shift + 2);
   const int64_t n = ((int64_t)t.tile_r << (a.shift + 2)) + r;
   double v = 0.0;
   if (n < a.N) {
@@ -321,7 +323,7 @@ __device__ __forceinline__ void all_sums(const NormArgs& a, const Seat_& t, doub
 
 template <int K>
 __device__ __forceinline__ bool whole_tile(const NormArgs& a, int bid) {
-  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)K * (kNormThreads >> a.shift);
+  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)K * (kTileThreads >> a.shift);
   return (bid % a.row_tiles + 1) * rows <= a.N && (bid / a.row_tiles + 1) * cols <= a.F;
 }
 
@@ -348,8 +350,8 @@ __device__ __forceinline__ void rms_norm_sum_tile(const NormArgs& a, double (*ld
   leave_sums(a, t, q, lds);
 }
 template <int K, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_sum_kernel(NormArgs a) {
-  __shared__ double lds[kNormWaves][256];
+__global__ void __launch_bounds__(kTileThreads) rms_norm_sum_kernel(NormArgs a) {
+  __shared__ double lds[kTileWaves][256];
   if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_sum_tile<K, DROP, true>(a, lds);
   else rms_norm_sum_tile<K, DROP, false>(a, lds);
 }
@@ -388,8 +390,8 @@ __device__ __forceinline__ void rms_norm_apply_tile(const NormArgs& a, double (*
   }
 }
 template <int K, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_apply_kernel(NormArgs a) {
-  __shared__ double lds[4][256];
+__global__ void __launch_bounds__(kTileThreads) rms_norm_apply_kernel(NormArgs a) {
+  __shared__ double lds[kTileThreads / 256][256];
   if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_apply_tile<K, DROP, true>(a, lds);
   else rms_norm_apply_tile<K, DROP, false>(a, lds);
 }
@@ -424,8 +426,8 @@ __device__ __forceinline__ void rms_norm_dots_tile(const NormArgs& a, double (*l
   leave_sums(a, t, q, lds);
 }
 template <int K>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_dots_kernel(NormArgs a) {
-  __shared__ double lds[kNormWaves][256];
+__global__ void __launch_bounds__(kTileThreads) rms_norm_dots_kernel(NormArgs a) {
+  __shared__ double lds[kTileWaves][256];
   if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_dots_tile<K, true>(a, lds);
   else rms_norm_dots_tile<K, false>(a, lds);
 }
@@ -464,11 +466,11 @@ __device__ __forceinline__ void rms_norm_grad_tile(const NormArgs& a, double (*l
   }
 }
 template <int K, bool DROP>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_grad_kernel(NormArgs a) {
-  __shared__ double lds[4][256];
+__global__ void __launch_bounds__(kTileThreads) rms_norm_grad_kernel(NormArgs a) {
+  __shared__ double lds[kTileThreads / 256][256];
   const int tiles = a.row_tiles * a.col_tiles;
   if ((int)blockIdx.x >= tiles) {
-    join_gamma(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
+    join_gamma<kTileWaves>(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
     return;
   }
   if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_grad_tile<K, DROP, true>(a, lds);
@@ -476,7 +478,9 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_grad_kernel(NormArgs a)
 }
 
 constexpr int kFewHeld = 16;  // features of a thread that a block of few rows holds
-constexpr int kTileCols = 4;  // columns of a thread in a tile (8 in the forward of many tiles)
+// Columns of a thread in a tile; twice as many where there are 512 tiles of that size
+// (8192 x 512 both ways 46 us, with 8 throughout 52; 4097 x 4099 177 us, with 4 212).
+constexpr int kTileCols = 4;
 
 // Few rows: up to 32, as many as a block holds.
 bool few_rows(NormArgs& a) {
@@ -487,15 +491,17 @@ bool few_rows(NormArgs& a) {
   return true;
 }
 
-// The tiles of K columns a thread; their number is checked by the caller.
-int64_t set_tiles(NormArgs& a, int K) {
+// The tiles, and how many columns a thread has in one.
+int set_tiles(NormArgs& a) {
   a.shift = 0;
   while (((int64_t)4 << a.shift) < a.N && a.shift < 6) ++a.shift;
-  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)K * (kNormThreads >> a.shift);
+  const int64_t rows = (int64_t)4 << a.shift;
   a.row_tiles = (int)((a.N + rows - 1) / rows);
-  const int64_t c = (a.F + cols - 1) / cols;
-  a.col_tiles = (int)c;
-  return a.row_tiles * c;
+  for (int K = 2 * kTileCols;; K = kTileCols) {
+    const int64_t cols = (int64_t)K * (kTileThreads >> a.shift);
+    a.col_tiles = (int)((a.F + cols - 1) / cols);
+    if (K == kTileCols || (int64_t)a.row_tiles * a.col_tiles >= 512) return K;
+  }
 }
 
 template <bool DROP>
@@ -507,19 +513,18 @@ int run_forward(NormArgs& a, hipStream_t st, const char* who) {
     else hipLaunchKernelGGL((rms_norm_few_fwd_kernel<kFewHeld, DROP>), dim3(1), threads, 0, st, a);
     return check_launch(who);
   }
-  int K = 2 * kTileCols;
-  if (set_tiles(a, K) < 512) set_tiles(a, K = kTileCols);
+  const int K = set_tiles(a);
   const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles;
   CNHIP_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too large", who);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, (size_t)a.col_tiles * (size_t)a.N * sizeof(double), &ws, who));
   a.part = static_cast<double*>(ws);
-  const dim3 grid((unsigned)tiles);
-  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_sum_kernel<kTileCols, DROP>), grid, threads, 0, st, a);
-  else hipLaunchKernelGGL((rms_norm_sum_kernel<2 * kTileCols, DROP>), grid, threads, 0, st, a);
+  const dim3 grid((unsigned)tiles), tile_threads(kTileThreads);
+  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_sum_kernel<kTileCols, DROP>), grid, tile_threads, 0, st, a);
+  else hipLaunchKernelGGL((rms_norm_sum_kernel<2 * kTileCols, DROP>), grid, tile_threads, 0, st, a);
   CNHIP_TRY(check_launch(who));
-  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_apply_kernel<kTileCols, DROP>), grid, threads, 0, st, a);
-  else hipLaunchKernelGGL((rms_norm_apply_kernel<2 * kTileCols, DROP>), grid, threads, 0, st, a);
+  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_apply_kernel<kTileCols, DROP>), grid, tile_threads, 0, st, a);
+  else hipLaunchKernelGGL((rms_norm_apply_kernel<2 * kTileCols, DROP>), grid, tile_threads, 0, st, a);
   return check_launch(who);
 }
 
@@ -528,7 +533,8 @@ int run_backward(NormArgs& a, hipStream_t st, const char* who) {
   const dim3 threads(kNormThreads);
   const bool few = few_rows(a);
   a.row_tiles = a.col_tiles = 1;
-  const int64_t tiles = few ? 1 : set_tiles(a, kTileCols), gamma_blocks = (a.F + 63) / 64;
+  const int K = few ? 0 : set_tiles(a);
+  const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles, gamma_blocks = (a.F + 63) / 64;
   CNHIP_REQUIRE(tiles + gamma_blocks < ((int64_t)1 << 31), "%s: too large", who);
   const size_t sums = few ? 0 : (size_t)a.col_tiles * (size_t)a.N * sizeof(double);
   void* ws = nullptr;
@@ -543,9 +549,12 @@ int run_backward(NormArgs& a, hipStream_t st, const char* who) {
     hipLaunchKernelGGL(rms_norm_gamma_kernel, dim3((unsigned)gamma_blocks), threads, 0, st, a);
     return check_launch(who);
   }
-  hipLaunchKernelGGL(rms_norm_dots_kernel<kTileCols>, dim3((unsigned)tiles), threads, 0, st, a);
+  const dim3 grid((unsigned)tiles), more((unsigned)(tiles + gamma_blocks)), tile_threads(kTileThreads);
+  if (K == kTileCols) hipLaunchKernelGGL(rms_norm_dots_kernel<kTileCols>, grid, tile_threads, 0, st, a);
+  else hipLaunchKernelGGL(rms_norm_dots_kernel<2 * kTileCols>, grid, tile_threads, 0, st, a);
   CNHIP_TRY(check_launch(who));
-  hipLaunchKernelGGL((rms_norm_grad_kernel<kTileCols, DROP>), dim3((unsigned)(tiles + gamma_blocks)), threads, 0, st, a);
+  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_grad_kernel<kTileCols, DROP>), more, tile_threads, 0, st, a);
+  else hipLaunchKernelGGL((rms_norm_grad_kernel<2 * kTileCols, DROP>), more, tile_threads, 0, st, a);
   return check_launch(who);
 }
 
