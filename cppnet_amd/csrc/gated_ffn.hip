@@ -30,6 +30,12 @@ struct FfnScales {
   uint32_t w, x, z;
 };
 // What the blocks that look for them found: of W, X and dZ.
+// The forward's epilogue is as long as many of its steps, so it runs in half tiles, two
+// to a CU (8192 x 1024 -> 4096, GELU, no Z: 459 us in both; 1021 x 513 -> 1365 38.8 us
+// in half tiles and 44.6 in whole ones, 300 rows 32.3 and 35.1); the backward in whole
+// ones (half tiles across the rows of both operands need more registers than there are).
+using Half = pr::Tile<2>;
+using Whole = pr::Tile<4>;
 constexpr int kMaxBlocks[3] = {256, 256, 512};
 constexpr int kMaxAt[3] = {0, 256, 512}, kMaxParts = 1024;
 
@@ -92,10 +98,11 @@ __device__ __forceinline__ void gate_both(int act, float z, float& y, float& d) 
 
 // ------------------------------------------------------------------ forward
 // X and W^T packed, every row of X and every 32 rows of W^T with an exponent of
-// their own: a block of eight waves for 32 rows, which reads them twice (the
-// second time from the L2).
-__global__ void __launch_bounds__(512) ffn_pack_own_kernel(FfnArgs a, int w_blocks) {
-  __shared__ uint32_t part[8][32];
+// their own: a block of sixteen waves for 32 rows, which keep their first kHeld steps
+// and read the others twice (the second time from the L2).
+__global__ void __launch_bounds__(1024) ffn_pack_own_kernel(FfnArgs a, int w_blocks) {
+  constexpr int kHeld = 4;
+  __shared__ uint32_t part[16][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
   const bool w = (int)blockIdx.x < w_blocks;
   const int64_t blk = w ? blockIdx.x : (int64_t)blockIdx.x - w_blocks, row = blk * 32 + r;
@@ -103,7 +110,10 @@ __global__ void __launch_bounds__(512) ffn_pack_own_kernel(FfnArgs a, int w_bloc
   const bool in = w ? col >= 0 : row < a.N;
   auto load = [&](int step, float (&x)[8]) {
     const int64_t d0 = step * 16 + 8 * h;
-    if (w) {
+    if (step >= a.steps_d) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    } else if (w) {
       const float* p = a.W + col * a.D + d0;
       if (in && d0 + 8 <= a.D) {
         const f32x4 lo = *reinterpret_cast<const f32x4u*>(p), hi = *reinterpret_cast<const f32x4u*>(p + 4);
@@ -122,16 +132,19 @@ __global__ void __launch_bounds__(512) ffn_pack_own_kernel(FfnArgs a, int w_bloc
     }
   };
   uint32_t m = 0;
-  for (int s0 = wave; s0 < a.steps_d; s0 += 32) {
-    float x[4][8];
+  float held[kHeld][8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (s0 + 8 * u < a.steps_d) load(s0 + 8 * u, x[u]);
-      else
-        for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
-    }
+  for (int u = 0; u < kHeld; ++u) load(wave + 16 * u, held[u]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+  for (int u = 0; u < kHeld; ++u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, pr::finite_bits(held[u][e]));
+  for (int s0 = wave + 16 * kHeld; s0 < a.steps_d; s0 += 32) {
+    float x[2][8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load(s0 + 16 * u, x[u]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = max(m, pr::finite_bits(x[u][e]));
   }
@@ -140,41 +153,47 @@ __global__ void __launch_bounds__(512) ffn_pack_own_kernel(FfnArgs a, int w_bloc
   if (lane < 32) part[wave][lane] = m;
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < 8; ++q) m = max(m, part[q][r]);
+  for (int q = 0; q < 16; ++q) m = max(m, part[q][r]);
   const int exp = pr::scale_exp(m);
   const float f = pr::exp2i(exp);
   if (wave == 0 && lane < 32) {
     if (!w && in) a.xe[row] = exp;
     if (w && lane == 0) a.we[blk] = exp;
   }
-  for (int step = wave; step < a.steps_d; step += 8) {
-    float x[8];
-    load(step, x);
+  auto put = [&](int step, float (&x)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= f;
     pr::put_frag(w ? a.wp : a.xp, blk, a.steps_d, step, x);
+  };
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (wave + 16 * u < a.steps_d) put(wave + 16 * u, held[u]);
+  for (int step = wave + 16 * kHeld; step < a.steps_d; step += 16) {
+    float x[8];
+    load(step, x);
+    put(step, x);
   }
 }
 
 // A: W^T (M: packed columns), B: X (N: rows); H and, where it is kept, Z.
-__global__ void __launch_bounds__(pr::GNT, 2) ffn_forward_kernel(pr::GemmArgs g, FfnArgs a, float* part) {
-  __shared__ __align__(16) char lds[pr::kGemmLds];
+__global__ void __launch_bounds__(Half::NT, 2) ffn_forward_kernel(pr::GemmArgs g, FfnArgs a, float* part) {
+  __shared__ __align__(16) char lds[Half::kLds];
   int tm, tn;
-  pr::tile_of((int)blockIdx.x, (g.M + pr::TM - 1) / pr::TM, (g.N + pr::TN - 1) / pr::TN, tm, tn);
+  pr::tile_of((int)blockIdx.x, (g.M + pr::TM - 1) / pr::TM, (g.N + Half::TN - 1) / Half::TN, tm, tn);
   pr::Acc acc;
   const int t0 = (int)blockIdx.y * g.steps_per_split;
-  pr::gemm_tile<false, false>(g, tm, tn, t0, min(g.steps, t0 + g.steps_per_split), lds, acc);
+  pr::gemm_tile<false, false, Half>(g, tm, tn, t0, min(g.steps, t0 + g.steps_per_split), lds, acc);
   if (part) {
-    pr::put_tile<false>(acc, tm, tn, g.M, g.N, part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float x) { return x; });
+    pr::put_tile<false, Half>(acc, tm, tn, g.M, g.N, part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float x) { return x; });
     return;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int block0 = tm * (pr::TM / 32) + (wave >> 2) * 4;  // the wave's first of 32 packed columns: a gate's
+  const int block0 = tm * (pr::TM / 32) + (wave / Half::WN) * 4;  // the wave's first of 32 packed columns: a gate's
   int64_t n[2];
   int ex[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    n[j] = (int64_t)tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
+    n[j] = (int64_t)tn * Half::TN + (wave % Half::WN) * 64 + 32 * j + (lane & 31);
     ex[j] = a.xe[n[j] < a.N ? n[j] : a.N - 1];
   }
 #pragma unroll
@@ -363,27 +382,23 @@ __global__ void __launch_bounds__(1024) ffn_max_kernel(FfnArgs a) {
     const int step_cols = step / chunks, step_chunks = step % chunks;
     int64_t col = (bid * 16 + wave) / chunks;
     int chunk = (bid * 16 + wave) % chunks;
+    // behind the last rows the last four again, so that no load stands behind a test of its
+    // own and is waited for (a piece of fewer than four rows: one row a lane)
     auto get = [&](const float* p, int n) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      if (n + 4 <= a.R) return f32x4(*reinterpret_cast<const f32x4u*>(p + n));
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < a.R) x[e] = p[n + e];
-      return x;
+      if (a.R >= 4) return f32x4(*reinterpret_cast<const f32x4u*>(p + (n + 4 <= a.R ? n : a.R - 4)));
+      const float x = p[n < a.R ? n : 0];
+      return f32x4{x, x, x, x};
     };
     while (col < cols) {
       f32x4 x[U], y[U], z[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int n = chunk * 256 + 4 * lane;
-        x[u] = y[u] = z[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (col < cols) {
-          const int64_t at = a.row0 + a.N * col;
-          x[u] = get((kind == 1 ? a.X : a.Z) + at, n);
-          if (kind == 2) {
-            y[u] = get(a.Z + a.N * a.F + at, n);
-            z[u] = get(a.dH + at, n);
-          }
+        const int n = chunk * 256 + (a.R >= 4 ? 4 * lane : lane);
+        const int64_t at = a.row0 + a.N * (col < cols ? col : cols - 1);
+        x[u] = get((kind == 1 ? a.X : a.Z) + at, n);
+        if (kind == 2) {
+          y[u] = get(a.Z + a.N * a.F + at, n);
+          z[u] = get(a.dH + at, n);
         }
         col += step_cols;
         chunk += step_chunks;
@@ -538,29 +553,29 @@ __device__ __forceinline__ void ffn_product(const FfnProduct& p, const FfnArgs& 
   const FfnOut& o = p.o;
   int tm, tn;
   const int split = bid / p.tiles;
-  pr::tile_of(bid % p.tiles, (g.M + pr::TM - 1) / pr::TM, (g.N + pr::TN - 1) / pr::TN, tm, tn);
+  pr::tile_of(bid % p.tiles, (g.M + pr::TM - 1) / pr::TM, (g.N + Whole::TN - 1) / Whole::TN, tm, tn);
   const int t0 = split * g.steps_per_split, t1 = min(g.steps, t0 + g.steps_per_split);
   pr::Acc acc;
-  pr::gemm_tile<TA, TB>(g, tm, tn, t0, t1, lds, acc);
+  pr::gemm_tile<TA, TB, Whole>(g, tm, tn, t0, t1, lds, acc);
   if (o.part) {
-    pr::put_tile<false>(acc, tm, tn, g.M, g.N, o.part + (int64_t)split * g.M * g.N, g.N, [](float x) { return x; });
+    pr::put_tile<false, Whole>(acc, tm, tn, g.M, g.N, o.part + (int64_t)split * g.M * g.N, g.N, [](float x) { return x; });
     return;
   }
   const int eo = scale_out<COLS>(a);
   auto value = [&](float x) { return pr::times_exp2(x, eo); };
   if constexpr (!COLS) {
-    pr::put_tile<false>(acc, tm, tn, g.M, g.N, o.p, o.ld, value);
+    pr::put_tile<false, Whole>(acc, tm, tn, g.M, g.N, o.p, o.ld, value);
   } else {
     // blocks of 32 packed columns lie together in the output: the even ones from its
     // start on, the odd ones from column F on
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int n = tn * pr::TN + (wave & 3) * 64 + 32 * j + (lane & 31);
+      const int n = tn * Whole::TN + (wave % Whole::WN) * 64 + 32 * j + (lane & 31);
       if (n >= g.N) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t blk = (int64_t)tm * (pr::TM / 32) + (wave >> 2) * 4 + i;
+        const int64_t blk = (int64_t)tm * (pr::TM / 32) + (wave / Whole::WN) * 4 + i;
         const int64_t f = (blk >> 1) * 32 + 4 * (lane >> 5), left = a.F - f;
         float* q = o.p + n + o.ld * (f + (blk & 1) * a.F);
         auto row = [](int e) { return 8 * (e / 4) + e % 4; };
@@ -583,8 +598,8 @@ __device__ __forceinline__ void ffn_product(const FfnProduct& p, const FfnArgs& 
 
 // Both products, and db (+)= the sums of the groups of rows, in order, in the blocks
 // behind them.
-__global__ void __launch_bounds__(pr::GNT, 2) ffn_grads_kernel(FfnArgs a, FfnProduct x, FfnProduct w, float* db, int add) {
-  __shared__ __align__(16) char lds[pr::kGemmLds];
+__global__ void __launch_bounds__(Whole::NT, 2) ffn_grads_kernel(FfnArgs a, FfnProduct x, FfnProduct w, float* db, int add) {
+  __shared__ __align__(16) char lds[Whole::kLds];
   int bid = (int)blockIdx.x;
   if (bid < x.tiles * x.splits) {
     ffn_product<true, false, false>(x, a, bid, lds);
@@ -596,7 +611,7 @@ __global__ void __launch_bounds__(pr::GNT, 2) ffn_grads_kernel(FfnArgs a, FfnPro
     return;
   }
   bid -= w.tiles * w.splits;
-  const int64_t v = (int64_t)bid * pr::GNT + threadIdx.x, blocks = (a.R + 31) / 32;
+  const int64_t v = (int64_t)bid * Whole::NT + threadIdx.x, blocks = (a.R + 31) / 32;
   if (v >= 2 * a.F) return;
   float s = 0.f;
 #pragma unroll 16
@@ -630,7 +645,10 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(FfnArgs a, FfnProduct x
   }
 }
 
-int64_t tiles_of(int64_t M, int64_t N) { return (M + pr::TM - 1) / pr::TM * ((N + pr::TN - 1) / pr::TN); }
+template <class T>
+int64_t tiles_of(int64_t M, int64_t N) {
+  return (M + pr::TM - 1) / pr::TM * ((N + T::TN - 1) / T::TN);
+}
 int64_t pad32(int64_t n) { return (n + 31) / 32 * 32; }
 
 struct Places {
@@ -650,15 +668,18 @@ int check_shape(int64_t N, int64_t D, int64_t F, int act, const char* who) {
   return CNHIP_OK;
 }
 
-// Steps of a block of a product that runs beside another one, so that all blocks
-// together are done soonest: rounds of 256 blocks, a block's own time and about 8 steps
-// for its beginning and end, and what the split sums move.
+// Steps of a block where all the products of a launch are done soonest: the rounds of
+// blocks that run together, a block's own time with what its beginning and end take,
+// and what split sums move.  Half tiles: one on a CU takes half the time of two.
 struct Job {
   int64_t M, N;
   int steps;
 };
+template <class T>
 int steps_of(const Job* jobs, int n) {
-  constexpr double kStepUs = 1.55, kBytesUs = 5e6;
+  constexpr bool kHalf = T::WN == 2;
+  constexpr double kStepUs = kHalf ? 1.2 : 1.55, kEnds = kHalf ? 6 : 8, kBytesUs = kHalf ? 8e6 : 5e6;
+  constexpr int64_t kSlots = kHalf ? 512 : 256;
   int longest = 2, best = 0;
   for (int i = 0; i < n; ++i) longest = jobs[i].steps > longest ? jobs[i].steps : longest;
   double least = 0;
@@ -669,10 +690,11 @@ int steps_of(const Job* jobs, int n) {
     double moved = 0;
     for (int i = 0; i < n; ++i) {
       const int64_t splits = (jobs[i].steps + per - 1) / per;
-      blocks += tiles_of(jobs[i].M, jobs[i].N) * splits;
+      blocks += tiles_of<T>(jobs[i].M, jobs[i].N) * splits;
       if (splits > 1) moved += 8.0 * (double)splits * (double)jobs[i].M * (double)jobs[i].N;
     }
-    const double us = (double)((blocks + 255) / 256) * (per + 8) * kStepUs + moved / kBytesUs + (moved > 0 ? 3.0 : 0.0);
+    const double rounds = kHalf && blocks <= 256 ? 0.625 : (double)((blocks + kSlots - 1) / kSlots);
+    const double us = rounds * (per + kEnds) * kStepUs + moved / kBytesUs + (moved > 0 ? 3.0 : 0.0);
     if (best == 0 || us < least) {
       least = us;
       best = per;
@@ -691,12 +713,13 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
     return check_launch(who);
   }
   a.steps_d = (int)(pad32(D) / 16);
-  CNHIP_REQUIRE(tiles_of(2 * Fp, N) < ((int64_t)1 << 31), "%s: too large", who);
+  CNHIP_REQUIRE(tiles_of<Half>(2 * Fp, N) < ((int64_t)1 << 31), "%s: too large", who);
   Places w;
   const size_t o_x = w.place((size_t)(pad32(N) * pad32(D)) * 4), o_w = w.place((size_t)(2 * Fp * pad32(D)) * 4),
                o_xe = w.place((size_t)N * 4), o_we = w.place((size_t)(2 * Fp / 32) * 4);
   const Job job{2 * Fp, N, a.steps_d};
-  const int per = F < 65536 ? steps_of(&job, 1) : a.steps_d, splits = (a.steps_d + per - 1) / per;
+  // (a row of the grid for every feature joins the splits)
+  const int per = F < 65536 ? steps_of<Half>(&job, 1) : a.steps_d, splits = (a.steps_d + per - 1) / per;
   const size_t o_part = w.place(splits > 1 ? (size_t)(splits * 2 * Fp * N) * 4 : 0);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, w.at, &ws, who));
@@ -705,14 +728,14 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
   a.wp = base + o_w;
   a.xe = reinterpret_cast<int*>(base + o_xe);
   a.we = reinterpret_cast<int*>(base + o_we);
-  hipLaunchKernelGGL(ffn_pack_own_kernel, dim3((unsigned)(2 * Fp / 32 + pad32(N) / 32)), dim3(512), 0, st, a,
+  hipLaunchKernelGGL(ffn_pack_own_kernel, dim3((unsigned)(2 * Fp / 32 + pad32(N) / 32)), dim3(1024), 0, st, a,
                      (int)(2 * Fp / 32));
   CNHIP_TRY(check_launch(who));
   const pr::GemmArgs g{pr::Packed{a.wp, (int)(2 * Fp / 32), a.steps_d}, pr::Packed{a.xp, (int)(pad32(N) / 32), a.steps_d},
                        (int)(2 * Fp), (int)N, a.steps_d, per, a.steps_d / 2};
   float* part = splits > 1 ? reinterpret_cast<float*>(base + o_part) : nullptr;
-  hipLaunchKernelGGL(ffn_forward_kernel, dim3((unsigned)tiles_of(2 * Fp, N), (unsigned)splits), dim3(pr::GNT), 0, st, g, a,
-                     part);
+  hipLaunchKernelGGL(ffn_forward_kernel, dim3((unsigned)tiles_of<Half>(2 * Fp, N), (unsigned)splits), dim3(Half::NT), 0, st,
+                     g, a, part);
   CNHIP_TRY(check_launch(who));
   if (!part) return CNHIP_OK;
   hipLaunchKernelGGL(ffn_join_kernel, dim3((unsigned)((N + 255) / 256), (unsigned)F), dim3(256), 0, st, a, part, 2 * Fp,
@@ -731,12 +754,13 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
   if (R > N) R = N;
   const int64_t Rp = pad32(R);
   const Job jobs[2] = {{D, R, 2 * a.steps_f}, {2 * Fp, D, (int)(Rp / 16)}};
-  const int per = steps_of(jobs, 2);
+  const int per = steps_of<Whole>(jobs, 2);
   auto parts = [&](const Job& j) {
     const int64_t splits = (j.steps + per - 1) / per;
     return splits > 1 ? (size_t)(splits * j.M * j.N) * 4 : 0;
   };
-  CNHIP_REQUIRE(tiles_of(D, R) * ((2 * a.steps_f + per - 1) / per) + tiles_of(2 * Fp, D) * ((Rp / 16 + per - 1) / per) <
+  CNHIP_REQUIRE(tiles_of<Whole>(D, R) * ((2 * a.steps_f + per - 1) / per) +
+                        tiles_of<Whole>(2 * Fp, D) * ((Rp / 16 + per - 1) / per) <
                     ((int64_t)1 << 30),
                 "%s: too large", who);
   // blocks of 32 rows of dZ a wave: as many as leave 4096 waves, so that a wave that has
@@ -762,7 +786,7 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
                      float* part, int add) {
     const int splits = (steps + per - 1) / per;
     return FfnProduct{pr::GemmArgs{A, B, (int)M, (int)Nn, steps, per, steps / 2},
-                      FfnOut{p, ld, splits > 1 ? part : nullptr, add}, (int)tiles_of(M, Nn), splits};
+                      FfnOut{p, ld, splits > 1 ? part : nullptr, add}, (int)tiles_of<Whole>(M, Nn), splits};
   };
   for (int64_t r0 = 0; r0 < N; r0 += R) {
     a.row0 = r0;
@@ -785,8 +809,9 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
     const pr::Packed px_{a.xp, rb, a.steps_d}, pz_{a.zp, rb, 2 * a.steps_f};
     const FfnProduct x = product(pw_, pz_, D, a.R, 2 * a.steps_f, dX + r0, N, reinterpret_cast<float*>(base + o_px), 0),
                      y = product(pz_, px_, 2 * Fp, D, 2 * rb, dW, D, reinterpret_cast<float*>(base + o_pw), add);
-    const int64_t blocks = (int64_t)x.tiles * x.splits + (int64_t)y.tiles * y.splits + (db ? (2 * F + pr::GNT - 1) / pr::GNT : 0);
-    hipLaunchKernelGGL(ffn_grads_kernel, dim3((unsigned)blocks), dim3(pr::GNT), 0, st, a, x, y, db, add);
+    const int64_t blocks =
+        (int64_t)x.tiles * x.splits + (int64_t)y.tiles * y.splits + (db ? (2 * F + Whole::NT - 1) / Whole::NT : 0);
+    hipLaunchKernelGGL(ffn_grads_kernel, dim3((unsigned)blocks), dim3(Whole::NT), 0, st, a, x, y, db, add);
     CNHIP_TRY(check_launch(who));
     if (!x.o.part && !y.o.part) continue;
     const int64_t most_out = (x.o.part ? D * a.R : 0) > (y.o.part ? 2 * Fp * D : 0) ? D * a.R : 2 * Fp * D;

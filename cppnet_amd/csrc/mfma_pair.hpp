@@ -158,33 +158,44 @@ struct GemmArgs {
   int half;              // the step where the second half begins
 };
 
-constexpr int TM = 256, TN = 256, GNT = 512;
-constexpr int kStage = 2 * 16 * kFrag;  // one step of both operands: 8 fragments of two planes each
-constexpr int kStages = 4;
-constexpr int kGemmLds = kStages * kStage;
+// A block of 2 x WN waves takes a tile of 256 x 64 WN.  WN = 4: one block to a CU, with
+// four LDS buffers for the steps; WN = 2: two, with three each, of which one computes
+// while the other stores its tile.
+constexpr int TM = 256;
+template <int WN_>
+struct Tile {
+  static constexpr int WN = WN_, TN = 64 * WN, NT = 128 * WN;
+  static constexpr int A = 16, B = 4 * WN;           // pieces of 1024 bytes a step
+  static constexpr int kStage = (A + B) * kFrag;
+  static constexpr int kStages = WN == 4 ? 4 : 3;
+  static constexpr int kLds = kStages * kStage;
+  static constexpr int kCopies = (A + B) / (2 * WN);  // a wave's of a step
+  static_assert(WN == 2 || WN == 4, "waves along the columns");
+};
+constexpr int TN = Tile<4>::TN, GNT = Tile<4>::NT, kGemmLds = Tile<4>::kLds;
 
-// Staging of one operand: 16 pieces of 1024 bytes a step, two a wave.
+// Staging of one operand: PIECES pieces of 1024 bytes a step, PER a wave.
 //   TR false: piece j = plane j & 1 of the fragment of row block j / 2
 //   TR true (contraction along the packed rows): piece j = for the 16 output
 //     rows of packed step j, both planes of the 16 packed rows of this step:
 //     [plane][k half of 8][slot of the row][8 halves]
-template <bool TR>
+template <bool TR, int PIECES, int PER>
 struct Stage {
-  const char* src[2];
+  const char* src[PER];
   int64_t step;  // bytes per step (TR: per two steps)
-  int lds[2];
+  int lds[PER];
   __device__ __forceinline__ void init(const Packed& o, int tile) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int j = 2 * wave + u;
+    for (int u = 0; u < PER; ++u) {
+      const int j = PER * wave + u;
       lds[u] = j * kFrag;
       if (TR) {
-        const int s = min(tile * 16 + j, o.steps - 1);
+        const int s = min(tile * PIECES + j, o.steps - 1);
         src[u] = o.p + (int64_t)s * (2 * kFrag) + (lane >> 5) * kFrag + ((lane >> 4 & 1) * 32 + (lane & 15)) * 16;
         step = (int64_t)o.steps * (2 * kFrag);
       } else {
-        const int b = min(tile * 8 + (j >> 1), o.blocks - 1);
+        const int b = min(tile * (PIECES / 2) + (j >> 1), o.blocks - 1);
         src[u] = o.p + (int64_t)b * o.steps * (2 * kFrag) + (j & 1) * kFrag + lane * 16;
         step = 2 * kFrag;
       }
@@ -239,41 +250,44 @@ __device__ __forceinline__ void tile_of(int bid, int nm, int nn, int& tm, int& t
   tn = in / size;
 }
 
-// The contraction [t0, t1) of a 256 x 256 tile; the sums' sign is right.  The
-// steps go through four LDS buffers, three on their way while one is read;
+// The contraction [t0, t1) of a tile; the sums' sign is right.  The steps go
+// through four LDS buffers (three), three (two) on their way while one is read;
 // the fragments of the next step are read while this one's MFMAs run.
-template <bool TA, bool TB>
+template <bool TA, bool TB, class T = Tile<4>>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int t0, int t1, char* lds, Acc& acc) {
-  const int wave = threadIdx.x >> 6, wm = wave >> 2, wn = wave & 3;
-  Stage<TA> sa;
-  Stage<TB> sb;
+  constexpr int kStage = T::kStage, kStages = T::kStages, kCopies = T::kCopies, kBehind = T::A * kFrag;
+  constexpr int kOfA = T::A / (2 * T::WN), kSlots = 12 / kCopies;
+  const int wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+  Stage<TA, T::A, kOfA> sa;
+  Stage<TB, T::B, kCopies - kOfA> sb;
+  auto buffer = [&](int t) { return lds + (kStages == 4 ? t & 3 : (int)((unsigned)t % 3u)) * kStage; };
   sa.init(g.a, tm);
   sb.init(g.b, tn);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc.x[i][j] = f32x16{};
-  // piece u (0 .. 3) of step t's copies; past the last step the last is copied
-  // again, so that the wait counts stay the same
+  // piece u (0 .. kCopies - 1) of step t's copies; past the last step the last is
+  // copied again, so that the wait counts stay the same
   auto copy = [&](int t, int u) {
-    char* buf = lds + (t & (kStages - 1)) * kStage;
+    char* buf = buffer(t);
     const int s = t < t1 ? t : t1 - 1;
-    if (u < 2) sa.copy(s, u, buf);
-    else sb.copy(s, u - 2, buf + kStage / 2);
+    if (u < kOfA) sa.copy(s, u, buf);
+    else sb.copy(s, u - kOfA, buf + kBehind);
   };
   // fragment u (0 .. 11) of step t, in the order of their first use
   auto read = [&](int t, int odd, int u, Frags& f) {
-    const char* buf = lds + (t & (kStages - 1)) * kStage;
-    if (u < 2) f.b[u][0] = frag<TB>(buf + kStage / 2, 2 * wn + u, 0, odd);
+    const char* buf = buffer(t);
+    if (u < 2) f.b[u][0] = frag<TB>(buf + kBehind, 2 * wn + u, 0, odd);
     else if (u < 6) f.a[u - 2][1] = frag<TA>(buf, 4 * wm + u - 2, 1, odd);
-    else if (u < 8) f.b[u - 6][1] = frag<TB>(buf + kStage / 2, 2 * wn + u - 6, 1, odd);
+    else if (u < 8) f.b[u - 6][1] = frag<TB>(buf + kBehind, 2 * wn + u - 6, 1, odd);
     else f.a[u - 8][0] = frag<TA>(buf, 4 * wm + u - 8, 0, odd);
   };
   Frags f0, f1;
   auto step = [&](int t, int odd, Frags& now, Frags& next) {
-    // step t + 1 has arrived (two younger ones may be on their way), and every
+    // step t + 1 has arrived (the younger ones may be on their way), and every
     // wave holds step t in registers: its buffer is free
-    wait_and_meet<8>();
+    wait_and_meet<(kStages - 2) * kCopies>();
     if (t == g.half) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -291,15 +305,15 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
       for (int j = 0; j < 2; ++j)
         acc.x[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.a[i][x], now.b[j][y], acc.x[i][j], 0, 0, 0);
       read(t + 1, 1 - odd, u, next);
-      if (u % 3 == 0) copy(t + 4, u / 3);
+      if (u % kSlots == 0) copy(t + kStages, u / kSlots);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < kStages; ++t)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) copy(t0 + t, u);
-  wait_and_meet<12>();
+    for (int u = 0; u < kCopies; ++u) copy(t0 + t, u);
+  wait_and_meet<(kStages - 1) * kCopies>();
 #pragma unroll
   for (int u = 0; u < 12; ++u) read(t0, 0, u, f0);
   // t0 is even, so a step's parity, and with it the slots, is known here
@@ -319,14 +333,14 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
 // p[n + ld m] = value(element), or += for ADD, for the elements of a tile that
 // this lane holds and that exist.  ADD reads all of a column before it writes
 // one, so the reads are under way together.
-template <bool ADD, class F>
+template <bool ADD, class T = Tile<4>, class F>
 __device__ __forceinline__ void put_tile(const Acc& acc, int tm, int tn, int M, int N, float* __restrict__ p,
                                          int64_t ld, F&& value) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = tm * TM + (wave >> 2) * 128, m1 = m0 + 4 * (lane >> 5);
+  const int m0 = tm * TM + (wave / T::WN) * 128, m1 = m0 + 4 * (lane >> 5);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int n = tn * TN + (wave & 3) * 64 + 32 * j + (lane & 31);
+    const int n = tn * T::TN + (wave % T::WN) * 64 + 32 * j + (lane & 31);
     if (n >= N) continue;
     float* q = p + n + ld * m1;
     auto row = [](int i, int e) { return 32 * i + 8 * (e / 4) + e % 4; };
