@@ -409,20 +409,24 @@ int run(RecArgs& a, int rows, hipStream_t st, const char* who) {
     return launch<kShort, BWD, IG, 1>(a, dim3((unsigned)blocks), 256, st, who);
   }
   // Teams: what one wave (or the waves that share the steps) takes.  Their waves are as
-  // many as fill the chip several times over and as there are steps for.
+  // many as are resident with all teams (a CU holds 16 of these kernels) and as there are
+  // steps for, and no more than the rounds that this makes need.
   const int64_t teams = side ? a.chains : a.D * ((a.B + 63) / 64);
   const int width = side ? 64 : a.B > 32 ? 1 : (int)(64 / a.B);
   const int u = BWD || (side && a.S <= 256) ? 1 : 2;
   const int64_t span = (int64_t)u * 4 * width;
-  while (a.waves < kMostWaves && teams * a.waves * 2 <= 4096 && span * a.waves < a.S) a.waves *= 2;
-  const int64_t round = span * a.waves;
-  if (a.waves == kMostWaves && teams * a.waves < 2048 && a.S >= 2 * round) {
-    int64_t n = 2048 / (teams * a.waves), most = a.S / round;
-    if (n > most) n = most;
-    a.segment = ((a.S + n - 1) / n + round - 1) / round * round;
+  const int64_t per_cu = (teams + 255) / 256, most = per_cu < kMostWaves ? kMostWaves / per_cu : 1;
+  const int64_t rounds = (a.S + span * most - 1) / (span * most);
+  a.waves = (int)((a.S + span * rounds - 1) / (span * rounds));
+  const int64_t full = span * kMostWaves;
+  if (teams < 128 && a.S >= 2 * full) {  // half the chip would idle
+    a.waves = kMostWaves;
+    int64_t n = 128 / teams;
+    if (n > a.S / full) n = a.S / full;
+    a.segment = ((a.S + n - 1) / n + full - 1) / full * full;
     a.segments = (int)((a.S + a.segment - 1) / a.segment);
   }
-  const int block_waves = a.waves < 4 ? 4 : a.waves, per = block_waves / a.waves;
+  const int per = a.waves < 4 ? 4 / a.waves : 1, block_waves = per * a.waves;
   const int64_t blocks = (teams + per - 1) / per;
   CNHIP_REQUIRE(blocks < ((int64_t)1 << 31), "%s: too large", who);
   if (a.segments > 1) {
