@@ -510,7 +510,7 @@ def _call_on(t, name: str, *args) -> None:
     index = t.get_device()
     # torch.cuda.current_stream() makes an object of it: 2.5 us, of 9 for a small call
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():  # (torch.cuda.current_device() without its check of what t has shown)
         _capi.call(name, *args, stream)
         return
     with torch.cuda.device(index):

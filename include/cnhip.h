@@ -873,7 +873,7 @@ int cnhip_dropout_advance(uint64_t* counter, uint64_t n, cnhip_stream_t stream);
  * sum: the forward's (x itself where there was no residual and p = 0).  dsum: the
  * gradient that reaches s past the norm, NULL: none.  dresidual may be NULL; with
  * p = 0 it equals dx.  dx and dresidual are overwritten, dgamma is added to with
- * accumulate 1.  eps > 0, N < 2^28, F < 2^31. */
+ * accumulate 1.  eps > 0, N < 2^28, F < 2^24. */
 int cnhip_rms_norm_forward(const float* x, const float* residual, const float* gamma, float* y,
                            float* sum, float* rstd, int64_t N, int64_t F, float eps, float p,
                            uint64_t seed, uint64_t offset, const uint64_t* counter,
