@@ -10,7 +10,7 @@
 // Matrices are ColMajor [N, F]: the features of a row lie N apart.  A block that held
 // whole rows would read a line or two of every column, each on a page of its own:
 // 4097 x 4099, forward, 203 us in blocks of 16 rows for 81 here.  So the matrix goes
-// through in tiles of 256 rows x 32 or 64 columns, a KiB in a row of every column,
+// through in tiles of 256 rows x 32 columns and more, a KiB in a row of every column,
 // twice: the first launch leaves each tile's sums over its columns, the second joins
 // them and reads s (and dy) again, for the most part from the caches.  Where a few
 // rows are all there is, one launch does both and holds them in registers.  The sums
@@ -76,6 +76,7 @@ struct NormArgs {
   int accumulate;
   int shift;          // few rows: log2 of the rows of a block; tiles: of the lanes along the rows
   int row_tiles, col_tiles;
+  int chunks;         // times that a block of a tile goes through K columns a thread
   double* part;       // [col_tiles][N]: sums over a tile's columns
   float* gamma_part;  // [row_tiles][F]: sums over a tile's rows
 };
@@ -222,11 +223,13 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_gamma_kernel(NormArgs a
 }
 
 // ---- tiles
-// 2^shift lanes along the rows, 4 rows each, and K times (kTileThreads >> shift) columns.
+constexpr int K = 4;  // a thread's columns at a time
+// 2^shift lanes along the rows, 4 rows each, and chunks times K times (kTileThreads >>
+// shift) columns; what stays in registers is a chunk's.
 // Row tiles lie side by side in the order of the blocks.  WHOLE: all of the tile's rows
 // and columns exist, and every thread's loads go out one after the other (behind the
 // tests of a ragged tile each would be waited for).
-template <int K, bool WHOLE>
+template <bool WHOLE>
 struct TileSeat {
   int64_t n, f0, base;  // the lane's first row; the wave's first column, its first element
   int64_t step;
@@ -240,7 +243,7 @@ struct TileSeat {
     row = 4 * (lane & ((1 << a.shift) - 1));
     lane_f = lane >> a.shift;
     const int64_t n0 = (int64_t)tile_r << (a.shift + 2);
-    f0 = (int64_t)tile_c * (K * cols) + (int64_t)wave * (64 >> a.shift);
+    f0 = (int64_t)tile_c * a.chunks * (K * cols) + (int64_t)wave * (64 >> a.shift);
     n = n0 + row;
     base = n0 + a.N * f0;
     step = a.N * cols;
@@ -321,58 +324,62 @@ __device__ __forceinline__ void all_sums(const NormArgs& a, const Seat_& t, doub
   }
 }
 
-template <int K>
 __device__ __forceinline__ bool whole_tile(const NormArgs& a, int bid) {
-  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)K * (kTileThreads >> a.shift);
+  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)a.chunks * K * (kTileThreads >> a.shift);
   return (bid % a.row_tiles + 1) * rows <= a.N && (bid / a.row_tiles + 1) * cols <= a.F;
 }
 
-template <int K, bool DROP, bool WHOLE>
+template <bool DROP, bool WHOLE>
 __device__ __forceinline__ void rms_norm_sum_tile(const NormArgs& a, double (*lds)[256]) {
 #pragma clang fp contract(off)
-  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
+  const TileSeat<WHOLE> t(a, (int)blockIdx.x);
   const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
-  f32x4 s[K], r[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    s[k] = t.get(a.x, k, a.F);
-    if (a.residual) r[k] = t.get(a.residual, k, a.F);
-  }
   double q[4] = {};
+  for (int k0 = 0; k0 < a.chunks * K; k0 += K) {
+    f32x4 s[K], r[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (DROP) s[k] = t.drop(a.drop, z0, k, s[k]);
-    if (a.residual) s[k] = r[k] + s[k];
-    if (a.sum) t.put(a.sum, k, a.F, s[k]);
+    for (int k = 0; k < K; ++k) {
+      s[k] = t.get(a.x, k0 + k, a.F);
+      if (a.residual) r[k] = t.get(a.residual, k0 + k, a.F);
+    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = fma((double)s[k][e], (double)s[k][e], q[e]);
+    for (int k = 0; k < K; ++k) {
+      if (DROP) s[k] = t.drop(a.drop, z0, k0 + k, s[k]);
+      if (a.residual) s[k] = r[k] + s[k];
+      if (a.sum) t.put(a.sum, k0 + k, a.F, s[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = fma((double)s[k][e], (double)s[k][e], q[e]);
+    }
   }
   leave_sums(a, t, q, lds);
 }
-template <int K, bool DROP>
+template <bool DROP>
 __global__ void __launch_bounds__(kTileThreads) rms_norm_sum_kernel(NormArgs a) {
   __shared__ double lds[kTileWaves][256];
-  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_sum_tile<K, DROP, true>(a, lds);
-  else rms_norm_sum_tile<K, DROP, false>(a, lds);
+  if (whole_tile(a, (int)blockIdx.x)) rms_norm_sum_tile<DROP, true>(a, lds);
+  else rms_norm_sum_tile<DROP, false>(a, lds);
 }
 
-template <int K, bool DROP, bool WHOLE>
+template <bool DROP, bool WHOLE>
 __device__ __forceinline__ void rms_norm_apply_tile(const NormArgs& a, double (*lds)[256]) {
 #pragma clang fp contract(off)
-  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
+  const TileSeat<WHOLE> t(a, (int)blockIdx.x);
+  const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
   f32x4 s[K];
-  if (a.sum) {
+  auto get = [&](int k0) {
+    if (a.sum) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) s[k] = t.get(a.sum, k, a.F);
-  } else {
-    const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
+      for (int k = 0; k < K; ++k) s[k] = t.get(a.sum, k0 + k, a.F);
+    } else {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      s[k] = t.get(a.x, k, a.F);
-      if (DROP) s[k] = t.drop(a.drop, z0, k, s[k]);
-      if (a.residual) s[k] = t.get(a.residual, k, a.F) + s[k];
+      for (int k = 0; k < K; ++k) {
+        s[k] = t.get(a.x, k0 + k, a.F);
+        if (DROP) s[k] = t.drop(a.drop, z0, k0 + k, s[k]);
+        if (a.residual) s[k] = t.get(a.residual, k0 + k, a.F) + s[k];
+      }
     }
-  }
+  };
+  get(0);
   double q[4];
   all_sums(a, t, q, lds);
   f32x4 rstd;
@@ -383,67 +390,78 @@ __device__ __forceinline__ void rms_norm_apply_tile(const NormArgs& a, double (*
     for (int e = 0; e < 4; ++e)
       if (e < t.left) a.rstd[t.n + e] = rstd[e];
   }
+  for (int k0 = 0;;) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const float g = t.of_column(a.gamma, k, a.F);
-    t.put(a.y, k, a.F, (s[k] * rstd) * g);
+    for (int k = 0; k < K; ++k) {
+      const float g = t.of_column(a.gamma, k0 + k, a.F);
+      t.put(a.y, k0 + k, a.F, (s[k] * rstd) * g);
+    }
+    k0 += K;
+    if (k0 >= a.chunks * K) break;
+    get(k0);
   }
 }
-template <int K, bool DROP>
+template <bool DROP>
 __global__ void __launch_bounds__(kTileThreads) rms_norm_apply_kernel(NormArgs a) {
   __shared__ double lds[kTileThreads / 256][256];
-  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_apply_tile<K, DROP, true>(a, lds);
-  else rms_norm_apply_tile<K, DROP, false>(a, lds);
+  if (whole_tile(a, (int)blockIdx.x)) rms_norm_apply_tile<DROP, true>(a, lds);
+  else rms_norm_apply_tile<DROP, false>(a, lds);
 }
 
 // First of the backward: the sums of d n over a tile's columns and of dy n over its rows.
-template <int K, bool WHOLE>
+template <bool WHOLE>
 __device__ __forceinline__ void rms_norm_dots_tile(const NormArgs& a, double (*lds)[256]) {
-  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
-  f32x4 u[K], d[K], rstd = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    u[k] = t.get(a.s, k, a.F);
-    d[k] = t.get(a.dy, k, a.F);
-  }
+  const TileSeat<WHOLE> t(a, (int)blockIdx.x);
+  f32x4 rstd = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (e < t.left) rstd[e] = a.rstd[t.n + e];
   double q[4] = {};
+  for (int k0 = 0; k0 < a.chunks * K; k0 += K) {
+    f32x4 u[K], d[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const float g = t.of_column(a.gamma, k, a.F);
-    float dg = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float n = u[k][e] * rstd[e];
-      if (e < t.left) dg = fmaf(d[k][e], n, dg);
-      q[e] = fma((double)(d[k][e] * g), (double)n, q[e]);
+    for (int k = 0; k < K; ++k) {
+      u[k] = t.get(a.s, k0 + k, a.F);
+      d[k] = t.get(a.dy, k0 + k, a.F);
     }
-    for (int o = (1 << a.shift) >> 1; o > 0; o >>= 1) dg += __shfl_xor(dg, o, 64);
-    if (t.row == 0 && t.has(k, a.F)) (a.gamma_part + (int64_t)t.tile_r * a.F + t.f0 + (int64_t)k * t.cols)[t.lane_f] = dg;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float g = t.of_column(a.gamma, k0 + k, a.F);
+      float dg = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float n = u[k][e] * rstd[e];
+        if (e < t.left) dg = fmaf(d[k][e], n, dg);
+        q[e] = fma((double)(d[k][e] * g), (double)n, q[e]);
+      }
+      for (int o = (1 << a.shift) >> 1; o > 0; o >>= 1) dg += __shfl_xor(dg, o, 64);
+      if (t.row == 0 && t.has(k0 + k, a.F))
+        (a.gamma_part + (int64_t)t.tile_r * a.F + t.f0 + (int64_t)(k0 + k) * t.cols)[t.lane_f] = dg;
+    }
   }
   leave_sums(a, t, q, lds);
 }
-template <int K>
 __global__ void __launch_bounds__(kTileThreads) rms_norm_dots_kernel(NormArgs a) {
   __shared__ double lds[kTileWaves][256];
-  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_dots_tile<K, true>(a, lds);
-  else rms_norm_dots_tile<K, false>(a, lds);
+  if (whole_tile(a, (int)blockIdx.x)) rms_norm_dots_tile<true>(a, lds);
+  else rms_norm_dots_tile<false>(a, lds);
 }
 
 // Second: dx and dresidual; the blocks behind the tiles join dgamma.
-template <int K, bool DROP, bool WHOLE>
+template <bool DROP, bool WHOLE>
 __device__ __forceinline__ void rms_norm_grad_tile(const NormArgs& a, double (*lds)[256]) {
-  const TileSeat<K, WHOLE> t(a, (int)blockIdx.x);
+  const TileSeat<WHOLE> t(a, (int)blockIdx.x);
   const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
   f32x4 u[K], d[K], p[K], rstd = {0.f, 0.f, 0.f, 0.f};
+  auto get = [&](int k0) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    u[k] = t.get(a.s, k, a.F);
-    d[k] = t.get(a.dy, k, a.F);
-    if (a.dsum) p[k] = t.get(a.dsum, k, a.F);
-  }
+    for (int k = 0; k < K; ++k) {
+      u[k] = t.get(a.s, k0 + k, a.F);
+      d[k] = t.get(a.dy, k0 + k, a.F);
+      if (a.dsum) p[k] = t.get(a.dsum, k0 + k, a.F);
+    }
+  };
+  get(0);
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (e < t.left) rstd[e] = a.rstd[t.n + e];
@@ -452,20 +470,25 @@ __device__ __forceinline__ void rms_norm_grad_tile(const NormArgs& a, double (*l
   float c[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) c[e] = (float)(q[e] * a.inv_f);
+  for (int k0 = 0;;) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const float gamma = t.of_column(a.gamma, k, a.F);
-    f32x4 g;
+    for (int k = 0; k < K; ++k) {
+      const float gamma = t.of_column(a.gamma, k0 + k, a.F);
+      f32x4 g;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      g[e] = rstd[e] * fmaf(-(u[k][e] * rstd[e]), c[e], d[k][e] * gamma);
-      if (a.dsum) g[e] += p[k][e];
+      for (int e = 0; e < 4; ++e) {
+        g[e] = rstd[e] * fmaf(-(u[k][e] * rstd[e]), c[e], d[k][e] * gamma);
+        if (a.dsum) g[e] += p[k][e];
+      }
+      if (a.dresidual) t.put(a.dresidual, k0 + k, a.F, g);
+      t.put(a.dx, k0 + k, a.F, DROP ? t.drop(a.drop, z0, k0 + k, g) : g);
     }
-    if (a.dresidual) t.put(a.dresidual, k, a.F, g);
-    t.put(a.dx, k, a.F, DROP ? t.drop(a.drop, z0, k, g) : g);
+    k0 += K;
+    if (k0 >= a.chunks * K) break;
+    get(k0);
   }
 }
-template <int K, bool DROP>
+template <bool DROP>
 __global__ void __launch_bounds__(kTileThreads) rms_norm_grad_kernel(NormArgs a) {
   __shared__ double lds[kTileThreads / 256][256];
   const int tiles = a.row_tiles * a.col_tiles;
@@ -473,8 +496,8 @@ __global__ void __launch_bounds__(kTileThreads) rms_norm_grad_kernel(NormArgs a)
     join_gamma<kTileWaves>(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
     return;
   }
-  if (whole_tile<K>(a, (int)blockIdx.x)) rms_norm_grad_tile<K, DROP, true>(a, lds);
-  else rms_norm_grad_tile<K, DROP, false>(a, lds);
+  if (whole_tile(a, (int)blockIdx.x)) rms_norm_grad_tile<DROP, true>(a, lds);
+  else rms_norm_grad_tile<DROP, false>(a, lds);
 }
 
 // Features of a thread that a block of few rows holds: in the forward as many as need
@@ -482,9 +505,10 @@ __global__ void __launch_bounds__(kTileThreads) rms_norm_grad_kernel(NormArgs a)
 // two launches either way, what one block does as fast as many (32 x 128: 18.5 us with
 // the forward for 20.9 in tiles, 32 x 512 26.7 and 21.0).
 constexpr int kFewHeld = 16, kFewHeldBack = 4;
-// Columns of a thread in a tile; twice as many where there are 512 tiles of that size
-// (8192 x 512 both ways 46 us, with 8 throughout 52; 4097 x 4099 177 us, with 4 212).
-constexpr int kTileCols = 4;
+// Blocks of a large matrix: fewer leave CUs without work, more leave more sums for every
+// block to join (4097 x 4099 both ways: 195 us with 256, 165 with 512 and 1024, 212 with
+// 2193, a tile of 32 columns each).
+constexpr int64_t kTileBlocks = 512;
 
 // Few rows: up to 32, as many as a block holds of them.
 bool few_rows(NormArgs& a, int held) {
@@ -495,17 +519,15 @@ bool few_rows(NormArgs& a, int held) {
   return true;
 }
 
-// The tiles, and how many columns a thread has in one.
-int set_tiles(NormArgs& a) {
+void set_tiles(NormArgs& a) {
   a.shift = 0;
   while (((int64_t)4 << a.shift) < a.N && a.shift < 6) ++a.shift;
-  const int64_t rows = (int64_t)4 << a.shift;
+  const int64_t rows = (int64_t)4 << a.shift, cols = (int64_t)K * (kTileThreads >> a.shift);
+  const int64_t col_tiles = (a.F + cols - 1) / cols;
   a.row_tiles = (int)((a.N + rows - 1) / rows);
-  for (int K = 2 * kTileCols;; K = kTileCols) {
-    const int64_t cols = (int64_t)K * (kTileThreads >> a.shift);
-    a.col_tiles = (int)((a.F + cols - 1) / cols);
-    if (K == kTileCols || (int64_t)a.row_tiles * a.col_tiles >= 512) return K;
-  }
+  const int64_t more = a.row_tiles * col_tiles / kTileBlocks;
+  a.chunks = (int)(more < 2 ? 1 : more < col_tiles ? more : col_tiles);
+  a.col_tiles = (int)((col_tiles + a.chunks - 1) / a.chunks);
 }
 
 template <bool DROP>
@@ -517,18 +539,16 @@ int run_forward(NormArgs& a, hipStream_t st, const char* who) {
     else hipLaunchKernelGGL((rms_norm_few_fwd_kernel<kFewHeld, DROP>), dim3(1), threads, 0, st, a);
     return check_launch(who);
   }
-  const int K = set_tiles(a);
+  set_tiles(a);
   const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles;
   CNHIP_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too large", who);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, (size_t)a.col_tiles * (size_t)a.N * sizeof(double), &ws, who));
   a.part = static_cast<double*>(ws);
   const dim3 grid((unsigned)tiles), tile_threads(kTileThreads);
-  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_sum_kernel<kTileCols, DROP>), grid, tile_threads, 0, st, a);
-  else hipLaunchKernelGGL((rms_norm_sum_kernel<2 * kTileCols, DROP>), grid, tile_threads, 0, st, a);
+  hipLaunchKernelGGL(rms_norm_sum_kernel<DROP>, grid, tile_threads, 0, st, a);
   CNHIP_TRY(check_launch(who));
-  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_apply_kernel<kTileCols, DROP>), grid, tile_threads, 0, st, a);
-  else hipLaunchKernelGGL((rms_norm_apply_kernel<2 * kTileCols, DROP>), grid, tile_threads, 0, st, a);
+  hipLaunchKernelGGL(rms_norm_apply_kernel<DROP>, grid, tile_threads, 0, st, a);
   return check_launch(who);
 }
 
@@ -536,8 +556,8 @@ template <bool DROP>
 int run_backward(NormArgs& a, hipStream_t st, const char* who) {
   const dim3 threads(kNormThreads);
   const bool few = few_rows(a, kFewHeldBack);
-  a.row_tiles = a.col_tiles = 1;
-  const int K = few ? 0 : set_tiles(a);
+  a.row_tiles = a.col_tiles = a.chunks = 1;
+  if (!few) set_tiles(a);
   const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles, gamma_blocks = (a.F + 63) / 64;
   CNHIP_REQUIRE(tiles + gamma_blocks < ((int64_t)1 << 31), "%s: too large", who);
   const size_t sums = few ? 0 : (size_t)a.col_tiles * (size_t)a.N * sizeof(double);
@@ -552,11 +572,9 @@ int run_backward(NormArgs& a, hipStream_t st, const char* who) {
     return check_launch(who);
   }
   const dim3 grid((unsigned)tiles), more((unsigned)(tiles + gamma_blocks)), tile_threads(kTileThreads);
-  if (K == kTileCols) hipLaunchKernelGGL(rms_norm_dots_kernel<kTileCols>, grid, tile_threads, 0, st, a);
-  else hipLaunchKernelGGL(rms_norm_dots_kernel<2 * kTileCols>, grid, tile_threads, 0, st, a);
+  hipLaunchKernelGGL(rms_norm_dots_kernel, grid, tile_threads, 0, st, a);
   CNHIP_TRY(check_launch(who));
-  if (K == kTileCols) hipLaunchKernelGGL((rms_norm_grad_kernel<kTileCols, DROP>), more, tile_threads, 0, st, a);
-  else hipLaunchKernelGGL((rms_norm_grad_kernel<2 * kTileCols, DROP>), more, tile_threads, 0, st, a);
+  hipLaunchKernelGGL(rms_norm_grad_kernel<DROP>, more, tile_threads, 0, st, a);
   return check_launch(who);
 }
 
