@@ -619,30 +619,25 @@ __global__ void __launch_bounds__(Whole::NT, 2) ffn_grads_kernel(FfnArgs a, FfnP
   db[v] = add ? db[v] + s : s;
 }
 
+// A row's 256 sums of a product that was split; block: [row][256 columns].
 template <bool COLS>
-__device__ __forceinline__ void ffn_reduce(const FfnProduct& p, const FfnArgs& a, int64_t first, int64_t step) {
-  const int64_t total = (int64_t)p.g.M * p.g.N;
-  const int eo = scale_out<COLS>(a);
-  for (int64_t i = first; i < total; i += step) {
-    const int64_t m = i / p.g.N, to = COLS ? column_of(m, a.F) : m;
-    if (to < 0) continue;
-    float x = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) x += p.o.part[s * total + i];
-    float* q = p.o.p + i % p.g.N + p.o.ld * to;
-    x = pr::times_exp2(x, eo);
-    *q = p.o.accumulate ? *q + x : x;
-  }
+__device__ __forceinline__ void ffn_reduce(const FfnProduct& p, const FfnArgs& a, int block) {
+  const int chunks = (p.g.N + 255) / 256, m = block / chunks, n = block % chunks * 256 + threadIdx.x;
+  const int64_t to = COLS ? column_of(m, a.F) : m, total = (int64_t)p.g.M * p.g.N;
+  if (to < 0 || n >= p.g.N) return;
+  const float* from = p.o.part + (int64_t)m * p.g.N + n;
+  float x = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < p.splits; ++s) x += from[s * total];
+  float* q = p.o.p + n + p.o.ld * to;
+  x = pr::times_exp2(x, scale_out<COLS>(a));
+  *q = p.o.accumulate ? *q + x : x;
 }
-// The products that were split, each over the blocks of its half of the grid.
-__global__ void __launch_bounds__(256) ffn_reduce_kernel(FfnArgs a, FfnProduct x, FfnProduct w) {
-  const int64_t half = gridDim.x / 2, bid = blockIdx.x % half;
-  const int64_t first = bid * 256 + threadIdx.x;
-  if (blockIdx.x < half) {
-    if (x.o.part) ffn_reduce<false>(x, a, first, half * 256);
-  } else {
-    if (w.o.part) ffn_reduce<true>(w, a, first, half * 256);
-  }
+// The products that were split, the x_blocks blocks of the first before the second's.
+__global__ void __launch_bounds__(256) ffn_reduce_kernel(FfnArgs a, FfnProduct x, FfnProduct w, int x_blocks) {
+  const int bid = (int)blockIdx.x;
+  if (bid < x_blocks) ffn_reduce<false>(x, a, bid);
+  else ffn_reduce<true>(w, a, bid - x_blocks);
 }
 
 template <class T>
@@ -678,7 +673,7 @@ struct Job {
 template <class T>
 int steps_of(const Job* jobs, int n) {
   constexpr bool kHalf = T::WN == 2;
-  constexpr double kStepUs = kHalf ? 1.2 : 1.55, kEnds = kHalf ? 6 : 8, kBytesUs = kHalf ? 8e6 : 5e6;
+  constexpr double kStepUs = kHalf ? 1.2 : 1.55, kEnds = kHalf ? 6 : 8, kBytesUs = kHalf ? 8e6 : 2.5e6;
   constexpr int64_t kSlots = kHalf ? 512 : 256;
   int longest = 2, best = 0;
   for (int i = 0; i < n; ++i) longest = jobs[i].steps > longest ? jobs[i].steps : longest;
@@ -814,8 +809,10 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
     hipLaunchKernelGGL(ffn_grads_kernel, dim3((unsigned)blocks), dim3(Whole::NT), 0, st, a, x, y, db, add);
     CNHIP_TRY(check_launch(who));
     if (!x.o.part && !y.o.part) continue;
-    const int64_t most_out = (x.o.part ? D * a.R : 0) > (y.o.part ? 2 * Fp * D : 0) ? D * a.R : 2 * Fp * D;
-    hipLaunchKernelGGL(ffn_reduce_kernel, dim3(2 * elementwise_grid(most_out, 256)), dim3(256), 0, st, a, x, y);
+    auto reduce_blocks = [](const FfnProduct& q) { return q.o.part ? (int64_t)q.g.M * ((q.g.N + 255) / 256) : 0; };
+    const int64_t xb = reduce_blocks(x), wb = reduce_blocks(y);
+    CNHIP_REQUIRE(xb + wb < ((int64_t)1 << 31), "%s: too large", who);
+    hipLaunchKernelGGL(ffn_reduce_kernel, dim3((unsigned)(xb + wb)), dim3(256), 0, st, a, x, y, (int)xb);
     CNHIP_TRY(check_launch(who));
   }
   return CNHIP_OK;
