@@ -673,7 +673,7 @@ struct Job {
 template <class T>
 int steps_of(const Job* jobs, int n) {
   constexpr bool kHalf = T::WN == 2;
-  constexpr double kStepUs = kHalf ? 1.2 : 1.55, kEnds = kHalf ? 6 : 8, kBytesUs = kHalf ? 8e6 : 2.5e6;
+  constexpr double kStepUs = kHalf ? 1.2 : 1.55, kEnds = kHalf ? 6 : 8, kBytesUs = kHalf ? 8e6 : 5e6;
   constexpr int64_t kSlots = kHalf ? 512 : 256;
   int longest = 2, best = 0;
   for (int i = 0; i < n; ++i) longest = jobs[i].steps > longest ? jobs[i].steps : longest;
