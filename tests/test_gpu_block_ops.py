@@ -264,7 +264,7 @@ NORM = [  # N, F, p, residual, dsum
     (8, 512, 0.1, True, True), (17, 100, 0.0, False, True), (32, 33, 0.5, True, True), (33, 1024, 0.0, True, True),
     (64, 513, 0.1, False, True), (257, 512, 0.1, True, True), (100, 2000, 0.0, True, True), (1000, 40, 0.0, True, False),
     (45, 4099, 0.1, True, True), (70, 2049, 0.0, True, True), (5, 20001, 0.2, True, True), (20000, 12, 0.0, True, True),
-    (16500, 64, 0.1, True, True),  # more tiles of rows than blocks
+    (16500, 64, 0.1, True, True), (1300, 6001, 0.1, True, True), (2100, 8300, 0.0, True, False),  # several tiles a block
 ]
 
 
@@ -384,6 +384,7 @@ FFN = [  # N, D, F, activation, bias
     (17, 300, 100, "sigmoid", False), (33, 64, 65, "silu", True), (64, 257, 31, "gelu", True), (65, 33, 31, "silu", True),
     (100, 64, 128, "gelu", False), (130, 1, 40, "silu", True), (70, 40, 1, "relu", False), (257, 100, 300, "silu", True),
     (300, 513, 97, "gelu", True), (1021, 257, 130, "silu", False), (1300, 96, 64, "sigmoid", True), (2050, 40, 33, "relu", True),
+    (70, 1100, 33, "silu", True), (9, 1500, 12, "gelu", False), (600, 33, 400, "silu", False),
 ]
 
 
