@@ -14,6 +14,8 @@
 // backward, once along its columns and once along its rows.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "act_math.hpp"
 #include "common.hpp"
 #include "mfma_pair.hpp"
@@ -30,10 +32,11 @@ struct FfnScales {
   uint32_t w, x, z;
 };
 // What the blocks that look for them found: of W, X and dZ.
-// The forward's epilogue is as long as many of its steps, so it runs in half tiles, two
-// to a CU (8192 x 1024 -> 4096, GELU, no Z: 459 us in both; 1021 x 513 -> 1365 38.8 us
-// in half tiles and 44.6 in whole ones, 300 rows 32.3 and 35.1); the backward in whole
-// ones (half tiles across the rows of both operands need more registers than there are).
+// The forward runs in half tiles, two to a CU, of which one stores while the other
+// computes, and which leave less of a small call's grid empty (half and whole tiles, us:
+// 1021 x 513 -> 1365 both directions 103.6 and 108.7, 256 x 1024 -> 4096 50 and 55, 8192 x
+// 1024 -> 4096 393 and 386); the backward in whole ones (half tiles across the rows of
+// both operands need more registers than there are).
 using Half = pr::Tile<2>;
 using Whole = pr::Tile<4>;
 constexpr int kMaxBlocks[3] = {256, 256, 512};
@@ -94,6 +97,15 @@ __device__ __forceinline__ void gate_both(int act, float z, float& y, float& d) 
   sigmoid_parts(z, on, off);
   y = act == CNHIP_GATE_SILU ? z * on : on;
   d = act == CNHIP_GATE_SILU ? on * fmaf(z, off, 1.f) : on * off;
+}
+
+// f(act), act a constant
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  if (act == CNHIP_GATE_SILU) f(std::integral_constant<int, CNHIP_GATE_SILU>{});
+  else if (act == CNHIP_GATE_GELU) f(std::integral_constant<int, CNHIP_GATE_GELU>{});
+  else if (act == CNHIP_GATE_SIGMOID) f(std::integral_constant<int, CNHIP_GATE_SIGMOID>{});
+  else f(std::integral_constant<int, CNHIP_GATE_RELU>{});
 }
 
 // ------------------------------------------------------------------ forward
@@ -189,36 +201,59 @@ __global__ void __launch_bounds__(Half::NT, 2) ffn_forward_kernel(pr::GemmArgs g
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int block0 = tm * (pr::TM / 32) + (wave / Half::WN) * 4;  // the wave's first of 32 packed columns: a gate's
-  int64_t n[2];
-  int ex[2];
+  const int64_t n0 = (int64_t)tn * Half::TN + (wave % Half::WN) * 64 + (lane & 31);
+  // A test for every element would end the run of loads, functions and stores behind it
+  // (1024 rows, 64 -> 1024: 24 us for 12; 8192 rows, 1024 -> 4096 475 us for 411), so the activation and whole tiles are told
+  // apart here.
+  with_act(a.act, [&](auto act) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    n[j] = (int64_t)tn * Half::TN + (wave % Half::WN) * 64 + 32 * j + (lane & 31);
-    ex[j] = a.xe[n[j] < a.N ? n[j] : a.N - 1];
-  }
+    for (int i = 0; i < 4; i += 2) {
+      if (block0 + i >= g.M / 32) break;
+      const int64_t first = (int64_t)(block0 + i) * 16, f0 = first + 4 * (lane >> 5);
+      const bool whole = first + 32 <= a.F && (int64_t)tn * Half::TN + (wave % Half::WN) * 64 + 64 <= a.N;
+      auto row = [](int e) { return 8 * (e / 4) + e % 4; };
+      float bg[16], bu[16];
 #pragma unroll
-  for (int i = 0; i < 4; i += 2) {
-    if (block0 + i >= g.M / 32) break;
-    const int eg = a.we[block0 + i], eu = a.we[block0 + i + 1];
-    const int64_t f0 = (int64_t)(block0 + i) * 16 + 4 * (lane >> 5);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int64_t f = f0 + 8 * (e / 4) + e % 4;
-      if (f >= a.F) continue;
-      const float bg = a.b ? a.b[f] : 0.f, bu = a.b ? a.b[a.F + f] : 0.f;
+      for (int e = 0; e < 16; ++e) {
+        const int64_t f = f0 + row(e) < a.F ? f0 + row(e) : a.F - 1;
+        bg[e] = a.b ? a.b[f] : 0.f;
+        bu[e] = a.b ? a.b[a.F + f] : 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (n[j] >= a.N) continue;
-        const float gate = pr::times_exp2(acc.x[i][j][e], -ex[j] - eg) + bg;
-        const float up = pr::times_exp2(acc.x[i + 1][j][e], -ex[j] - eu) + bu;
-        if (a.Zout) {
-          a.Zout[n[j] + a.N * f] = gate;
-          a.Zout[n[j] + a.N * (a.F + f)] = up;
+        const int64_t n = n0 + 32 * j;
+        const int ex = a.xe[n < a.N ? n : a.N - 1], eg = -ex - a.we[block0 + i], eu = -ex - a.we[block0 + i + 1];
+        float h[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          acc.x[i][j][e] = pr::times_exp2(acc.x[i][j][e], eg) + bg[e];
+          acc.x[i + 1][j][e] = pr::times_exp2(acc.x[i + 1][j][e], eu) + bu[e];
+          h[e] = gate_f(act, acc.x[i][j][e]) * acc.x[i + 1][j][e];
         }
-        a.H[n[j] + a.N * f] = gate_f(a.act, gate) * up;
+        float* to = a.H + n + a.N * f0;
+        float* zg = a.Zout + n + a.N * f0;
+        float* zu = zg + a.N * a.F;
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) to[a.N * row(e)] = h[e];
+          if (!a.Zout) continue;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) zg[a.N * row(e)] = acc.x[i][j][e];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) zu[a.N * row(e)] = acc.x[i + 1][j][e];
+        } else if (n < a.N) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (f0 + row(e) >= a.F) continue;
+            to[a.N * row(e)] = h[e];
+            if (!a.Zout) continue;
+            zg[a.N * row(e)] = acc.x[i][j][e];
+            zu[a.N * row(e)] = acc.x[i + 1][j][e];
+          }
+        }
       }
     }
-  }
+  });
 }
 
 // The same from split sums, [splits][M][N].
@@ -243,22 +278,32 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(FfnArgs a, const float* _
   a.H[n + a.N * f] = gate_f(a.act, gate) * up;
 }
 
-// Few rows: W is read once and each value used for a handful of products, so the
-// fp32 matrix cores keep up with memory and nothing is packed.  A block takes 8
-// hidden features (16 columns of W, the rows of the 16 x 16 tiles); its eight
-// waves share out D and meet in LDS.
-constexpr int kFewRows = 64;
+// Few rows: each value of W is used for a handful of products, so the fp32 matrix
+// cores keep up with memory and nothing is packed.  A block takes 8 hidden features
+// (16 columns of W, the rows of the 16 x 16 tiles) and up to 128 rows; its eight waves
+// share out D and meet in LDS.
+// Packed, a call takes about 15 us more for its launches and 3.6 us for every million of D
+// F to pack W, but a quarter of the time for a row's products.  This way and packed, us:
+// 128 rows, 512 -> 2048 10.7 and 26.7, 1024 -> 4096 39 and 47; 256 rows, 512 -> 2048
+// 21.8 and 26.6; 384 rows 32.6 and 29.5; 1024 rows, 256 -> 512 12.0 and 23.7.
+constexpr int kFewBlock = 128;
+bool few_rows(int64_t N, int64_t D, int64_t F) {
+  const double rows = (double)(N <= 64 ? (N + 15) / 16 * 16 : (N + kFewBlock - 1) / kFewBlock * kFewBlock);
+  return N <= 65535 * (int64_t)kFewBlock && 1e-6 * (double)D * (double)F * (0.05 * rows - 3.6) <= 15.0;
+}
 template <int NB>
 __global__ void __launch_bounds__(512) ffn_few_kernel(FfnArgs a) {
   __shared__ float part[8][16][16 * NB + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int64_t f0 = (int64_t)blockIdx.x * 8, f = f0 + (r & 7);
   const float* w = a.W + ((r >> 3) * a.F + (f < a.F ? f : a.F - 1)) * a.D;
-  const int N = (int)a.N;
+  const int64_t n0 = (int64_t)blockIdx.y * kFewBlock;
+  const float* X = a.X + n0;
+  const int N = (int)(a.N - n0 < 16 * NB ? a.N - n0 : 16 * NB);
   f32x4 acc[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int U = NB > 2 ? 2 : 4;  // steps of 16 features under way
+  constexpr int U = NB > 4 ? 1 : NB > 2 ? 2 : 4;  // steps of 16 features under way
   for (int64_t d0 = 16 * wave; d0 < a.D; d0 += 128 * U) {
     f32x4 wv[U];
     float xv[U][NB][4];
@@ -275,7 +320,7 @@ __global__ void __launch_bounds__(512) ffn_few_kernel(FfnArgs a) {
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          xv[u][j][e] = d + e < a.D && 16 * j + r < N ? a.X[16 * j + r + a.N * (d + e)] : 0.f;
+          xv[u][j][e] = d + e < a.D && 16 * j + r < N ? X[16 * j + r + a.N * (d + e)] : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -303,11 +348,12 @@ __global__ void __launch_bounds__(512) ffn_few_kernel(FfnArgs a) {
       gate += a.b[f0 + k];
       up += a.b[a.F + f0 + k];
     }
+    const int64_t at = n0 + n + a.N * (f0 + k);
     if (a.Zout) {
-      a.Zout[n + a.N * (f0 + k)] = gate;
-      a.Zout[n + a.N * (a.F + f0 + k)] = up;
+      a.Zout[at] = gate;
+      a.Zout[at + a.N * a.F] = up;
     }
-    a.H[n + a.N * (f0 + k)] = gate_f(a.act, gate) * up;
+    a.H[at] = gate_f(a.act, gate) * up;
   }
 }
 
@@ -580,9 +626,14 @@ __device__ __forceinline__ void ffn_product(const FfnProduct& p, const FfnArgs& 
         float* q = o.p + n + o.ld * (f + (blk & 1) * a.F);
         auto row = [](int e) { return 8 * (e / 4) + e % 4; };
         if (!o.accumulate) {
+          if (left >= 32) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (row(e) < left) q[o.ld * row(e)] = value(acc.x[i][j][e]);
+            for (int e = 0; e < 16; ++e) q[o.ld * row(e)] = value(acc.x[i][j][e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (row(e) < left) q[o.ld * row(e)] = value(acc.x[i][j][e]);
+          }
           continue;
         }
         float old[16];
@@ -700,11 +751,12 @@ int steps_of(const Job* jobs, int n) {
 
 int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
   const int64_t N = a.N, D = a.D, F = a.F, Fp = pad32(F);
-  if (N <= kFewRows) {
-    const dim3 grid((unsigned)((F + 7) / 8)), threads(512);
+  if (few_rows(N, D, F)) {
+    const dim3 grid((unsigned)((F + 7) / 8), (unsigned)((N + kFewBlock - 1) / kFewBlock)), threads(512);
     if (N <= 16) hipLaunchKernelGGL(ffn_few_kernel<1>, grid, threads, 0, st, a);
     else if (N <= 32) hipLaunchKernelGGL(ffn_few_kernel<2>, grid, threads, 0, st, a);
-    else hipLaunchKernelGGL(ffn_few_kernel<4>, grid, threads, 0, st, a);
+    else if (N <= 64) hipLaunchKernelGGL(ffn_few_kernel<4>, grid, threads, 0, st, a);
+    else hipLaunchKernelGGL(ffn_few_kernel<8>, grid, threads, 0, st, a);
     return check_launch(who);
   }
   a.steps_d = (int)(pad32(D) / 16);

@@ -385,6 +385,9 @@ FFN = [  # N, D, F, activation, bias
     (100, 64, 128, "gelu", False), (130, 1, 40, "silu", True), (70, 40, 1, "relu", False), (257, 100, 300, "silu", True),
     (300, 513, 97, "gelu", True), (1021, 257, 130, "silu", False), (1300, 96, 64, "sigmoid", True), (2050, 40, 33, "relu", True),
     (70, 1100, 33, "silu", True), (9, 1500, 12, "gelu", False), (600, 33, 400, "silu", False),
+    # the forward on packed operands too
+    (1021, 257, 1300, "silu", False), (2050, 300, 700, "relu", True), (3000, 130, 1000, "gelu", True),
+    (700, 1100, 600, "sigmoid", False), (5000, 33, 1900, "silu", True), (513, 1000, 999, "gelu", False),
 ]
 
 
@@ -443,13 +446,13 @@ def test_ffn(gpu, N, D, F, act, bias):
     c.check(accumulate=True)
 
 
-@pytest.mark.parametrize("N", [20, 200])
-def test_ffn_rows_and_columns_of_any_size(gpu, N):
+@pytest.mark.parametrize("N,D,F", [(20, 70, 96), (200, 70, 96), (1100, 260, 1312)])
+def test_ffn_rows_and_columns_of_any_size(gpu, N, D, F):
     """Forward: a row of X and a block of W's columns have scales of their own."""
-    c = Ffn(N, 70, 96, "silu", False)
+    c = Ffn(N, D, F, "silu", False)
     c.X *= np.float32(2.0) ** np.random.default_rng(1).integers(-60, 30, (N, 1)).astype(np.float32)
     c.W[:, :32] *= np.float32(2.0 ** -40)
-    c.W[:, 96:128] *= np.float32(2.0 ** 20)
+    c.W[:, F:F + 32] *= np.float32(2.0 ** 20)
     got, want = c.forward(), ref.ffn_forward(c.X, c.W, None, "silu")
     for name in got:
         ref.check(name, got[name], *want[name])
@@ -468,8 +471,8 @@ def test_ffn_gates_far_out(gpu, act):
 
 
 def test_ffn_rows_that_are_not_finite_stay_alone(gpu):
-    for N in (30, 300):
-        c = Ffn(N, 40, 50, "silu", True)
+    for N, D, F in ((30, 40, 50), (300, 40, 50), (1100, 260, 1300)):
+        c = Ffn(N, D, F, "silu", True)
         plain = c.forward()
         c.X[7, 3], c.X[20, :] = np.nan, np.inf
         got = c.forward()
