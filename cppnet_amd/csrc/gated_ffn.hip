@@ -6,7 +6,7 @@
 //   dgate = dH up act'(gate), dup = dH act(gate), dZ = [dgate dup],
 //   dX = dZ W^T,  dW (+)= X^T dZ,  db (+)= column sums of dZ
 //
-// The products run on the fp16 matrix cores over operands packed as pairs
+// Products of many rows run on the fp16 matrix cores over operands packed as pairs
 // (mfma_pair.hpp).  W's columns are packed in blocks of 32, a gate's and then its
 // up's, so one wave's accumulators hold both values of an element and the
 // activation and the product are done where the sums are.  dZ is packed in the
@@ -363,6 +363,43 @@ __device__ __forceinline__ void grads_of(const FfnArgs& a, float gate, float up,
   gate_both(a.act, gate, y, d);
   dg = dh * up * d;
   du = dh * y;
+}
+
+// dZ, [N, 2 F] as Z is stored: 4 values a thread.
+__global__ void __launch_bounds__(256) ffn_dz_kernel(FfnArgs a, float* __restrict__ dZ) {
+  const int64_t n = a.N * a.F, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int left = n - i < 4 ? (int)(n - i) : 4;
+  f32x4 zg = {0.f, 0.f, 0.f, 0.f}, zu = zg, dh = zg;
+  if (left == 4) {
+    zg = *reinterpret_cast<const f32x4u*>(a.Z + i);
+    zu = *reinterpret_cast<const f32x4u*>(a.Z + n + i);
+    dh = *reinterpret_cast<const f32x4u*>(a.dH + i);
+  } else {
+    for (int e = 0; e < left; ++e) {
+      zg[e] = a.Z[i + e];
+      zu[e] = a.Z[n + i + e];
+      dh[e] = a.dH[i + e];
+    }
+  }
+  with_act(a.act, [&](auto act) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float y, d;
+      gate_both(act, zg[e], y, d);
+      zg[e] = dh[e] * zu[e] * d;
+      zu[e] = dh[e] * y;
+    }
+  });
+  if (left == 4) {
+    *reinterpret_cast<f32x4u*>(dZ + i) = zg;
+    *reinterpret_cast<f32x4u*>(dZ + n + i) = zu;
+  } else {
+    for (int e = 0; e < left; ++e) {
+      dZ[i + e] = zg[e];
+      dZ[n + i + e] = zu[e];
+    }
+  }
 }
 
 // An upper bound of |dgate| and |dup|, a few times their size at most but next to a zero
@@ -790,6 +827,24 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
   return check_launch(who);
 }
 
+// Few rows: dZ, and the Linear's backward over it.  This way and packed, us: 32 rows,
+// 512 -> 2048 20 and 37, 256 rows 37 and 44, 512 rows 54 and 55; 1024 -> 4096 64 rows 40
+// and 54, 256 rows 76 and 73.  64 rows fill a quarter of a packed tile, so they take
+// this way at any size.
+bool few_rows_back(int64_t N, int64_t D, int64_t F) {
+  return N <= 64 || (N <= 256 && (double)N * (double)D * (double)F <= 5e8);
+}
+
+int run_backward_few(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hipStream_t st, const char* who) {
+  void* dZ = nullptr;
+  const int64_t n = a.N * a.F;
+  CNHIP_REQUIRE((n + 1023) / 1024 < ((int64_t)1 << 31), "%s: too large", who);
+  CNHIP_TRY(scratch(st, kScratchLayer, (size_t)(2 * n) * sizeof(float), &dZ, who));
+  hipLaunchKernelGGL(ffn_dz_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, a, static_cast<float*>(dZ));
+  CNHIP_TRY(check_launch(who));
+  return cnhip_linear_backward(a.X, a.W, static_cast<float*>(dZ), dW, db, dX, a.N, a.D, 2 * a.F, 1, accumulate, st);
+}
+
 int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hipStream_t st, const char* who) {
   const int64_t N = a.N, D = a.D, F = a.F, Fp = pad32(F), Dp = pad32(D);
   a.steps_d = (int)(Dp / 16);
@@ -909,7 +964,9 @@ int cnhip_gated_ffn_backward(const float* X, const float* W, const float* Z, con
   a.D = in_features;
   a.F = hidden;
   a.act = act;
-  return cnhip::run_backward(a, dX, dW, db, accumulate, cnhip::as_stream(stream), who);
+  const hipStream_t st = cnhip::as_stream(stream);
+  return cnhip::few_rows_back(batch, in_features, hidden) ? cnhip::run_backward_few(a, dX, dW, db, accumulate, st, who)
+                                                          : cnhip::run_backward(a, dX, dW, db, accumulate, st, who);
 }
 
 }  // extern "C"

@@ -913,14 +913,13 @@ int cnhip_linear_recurrence_backward(const float* x, const float* f, const float
  * Z [batch, 2 hidden] is what the backward reads; NULL: not wanted.
  * backward: dX (overwritten), dW and db (added to with accumulate 1, else
  * overwritten; db NULL exactly where b was) from X, W, Z and dH.
- * The backward's products, and the forward's of many rows, run on pairs of fp16
- * terms as above; the operands with a largest value of their own are a row of X and
- * 32 columns of W in the forward; W, the rows of X and those of Z's gradient that go
- * through together in the backward (2^26 / hidden, at least 1024).  For Z's gradient
- * a bound stands for the largest value, a few times it unless every gate lies next to
- * a zero of act'.  An infinity in such an operand comes out as NaN.  The stream's
- * scratch holds X and W as packed, in the backward those rows of Z's gradient, and
- * the parts of products that are split. */
+ * Products of many rows run on pairs of fp16 terms as above; the operands with a
+ * largest value of their own are a row of X and 32 columns of W in the forward; W, the
+ * rows of X and those of Z's gradient that go through together in the backward (2^26 /
+ * hidden, at least 1024).  For Z's gradient a bound stands for the largest value, a few
+ * times it unless every gate lies next to a zero of act'.  An infinity in such an
+ * operand comes out as NaN.  The stream's scratch holds X and W as packed, in the
+ * backward (a piece of) Z's gradient, and the parts of products that are split. */
 #define CNHIP_GATE_SILU 0     /* z sigmoid(z) */
 #define CNHIP_GATE_GELU 1     /* z Phi(z), as CNHIP_ACT_GELU */
 #define CNHIP_GATE_SIGMOID 2

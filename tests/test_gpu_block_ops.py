@@ -482,12 +482,12 @@ def test_ffn_rows_that_are_not_finite_stay_alone(gpu):
             assert not np.isfinite(got[name][[7, 20]]).any()
 
 
-def test_ffn_in_pieces(gpu):
+@pytest.mark.parametrize("last", [777, 2])
+def test_ffn_in_pieces(gpu, last):
     """More values of dZ than one piece holds: a million rows of 40 hidden features go
     through in two, each with scales of its own; checked against calls on the parts."""
     D, F, act = 2, 40, "silu"
     piece = (1 << 27) // 128 // 256 * 256  # 40 features are packed as 64
-    last = 777
     N = piece + last
     g = torch.Generator(device="cuda").manual_seed(5)
     new = lambda n: torch.randn(n, generator=g, device="cuda")  # noqa: E731
