@@ -12,6 +12,12 @@
 // activation and the product are done where the sums are.  dZ is packed in the
 // same order of columns straight from Z and dH, and serves both products of the
 // backward, once along its columns and once along its rows.
+//
+// Bound by the fp16 matrix cores at the clock that the power limit leaves.  8192 rows,
+// 1024 -> 4096, GELU: forward 411 to 468 us (294 to 334 TFLOP/s of fp32 products, where a
+// third of a library's fp16 rate is 387) and packing 38; back 711 to 783 (351 to 387),
+// packing 152 (5.3 TB/s) and the bound of dZ 103 (4.6 TB/s).  Few rows by W: 4 rows, 512 ->
+// 2048 4.7 us.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -747,7 +753,8 @@ int check_shape(int64_t N, int64_t D, int64_t F, int act, const char* who) {
   CNHIP_REQUIRE(N > 0 && D > 0 && F > 0, "%s: bad shape batch=%lld in_features=%lld hidden=%lld", who, (long long)N,
                 (long long)D, (long long)F);
   CNHIP_REQUIRE(act >= CNHIP_GATE_SILU && act <= CNHIP_GATE_RELU, "%s: bad activation %d", who, act);
-  CNHIP_REQUIRE(N < ((int64_t)1 << 30) && D < ((int64_t)1 << 22) && F < ((int64_t)1 << 28), "%s: too large", who);
+  // (a grid has fewer than 2^32 threads; the packing has 32 for a row or a column of W)
+  CNHIP_REQUIRE(N < ((int64_t)1 << 26) && D < ((int64_t)1 << 22) && F < ((int64_t)1 << 25), "%s: too large", who);
   return CNHIP_OK;
 }
 
@@ -797,7 +804,7 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
     return check_launch(who);
   }
   a.steps_d = (int)(pad32(D) / 16);
-  CNHIP_REQUIRE(tiles_of<Half>(2 * Fp, N) < ((int64_t)1 << 31), "%s: too large", who);
+  CNHIP_REQUIRE(tiles_of<Half>(2 * Fp, N) < ((int64_t)1 << 23), "%s: too large", who);
   Places w;
   const size_t o_x = w.place((size_t)(pad32(N) * pad32(D)) * 4), o_w = w.place((size_t)(2 * Fp * pad32(D)) * 4),
                o_xe = w.place((size_t)N * 4), o_we = w.place((size_t)(2 * Fp / 32) * 4);
@@ -838,7 +845,7 @@ bool few_rows_back(int64_t N, int64_t D, int64_t F) {
 int run_backward_few(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hipStream_t st, const char* who) {
   void* dZ = nullptr;
   const int64_t n = a.N * a.F;
-  CNHIP_REQUIRE((n + 1023) / 1024 < ((int64_t)1 << 31), "%s: too large", who);
+  CNHIP_REQUIRE((n + 1023) / 1024 < ((int64_t)1 << 24), "%s: too large", who);
   CNHIP_TRY(scratch(st, kScratchLayer, (size_t)(2 * n) * sizeof(float), &dZ, who));
   hipLaunchKernelGGL(ffn_dz_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, a, static_cast<float*>(dZ));
   CNHIP_TRY(check_launch(who));
@@ -863,7 +870,7 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
   };
   CNHIP_REQUIRE(tiles_of<Whole>(D, R) * ((2 * a.steps_f + per - 1) / per) +
                         tiles_of<Whole>(2 * Fp, D) * ((Rp / 16 + per - 1) / per) <
-                    ((int64_t)1 << 30),
+                    ((int64_t)1 << 22),
                 "%s: too large", who);
   // blocks of 32 rows of dZ a wave: as many as leave 4096 waves, so that a wave that has
   // several keeps its loads going
@@ -904,7 +911,7 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
     CNHIP_TRY(check_launch(who));
     const int64_t zw = (int64_t)((rb + a.z_blocks - 1) / a.z_blocks) * a.steps_f, wf = r0 ? 0 : 2 * Fp / 32 * a.steps_d,
                   xf = (int64_t)rb * a.steps_d;
-    CNHIP_REQUIRE(zw + wf + xf < ((int64_t)1 << 32), "%s: too large", who);
+    CNHIP_REQUIRE(zw + wf + xf < ((int64_t)1 << 25), "%s: too large", who);
     hipLaunchKernelGGL(ffn_pack_kernel, dim3((unsigned)((zw + wf + xf + 3) / 4)), dim3(256), 0, st, a, zw, wf, xf);
     CNHIP_TRY(check_launch(who));
     const int add = accumulate || r0 > 0;
@@ -918,7 +925,7 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
     if (!x.o.part && !y.o.part) continue;
     auto reduce_blocks = [](const FfnProduct& q) { return q.o.part ? (int64_t)q.g.M * ((q.g.N + 255) / 256) : 0; };
     const int64_t xb = reduce_blocks(x), wb = reduce_blocks(y);
-    CNHIP_REQUIRE(xb + wb < ((int64_t)1 << 31), "%s: too large", who);
+    CNHIP_REQUIRE(xb + wb < ((int64_t)1 << 24), "%s: too large", who);
     hipLaunchKernelGGL(ffn_reduce_kernel, dim3((unsigned)(xb + wb)), dim3(256), 0, st, a, x, y, (int)xb);
     CNHIP_TRY(check_launch(who));
   }

@@ -912,7 +912,8 @@ int cnhip_linear_recurrence_backward(const float* x, const float* f, const float
  * hidden] or NULL;  H [batch, hidden] = act(Z[:, :hidden]) * Z[:, hidden:].
  * Z [batch, 2 hidden] is what the backward reads; NULL: not wanted.
  * backward: dX (overwritten), dW and db (added to with accumulate 1, else
- * overwritten; db NULL exactly where b was) from X, W, Z and dH.
+ * overwritten; db NULL exactly where b was) from X, W, Z and dH.  batch < 2^26,
+ * hidden < 2^25, in_features < 2^22.
  * Products of many rows run on pairs of fp16 terms as above; the operands with a
  * largest value of their own are a row of X and 32 columns of W in the forward; W, the
  * rows of X and those of Z's gradient that go through together in the backward (2^26 /

@@ -82,7 +82,7 @@ def test_recurrence_gradient_of_the_input_gate_goes_with_it():
 @pytest.mark.parametrize("change,word", [
     ({"N": 0}, "bad shape"), ({"D": 0}, "bad shape"), ({"F": -1}, "bad shape"), ({"act": 4}, "activation"),
     ({"act": -1}, "activation"), ({"X": None}, "NULL"), ({"N": 1 << 30}, "too large"), ({"F": 1 << 28}, "too large"),
-    ({"D": 1 << 22}, "too large"),
+    ({"D": 1 << 22}, "too large"), ({"N": 1 << 26}, "too large"), ({"F": 1 << 25}, "too large"),
 ])
 def test_ffn_refusals(change, word):
     a = dict(X=P, N=2, D=3, F=4, act=0) | change

@@ -244,3 +244,20 @@ def test_positions_past_32_bits(gpu):
     np.testing.assert_array_equal(last.cpu().numpy(), [1.0, 0.0, 0.0, 9.0])
     np.testing.assert_array_equal(h[S - 4:S].cpu().numpy(), [0.0, 4.0, 2.0, 1.0])
     np.testing.assert_array_equal(h[-3:].cpu().numpy(), [0.0, 2.0, 9.0])
+
+
+def test_more_chains_than_a_launch_takes(gpu):
+    """2^29 + 2^16 chains of one step: a second launch has the last of them."""
+    B, D = 1 << 16, (1 << 13) + 1
+    n = B * D
+    x, f, h = (torch.empty(n, device="cuda") for _ in range(3))
+    f.zero_()  # a = 1 / 2
+    h.fill_(-1.0)
+    last = torch.full((n,), 6.0, device="cuda")
+    for i in range(0, n, 1 << 24):
+        k = min(1 << 24, n - i)
+        x[i:i + k] = torch.arange(i % 1021, i % 1021 + k, device="cuda", dtype=torch.int32) % 1021
+    ops.linear_recurrence_forward(x, f, None, last, h, last, B, 1, D)
+    x.add_(6.0).mul_(0.5)
+    assert torch.equal(h, x)
+    assert torch.equal(last, x)
