@@ -7,21 +7,29 @@
 //   ds = dsum + rstd (d - n mean_f(d n)),  dresidual = ds, dx = drop(ds),
 //   dgamma_f (+)= sum_n dy_nf n_nf
 //
-// Matrices are ColMajor [N, F]: the features of a row lie N apart.  A block that held
-// whole rows would read a line or two of every column, each on a page of its own:
-// 4097 x 4099, forward, 203 us in blocks of 16 rows for 81 here.  So the matrix goes
-// through in tiles of 256 rows x 32 columns and more, a KiB in a row of every column,
-// twice: the first launch leaves each tile's sums over its columns, the second joins
-// them and reads s (and dy) again, for the most part from the caches.  Where a few
-// rows are all there is, one launch does both and holds them in registers.  The sums
-// over a row are kept in 64 bits, which neither overflow nor vanish for any finite
-// fp32 row.
+// Matrices are ColMajor [N, F]: the features of a row lie N apart.  Up to 1024 features,
+// a block holds 32 rows, a line of every column, in registers and reads everything once.
+// Of longer rows it would hold a part of a line of every column, each on a page of its
+// own (4097 x 4099, forward, 203 us in blocks of 16 rows for 81 here), so a larger matrix
+// goes through in tiles of 256 rows x 32 columns and more, a KiB in a row of every
+// column, twice: the first launch leaves each tile's sums over its columns, the second
+// joins them and reads s (and dy) again, for the most part from the caches.  Where a few
+// rows are all there is, one block does it.  The sums over a row are kept in 64 bits,
+// which neither overflow nor vanish for any finite fp32 row.
+//
+// Bound by memory: 8192 x 512 with dropout takes 14.4 us forward (67 MB, 4.7 TB/s) and 18.0
+// back (84 MB, 4.7 TB/s), a round of one block a CU, which loads, adds up and then stores,
+// and 3.8 for dgamma; 8192 x 1024 without 23.5 and 24.3; 4097 x 4099 in tiles 48 + 29 us
+// forward (375 MB, 4.9 TB/s) and 30 + 57 back (462 MB, 5.3 TB/s), of which reading s and dy
+// again is a fifth and a third.  Dropout alone: 8192 x 2048 20.6 us, 6.5 TB/s with its
+// input in the caches (24 among other work).
 //
 // Element j of the [N, F] storage is kept where the generator's word for
 // position + j says so; the backward draws the same words again.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 #include "dropout_rng.hpp"
@@ -202,24 +210,39 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_few_bwd_kernel(NormArgs
 }
 
 // dgamma (+)= the tiles' parts, in order: 64 features a block, its waves share the parts.
-template <int WAVES>
 __device__ __forceinline__ void join_gamma(const NormArgs& a, int64_t block, float (*sum)[64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t f = block * 64 + lane;
   float t = 0.f;
   if (f < a.F) {
 #pragma unroll 8
-    for (int b = wave; b < a.row_tiles; b += WAVES) t += a.gamma_part[(int64_t)b * a.F + f];
+    for (int b = wave; b < a.row_tiles; b += kTileWaves) t += a.gamma_part[(int64_t)b * a.F + f];
   }
   sum[wave][lane] = t;
   __syncthreads();
   if (wave || f >= a.F) return;
-  for (int w = 1; w < WAVES; ++w) t += sum[w][lane];
+  for (int w = 1; w < kTileWaves; ++w) t += sum[w][lane];
   a.dgamma[f] = a.accumulate ? a.dgamma[f] + t : t;
 }
+// The same in a launch of its own, 16 features a block.
 __global__ void __launch_bounds__(kNormThreads) rms_norm_gamma_kernel(NormArgs a) {
-  __shared__ float sum[kNormWaves][64];
-  join_gamma<kNormWaves>(a, blockIdx.x, sum);
+  __shared__ float sum[kNormWaves][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t f = (int64_t)blockIdx.x * 16 + (lane & 15);
+  float t = 0.f;
+  if (f < a.F) {
+#pragma unroll 4
+    for (int b = threadIdx.x >> 4; b < a.row_tiles; b += kNormThreads / 16) t += a.gamma_part[(int64_t)b * a.F + f];
+  }
+  t += __shfl_xor(t, 16, 64);
+  t += __shfl_xor(t, 32, 64);
+  if (lane < 16) sum[wave][lane] = t;
+  __syncthreads();
+  if (threadIdx.x >= 16 || f >= a.F) return;
+  t = 0.f;
+#pragma unroll
+  for (int w = 0; w < kNormWaves; ++w) t += sum[w][lane];
+  a.dgamma[f] = a.accumulate ? a.dgamma[f] + t : t;
 }
 
 // ---- tiles
@@ -493,11 +516,195 @@ __global__ void __launch_bounds__(kTileThreads) rms_norm_grad_kernel(NormArgs a)
   __shared__ double lds[kTileThreads / 256][256];
   const int tiles = a.row_tiles * a.col_tiles;
   if ((int)blockIdx.x >= tiles) {
-    join_gamma<kTileWaves>(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
+    join_gamma(a, (int)blockIdx.x - tiles, reinterpret_cast<float(*)[64]>(&lds[0][0]));
     return;
   }
   if (whole_tile(a, (int)blockIdx.x)) rms_norm_grad_tile<DROP, true>(a, lds);
   else rms_norm_grad_tile<DROP, false>(a, lds);
+}
+
+// ---- rows held
+// Up to kHeldFeatures features: a block holds 32 rows, a line of every column, with all
+// of their features in registers, and one launch does it.  8 lanes go along the rows, 4
+// rows each, and CH times kNormWaves kCols features, of which a wave has kCols side by
+// side.  Behind the last feature a wave reads the last ones again and counts and writes
+// nothing (a test around its loads takes registers that there are not: 8192 x 1024, back,
+// 77 us for 24).
+constexpr int kHeldRows = 32;
+// The blocks of an XCD (every eighth) take row tiles side by side: of an odd number of rows
+// neighbours share lines.
+__device__ __forceinline__ int held_tile(const NormArgs& a) {
+  const int b = (int)blockIdx.x, n = a.row_tiles, x = b % 8;
+  return x * (n / 8) + min(x, n % 8) + b / 8;
+}
+
+template <bool WHOLE>
+struct HeldSeat {
+  static constexpr int kCols = 256 / kHeldRows;  // of a wave, side by side
+  int64_t n0, F, N;          // the block's first row
+  int tile, row, left, f0;   // the lane's first of its rows, how many of them exist; the wave's first feature
+  uint32_t lane_f, j;
+  __device__ __forceinline__ HeldSeat(const NormArgs& a, int bid) : F(a.F), N(a.N), tile(bid) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    row = 4 * (lane & (kHeldRows / 4 - 1));
+    lane_f = lane / (kHeldRows / 4);
+    f0 = kCols * wave;
+    n0 = (int64_t)bid * kHeldRows;
+    j = (uint32_t)row + (uint32_t)a.N * lane_f;
+    left = WHOLE || n0 + row + 4 <= N ? 4 : n0 + row < N ? (int)(N - n0 - row) : 0;
+  }
+  __device__ __forceinline__ bool has(int k) const { return f0 + k * (kNormWaves * kCols) < F; }
+  __device__ __forceinline__ int64_t column(int k) const { return has(k) ? f0 + k * (kNormWaves * kCols) : F - kCols; }
+  __device__ __forceinline__ int64_t at(int k) const { return n0 + N * column(k); }
+  __device__ __forceinline__ f32x4 get(const float* p, int k) const {
+    const float* q = p + at(k) + j;
+    if (WHOLE || left == 4) return f32x4(*reinterpret_cast<const f32x4u*>(q));
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < left) v[e] = q[e];
+    return v;
+  }
+  __device__ __forceinline__ void put(float* p, int k, const f32x4& v) const {
+    if (!has(k)) return;
+    float* q = p + at(k) + j;
+    if (WHOLE || left == 4) {
+      *reinterpret_cast<f32x4u*>(q) = v;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < left) q[e] = v[e];
+  }
+  __device__ __forceinline__ float of_column(const float* p, int k) const { return (p + column(k))[lane_f]; }
+  __device__ __forceinline__ f32x4 drop(const Drop& d, uint64_t z0, int k, f32x4 v) const {
+    const uint64_t z = z0 + (uint64_t)at(k) * kDropoutStep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = dropped(d, z + (uint64_t)e * kDropoutStep, v[e]);
+    return v;
+  }
+};
+
+// The sums over the block's features of the thread's 4 rows.
+__device__ __forceinline__ void held_sums(double (&q)[4], int row, double (*part)[kHeldRows], double* sum) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    for (int o = kHeldRows / 4; o < 64; o <<= 1) q[e] += __shfl_xor(q[e], o, 64);
+    if (lane < kHeldRows / 4) part[wave][row + e] = q[e];
+  }
+  __syncthreads();
+  if (threadIdx.x < kHeldRows) {
+    double v = 0.0;
+#pragma unroll
+    for (int w = 0; w < kNormWaves; ++w) v += part[w][threadIdx.x];
+    sum[threadIdx.x] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 4; ++e) q[e] = sum[row + e];
+}
+
+template <int CH, bool DROP, bool WHOLE>
+__device__ __forceinline__ void rms_norm_held_fwd_tile(const NormArgs& a, int bid, double (*part)[kHeldRows], double* sum) {
+#pragma clang fp contract(off)
+  const HeldSeat<WHOLE> t(a, bid);
+  const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
+  f32x4 s[CH], r[CH];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) s[k] = t.get(a.x, k);
+  if (a.residual) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) r[k] = t.get(a.residual, k);
+  }
+  double q[4] = {};
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    if (DROP) s[k] = t.drop(a.drop, z0, k, s[k]);
+    if (a.residual) s[k] = r[k] + s[k];
+    if (a.sum) t.put(a.sum, k, s[k]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const double v = t.has(k) ? (double)s[k][e] : 0.0;
+      q[e] = fma(v, v, q[e]);
+    }
+  }
+  held_sums(q, t.row, part, sum);
+  f32x4 rstd;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) rstd[e] = inv_sqrt(q[e] * a.inv_f + a.eps);
+  if (a.rstd && threadIdx.x < kHeldRows / 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < t.left) a.rstd[t.n0 + t.row + e] = rstd[e];
+  }
+#pragma unroll
+  for (int k = 0; k < CH; ++k) t.put(a.y, k, (s[k] * rstd) * t.of_column(a.gamma, k));
+}
+template <int CH, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_held_fwd_kernel(NormArgs a) {
+  __shared__ double part[kNormWaves][kHeldRows], sum[kHeldRows];
+  const int bid = held_tile(a);
+  if ((int64_t)(bid + 1) * kHeldRows <= a.N) rms_norm_held_fwd_tile<CH, DROP, true>(a, bid, part, sum);
+  else rms_norm_held_fwd_tile<CH, DROP, false>(a, bid, part, sum);
+}
+
+template <int CH, bool DROP, bool WHOLE>
+__device__ __forceinline__ void rms_norm_held_bwd_tile(const NormArgs& a, int bid, double (*part)[kHeldRows], double* sum) {
+  constexpr int P = CH < 4 ? CH : 4;  // of dsum under way
+  const HeldSeat<WHOLE> t(a, bid);
+  const uint64_t z0 = DROP ? first_word(a.drop) + (uint64_t)t.j * kDropoutStep : 0;
+  f32x4 u[CH], d[CH], p[P], rstd = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < t.left) rstd[e] = a.rstd[t.n0 + t.row + e];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    u[k] = t.get(a.s, k);
+    d[k] = t.get(a.dy, k);
+  }
+  if (a.dsum) {
+#pragma unroll
+    for (int k = 0; k < P; ++k) p[k] = t.get(a.dsum, k);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  double q[4] = {};
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const float g = t.has(k) ? t.of_column(a.gamma, k) : 0.f;
+    float dg = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      u[k][e] *= rstd[e];
+      if (e < t.left) dg = fmaf(d[k][e], u[k][e], dg);
+      d[k][e] *= g;
+      q[e] = t.has(k) ? fma((double)d[k][e], (double)u[k][e], q[e]) : q[e];
+    }
+    for (int o = kHeldRows / 8; o > 0; o >>= 1) dg += __shfl_xor(dg, o, 64);
+    if (t.row == 0 && t.has(k)) (a.gamma_part + (int64_t)t.tile * a.F + t.column(k))[t.lane_f] = dg;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  held_sums(q, t.row, part, sum);
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    f32x4 g;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      g[e] = rstd[e] * fmaf(-u[k][e], (float)(q[e] * a.inv_f), d[k][e]);
+      if (a.dsum) g[e] += p[k % P][e];
+    }
+    if (a.dsum && k + P < CH) p[k % P] = t.get(a.dsum, k + P);
+    __builtin_amdgcn_sched_barrier(0);
+    if (a.dresidual) t.put(a.dresidual, k, g);
+    t.put(a.dx, k, DROP ? t.drop(a.drop, z0, k, g) : g);
+  }
+}
+template <int CH, bool DROP>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_held_bwd_kernel(NormArgs a) {
+  __shared__ double part[kNormWaves][kHeldRows], sum[kHeldRows];
+  const int bid = held_tile(a);
+  if ((int64_t)(bid + 1) * kHeldRows <= a.N) rms_norm_held_bwd_tile<CH, DROP, true>(a, bid, part, sum);
+  else rms_norm_held_bwd_tile<CH, DROP, false>(a, bid, part, sum);
 }
 
 // Features of a thread that a block of few rows holds: in the forward as many as need
@@ -530,6 +737,32 @@ void set_tiles(NormArgs& a) {
   a.col_tiles = (int)((col_tiles + a.chunks - 1) / a.chunks);
 }
 
+// Rows held: their features, at most as many as the registers of a block hold, and a
+// multiple of what a wave has side by side.  Both ways in tiles and held, us: 8192 x 512 42.4
+// and 36.6, 1000 x 512 22.7 and 18.5, 8191 x 512 49 and 35, 131072 x 256 317 and 263, 8192 x
+// 1024 94 and 67; more than 512 features need as many registers as there are and one
+// block's backward runs as long as two launches, so that few rows of them stay with
+// tiles there (1000 x 1024 11.5 + 13.5 and 13.4 + 15.8, 4096 x 1024 20.3 + 23.3 and 15.0 +
+// 31.1, 6000 x 1024 28.3 + 35.4 and 21.8 + 28.5).
+constexpr int kHeldFeatures = 1024;
+bool rows_held(NormArgs& a, bool backward) {
+  if (a.F % (256 / kHeldRows) || a.F > kHeldFeatures || (backward && a.F > 512 && a.N < 6000)) return false;
+  if (a.N >= (int64_t)1 << 26) return false;  // (a grid has fewer than 2^32 threads)
+  a.row_tiles = (int)((a.N + kHeldRows - 1) / kHeldRows);
+  return true;
+}
+// f(the times that a block's threads go through its features)
+template <class F>
+void with_passes(const NormArgs& a, F&& f) {
+  const int n = (int)((a.F * kHeldRows + 4 * kNormThreads - 1) / (4 * kNormThreads));
+  if (n <= 1) f(std::integral_constant<int, 1>{});
+  else if (n <= 2) f(std::integral_constant<int, 2>{});
+  else if (n <= 3) f(std::integral_constant<int, 3>{});
+  else if (n <= 4) f(std::integral_constant<int, 4>{});
+  else if (n <= 6) f(std::integral_constant<int, 6>{});
+  else f(std::integral_constant<int, 8>{});
+}
+
 template <bool DROP>
 int run_forward(NormArgs& a, hipStream_t st, const char* who) {
   const dim3 threads(kNormThreads);
@@ -537,6 +770,12 @@ int run_forward(NormArgs& a, hipStream_t st, const char* who) {
     const int64_t per = ((a.F << a.shift) + kNormThreads - 1) / kNormThreads;
     if (per <= 4) hipLaunchKernelGGL((rms_norm_few_fwd_kernel<4, DROP>), dim3(1), threads, 0, st, a);
     else hipLaunchKernelGGL((rms_norm_few_fwd_kernel<kFewHeld, DROP>), dim3(1), threads, 0, st, a);
+    return check_launch(who);
+  }
+  if (rows_held(a, false)) {
+    with_passes(a, [&](auto n) {
+      hipLaunchKernelGGL((rms_norm_held_fwd_kernel<n.value, DROP>), dim3((unsigned)a.row_tiles), threads, 0, st, a);
+    });
     return check_launch(who);
   }
   set_tiles(a);
@@ -557,18 +796,23 @@ int run_backward(NormArgs& a, hipStream_t st, const char* who) {
   const dim3 threads(kNormThreads);
   const bool few = few_rows(a, kFewHeldBack);
   a.row_tiles = a.col_tiles = a.chunks = 1;
-  if (!few) set_tiles(a);
+  const bool held = !few && rows_held(a, true);
+  if (!few && !held) set_tiles(a);
   const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles, gamma_blocks = (a.F + 63) / 64;
   CNHIP_REQUIRE(tiles + gamma_blocks < ((int64_t)1 << 31), "%s: too large", who);
-  const size_t sums = few ? 0 : (size_t)a.col_tiles * (size_t)a.N * sizeof(double);
+  const size_t sums = few || held ? 0 : (size_t)a.col_tiles * (size_t)a.N * sizeof(double);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, sums + (size_t)a.row_tiles * (size_t)a.F * sizeof(float), &ws, who));
   a.part = static_cast<double*>(ws);
   a.gamma_part = reinterpret_cast<float*>(static_cast<char*>(ws) + sums);
-  if (few) {
-    hipLaunchKernelGGL((rms_norm_few_bwd_kernel<kFewHeldBack, DROP>), dim3(1), threads, 0, st, a);
+  if (few || held) {
+    if (few) hipLaunchKernelGGL((rms_norm_few_bwd_kernel<kFewHeldBack, DROP>), dim3(1), threads, 0, st, a);
+    else
+      with_passes(a, [&](auto n) {
+        hipLaunchKernelGGL((rms_norm_held_bwd_kernel<n.value, DROP>), dim3((unsigned)a.row_tiles), threads, 0, st, a);
+      });
     CNHIP_TRY(check_launch(who));
-    hipLaunchKernelGGL(rms_norm_gamma_kernel, dim3((unsigned)gamma_blocks), threads, 0, st, a);
+    hipLaunchKernelGGL(rms_norm_gamma_kernel, dim3((unsigned)((a.F + 15) / 16)), threads, 0, st, a);
     return check_launch(who);
   }
   const dim3 grid((unsigned)tiles), more((unsigned)(tiles + gamma_blocks)), tile_threads(kTileThreads);

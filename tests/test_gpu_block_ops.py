@@ -265,6 +265,11 @@ NORM = [  # N, F, p, residual, dsum
     (64, 513, 0.1, False, True), (257, 512, 0.1, True, True), (100, 2000, 0.0, True, True), (1000, 40, 0.0, True, False),
     (45, 4099, 0.1, True, True), (70, 2049, 0.0, True, True), (5, 20001, 0.2, True, True), (20000, 12, 0.0, True, True),
     (16500, 64, 0.1, True, True), (1300, 6001, 0.1, True, True), (2100, 8300, 0.0, True, False),  # several tiles a block
+    # features a multiple of 8, up to 1024, and next to that
+    (34, 8, 0.0, True, True), (95, 24, 0.2, True, True), (63, 128, 0.0, False, False), (65, 136, 0.1, True, True),
+    (100, 256, 0.0, True, True), (131, 336, 0.1, True, False), (96, 384, 0.0, False, True), (70, 520, 0.0, True, True),
+    (47, 768, 0.3, True, True), (6001, 1024, 0.1, True, True), (6040, 776, 0.0, True, True), (700, 640, 0.0, True, True),
+    (300, 1032, 0.0, True, True), (1000, 39, 0.1, True, True), (20000, 13, 0.0, True, True), (16500, 65, 0.1, True, True),
 ]
 
 
