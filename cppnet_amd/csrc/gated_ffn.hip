@@ -20,6 +20,7 @@
 // 2048 4.7 us.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "act_math.hpp"
@@ -37,14 +38,19 @@ using pr::f32x4u;
 struct FfnScales {
   uint32_t w, x, z;
 };
-// What the blocks that look for them found: of W, X and dZ.
-// The forward runs in half tiles, two to a CU, of which one stores while the other
-// computes, and which leave less of a small call's grid empty (half and whole tiles, us:
-// 1021 x 513 -> 1365 both directions 103.6 and 108.7, 256 x 1024 -> 4096 50 and 55, 8192 x
-// 1024 -> 4096 393 and 386); the backward in whole ones (half tiles across the rows of
-// both operands need more registers than there are).
+// The products' tiles.  The forward's are Half, two to a CU, of which one stores while the
+// other computes, which leaves less of a call's grid empty (half and whole tiles, us: 1021 x
+// 513 -> 1365 both directions 103.6 and 108.7, 256 x 1024 -> 4096 50 and 55, 8192 x 1024 ->
+// 4096 393 and 386), or Small; the backward's Whole (half tiles across the rows of both
+// operands need more registers than there are) or Small: where there are few tiles these
+// need fewer splits or none and pad less, and a step of them costs half as much again for
+// a product (Small and the others, kernels with the joining of splits, us: 1021 x 513 ->
+// 1365 forward 21 and 30, back 40 and 50; 1024 x 512 -> 2048 22 and 32.5, 41 and 60; 512 x
+// 512 -> 2048 back 27 and 38; 2048 x 1024 -> 4096 127 and 104, 227 and 207).
 using Half = pr::Tile<2>;
 using Whole = pr::Tile<4>;
+using Small = pr::Tile<2, 2, 2>;
+// What the blocks that look for them found: of W, X and dZ.
 constexpr int kMaxBlocks[3] = {256, 256, 512};
 constexpr int kMaxAt[3] = {0, 256, 512}, kMaxParts = 1024;
 
@@ -194,29 +200,30 @@ __global__ void __launch_bounds__(1024) ffn_pack_own_kernel(FfnArgs a, int w_blo
 }
 
 // A: W^T (M: packed columns), B: X (N: rows); H and, where it is kept, Z.
-__global__ void __launch_bounds__(Half::NT, 2) ffn_forward_kernel(pr::GemmArgs g, FfnArgs a, float* part) {
-  __shared__ __align__(16) char lds[Half::kLds];
+template <class T>
+__global__ void __launch_bounds__(T::NT, 2) ffn_forward_kernel(pr::GemmArgs g, FfnArgs a, float* part) {
+  __shared__ __align__(16) char lds[T::kLds];
   int tm, tn;
-  pr::tile_of((int)blockIdx.x, (g.M + pr::TM - 1) / pr::TM, (g.N + Half::TN - 1) / Half::TN, tm, tn);
-  pr::Acc acc;
+  pr::tile_of((int)blockIdx.x, (g.M + T::TM - 1) / T::TM, (g.N + T::TN - 1) / T::TN, tm, tn);
+  pr::AccOf<T::MI> acc;
   const int t0 = (int)blockIdx.y * g.steps_per_split;
-  pr::gemm_tile<false, false, Half>(g, tm, tn, t0, min(g.steps, t0 + g.steps_per_split), lds, acc);
+  pr::gemm_tile<false, false, T>(g, tm, tn, t0, min(g.steps, t0 + g.steps_per_split), lds, acc);
   if (part) {
-    pr::put_tile<false, Half>(acc, tm, tn, g.M, g.N, part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float x) { return x; });
+    pr::put_tile<false, T>(acc, tm, tn, g.M, g.N, part + (int64_t)blockIdx.y * g.M * g.N, g.N, [](float x) { return x; });
     return;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int block0 = tm * (pr::TM / 32) + (wave / Half::WN) * 4;  // the wave's first of 32 packed columns: a gate's
-  const int64_t n0 = (int64_t)tn * Half::TN + (wave % Half::WN) * 64 + (lane & 31);
+  const int lane = threadIdx.x & 63;
+  const int block0 = (tm * T::TM + T::row0()) / 32;  // the wave's first of 32 packed columns: a gate's
+  const int64_t n0 = (int64_t)tn * T::TN + T::column(0);
   // A test for every element would end the run of loads, functions and stores behind it
   // (1024 rows, 64 -> 1024: 24 us for 12; 8192 rows, 1024 -> 4096 475 us for 411), so the activation and whole tiles are told
   // apart here.
   with_act(a.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
+    for (int i = 0; i < T::MI; i += 2) {
       if (block0 + i >= g.M / 32) break;
       const int64_t first = (int64_t)(block0 + i) * 16, f0 = first + 4 * (lane >> 5);
-      const bool whole = first + 32 <= a.F && (int64_t)tn * Half::TN + (wave % Half::WN) * 64 + 64 <= a.N;
+      const bool whole = first + 32 <= a.F && n0 - (lane & 31) + 32 * T::J <= a.N;
       auto row = [](int e) { return 8 * (e / 4) + e % 4; };
       float bg[16], bu[16];
 #pragma unroll
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(Half::NT, 2) ffn_forward_kernel(pr::GemmArgs g
         bu[e] = a.b ? a.b[a.F + f] : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < T::J; ++j) {
         const int64_t n = n0 + 32 * j;
         const int ex = a.xe[n < a.N ? n : a.N - 1], eg = -ex - a.we[block0 + i], eu = -ex - a.we[block0 + i + 1];
         float h[16];
@@ -636,35 +643,35 @@ struct FfnProduct {
 
 // dX (A: W across its rows, B: dZ), COLS false, and dW (A: dZ, B: X, both across
 // their rows), COLS true.
-template <bool TA, bool TB, bool COLS>
+template <class T, bool TA, bool TB, bool COLS>
 __device__ __forceinline__ void ffn_product(const FfnProduct& p, const FfnArgs& a, int bid, char* lds) {
   const pr::GemmArgs& g = p.g;
   const FfnOut& o = p.o;
   int tm, tn;
   const int split = bid / p.tiles;
-  pr::tile_of(bid % p.tiles, (g.M + pr::TM - 1) / pr::TM, (g.N + Whole::TN - 1) / Whole::TN, tm, tn);
+  pr::tile_of(bid % p.tiles, (g.M + T::TM - 1) / T::TM, (g.N + T::TN - 1) / T::TN, tm, tn);
   const int t0 = split * g.steps_per_split, t1 = min(g.steps, t0 + g.steps_per_split);
-  pr::Acc acc;
-  pr::gemm_tile<TA, TB, Whole>(g, tm, tn, t0, t1, lds, acc);
+  pr::AccOf<T::MI> acc;
+  pr::gemm_tile<TA, TB, T>(g, tm, tn, t0, t1, lds, acc);
   if (o.part) {
-    pr::put_tile<false, Whole>(acc, tm, tn, g.M, g.N, o.part + (int64_t)split * g.M * g.N, g.N, [](float x) { return x; });
+    pr::put_tile<false, T>(acc, tm, tn, g.M, g.N, o.part + (int64_t)split * g.M * g.N, g.N, [](float x) { return x; });
     return;
   }
   const int eo = scale_out<COLS>(a);
   auto value = [&](float x) { return pr::times_exp2(x, eo); };
   if constexpr (!COLS) {
-    pr::put_tile<false, Whole>(acc, tm, tn, g.M, g.N, o.p, o.ld, value);
+    pr::put_tile<false, T>(acc, tm, tn, g.M, g.N, o.p, o.ld, value);
   } else {
     // blocks of 32 packed columns lie together in the output: the even ones from its
     // start on, the odd ones from column F on
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = tn * Whole::TN + (wave % Whole::WN) * 64 + 32 * j + (lane & 31);
+    for (int j = 0; j < T::J; ++j) {
+      const int n = tn * T::TN + T::column(j);
       if (n >= g.N) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t blk = (int64_t)tm * (pr::TM / 32) + (wave / Whole::WN) * 4 + i;
+      for (int i = 0; i < T::MI; ++i) {
+        const int64_t blk = (tm * T::TM + T::row0()) / 32 + i;
         const int64_t f = (blk >> 1) * 32 + 4 * (lane >> 5), left = a.F - f;
         float* q = o.p + n + o.ld * (f + (blk & 1) * a.F);
         auto row = [](int e) { return 8 * (e / 4) + e % 4; };
@@ -692,20 +699,21 @@ __device__ __forceinline__ void ffn_product(const FfnProduct& p, const FfnArgs& 
 
 // Both products, and db (+)= the sums of the groups of rows, in order, in the blocks
 // behind them.
-__global__ void __launch_bounds__(Whole::NT, 2) ffn_grads_kernel(FfnArgs a, FfnProduct x, FfnProduct w, float* db, int add) {
-  __shared__ __align__(16) char lds[Whole::kLds];
+template <class T>
+__global__ void __launch_bounds__(T::NT, 2) ffn_grads_kernel(FfnArgs a, FfnProduct x, FfnProduct w, float* db, int add) {
+  __shared__ __align__(16) char lds[T::kLds];
   int bid = (int)blockIdx.x;
   if (bid < x.tiles * x.splits) {
-    ffn_product<true, false, false>(x, a, bid, lds);
+    ffn_product<T, true, false, false>(x, a, bid, lds);
     return;
   }
   bid -= x.tiles * x.splits;
   if (bid < w.tiles * w.splits) {
-    ffn_product<true, true, true>(w, a, bid, lds);
+    ffn_product<T, true, true, true>(w, a, bid, lds);
     return;
   }
   bid -= w.tiles * w.splits;
-  const int64_t v = (int64_t)bid * Whole::NT + threadIdx.x, blocks = (a.R + 31) / 32;
+  const int64_t v = (int64_t)bid * T::NT + threadIdx.x, blocks = (a.R + 31) / 32;
   if (v >= 2 * a.F) return;
   float s = 0.f;
 #pragma unroll 16
@@ -736,7 +744,7 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(FfnArgs a, FfnProduct x
 
 template <class T>
 int64_t tiles_of(int64_t M, int64_t N) {
-  return (M + pr::TM - 1) / pr::TM * ((N + T::TN - 1) / T::TN);
+  return (M + T::TM - 1) / T::TM * ((N + T::TN - 1) / T::TN);
 }
 int64_t pad32(int64_t n) { return (n + 31) / 32 * 32; }
 
@@ -758,39 +766,63 @@ int check_shape(int64_t N, int64_t D, int64_t F, int act, const char* who) {
   return CNHIP_OK;
 }
 
-// Steps of a block where all the products of a launch are done soonest: the rounds of
-// blocks that run together, a block's own time with what its beginning and end take,
-// and what split sums move.  Half tiles: one on a CU takes half the time of two.
 struct Job {
   int64_t M, N;
   int steps;
 };
+struct Plan {
+  int per[2] = {};  // steps of a block of each product
+  double us = 0;
+};
+// What a step costs a block that has the chip's caches to itself and one among as many as
+// run at a time, us; steps that a block's beginning and end take, where it stores split
+// sums and where it does not; bytes of split sums a us.
+struct Rates {
+  double light, full, ends_split, ends, bytes;
+  int slots;  // blocks at a time
+};
+// Read off the kernels' times for 13 shapes from 300 x 256 -> 512 to 16384 x 128 -> 256 and 2048 x
+// 1024 -> 4096, which these give again to some 15%.
 template <class T>
-int steps_of(const Job* jobs, int n) {
-  constexpr bool kHalf = T::WN == 2;
-  constexpr double kStepUs = kHalf ? 1.2 : 1.55, kEnds = kHalf ? 6 : 8, kBytesUs = kHalf ? 8e6 : 5e6;
-  constexpr int64_t kSlots = kHalf ? 512 : 256;
-  int longest = 2, best = 0;
+constexpr Rates kRates = T::G == 2   ? Rates{0.28, 0.42, 18, 18, 6e6, 256}
+                         : T::WN == 2 ? Rates{0.75, 1.2, 7, 17, 8e6, 512}
+                                      : Rates{1.45, 1.45, 8, 8, 9e6, 256};
+int even(int64_t n) { return (int)((n + 1) / 2 * 2); }
+// The splits where all the products of a launch are done soonest.
+template <class T>
+Plan plan_of(const Job* jobs, int n) {
+  constexpr Rates r = kRates<T>;
+  int longest = 2;
   for (int i = 0; i < n; ++i) longest = jobs[i].steps > longest ? jobs[i].steps : longest;
-  double least = 0;
+  Plan best;
   for (int parts = 1; parts <= 64; ++parts) {
-    const int per = ((longest + parts - 1) / parts + 1) / 2 * 2;
-    if (parts > 1 && per < 6) break;
-    int64_t blocks = 0;
-    double moved = 0;
+    const int most = even((longest + parts - 1) / parts);
+    if (parts > 1 && most < 6) break;
+    Plan p;
+    double moved = 0, work = 0, blocks = 0, block = 0;
     for (int i = 0; i < n; ++i) {
-      const int64_t splits = (jobs[i].steps + per - 1) / per;
-      blocks += tiles_of<T>(jobs[i].M, jobs[i].N) * splits;
-      if (splits > 1) moved += 8.0 * (double)splits * (double)jobs[i].M * (double)jobs[i].N;
+      const int steps = jobs[i].steps, alike = (steps + most - 1) / most;
+      p.per[i] = even((steps + alike - 1) / alike);
+      const int splits = (steps + p.per[i] - 1) / p.per[i];
+      const double b = (double)(tiles_of<T>(jobs[i].M, jobs[i].N) * splits), own = p.per[i] + (splits > 1 ? r.ends_split : r.ends);
+      blocks += b;
+      work += b * own;
+      block = own > block ? own : block;
+      if (splits > 1) moved += 8.0 * splits * (double)jobs[i].M * (double)jobs[i].N;
     }
-    const double rounds = kHalf && blocks <= 256 ? 0.625 : (double)((blocks + kSlots - 1) / kSlots);
-    const double us = rounds * (per + kEnds) * kStepUs + moved / kBytesUs + (moved > 0 ? 3.0 : 0.0);
-    if (best == 0 || us < least) {
-      least = us;
-      best = per;
-    }
+    const double rounds = work / block / r.slots;
+    const double step = T::G == 2 ? r.full * rounds : blocks <= 256 ? r.light : r.full * std::ceil(rounds);
+    p.us = 3 + block * (step > r.light ? step : r.light) + (moved > 0 ? 4 + moved / r.bytes : 0);
+    if (best.us == 0 || p.us < best.us) best = p;
+    if (blocks > 4 * r.slots) break;  // more of them win nothing
   }
   return best;
+}
+// f(a tile): Small's or T
+template <class T, class F>
+void with_tile(bool small, F&& f) {
+  if (small) f(Small{});
+  else f(T{});
 }
 
 int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
@@ -804,13 +836,15 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
     return check_launch(who);
   }
   a.steps_d = (int)(pad32(D) / 16);
-  CNHIP_REQUIRE(tiles_of<Half>(2 * Fp, N) < ((int64_t)1 << 23), "%s: too large", who);
+  CNHIP_REQUIRE(tiles_of<Small>(2 * Fp, N) < ((int64_t)1 << 23), "%s: too large", who);
   Places w;
   const size_t o_x = w.place((size_t)(pad32(N) * pad32(D)) * 4), o_w = w.place((size_t)(2 * Fp * pad32(D)) * 4),
                o_xe = w.place((size_t)N * 4), o_we = w.place((size_t)(2 * Fp / 32) * 4);
   const Job job{2 * Fp, N, a.steps_d};
   // (a row of the grid for every feature joins the splits)
-  const int per = F < 65536 ? steps_of<Half>(&job, 1) : a.steps_d, splits = (a.steps_d + per - 1) / per;
+  const Plan half = plan_of<Half>(&job, 1), few = plan_of<Small>(&job, 1);
+  const bool small = few.us < half.us;
+  const int per = F < 65536 ? (small ? few : half).per[0] : a.steps_d, splits = (a.steps_d + per - 1) / per;
   const size_t o_part = w.place(splits > 1 ? (size_t)(splits * 2 * Fp * N) * 4 : 0);
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, w.at, &ws, who));
@@ -825,8 +859,11 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
   const pr::GemmArgs g{pr::Packed{a.wp, (int)(2 * Fp / 32), a.steps_d}, pr::Packed{a.xp, (int)(pad32(N) / 32), a.steps_d},
                        (int)(2 * Fp), (int)N, a.steps_d, per, a.steps_d / 2};
   float* part = splits > 1 ? reinterpret_cast<float*>(base + o_part) : nullptr;
-  hipLaunchKernelGGL(ffn_forward_kernel, dim3((unsigned)tiles_of<Half>(2 * Fp, N), (unsigned)splits), dim3(Half::NT), 0, st,
-                     g, a, part);
+  with_tile<Half>(small, [&](auto t) {
+    using T = decltype(t);
+    hipLaunchKernelGGL(ffn_forward_kernel<T>, dim3((unsigned)tiles_of<T>(2 * Fp, N), (unsigned)splits), dim3(T::NT), 0, st, g,
+                       a, part);
+  });
   CNHIP_TRY(check_launch(who));
   if (!part) return CNHIP_OK;
   hipLaunchKernelGGL(ffn_join_kernel, dim3((unsigned)((N + 255) / 256), (unsigned)F), dim3(256), 0, st, a, part, 2 * Fp,
@@ -863,13 +900,15 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
   if (R > N) R = N;
   const int64_t Rp = pad32(R);
   const Job jobs[2] = {{D, R, 2 * a.steps_f}, {2 * Fp, D, (int)(Rp / 16)}};
-  const int per = steps_of<Whole>(jobs, 2);
-  auto parts = [&](const Job& j) {
-    const int64_t splits = (j.steps + per - 1) / per;
-    return splits > 1 ? (size_t)(splits * j.M * j.N) * 4 : 0;
+  const Plan whole = plan_of<Whole>(jobs, 2), few = plan_of<Small>(jobs, 2);
+  const bool small = few.us < whole.us;
+  const Plan& plan = small ? few : whole;
+  auto parts = [&](int i) {
+    const int64_t splits = (jobs[i].steps + plan.per[i] - 1) / plan.per[i];
+    return splits > 1 ? (size_t)(splits * jobs[i].M * jobs[i].N) * 4 : 0;
   };
-  CNHIP_REQUIRE(tiles_of<Whole>(D, R) * ((2 * a.steps_f + per - 1) / per) +
-                        tiles_of<Whole>(2 * Fp, D) * ((Rp / 16 + per - 1) / per) <
+  CNHIP_REQUIRE(tiles_of<Small>(D, R) * ((2 * a.steps_f + plan.per[0] - 1) / plan.per[0]) +
+                        tiles_of<Small>(2 * Fp, D) * ((Rp / 16 + plan.per[1] - 1) / plan.per[1]) <
                     ((int64_t)1 << 22),
                 "%s: too large", who);
   // blocks of 32 rows of dZ a wave: as many as leave 4096 waves, so that a wave that has
@@ -880,7 +919,7 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
   const size_t o_max = w.place(kMaxParts * 4 + sizeof(FfnScales)), o_x = w.place((size_t)(Rp * Dp) * 4),
                o_w = w.place((size_t)(2 * Fp * Dp) * 4), o_z = w.place((size_t)(Rp * 2 * Fp) * 4),
                o_db = w.place(db ? (size_t)((Rp / 32 + a.z_blocks - 1) / a.z_blocks * 2 * F) * 4 : 0),
-               o_px = w.place(parts(jobs[0])), o_pw = w.place(parts(jobs[1]));
+               o_px = w.place(parts(0)), o_pw = w.place(parts(1));
   void* ws = nullptr;
   CNHIP_TRY(scratch(st, kScratchLayer, w.at, &ws, who));
   char* base = static_cast<char*>(ws);
@@ -891,11 +930,12 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
   a.zp = base + o_z;
   a.db_part = db ? reinterpret_cast<float*>(base + o_db) : nullptr;
   const pr::Packed pw_{a.wp, (int)(2 * Fp / 32), a.steps_d};
-  auto product = [&](const pr::Packed& A, const pr::Packed& B, int64_t M, int64_t Nn, int steps, float* p, int64_t ld,
-                     float* part, int add) {
+  auto product = [&](const pr::Packed& A, const pr::Packed& B, int64_t M, int64_t Nn, int steps, int per, float* p,
+                     int64_t ld, float* part, int add) {
     const int splits = (steps + per - 1) / per;
     return FfnProduct{pr::GemmArgs{A, B, (int)M, (int)Nn, steps, per, steps / 2},
-                      FfnOut{p, ld, splits > 1 ? part : nullptr, add}, (int)tiles_of<Whole>(M, Nn), splits};
+                      FfnOut{p, ld, splits > 1 ? part : nullptr, add},
+                      (int)(small ? tiles_of<Small>(M, Nn) : tiles_of<Whole>(M, Nn)), splits};
   };
   for (int64_t r0 = 0; r0 < N; r0 += R) {
     a.row0 = r0;
@@ -916,11 +956,13 @@ int run_backward(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hi
     CNHIP_TRY(check_launch(who));
     const int add = accumulate || r0 > 0;
     const pr::Packed px_{a.xp, rb, a.steps_d}, pz_{a.zp, rb, 2 * a.steps_f};
-    const FfnProduct x = product(pw_, pz_, D, a.R, 2 * a.steps_f, dX + r0, N, reinterpret_cast<float*>(base + o_px), 0),
-                     y = product(pz_, px_, 2 * Fp, D, 2 * rb, dW, D, reinterpret_cast<float*>(base + o_pw), add);
-    const int64_t blocks =
-        (int64_t)x.tiles * x.splits + (int64_t)y.tiles * y.splits + (db ? (2 * F + Whole::NT - 1) / Whole::NT : 0);
-    hipLaunchKernelGGL(ffn_grads_kernel, dim3((unsigned)blocks), dim3(Whole::NT), 0, st, a, x, y, db, add);
+    const FfnProduct x = product(pw_, pz_, D, a.R, 2 * a.steps_f, plan.per[0], dX + r0, N, reinterpret_cast<float*>(base + o_px), 0),
+                     y = product(pz_, px_, 2 * Fp, D, 2 * rb, plan.per[1], dW, D, reinterpret_cast<float*>(base + o_pw), add);
+    with_tile<Whole>(small, [&](auto t) {
+      using T = decltype(t);
+      const int64_t blocks = (int64_t)x.tiles * x.splits + (int64_t)y.tiles * y.splits + (db ? (2 * F + T::NT - 1) / T::NT : 0);
+      hipLaunchKernelGGL(ffn_grads_kernel<T>, dim3((unsigned)blocks), dim3(T::NT), 0, st, a, x, y, db, add);
+    });
     CNHIP_TRY(check_launch(who));
     if (!x.o.part && !y.o.part) continue;
     auto reduce_blocks = [](const FfnProduct& q) { return q.o.part ? (int64_t)q.g.M * ((q.g.N + 255) / 256) : 0; };

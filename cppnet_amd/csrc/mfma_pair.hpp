@@ -158,21 +158,32 @@ struct GemmArgs {
   int half;              // the step where the second half begins
 };
 
-// A block of 2 x WN waves takes a tile of 256 x 64 WN.  WN = 4: one block to a CU, with
-// four LDS buffers for the steps; WN = 2: two, with three each, of which one computes
-// while the other stores its tile.
-constexpr int TM = 256;
-template <int WN_>
+// A block of 2 x WN waves, each with 32 MI x 64 of the product, takes a tile of 64 MI x 64
+// WN.  WN = 4: one block to a CU, with four LDS buffers for the steps; WN = 2: two, with
+// three each, of which one computes while the other stores its tile.  G = 2, for products
+// of few tiles: two such groups of waves, four buffers each, share the steps of a tile of
+// 128 x 128, so that a SIMD still has two waves, and exchange their sums in LDS: each
+// ends with one of the two blocks of 32 columns.
+template <int WN_, int MI_ = 4, int G_ = 1>
 struct Tile {
-  static constexpr int WN = WN_, TN = 64 * WN, NT = 128 * WN;
-  static constexpr int A = 16, B = 4 * WN;           // pieces of 1024 bytes a step
+  static constexpr int WN = WN_, MI = MI_, G = G_, TM = 64 * MI, TN = 64 * WN, NT = 128 * WN * G;
+  static constexpr int J = 2 / G;                    // blocks of 32 columns that a wave ends with
+  static constexpr int A = 4 * MI, B = 4 * WN;       // pieces of 1024 bytes a step
   static constexpr int kStage = (A + B) * kFrag;
-  static constexpr int kStages = WN == 4 ? 4 : 3;
-  static constexpr int kLds = kStages * kStage;
+  static constexpr int kStages = WN == 4 || G == 2 ? 4 : 3;
+  static constexpr int kLds = G * kStages * kStage;
   static constexpr int kCopies = (A + B) / (2 * WN);  // a wave's of a step
-  static_assert(WN == 2 || WN == 4, "waves along the columns");
+  static_assert(G == 2 ? WN == 2 && MI == 2 : MI == 4 && (WN == 2 || WN == 4), "tiles");
+  static __device__ __forceinline__ int wave() {
+    const int w = threadIdx.x >> 6;
+    return G == 1 ? w : w % (2 * WN);
+  }
+  static __device__ __forceinline__ int group() { return G == 1 ? 0 : (int)(threadIdx.x >> 6) / (2 * WN); }
+  // the wave's first row and, of its block j, this lane's column in the tile
+  static __device__ __forceinline__ int row0() { return wave() / WN * (32 * MI); }
+  static __device__ __forceinline__ int column(int j) { return wave() % WN * 64 + 32 * (j + group()) + (int)(threadIdx.x & 31); }
 };
-constexpr int TN = Tile<4>::TN, GNT = Tile<4>::NT, kGemmLds = Tile<4>::kLds;
+constexpr int TM = Tile<4>::TM, TN = Tile<4>::TN, GNT = Tile<4>::NT, kGemmLds = Tile<4>::kLds;
 
 // Staging of one operand: PIECES pieces of 1024 bytes a step, PER a wave.
 //   TR false: piece j = plane j & 1 of the fragment of row block j / 2
@@ -184,8 +195,8 @@ struct Stage {
   const char* src[PER];
   int64_t step;  // bytes per step (TR: per two steps)
   int lds[PER];
-  __device__ __forceinline__ void init(const Packed& o, int tile) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __device__ __forceinline__ void init(const Packed& o, int tile, int wave) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int j = PER * wave + u;
@@ -228,14 +239,17 @@ __device__ __forceinline__ f16x8 flip(f16x8 x, uint32_t sign) {
   return __builtin_bit_cast(f16x8, w);
 }
 
-// What a wave holds: 4 x 2 accumulators, block (i, j) rows 32 i .. of its 128
+// What a wave holds: MI x 2 accumulators, block (i, j) rows 32 i .. of its 32 MI
 // (row 8 (e / 4) + 4 (lane / 32) + e % 4 in element e), columns 32 j + lane % 32
 // of its 64.
-struct Acc {
-  f32x16 x[4][2];
+template <int MI>
+struct AccOf {
+  f32x16 x[MI][2];
 };
+using Acc = AccOf<4>;
+template <int MI>
 struct Frags {
-  f16x8 a[4][2], b[2][2];
+  f16x8 a[MI][2], b[2][2];
 };
 
 // Block -> tile.  Consecutive blocks go to the 8 XCDs in turn; each XCD takes
@@ -250,21 +264,31 @@ __device__ __forceinline__ void tile_of(int bid, int nm, int nn, int& tm, int& t
   tn = in / size;
 }
 
-// The contraction [t0, t1) of a tile; the sums' sign is right.  The steps go
+// The contraction [t0, t1) of a tile; the sums' sign is right, and with two groups a
+// wave's are in x[.][0].  The steps go
 // through four LDS buffers (three), three (two) on their way while one is read;
 // the fragments of the next step are read while this one's MFMAs run.
 template <bool TA, bool TB, class T = Tile<4>>
-__device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int t0, int t1, char* lds, Acc& acc) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int t0, int t1, char* lds,
+                                          AccOf<T::MI>& acc) {
   constexpr int kStage = T::kStage, kStages = T::kStages, kCopies = T::kCopies, kBehind = T::A * kFrag;
-  constexpr int kOfA = T::A / (2 * T::WN), kSlots = 12 / kCopies;
-  const int wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+  constexpr int MI = T::MI, kOfA = T::A / (2 * T::WN), kTurns = 3 * MI, kReads = 2 * MI + 4, kSlots = kTurns / kCopies;
+  const int wave = T::wave(), wm = wave / T::WN, wn = wave % T::WN;
+  // two groups: the steps of the first, which are as many as the second's or two more
+  const int shared = T::G == 1 ? 0 : ((t1 - t0) / 2 + 1) / 2 * 2;
+  char* const box = lds;
+  if (T::G == 2) {
+    lds += __builtin_amdgcn_readfirstlane(T::group()) * (T::kStages * T::kStage);
+    if (__builtin_amdgcn_readfirstlane(T::group())) t0 += shared;
+    else t1 = t0 + shared;
+  }
   Stage<TA, T::A, kOfA> sa;
   Stage<TB, T::B, kCopies - kOfA> sb;
   auto buffer = [&](int t) { return lds + (kStages == 4 ? t & 3 : (int)((unsigned)t % 3u)) * kStage; };
-  sa.init(g.a, tm);
-  sb.init(g.b, tn);
+  sa.init(g.a, tm, wave);
+  sb.init(g.b, tn, wave);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc.x[i][j] = f32x16{};
   // piece u (0 .. kCopies - 1) of step t's copies; past the last step the last is
@@ -275,22 +299,22 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
     if (u < kOfA) sa.copy(s, u, buf);
     else sb.copy(s, u - kOfA, buf + kBehind);
   };
-  // fragment u (0 .. 11) of step t, in the order of their first use
-  auto read = [&](int t, int odd, int u, Frags& f) {
+  // fragment u (0 .. kReads - 1) of step t, in the order of their first use
+  auto read = [&](int t, int odd, int u, Frags<MI>& f) {
     const char* buf = buffer(t);
     if (u < 2) f.b[u][0] = frag<TB>(buf + kBehind, 2 * wn + u, 0, odd);
-    else if (u < 6) f.a[u - 2][1] = frag<TA>(buf, 4 * wm + u - 2, 1, odd);
-    else if (u < 8) f.b[u - 6][1] = frag<TB>(buf + kBehind, 2 * wn + u - 6, 1, odd);
-    else f.a[u - 8][0] = frag<TA>(buf, 4 * wm + u - 8, 0, odd);
+    else if (u < MI + 2) f.a[u - 2][1] = frag<TA>(buf, MI * wm + u - 2, 1, odd);
+    else if (u < MI + 4) f.b[u - MI - 2][1] = frag<TB>(buf + kBehind, 2 * wn + u - MI - 2, 1, odd);
+    else f.a[u - MI - 4][0] = frag<TA>(buf, MI * wm + u - MI - 4, 0, odd);
   };
-  Frags f0, f1;
-  auto step = [&](int t, int odd, Frags& now, Frags& next) {
+  Frags<MI> f0, f1;
+  auto step = [&](int t, int odd, Frags<MI>& now, Frags<MI>& next) {
     // step t + 1 has arrived (the younger ones may be on their way), and every
     // wave holds step t in registers: its buffer is free
     wait_and_meet<(kStages - 2) * kCopies>();
     if (t == g.half) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc.x[i][j] = -acc.x[i][j];
     }
@@ -298,14 +322,16 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
     // a MFMA keeps the matrix pipe for 32 cycles and the wave for 4: the reads,
     // copies and sign changes go between them
 #pragma unroll
-    for (int u = 0; u < 12; ++u) {
-      const int i = u % 4, x = u < 4 ? 1 : 0, y = u >= 4 && u < 8 ? 1 : 0;
-      if (u < 8) now.a[i][x] = flip(now.a[i][x], sign);
+    for (int u = 0; u < kTurns; ++u) {
+      const int i = u % MI, x = u < MI ? 1 : 0, y = u >= MI && u < 2 * MI ? 1 : 0;
+      if (u < 2 * MI) now.a[i][x] = flip(now.a[i][x], sign);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         acc.x[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now.a[i][x], now.b[j][y], acc.x[i][j], 0, 0, 0);
-      read(t + 1, 1 - odd, u, next);
-      if (u % kSlots == 0) copy(t + kStages, u / kSlots);
+      constexpr int kTwo = kReads - kTurns;  // turns that read two
+      read(t + 1, 1 - odd, u < kTwo ? 2 * u : u + kTwo, next);
+      if (u < kTwo) read(t + 1, 1 - odd, 2 * u + 1, next);
+      if (u % kSlots == 0 && u / kSlots < kCopies) copy(t + kStages, u / kSlots);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -315,18 +341,42 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
     for (int u = 0; u < kCopies; ++u) copy(t0 + t, u);
   wait_and_meet<(kStages - 1) * kCopies>();
 #pragma unroll
-  for (int u = 0; u < 12; ++u) read(t0, 0, u, f0);
+  for (int u = 0; u < kReads; ++u) read(t0, 0, u, f0);
   // t0 is even, so a step's parity, and with it the slots, is known here
   for (int t = t0; t < t1; t += 2) {
     step(t, 0, f0, f1);
     if (t + 1 < t1) step(t + 1, 1, f1, f0);
   }
+  if (T::G == 2) {  // both groups meet equally often
+    for (int t = t1 - t0; t < shared; ++t) wait_and_meet<0>();
+  }
   wait_and_meet<0>();  // the copies that went past the end
   if (t1 > g.half) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) acc.x[i][j] = -acc.x[i][j];
+  }
+  if constexpr (T::G == 2) {
+    const int lane = threadIdx.x & 63, from = __builtin_amdgcn_readfirstlane(T::group());
+    f32x4* to = reinterpret_cast<f32x4*>(box) + (threadIdx.x >> 6) * (4 * MI * 64) + lane;
+    const f32x4* other = reinterpret_cast<const f32x4*>(box) + ((threadIdx.x >> 6) ^ 4) * (4 * MI * 64) + lane;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const f32x16 give = from ? acc.x[i][0] : acc.x[i][1];
+      if (from) acc.x[i][0] = acc.x[i][1];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) to[(4 * i + q) * 64] = f32x4{give[4 * q], give[4 * q + 1], give[4 * q + 2], give[4 * q + 3]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 v = other[(4 * i + q) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc.x[i][0][4 * q + e] += v[e];
+      }
   }
 }
 
@@ -334,31 +384,31 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, int tm, int tn, int
 // this lane holds and that exist.  ADD reads all of a column before it writes
 // one, so the reads are under way together.
 template <bool ADD, class T = Tile<4>, class F>
-__device__ __forceinline__ void put_tile(const Acc& acc, int tm, int tn, int M, int N, float* __restrict__ p,
+__device__ __forceinline__ void put_tile(const AccOf<T::MI>& acc, int tm, int tn, int M, int N, float* __restrict__ p,
                                          int64_t ld, F&& value) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = tm * TM + (wave / T::WN) * 128, m1 = m0 + 4 * (lane >> 5);
+  const int lane = threadIdx.x & 63;
+  const int m0 = tm * T::TM + T::row0(), m1 = m0 + 4 * (lane >> 5);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = tn * T::TN + (wave % T::WN) * 64 + 32 * j + (lane & 31);
+  for (int j = 0; j < T::J; ++j) {
+    const int n = tn * T::TN + T::column(j);
     if (n >= N) continue;
     float* q = p + n + ld * m1;
     auto row = [](int i, int e) { return 32 * i + 8 * (e / 4) + e % 4; };
-    if (m0 + 128 <= M) {
-      float old[4][16];
+    if (m0 + 32 * T::MI <= M) {
+      float old[T::MI][16];
       if (ADD) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < T::MI; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e) old[i][e] = q[ld * row(i, e)];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < T::MI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) q[ld * row(i, e)] = ADD ? old[i][e] + value(acc.x[i][j][e]) : value(acc.x[i][j][e]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < T::MI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (m1 + row(i, e) < M) {

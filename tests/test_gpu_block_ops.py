@@ -393,6 +393,10 @@ FFN = [  # N, D, F, activation, bias
     # the forward on packed operands too
     (1021, 257, 1300, "silu", False), (2050, 300, 700, "relu", True), (3000, 130, 1000, "gelu", True),
     (700, 1100, 600, "sigmoid", False), (5000, 33, 1900, "silu", True), (513, 1000, 999, "gelu", False),
+    # every size of tile, with sums that are split and whole
+    (520, 2100, 260, "relu", True), (300, 4100, 260, "sigmoid", False), (1000, 130, 4000, "silu", True),
+    (1000, 4100, 1050, "gelu", False), (4100, 4100, 20, "silu", True), (65, 2100, 4000, "gelu", True),
+    (4100, 130, 4000, "relu", False),
 ]
 
 
