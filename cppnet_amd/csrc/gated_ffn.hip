@@ -295,14 +295,15 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(FfnArgs a, const float* _
 // cores keep up with memory and nothing is packed.  A block takes 8 hidden features
 // (16 columns of W, the rows of the 16 x 16 tiles) and up to 128 rows; its eight waves
 // share out D and meet in LDS.
-// Packed, a call takes about 15 us more for its launches and 3.6 us for every million of D
+// Packed, a call takes about 12 us more for its launches and 3.6 us for every million of D
 // F to pack W, but a quarter of the time for a row's products.  This way and packed, us:
-// 128 rows, 512 -> 2048 10.7 and 26.7, 1024 -> 4096 39 and 47; 256 rows, 512 -> 2048
-// 21.8 and 26.6; 384 rows 32.6 and 29.5; 1024 rows, 256 -> 512 12.0 and 23.7.
+// 128 rows, 512 -> 2048 11.1 and 25, 1024 -> 4096 40 and 44; 256 rows, 512 -> 2048 22 and
+// 26.7; 384 rows 35 and 27.5; 512 rows, 512 -> 1024 21.8 and 24; 1024 rows, 256 -> 512 12.4
+// and 16.8, 2048 rows 21.4 and 18.1.
 constexpr int kFewBlock = 128;
 bool few_rows(int64_t N, int64_t D, int64_t F) {
   const double rows = (double)(N <= 64 ? (N + 15) / 16 * 16 : (N + kFewBlock - 1) / kFewBlock * kFewBlock);
-  return N <= 65535 * (int64_t)kFewBlock && 1e-6 * (double)D * (double)F * (0.05 * rows - 3.6) <= 15.0;
+  return N <= 65535 * (int64_t)kFewBlock && 1e-6 * (double)D * (double)F * (0.05 * rows - 3.6) <= 12.0;
 }
 template <int NB>
 __global__ void __launch_bounds__(512) ffn_few_kernel(FfnArgs a) {
@@ -871,12 +872,12 @@ int run_forward(FfnArgs& a, hipStream_t st, const char* who) {
   return check_launch(who);
 }
 
-// Few rows: dZ, and the Linear's backward over it.  This way and packed, us: 32 rows,
-// 512 -> 2048 20 and 37, 256 rows 37 and 44, 512 rows 54 and 55; 1024 -> 4096 64 rows 40
-// and 54, 256 rows 76 and 73.  64 rows fill a quarter of a packed tile, so they take
-// this way at any size.
+// Few rows: dZ, and the Linear's backward over it.  This way and packed, both with the
+// forward, us: 512 -> 2048 65 rows 40 and 44, 128 rows 43 and 44, 256 rows 64 and 58; 1024 ->
+// 4096 64 rows 67 and 82, 128 rows 103 and 106, 256 rows 147 and 132; 1024 -> 1024 96 rows 47
+// and 51; 256 -> 512 256 rows 31.5 and 36; 2048 -> 8192 64 rows 204 and 251.
 bool few_rows_back(int64_t N, int64_t D, int64_t F) {
-  return N <= 64 || (N <= 256 && (double)N * (double)D * (double)F <= 5e8);
+  return N <= 96 || (N <= 256 && (double)N * (double)D * (double)F <= 1.5e8);
 }
 
 int run_backward_few(FfnArgs& a, float* dX, float* dW, float* db, int accumulate, hipStream_t st, const char* who) {
