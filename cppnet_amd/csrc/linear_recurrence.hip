@@ -400,7 +400,7 @@ int launch(RecArgs& a, int64_t blocks, int threads, hipStream_t st, const char* 
     return CNHIP_OK;
   }
   const dim3 grid((unsigned)blocks, (unsigned)a.segments);
-  if constexpr (LAY != kShort) {
+  if constexpr (LAY != kShort && (BWD || U == 2)) {  // (the forward's U = 1 is for short sequences)
     hipLaunchKernelGGL((recurrence_kernel<LAY, BWD, IG, U, 1>), grid, dim3(threads), 0, st, a);
     CNHIP_TRY(check_launch(who));
     hipLaunchKernelGGL((recurrence_kernel<LAY, BWD, IG, U, 2>), grid, dim3(threads), 0, st, a);

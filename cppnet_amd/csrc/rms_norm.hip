@@ -527,9 +527,9 @@ __global__ void __launch_bounds__(kTileThreads) rms_norm_grad_kernel(NormArgs a)
 // Up to kHeldFeatures features: a block holds 32 rows, a line of every column, with all
 // of their features in registers, and one launch does it.  8 lanes go along the rows, 4
 // rows each, and CH times kNormWaves kCols features, of which a wave has kCols side by
-// side.  Behind the last feature a wave reads the last ones again and counts and writes
-// nothing (a test around its loads takes registers that there are not: 8192 x 1024, back,
-// 77 us for 24).
+// side.  Behind the last feature a wave reads the last kCols again and counts and writes
+// those that no other has (a test around its loads takes registers that there are not:
+// 8192 x 1024, back, 77 us for 24).
 constexpr int kHeldRows = 32;
 // The blocks of an XCD (every eighth) take row tiles side by side: of an odd number of rows
 // neighbours share lines.
@@ -553,8 +553,10 @@ struct HeldSeat {
     j = (uint32_t)row + (uint32_t)a.N * lane_f;
     left = WHOLE || n0 + row + 4 <= N ? 4 : n0 + row < N ? (int)(N - n0 - row) : 0;
   }
-  __device__ __forceinline__ bool has(int k) const { return f0 + k * (kNormWaves * kCols) < F; }
-  __device__ __forceinline__ int64_t column(int k) const { return has(k) ? f0 + k * (kNormWaves * kCols) : F - kCols; }
+  // The first of the wave's features: where they would end behind the last, those before.
+  __device__ __forceinline__ int column(int k) const { return min(first(k), (int)F - kCols); }
+  __device__ __forceinline__ int first(int k) const { return f0 + k * (kNormWaves * kCols); }
+  __device__ __forceinline__ bool has(int k) const { return column(k) + (int)lane_f >= first(k); }
   __device__ __forceinline__ int64_t at(int k) const { return n0 + N * column(k); }
   __device__ __forceinline__ f32x4 get(const float* p, int k) const {
     const float* q = p + at(k) + j;
@@ -737,8 +739,8 @@ void set_tiles(NormArgs& a) {
   a.col_tiles = (int)((col_tiles + a.chunks - 1) / a.chunks);
 }
 
-// Rows held: their features, at most as many as the registers of a block hold, and a
-// multiple of what a wave has side by side.  Both ways in tiles and held, us: 8192 x 512 42.4
+// Rows held: at least the features that a wave has side by side, and at most as many as
+// the registers of a block hold.  Both ways in tiles and held, us: 8192 x 512 42.4
 // and 36.6, 1000 x 512 22.7 and 18.5, 8191 x 512 49 and 35, 131072 x 256 317 and 263, 8192 x
 // 1024 94 and 67; more than 512 features need as many registers as there are and one
 // block's backward runs as long as two launches, so that few rows of them stay with
@@ -746,7 +748,7 @@ void set_tiles(NormArgs& a) {
 // 31.1, 6000 x 1024 28.3 + 35.4 and 21.8 + 28.5).
 constexpr int kHeldFeatures = 1024;
 bool rows_held(NormArgs& a, bool backward) {
-  if (a.F % (256 / kHeldRows) || a.F > kHeldFeatures || (backward && a.F > 512 && a.N < 6000)) return false;
+  if (a.F < 256 / kHeldRows || a.F > kHeldFeatures || (backward && a.F > 512 && a.N < 6000)) return false;
   if (a.N >= (int64_t)1 << 26) return false;  // (a grid has fewer than 2^32 threads)
   a.row_tiles = (int)((a.N + kHeldRows - 1) / kHeldRows);
   return true;

@@ -270,6 +270,8 @@ NORM = [  # N, F, p, residual, dsum
     (100, 256, 0.0, True, True), (131, 336, 0.1, True, False), (96, 384, 0.0, False, True), (70, 520, 0.0, True, True),
     (47, 768, 0.3, True, True), (6001, 1024, 0.1, True, True), (6040, 776, 0.0, True, True), (700, 640, 0.0, True, True),
     (300, 1032, 0.0, True, True), (1000, 39, 0.1, True, True), (20000, 13, 0.0, True, True), (16500, 65, 0.1, True, True),
+    (77, 9, 0.0, True, True), (300, 333, 0.1, True, True), (513, 517, 0.0, True, False), (6100, 1021, 0.1, True, True),
+    (90, 771, 0.0, True, True), (20000, 5, 0.1, True, True), (70, 3, 0.0, False, True),
 ]
 
 
