@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(T::NT, 2) ffn_forward_kernel(pr::GemmArgs g, F
   const int block0 = (tm * T::TM + T::row0()) / 32;  // the wave's first of 32 packed columns: a gate's
   const int64_t n0 = (int64_t)tn * T::TN + T::column(0);
   // A test for every element would end the run of loads, functions and stores behind it
-  // (1024 rows, 64 -> 1024: 24 us for 12; 8192 rows, 1024 -> 4096 475 us for 411), so the activation and whole tiles are told
-  // apart here.
+  // (in tiles of 256 x 128: 1024 rows, 64 -> 1024 24 us for 12; 8192 rows, 1024 -> 4096 475 us
+  // for 411), so the activation and whole tiles are told apart here.
   with_act(a.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < T::MI; i += 2) {
@@ -700,8 +700,8 @@ __device__ __forceinline__ void ffn_product(const FfnProduct& p, const FfnArgs& 
 }
 
 // Both products, the one of the longer blocks first, so that the shorter ones fill what is
-// left (3822 x 652 -> 1121 in small tiles: 30 us of 180), and db (+)= the sums of the groups of rows, in order, in the blocks
-// behind them.
+// left (3822 x 652 -> 1121 in small tiles: 30 us of 180), and db (+)= the sums of the
+// groups of rows, in order, in the blocks behind them.
 template <class T>
 __global__ void __launch_bounds__(T::NT, 2) ffn_grads_kernel(FfnArgs a, FfnProduct x, FfnProduct w, float* db, int add) {
   __shared__ __align__(16) char lds[T::kLds];
