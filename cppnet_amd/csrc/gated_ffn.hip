@@ -35,7 +35,7 @@ using pr::f32x16;
 using pr::f32x4;
 using pr::f32x4u;
 
-// Largest finite values, as bits: of W, of a piece's X and a bound of its dZ.
+// Largest finite values, as bits: of W, of a piece's X and half a bound of its dZ.
 struct FfnScales {
   uint32_t w, x, z;
 };
@@ -423,27 +423,31 @@ __global__ void __launch_bounds__(256) ffn_dz_kernel(FfnArgs a, float* __restric
 //   z >= 0: |act| <= z (sigmoid: 1), |act'| <= 1.13
 //   z < 0:  with r = e^z, or e^(-z^2 / 2) for GELU, |act| <= r |z|, |act'| <= r (1 + |z|);
 //   sigmoid: act <= r, and act' <= e^-|z| everywhere.  ReLU: as they are.
-__device__ __forceinline__ uint32_t grad_bound(int act, float gate, float up, float dh) {
+// Half of it is kept: the whole may lie past fp32's range where the gradient does not, and
+// a bound that is not finite does not count.
+__device__ __forceinline__ uint32_t half_grad_bound(int act, float gate, float up, float dh) {
   constexpr float kLog2e = 1.4426950408889634f;
   const float m = fabsf(gate);
   float y, d;
   if (act == CNHIP_GATE_RELU) {
-    y = relu_f(gate);
-    d = relu_mask(y);
+    y = 0.5f * relu_f(gate);
+    d = 0.5f * relu_mask(gate);
   } else {
-    const float r = __builtin_amdgcn_exp2f(-kLog2e * (act == CNHIP_GATE_GELU ? 0.5f * m * m : m));
+    const float r = 0.5f * __builtin_amdgcn_exp2f(-kLog2e * (act == CNHIP_GATE_GELU ? 0.5f * m * m : m));
     if (act == CNHIP_GATE_SIGMOID) {
-      y = gate < 0.f ? r : 1.f;
+      y = gate < 0.f ? r : 0.5f;
       d = r;
     } else {
-      y = gate < 0.f ? r * m : gate;
-      d = gate < 0.f ? fmaf(r, m, r) : 1.13f;
+      y = gate < 0.f ? r * m : 0.5f * gate;
+      d = gate < 0.f ? fmaf(r, m, r) : 0.5f * 1.13f;
     }
   }
   return max(pr::finite_bits(dh * up * d), pr::finite_bits(dh * y));
 }
+// dZ's exponent from the largest of those.
+__device__ __forceinline__ int dz_exp(uint32_t half) { return pr::scale_exp(half) - 1; }
 
-// The largest finite |W|, |X| and bound of |dZ| of a piece's rows, by blocks.
+// The largest finite |W|, |X| and half the bound of |dZ| of a piece's rows, by blocks.
 __global__ void __launch_bounds__(1024) ffn_max_kernel(FfnArgs a) {
   __shared__ uint32_t part[16];
   uint32_t m = 0;
@@ -509,7 +513,7 @@ __global__ void __launch_bounds__(1024) ffn_max_kernel(FfnArgs a) {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          m = max(m, kind == 1 ? pr::finite_bits(x[u][e]) : grad_bound(a.act, x[u][e], y[u][e], z[u][e]));
+          m = max(m, kind == 1 ? pr::finite_bits(x[u][e]) : half_grad_bound(a.act, x[u][e], y[u][e], z[u][e]));
     }
   }
   m = pr::wave_max(m);
@@ -543,7 +547,7 @@ __global__ void __launch_bounds__(256) ffn_pack_kernel(FfnArgs a, int64_t z_wave
     const int64_t groups = (blocks + a.z_blocks - 1) / a.z_blocks, grp = f % groups;
     const int step = (int)(f / groups);
     const int64_t f0 = (int64_t)step * 16 + 8 * h;
-    const float s = pr::exp2i(pr::scale_exp(max_of(a, 2)));
+    const float s = pr::exp2i(dz_exp(max_of(a, 2)));
     float sg[8] = {}, su[8] = {};
     for (int64_t b = grp * a.z_blocks; b < (grp + 1) * a.z_blocks && b < blocks; ++b) {
       const int64_t n = b * 32 + r;
@@ -633,7 +637,7 @@ struct FfnOut {
 // COLS: row m of the product is column_of(m) of the output.
 template <bool COLS>
 __device__ __forceinline__ int scale_out(const FfnArgs& a) {
-  return -pr::scale_exp(a.scales->z) - pr::scale_exp(COLS ? a.scales->x : a.scales->w);
+  return -dz_exp(a.scales->z) - pr::scale_exp(COLS ? a.scales->x : a.scales->w);
 }
 
 // A product of the backward as blocks [tile][split].
