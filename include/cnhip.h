@@ -917,8 +917,9 @@ int cnhip_linear_recurrence_backward(const float* x, const float* f, const float
  * Products of many rows run on pairs of fp16 terms as above; the operands with a
  * largest value of their own are a row of X and 32 columns of W in the forward; W, the
  * rows of X and those of Z's gradient that go through together in the backward (2^26 /
- * hidden, at least 1024).  For Z's gradient a bound stands for the largest value, a few
- * times it unless every gate lies next to a zero of act'.  An infinity in such an
+ * hidden, at least 1024).  For Z's gradient a bound stands for the largest value: at most
+ * twice that of the up half, and 6 times that of the gate's unless its gate lies next to
+ * the zero of SiLU's or GELU's act' (between -1.8 and -0.37).  An infinity in such an
  * operand comes out as NaN.  The stream's scratch holds X and W as packed, in the
  * backward (a piece of) Z's gradient, and the parts of products that are split. */
 #define CNHIP_GATE_SILU 0     /* z sigmoid(z) */
