@@ -1,12 +1,89 @@
 """GPU tests of a recurrent block's operators where their ranges end."""
 import numpy as np
 import pytest
+import torch
 
 import block_ops_ref as ref
-from test_gpu_block_ops import Ffn
+from cppnet_amd import ops
+from test_gpu_block_ops import Ffn, Recurrence
+from test_gpu_lm_ops import REF, SAMPLE
 
 pytestmark = pytest.mark.gpu
 U = ref.U
+
+
+# --------------------------------------------------------------- recurrence
+SHAPES = [(5, 1, 9), (5, 30, 9), (5, 600, 9), (2, 40000, 2)]  # the last in segments of its steps
+
+
+def same(got, plain, where):
+    for name in ("h", "dx", "df", "di"):
+        if name in got:
+            np.testing.assert_array_equal(got[name][where], plain[name][where])
+
+
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("B,S,D", SHAPES)
+def test_recurrence_inputs_that_are_not_finite(gpu, B, S, D, gate, rows):
+    """x at a step reaches h from there on and its own and later gates' gradients; f the
+    gradients of earlier steps too.  No other sequence, and no step that it does not reach,
+    changes a bit."""
+    print(f"[recurrence] {B}x{S} D={D} rows={rows} gate={gate}", flush=True)
+    r = Recurrence(B, S, D, rows, gate, True, None)
+    plain, at = r.run(), S // 2
+    r.x[1, at, 0], r.f[0, at, 1] = np.nan, np.nan
+    got = r.run()
+    clean = np.ones((B, S, D), bool)
+    clean[1, :, 0] = clean[0, :, 1] = False
+    same(got, plain, clean)
+    for b, d in ((1, 0), (0, 1)):
+        np.testing.assert_array_equal(got["h"][b, :at, d], plain["h"][b, :at, d])
+        assert np.isnan(got["h"][b, at:, d]).all() and np.isnan(got["last"][b, d])
+    np.testing.assert_array_equal(got["dx"][1, :, 0], plain["dx"][1, :, 0])  # has neither x nor h
+    np.testing.assert_array_equal(got["dh0"][1, 0], plain["dh0"][1, 0])
+    np.testing.assert_array_equal(got["df"][1, :at, 0], plain["df"][1, :at, 0])
+    assert np.isnan(got["df"][1, at + (1 if gate else 0):, 0]).all()
+    np.testing.assert_array_equal(got["dx"][0, at + 1:, 1], plain["dx"][0, at + 1:, 1])
+    assert np.isnan(got["df"][0, :, 1]).all() and np.isnan(got["dx"][0, :at, 1]).all() and np.isnan(got["dh0"][0, 1])
+
+
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("B,S,D", SHAPES)
+def test_recurrence_gradients_that_are_not_finite(gpu, B, S, D, gate, rows):
+    """dh at a step reaches that step and the earlier ones of its sequence, dh_last all of
+    them, and nothing else changes a bit."""
+    print(f"[recurrence] {B}x{S} D={D} rows={rows} gate={gate}", flush=True)
+    r = Recurrence(B, S, D, rows, gate, True, None)
+    plain, at = r.run(), S // 2
+    r.dh[1, at, 0], r.dh[0, at, 0], r.dl[1, 1] = np.nan, -np.inf, np.inf
+    got = r.run()
+    np.testing.assert_array_equal(got["h"], plain["h"])
+    clean = np.ones((B, S, D), bool)
+    clean[1, :at + 1, 0] = clean[0, :at + 1, 0] = clean[1, :, 1] = False
+    same(got, plain, clean)
+    for name in ("dx", "df", "di") if gate else ("dx", "df"):
+        assert not np.isfinite(got[name][~clean]).any(), name
+    assert not np.isfinite(got["dh0"][[1, 0, 1], [0, 0, 1]]).any()
+    others = np.ones((B, D), bool)
+    others[[1, 0, 1], [0, 0, 1]] = False
+    np.testing.assert_array_equal(got["dh0"][others], plain["dh0"][others])
+
+
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+def test_recurrence_infinite_gates_in_segments(gpu, rows):
+    """-inf drops the state and takes the input, +inf keeps the state, over every border."""
+    B, S, D = 2, 40000, 2
+    r = Recurrence(B, S, D, rows, False, True, None)
+    r.f[:, 1::2], r.f[:, 0::2] = np.inf, -np.inf
+    got = r.run()
+    np.testing.assert_array_equal(got["h"], np.repeat(r.x[:, 0::2], 2, 1))
+    assert (got["df"] == 0).all() and (got["dh0"] == 0).all() and (got["dx"][:, 1::2] == 0).all()
+    r.f[:] = np.inf
+    got = r.run()
+    np.testing.assert_array_equal(got["h"], np.broadcast_to(r.h0[:, None], (B, S, D)))
+    assert (got["dx"] == 0).all() and (got["df"] == 0).all()
 
 
 # ------------------------------------------------------ gated feed-forward
