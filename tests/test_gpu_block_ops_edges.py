@@ -1,4 +1,5 @@
-"""GPU tests of a recurrent block's operators where their ranges end."""
+"""GPU tests of a recurrent block's operators where their ranges end, on what is not finite,
+and at positions past 32 bits."""
 import numpy as np
 import pytest
 import torch
@@ -127,3 +128,109 @@ def test_ffn_scale_of_the_gradient(gpu, act, gate):
     bound = 1.05 * (34 * U * np.abs(want) + 2 * ref.F * np.abs(y).max() * c.W.max())
     print("  worst share of the bound", ref.check("dX", got, want, bound))
     c.buf.intact()
+
+
+# ----------------------------------------------------- positions past 32 bits
+def spare(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of free device memory")
+
+
+def filled(n, value):
+    """n floats, filled in parts."""
+    t = torch.empty(n, device="cuda")
+    for i in range(0, n, 1 << 28):
+        t[i:i + (1 << 28)] = value
+    return t
+
+
+@pytest.mark.parametrize("F", [1024, 2048])  # rows held, tiles
+def test_norm_backward_past_32_bits(gpu, F):
+    """2^31 + 2^21 values.  dy is one in the last column and zero elsewhere,
+    so every element has a value of its own form:  n = s r, c = gamma n_last / F,
+    ds_last = r (gamma - n_last c), ds_j = -r n_j c.  A value passes fewer than ten roundings;
+    one of dgamma's terms fewer than 2000 (32 rows of a block, or 256, then up to 66000 blocks
+    over 64 sums side by side, or 4100 over 8)."""
+    spare(60)
+    N = ((1 << 31) + (1 << 21)) // F
+    tail = 5000
+    s = filled(N * F, 1.0)
+    s[-tail:] = 2.0  # the last rows' last feature
+    size = np.where(np.arange(N) < N - tail, 1.0, 2.0)
+    r = 1 / np.sqrt((F - 1 + size ** 2) / F + float(np.float32(1e-5)))
+    rstd, gamma = torch.from_numpy(r.astype(np.float32)).cuda(), torch.full((F,), 3.0, device="cuda")
+    dy = filled(N * F, 0.0)
+    dy[-N:] = 1.0
+    dx, dg = torch.empty(N * F, device="cuda"), torch.empty(F, device="cuda")
+    ops.rms_norm_backward(s, rstd, gamma, dy, None, dx, None, dg, N, F)
+    c = 3 * size * r / F
+    np.testing.assert_allclose(dx[-N:].cpu().numpy(), r * (3 - size * r * c), rtol=20 * U)
+    for f in (0, 511, F - 2):
+        np.testing.assert_allclose(dx[f * N:(f + 1) * N].cpu().numpy(), -r * r * c, rtol=20 * U)
+    got = dg.cpu().numpy()
+    assert (got[:-1] == 0).all()
+    np.testing.assert_allclose(got[-1], (size * r).sum(), rtol=2000 * U)
+
+
+@pytest.mark.parametrize("rows", [REF, SAMPLE])
+def test_recurrence_backward_past_32_bits(gpu, rows):
+    """Four chains of 2^29 + 2^19 steps whose gate is one half: every value is a power of two
+    times a small number, and exact."""
+    spare(70)
+    B, D = 2, 2
+    n = (1 << 31) + (1 << 21)
+    S = n // 4
+    zero, h, dh = filled(n, 0.0), filled(n, 0.0), filled(n, 0.0)
+    at = lambda b, t, d: b + B * t + B * S * d if rows == REF else t + S * b + B * S * d  # noqa: E731
+    dh[at(0, 2, 0)], dh[at(1, S - 1, 1)], dh[at(0, S - 2, 1)] = 16.0, 64.0, 32.0
+    h[at(1, S - 2, 1)], h[at(0, 0, 0)] = 8.0, 4.0
+    last = torch.tensor([0.0, 128.0, 0.0, 0.0], device="cuda")  # [B, D] as it is stored: b + B d
+    dx, df, dh0 = filled(n, 7.0), filled(n, 7.0), torch.empty(4, device="cuda")
+    ops.linear_recurrence_backward(zero, zero, None, None, h, dh, last, dx, df, None, dh0, B, S, D, rows=rows)
+    # g halves from step to step towards the first; dx = g / 2, df = g h_{t-1} / 4
+    for b, t, d, g in ((0, 2, 0, 16.0), (1, S - 1, 1, 64.0), (0, S - 2, 1, 32.0), (1, S - 1, 0, 128.0)):
+        for k in range(3):
+            assert float(dx[at(b, t - k, d)]) == g / 2 ** k / 2, (b, t, d, k)
+    for b, t, d in ((0, 3, 0), (0, S - 1, 1), (0, S - 1, 0), (0, S // 2, 0), (1, 0, 0), (1, 1, 1)):
+        assert float(dx[at(b, t, d)]) == 0
+    assert float(df[at(1, S - 1, 1)]) == 64.0 * 8 / 4 and float(df[at(0, 1, 0)]) == 8.0 * 4 / 4
+    df[at(1, S - 1, 1)] = df[at(0, 1, 0)] = 0
+    assert sum(float(df[i:i + (1 << 28)].abs().max()) for i in range(0, n, 1 << 28)) == 0
+    np.testing.assert_array_equal(dh0.cpu().numpy(), [2.0, 0.0, 0.0, 0.0])
+
+
+def test_ffn_past_32_bits(gpu):
+    """2^20 + 3 rows and 1025 hidden features, so that Z has more than 2^31 values; all of them
+    small whole numbers, and every sum below 2^24, so that both directions are exact.
+      Z = (n % 3) (1 + j % 2) + 1 + j % 3 (ReLU keeps it), dH = 1 or -1 in turn."""
+    spare(40)
+    N, D, F = (1 << 20) + 3, 2, 1025
+    n, j = torch.arange(N, device="cuda"), torch.arange(2 * F, device="cuda")
+    X = torch.stack([n % 3, torch.ones_like(n)]).float()                     # (D, N)
+    W = torch.stack([1 + j % 2, j % 3], 1).float().contiguous()              # (2 F, D)
+    b = torch.ones(2 * F, device="cuda")
+    H, Z = torch.empty(F, N, device="cuda"), torch.empty(2 * F, N, device="cuda")
+    ops.gated_ffn_forward(X, W, b, H, Z, N, D, F, act="relu")
+
+    def z_of(a, e):
+        return X[0] * W[a:e, :1] + (W[a:e, 1:] + 1)
+    step = 41  # 1025 = 25 41
+    for a in range(0, F, step):
+        g, u = z_of(a, a + step), z_of(F + a, F + a + step)
+        assert torch.equal(Z[a:a + step], g) and torch.equal(Z[F + a:F + a + step], u)
+        assert torch.equal(H[a:a + step], g * u)
+    dH = H
+    for f in range(F):
+        dH[f] = 1 - 2 * ((n + f) % 2)
+    dX, dW, db = torch.empty(D, N, device="cuda"), torch.empty(2 * F, D, device="cuda"), torch.empty(2 * F, device="cuda")
+    ops.gated_ffn_backward(X, W, Z, dH, dX, dW, db, N, D, F, act="relu")
+    wX = torch.zeros(D, N, device="cuda", dtype=torch.float64)
+    for a in range(0, F, step):
+        dg, du = (dH[a:a + step] * z_of(F + a, F + a + step)).double(), (dH[a:a + step] * z_of(a, a + step)).double()
+        for at, dz in ((a, dg), (F + a, du)):
+            w = W[at:at + step].double()
+            for d in range(D):
+                wX[d] += (dz * w[:, d:d + 1]).sum(0)
+                assert torch.equal(dW[at:at + step, d].double(), (dz * X[d].double()).sum(1))
+            assert torch.equal(db[at:at + step].double(), dz.sum(1))
+    assert torch.equal(dX.double(), wX)
