@@ -84,9 +84,16 @@ __device__ __forceinline__ void sigmoid_parts(float z, float& on, float& off) {
   off = z >= 0.f ? e * r : r;
   if (z != z) on = off = z;
 }
+// Phi(z), and exp(-z^2 / 2); beyond 200 it is 0 or 1, and the square would leave fp32's range.
+__device__ __forceinline__ float gate_cdf(float z, float& e) {
+  return ncdf_f(z, fminf(fabsf(z), 200.f) * 0.70710678118654752440f, &e);
+}
 // act(z)
 __device__ __forceinline__ float gate_f(int act, float z) {
-  if (act == CNHIP_GATE_GELU) return gelu_f(z);
+  if (act == CNHIP_GATE_GELU) {
+    float e;
+    return z * gate_cdf(z, e);
+  }
   if (act == CNHIP_GATE_RELU) return relu_f(z);
   float on, off;
   sigmoid_parts(z, on, off);
@@ -95,8 +102,8 @@ __device__ __forceinline__ float gate_f(int act, float z) {
 // act(z) and act'(z)
 __device__ __forceinline__ void gate_both(int act, float z, float& y, float& d) {
   if (act == CNHIP_GATE_GELU) {
-    float e;  // exp(-z^2 / 2)
-    const float cdf = ncdf_f(z, fabsf(z) * 0.70710678118654752440f, &e);
+    float e;
+    const float cdf = gate_cdf(z, e);
     y = z * cdf;
     d = fmaf(z, 0.39894228040143267794f * e, cdf);
     return;

@@ -923,7 +923,7 @@ int cnhip_linear_recurrence_backward(const float* x, const float* f, const float
  * operand comes out as NaN.  The stream's scratch holds X and W as packed, in the
  * backward (a piece of) Z's gradient, and the parts of products that are split. */
 #define CNHIP_GATE_SILU 0     /* z sigmoid(z) */
-#define CNHIP_GATE_GELU 1     /* z Phi(z), as CNHIP_ACT_GELU */
+#define CNHIP_GATE_GELU 1     /* z Phi(z), as CNHIP_ACT_GELU; gates past +-2^64 too */
 #define CNHIP_GATE_SIGMOID 2
 #define CNHIP_GATE_RELU 3
 int cnhip_gated_ffn_forward(const float* X, const float* W, const float* b, float* H, float* Z,

@@ -130,6 +130,24 @@ def test_ffn_scale_of_the_gradient(gpu, act, gate):
     c.buf.intact()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "relu"])
+@pytest.mark.parametrize("N,D,F", [(20, 8, 40), (300, 1100, 700)])  # fp32 MFMAs and the Linear's backward; packed
+def test_ffn_gates_of_any_size(gpu, act, N, D, F):
+    """Gates up to 1e30, whose squares are past fp32's range."""
+    c = Ffn(N, D, F, act, True)
+    far = np.float32(10.0) ** np.linspace(2, 30, F // 2).astype(np.float32)
+    c.b = np.concatenate([far, -far, np.full(F, 3.0)]).astype(np.float32)
+    c.X[:] = 0
+    got, want = c.forward(), ref.ffn_forward(c.X, c.W, c.b, act)
+    c.Z = np.broadcast_to(c.b, (N, 2 * F)).astype(np.float32).copy()
+    c.X = np.random.default_rng(1).standard_normal(c.X.shape).astype(np.float32)
+    want |= ref.ffn_backward(c.X, c.W, c.Z, c.dH, act)
+    for name, value in (got | c.backward()).items():
+        assert np.isfinite(value).all(), name
+        ref.check(name, value, *want[name])
+    c.buf.intact()
+
+
 # ----------------------------------------------------- positions past 32 bits
 def spare(gib):
     if torch.cuda.mem_get_info()[0] < gib << 30:
