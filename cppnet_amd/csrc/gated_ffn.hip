@@ -16,9 +16,9 @@
 // Bound by the fp16 matrix cores at the clock that the power limit leaves, which differs
 // from card to card.  8192 rows, 1024 -> 4096, GELU: forward 411 to 490 us (280 to 334
 // TFLOP/s of fp32 products, where a third of a library's fp16 rate is 387) and packing 38;
-// back 711 to 813 (338 to 387), packing 152 (5.3 TB/s) and the bound of dZ 103 (4.6 TB/s).
+// back 711 to 813 (338 to 387), packing 152 (5.3 TB/s) and the bound of dZ 100 (4.7 TB/s).
 // Few tiles by latency and what is moved between the launches: 1021 rows, 513 -> 1365, 9 +
-// 21.5 us forward and 10 + 10.8 + 36 + 4.5 back.  Few rows by W: 4 rows, 512 -> 2048 4.7 us.
+// 21.5 us forward and 9.3 + 10.8 + 36 + 4.5 back.  Few rows by W: 4 rows, 512 -> 2048 4.7 us.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -432,7 +432,9 @@ int run(RecArgs& a, int rows, hipStream_t st, const char* who) {
   const int64_t rounds = (a.S + span * most - 1) / (span * most);
   a.waves = (int)((a.S + span * rounds - 1) / (span * rounds));
   const int64_t full = span * kMostWaves;
-  if (teams < 128 && a.S >= 2 * full) {  // half the chip would idle
+  // Half the chip would idle: at most 128 blocks, so that from 65 teams on, or below twice
+  // the steps of a block of all waves, one block still takes a chain's steps from end to end.
+  if (teams < 128 && a.S >= 2 * full) {
     a.waves = kMostWaves;
     int64_t n = 128 / teams;
     if (n > a.S / full) n = a.S / full;

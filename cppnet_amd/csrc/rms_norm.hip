@@ -7,8 +7,9 @@
 //   ds = dsum + rstd (d - n mean_f(d n)),  dresidual = ds, dx = drop(ds),
 //   dgamma_f (+)= sum_n dy_nf n_nf
 //
-// Matrices are ColMajor [N, F]: the features of a row lie N apart.  Up to 1024 features,
-// a block holds 32 rows, a line of every column, in registers and reads everything once.
+// Matrices are ColMajor [N, F]: the features of a row lie N apart.  Up to 1024 features
+// (back, of less than 6000 rows, up to 512) a block holds 32 rows, a line of every column,
+// in registers and reads everything once.
 // Of longer rows it would hold a part of a line of every column, each on a page of its
 // own (4097 x 4099, forward, 203 us in blocks of 16 rows for 81 here), so a larger matrix
 // goes through in tiles of 256 rows x 32 columns and more, a KiB in a row of every
@@ -525,7 +526,8 @@ __global__ void __launch_bounds__(kTileThreads) rms_norm_grad_kernel(NormArgs a)
 
 // ---- rows held
 // Up to kHeldFeatures features: a block holds 32 rows, a line of every column, with all
-// of their features in registers, and one launch does it.  8 lanes go along the rows, 4
+// of their features in registers, and one launch does it (back, but for joining the blocks'
+// parts of dgamma).  8 lanes go along the rows, 4
 // rows each, and CH times kNormWaves kCols features, of which a wave has kCols side by
 // side.  Behind the last feature a wave reads the last kCols again and counts and writes
 // those that no other has (a test around its loads takes registers that there are not:
@@ -740,12 +742,22 @@ void set_tiles(NormArgs& a) {
 }
 
 // Rows held: at least the features that a wave has side by side, and at most as many as
-// the registers of a block hold.  Both ways in tiles and held, us: 8192 x 512 42.4
-// and 36.6, 1000 x 512 22.7 and 18.5, 8191 x 512 49 and 35, 131072 x 256 317 and 263, 8192 x
-// 1024 94 and 67; more than 512 features need as many registers as there are and one
-// block's backward runs as long as two launches, so that few rows of them stay with
-// tiles there (1000 x 1024 11.5 + 13.5 and 13.4 + 15.8, 4096 x 1024 20.3 + 23.3 and 15.0 +
-// 31.1, 6000 x 1024 28.3 + 35.4 and 21.8 + 28.5).
+// the registers of a block hold.  Forward in tiles and held, us, in a graph:
+//   rows      512 features    768             1024
+//   40        9.1 and 6.1     9.5 and 7.5     9.2 and 8.7
+//   300       9.2 and 6.3     9.6 and 8.0     10.1 and 9.6
+//   1000      9.7 and 6.7     10.4 and 8.5    11.1 and 10.5
+//   2000      9.8 and 7.1     10.8 and 9.3    11.9 and 11.8
+//   4000      11.1 and 8.2    15.8 and 11.0   19.9 and 13.9
+//   8000      19.1 and 11.6   25.5 and 16.2   29.8 and 21.0
+// Both ways in tiles and held: 8192 x 512 42.4 and 36.6, 1000 x 512 22.7 and 18.5, 8191 x 512
+// 49 and 35, 131072 x 256 317 and 263, 8192 x 1024 94 and 67.  More than 512 features need
+// as many registers as there are and one block's backward runs as long as two launches,
+// so that few rows of them stay with tiles there (kernels' times: 1000 x 1024 13.5 and
+// 15.8, 4096 x 1024 23.3 and 31.1, 6000 x 1024 35.4 and 28.5; of 513 to 1023 features it is
+// not measured apart).  A backward in tiles behind a held forward takes some 2 us longer at
+// 1000 x 1024 than behind one in tiles, 26.2 for 24.6 both ways, and no longer at 300 and
+// 2000.
 constexpr int kHeldFeatures = 1024;
 bool rows_held(NormArgs& a, bool backward) {
   if (a.F < 256 / kHeldRows || a.F > kHeldFeatures || (backward && a.F > 512 && a.N < 6000)) return false;

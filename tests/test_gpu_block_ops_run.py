@@ -1,6 +1,6 @@
 """The operators of a recurrent block together, as a training step and as generation
-use them: eager, captured and replayed, over two streams, on another device than
-the current one; and at sizes whose positions pass 32 bits."""
+use them: eager, captured and replayed, over two streams; and at sizes whose positions
+pass 32 bits."""
 import numpy as np
 import pytest
 import torch
